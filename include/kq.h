@@ -1,8 +1,9 @@
 /*
  * kq.h -- C ABI of libkq, the MI355X (gfx950) decode hot path:
  *   int4 group-affine GEMV / batched skinny GEMM, codebook (VQ) dequant-GEMV,
- *   and the three-kernel MoE block (router top-k, gathered gate/up + SwiGLU,
- *   gathered down + weighted combine).
+ *   the three-kernel MoE block (router top-k, gathered gate/up + SwiGLU,
+ *   gathered down + weighted combine), and an 8-bit paged key/value cache with
+ *   the attention that reads it.
  *
  * Every entry point is stream-ordered and asynchronous: it validates its
  * arguments on the host, enqueues kernels on `stream` and returns. Nothing
@@ -378,6 +379,132 @@ kq_status kq_moe_block_unfused(const uint8_t* pool, const kq_moe_desc* d,
                                uint32_t batch, uint32_t* idx, float* wgt, uint16_t* xh,
                                uint16_t* H, void* Y, kq_dtype y_dtype, void* ws, size_t ws_bytes,
                                uint32_t* n_launches, kq_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * 8-bit key/value cache, and the attention that reads it
+ *
+ * A paged cache: n_pages pages of `page` tokens of every head. A sequence is a
+ * row of page ids; its token p is token p % page of its page p / page.
+ *
+ *   k     : codes [n_pages][heads][page][head_dim]
+ *   v     : codes [n_pages][heads][page / 16][head_dim][16] -- the 16 tokens of
+ *           a column lie together, as the product with the probabilities
+ *           takes them
+ *   k_exp, v_exp : uint8 [n_pages][heads][page / block], a byte for each block
+ *           of `block` tokens and head: a code c of the block stands for
+ *           c * 2^(byte - 127). kq_kv_write keeps byte - 127 within [-64, 121]
+ *           (KQ_KV_I8) or [-64, 119] (KQ_KV_E4M3).
+ *
+ * A code is an int8 (KQ_KV_I8) or an OCP e4m3 (KQ_KV_E4M3). Powers of two as
+ * scales: every product with one is exact, so the codes do not depend on how
+ * they are computed, and a block that tokens are appended to one by one is
+ * rarely scaled anew (a running maximum would be, 3.4 times on average over 16
+ * tokens, and cost each older token half a step every time).
+ *
+ * Constraints: head_dim 64, 96, 128, 192 or 256 (else KQ_EUNSUPPORTED); block a
+ * power of two from 16 to 256; page a power of two from block to 4096; 1 <=
+ * heads <= 1024; k and v 16-byte aligned. Offsets are 64-bit: the cache may be
+ * of any size.
+ * No counterpart in the reference, which has no attention.
+ * ------------------------------------------------------------------------ */
+typedef enum kq_kv_type { KQ_KV_I8 = 0, KQ_KV_E4M3 = 1 } kq_kv_type;
+
+typedef struct kq_kv_cache {
+    void* k;
+    void* v;
+    uint8_t* k_exp;
+    uint8_t* v_exp;
+    uint32_t type; /* kq_kv_type */
+    uint32_t n_pages, page, block, heads, head_dim;
+} kq_kv_cache;
+
+/* The sequences of a call and their newest tokens, the rows of q, k, v and o:
+ * sequence i has rows q_start[i] .. q_start[i + 1] - 1, or with q_start NULL the
+ * max_q rows from i * max_q on. They are the last of its kv_len[i] tokens:
+ * kv_len counts them, in kq_kv_write too.
+ *
+ * pages   : int32 [n_seq][max_pages] page ids; what lies behind a sequence's
+ *           last token is not read
+ * kv_len  : int32 [n_seq], 0 <= kv_len[i] <= max_len
+ * q_start : int32 [n_seq + 1], ascending, q_start[n_seq] <= n_rows; or NULL
+ * max_q   : at least the most rows of a sequence;  n_rows: the rows of the
+ *           arrays (more than the sequences have: the rest is left as it was)
+ * max_len : at least the longest kv_len; both bounds shape the launch
+ *
+ * pages, kv_len and q_start are device memory and cannot be checked on the
+ * host. The kernels stay in bounds whatever they hold: lengths are cut to
+ * max_len and max_pages * page, rows to max_q and n_rows, and the tokens of a
+ * page id outside [0, n_pages) are left out -- not written, not attended to,
+ * read as zeros.
+ * Constraints: 1 <= n_seq <= 65535; max_q, max_pages, max_len >= 1; max_len, n_rows
+ * < 2^31 - 2^16; q_start NULL: n_seq * max_q <= n_rows. */
+typedef struct kq_kv_batch {
+    const int32_t* pages;
+    const int32_t* kv_len;
+    const int32_t* q_start;
+    uint32_t n_seq, max_pages, max_q, n_rows, max_len;
+} kq_kv_batch;
+
+/* The rows of a tensor [n_rows][heads][head_dim]: element strides of a row and of a
+ * head; head_dim is contiguous. Strides are non-negative multiples of 8, the
+ * pointer 16-byte aligned (a slice of a fused projection's output is). */
+typedef struct kq_kv_rows {
+    void* p;
+    int64_t row, head;
+} kq_kv_rows;
+
+/* Writes the newest tokens' keys and values K, V (dtype KQ_F16 or KQ_BF16).
+ * Per block and head: a = the largest |x| of the block's new values, e = the
+ * smallest integer within the type's range with a <= 127 * 2^e (448 * 2^e), at
+ * least the block's present one where it holds older tokens of the sequence;
+ * codes are x * 2^-e rounded to nearest even, saturated. Where an older block's
+ * e grows its codes are rounded anew from their present values. Infinities
+ * become the largest code (and do not count in a), NaN zero: what is written
+ * is finite. Nothing but those blocks' new and re-rounded codes and exponents
+ * changes. One launch. A page that the call writes must belong to one
+ * sequence of it (pages of a shared prefix are only read). */
+kq_status kq_kv_write(const kq_kv_cache* cache, const kq_kv_batch* batch, const kq_kv_rows* K,
+                      const kq_kv_rows* V, kq_dtype dtype, kq_stream_t stream);
+
+/* Reads the newest tokens of each sequence -- q_start of whole lengths: the whole
+ * sequences -- into K, V (dtype KQ_F16, KQ_BF16 or KQ_F32): code * 2^e rounded to
+ * nearest even; values beyond the type's largest finite one become that. Rows
+ * at negative positions (more rows than tokens) are left as they were. */
+kq_status kq_kv_read(const kq_kv_cache* cache, const kq_kv_batch* batch, const kq_kv_rows* K,
+                     const kq_kv_rows* V, kq_dtype dtype, kq_stream_t stream);
+
+/* Attention of each row over its sequence's tokens in the cache. Query head h
+ * reads head h / (q_heads / heads). Row j of a sequence's n is at position
+ * pos = kv_len - n + j and sees tokens p with
+ *   causal:     p <= pos, and with window > 0 also p > pos - window
+ *   not causal: every p < kv_len (window must be 0).
+ *   O = sum_p exp(s_p) v_p / L,  L = sum_p exp(s_p) + exp(sinks[h]),
+ *   s_p = scale * (q . k_p);  lse = log L
+ * sinks: float [q_heads], or NULL for none. lse: float [n_rows][q_heads], or
+ * NULL. A row that sees nothing gets zeros (lse: the sink, or -inf). Rows of
+ * no sequence are left as they were. Q and O have q_heads heads, of dtype KQ_F16
+ * or KQ_BF16; O may not overlap Q.
+ * Scores, softmax and sums are fp32. The products run in fp16 on exact
+ * codes: bf16 queries are scaled to fp16 by a power of two for each row, which
+ * keeps every bit down to 2^-28 of the row's largest; probabilities are
+ * rounded to fp16, scaled so that 2^-28 of the row's largest is still normal.
+ * ws: kq_kv_attn_workspace_size bytes, 256-byte aligned, no initialisation and
+ * nothing kept in it between calls: a range of it for the partial results of
+ * sequences that are split among workgroups. Calls that share one must be
+ * stream-ordered. 0 from kq_kv_attn_workspace_size means invalid arguments.
+ * q_heads: a multiple of cache->heads, at most 64 times as many. Results do
+ * not change from run to run (no atomics). */
+typedef struct kq_kv_attn_desc {
+    uint32_t q_heads;
+    float scale;
+    uint32_t causal, window;
+    const float* sinks;
+} kq_kv_attn_desc;
+size_t kq_kv_attn_workspace_size(const kq_kv_cache* cache, const kq_kv_batch* batch,
+                                 uint32_t q_heads);
+kq_status kq_kv_attn(const kq_kv_cache* cache, const kq_kv_batch* batch, const kq_kv_attn_desc* d,
+                     const kq_kv_rows* Q, const kq_kv_rows* O, kq_dtype dtype, float* lse,
+                     void* ws, size_t ws_bytes, kq_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -166,6 +166,63 @@ kq_status check_ws(const kq_moe_desc* d, uint32_t batch, const void* ws, size_t 
     return KQ_OK;
 }
 
+// ---- 8-bit key/value cache
+uint32_t log2_of(uint32_t v) { return 31u - (uint32_t)__builtin_clz(v); }
+
+kq_status check_kv(const kq_kv_cache* c, const kq_kv_batch* b) {
+    if (!c || !b) return KQ_ENULL;
+    if (!(c->type == KQ_KV_I8 || c->type == KQ_KV_E4M3)) return KQ_EUNSUPPORTED;
+    if (!(c->head_dim == 64 || c->head_dim == 96 || c->head_dim == 128 || c->head_dim == 192 || c->head_dim == 256))
+        return KQ_EUNSUPPORTED;
+    if (!pow2(c->block) || c->block < 16 || c->block > 256) return KQ_EINVAL;
+    if (!pow2(c->page) || c->page < c->block || c->page > 4096) return KQ_EINVAL;
+    if (c->heads == 0 || c->heads > 1024 || c->n_pages == 0 || c->n_pages > 0x7FFFFFFFu) return KQ_EINVAL;
+    constexpr uint32_t kMost = 0x7FFF0000u;  // tokens and rows are ints in the kernels, with room for a tile
+    if (b->n_seq == 0 || b->n_seq > 65535 || b->max_pages == 0 || b->max_q == 0 || b->max_len == 0) return KQ_EINVAL;
+    if (b->max_len >= kMost || b->max_q >= kMost || b->n_rows >= kMost) return KQ_EINVAL;
+    if (!b->q_start && (uint64_t)b->n_seq * b->max_q > b->n_rows) return KQ_EINVAL;
+    return KQ_OK;
+}
+
+// The device memory of a call, which kq_kv_attn_workspace_size does without.
+kq_status check_kv_pointers(const kq_kv_cache* c, const kq_kv_batch* b) {
+    if (!c->k || !c->v || !c->k_exp || !c->v_exp || !b->pages || !b->kv_len) return KQ_ENULL;
+    if (!aligned(c->k, 16) || !aligned(c->v, 16)) return KQ_EALIGN;
+    if (!aligned(b->pages, 4) || !aligned(b->kv_len, 4) || !aligned(b->q_start, 4)) return KQ_EALIGN;
+    return KQ_OK;
+}
+
+kq_status check_kv_rows(const kq_kv_rows* r, const kq_kv_batch* b, uint32_t heads, uint32_t D, bool written) {
+    if (!r || !r->p) return KQ_ENULL;
+    if (r->row < 0 || r->head < 0 || r->row % 8 || r->head % 8) return KQ_EINVAL;
+    // rows and heads that overlap cannot be written
+    if (written && ((b->n_rows > 1 && r->row < (int64_t)D) || (heads > 1 && r->head < (int64_t)D))) return KQ_EINVAL;
+    return aligned(r->p, 16) ? KQ_OK : KQ_EALIGN;
+}
+
+kq::kv::Cache kv_cache(const kq_kv_cache& c) {
+    return {static_cast<uint8_t*>(c.k), static_cast<uint8_t*>(c.v), c.k_exp, c.v_exp, c.n_pages, c.heads,
+            log2_of(c.page), log2_of(c.block)};
+}
+kq::kv::Batch kv_batch(const kq_kv_batch& b) {
+    return {b.pages, b.kv_len, b.q_start, b.n_seq, b.max_pages, b.max_q, b.n_rows, b.max_len};
+}
+kq::kv::Rows kv_rows(const kq_kv_rows& r) { return {r.p, r.row, r.head}; }
+
+// Workgroups of a launch over the `unit`-token blocks of max_q tokens (grid.x).
+bool kv_blocks_fit(const kq_kv_cache* c, const kq_kv_batch* b, uint32_t unit) {
+    return ((uint64_t)(b->max_q / unit) + 2) * ((2 * c->heads + 3) / 4) < 0x7FFFFFFFull;
+}
+
+bool kv_attn_fits(const kq_kv_cache* c, const kq_kv_batch* b, uint32_t q_heads, const kq::kv::Plan& p) {
+    return (uint64_t)b->n_seq * p.tiles * c->heads < 0x7FFFFFFFull / p.splits &&
+           (uint64_t)b->n_seq * b->max_q < 0x7FFFFFFFull / q_heads;
+}
+
+kq_status check_kv_heads(const kq_kv_cache* c, uint32_t q_heads) {
+    return q_heads == 0 || q_heads % c->heads || q_heads / c->heads > 64 ? KQ_EINVAL : KQ_OK;
+}
+
 }  // namespace
 
 namespace kq {
@@ -529,6 +586,70 @@ kq_status kq_moe_block_unfused(const uint8_t* pool, const kq_moe_desc* d, const 
                                            reinterpret_cast<hipStream_t>(stream)));
     if (n_launches) *n_launches = st == KQ_OK ? kq::moe_unfused_launches(*d) : 0;
     return st;
+}
+
+// ------------------------------------------------------------ key/value cache
+kq_status kq_kv_write(const kq_kv_cache* cache, const kq_kv_batch* batch, const kq_kv_rows* K,
+                      const kq_kv_rows* V, kq_dtype dtype, kq_stream_t stream) {
+    kq_status st = check_kv(cache, batch);
+    if (st == KQ_OK) st = check_kv_pointers(cache, batch);
+    if (st != KQ_OK) return st;
+    if (!(dtype == KQ_F16 || dtype == KQ_BF16)) return KQ_EUNSUPPORTED;
+    st = check_kv_rows(K, batch, cache->heads, cache->head_dim, false);
+    if (st == KQ_OK) st = check_kv_rows(V, batch, cache->heads, cache->head_dim, false);
+    if (st != KQ_OK) return st;
+    if (!kv_blocks_fit(cache, batch, cache->block)) return KQ_EUNSUPPORTED;
+    return hip_status(kq::launch_kv_write(kv_cache(*cache), kv_batch(*batch), cache->head_dim, (int)cache->type,
+                                          kv_rows(*K), kv_rows(*V), dtype == KQ_BF16,
+                                          reinterpret_cast<hipStream_t>(stream)));
+}
+
+kq_status kq_kv_read(const kq_kv_cache* cache, const kq_kv_batch* batch, const kq_kv_rows* K,
+                     const kq_kv_rows* V, kq_dtype dtype, kq_stream_t stream) {
+    kq_status st = check_kv(cache, batch);
+    if (st == KQ_OK) st = check_kv_pointers(cache, batch);
+    if (st != KQ_OK) return st;
+    if (!(dtype == KQ_F16 || dtype == KQ_BF16 || dtype == KQ_F32)) return KQ_EUNSUPPORTED;
+    st = check_kv_rows(K, batch, cache->heads, cache->head_dim, true);
+    if (st == KQ_OK) st = check_kv_rows(V, batch, cache->heads, cache->head_dim, true);
+    if (st != KQ_OK) return st;
+    if (!kv_blocks_fit(cache, batch, 16)) return KQ_EUNSUPPORTED;
+    return hip_status(kq::launch_kv_read(kv_cache(*cache), kv_batch(*batch), cache->head_dim, (int)cache->type,
+                                         kv_rows(*K), kv_rows(*V), dtype, reinterpret_cast<hipStream_t>(stream)));
+}
+
+size_t kq_kv_attn_workspace_size(const kq_kv_cache* cache, const kq_kv_batch* batch, uint32_t q_heads) {
+    if (check_kv(cache, batch) != KQ_OK || check_kv_heads(cache, q_heads) != KQ_OK) return 0;
+    const size_t n = kq::kv_attn_ws_bytes(kv_cache(*cache), kv_batch(*batch), cache->head_dim, q_heads / cache->heads);
+    return n > 256 ? (n + 255) / 256 * 256 : 256;
+}
+
+kq_status kq_kv_attn(const kq_kv_cache* cache, const kq_kv_batch* batch, const kq_kv_attn_desc* d,
+                     const kq_kv_rows* Q, const kq_kv_rows* O, kq_dtype dtype, float* lse,
+                     void* ws, size_t ws_bytes, kq_stream_t stream) {
+    kq_status st = check_kv(cache, batch);
+    if (st == KQ_OK) st = check_kv_pointers(cache, batch);
+    if (st != KQ_OK) return st;
+    if (!d) return KQ_ENULL;
+    if (!(dtype == KQ_F16 || dtype == KQ_BF16)) return KQ_EUNSUPPORTED;
+    st = check_kv_heads(cache, d->q_heads);
+    if (st != KQ_OK) return st;
+    if (!(d->scale - d->scale == 0.0f) || (d->window && !d->causal)) return KQ_EINVAL;
+    st = check_kv_rows(Q, batch, d->q_heads, cache->head_dim, false);
+    if (st == KQ_OK) st = check_kv_rows(O, batch, d->q_heads, cache->head_dim, true);
+    if (st != KQ_OK) return st;
+    if (!aligned(d->sinks, 4) || !aligned(lse, 4)) return KQ_EALIGN;
+    const kq::kv::Cache c = kv_cache(*cache);
+    const kq::kv::Batch b = kv_batch(*batch);
+    const uint32_t group = d->q_heads / cache->heads;
+    const uint32_t window = d->window < batch->max_len ? d->window : 0;  // as wide as all there is: none
+    const kq::kv::Plan p = kq::kv_attn_plan(c, b, group, window);
+    if (!kv_attn_fits(cache, batch, d->q_heads, p)) return KQ_EUNSUPPORTED;
+    if (!ws || ws_bytes < kq_kv_attn_workspace_size(cache, batch, d->q_heads)) return KQ_EWORKSPACE;
+    if (!aligned(ws, 256)) return KQ_EALIGN;
+    const kq::kv::Attn a = {d->scale * 1.4426950408889634f, group, d->causal != 0, window, d->sinks, lse};
+    return hip_status(kq::launch_kv_attn(c, b, cache->head_dim, (int)cache->type, a, p, kv_rows(*Q), kv_rows(*O),
+                                         dtype == KQ_BF16, ws, reinterpret_cast<hipStream_t>(stream)));
 }
 
 }  // extern "C"

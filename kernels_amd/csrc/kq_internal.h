@@ -158,4 +158,60 @@ bool moe_one_supported(const kq_moe_desc& d, uint32_t batch);
 // The atomic sum(h) block's limits (the streaming gate/up and down).
 bool moe_atomic_supported(const kq_moe_desc& d, uint32_t batch);
 
+
+// 8-bit key/value cache (kq_kv_cache.hip, kq_kv_attn.hip).
+namespace kv {
+// The cache, with shifts for its powers of two.
+struct Cache {
+    uint8_t *k, *v, *k_exp, *v_exp;
+    uint32_t n_pages, heads, page_log2, block_log2;
+};
+// kq_kv_batch as the kernels take it.
+struct Batch {
+    const int32_t *pages, *kv_len, *q_start;
+    uint32_t n_seq, max_pages, max_q, n_rows, max_len;
+};
+struct Rows {
+    void* p;
+    int64_t row, head;
+};
+// What a call of the attention asks for, and its launch plan.
+struct Attn {
+    float scale_log2;  // scale * log2(e)
+    uint32_t group, causal, window;
+    const float* sinks;
+    float* lse;
+};
+struct Plan {
+    uint32_t tiles;   // row tiles of a sequence and head
+    uint32_t chunk;   // tokens of a split, a multiple of 64
+    uint32_t splits;  // at most, of a row tile
+};
+template <int N>
+struct Int {
+    static constexpr int value = N;
+};
+// f(Int<head_dim>, Int<type>) for a checked head_dim and type.
+template <class Fn>
+hipError_t by_dim(uint32_t D, int type, Fn f) {
+    auto of = [&](auto d) { return type == KQ_KV_I8 ? f(d, Int<KQ_KV_I8>()) : f(d, Int<KQ_KV_E4M3>()); };
+    switch (D) {
+        case 64: return of(Int<64>());
+        case 96: return of(Int<96>());
+        case 128: return of(Int<128>());
+        case 192: return of(Int<192>());
+        case 256: return of(Int<256>());
+        default: return hipErrorInvalidValue;
+    }
+}
+}  // namespace kv
+hipError_t launch_kv_write(const kv::Cache& c, const kv::Batch& b, uint32_t D, int type, const kv::Rows& K,
+                           const kv::Rows& V, bool bf, hipStream_t s);
+hipError_t launch_kv_read(const kv::Cache& c, const kv::Batch& b, uint32_t D, int type, const kv::Rows& K,
+                          const kv::Rows& V, kq_dtype f, hipStream_t s);
+size_t kv_attn_ws_bytes(const kv::Cache& c, const kv::Batch& b, uint32_t D, uint32_t group);  // of any window
+kv::Plan kv_attn_plan(const kv::Cache& c, const kv::Batch& b, uint32_t group, uint32_t window);
+hipError_t launch_kv_attn(const kv::Cache& c, const kv::Batch& b, uint32_t D, int type, const kv::Attn& a,
+                          const kv::Plan& p, const kv::Rows& Q, const kv::Rows& O, bool bf, void* ws, hipStream_t s);
+
 }  // namespace kq

@@ -29,7 +29,8 @@ EXPORTS = ("kq_status_str", "kq_last_hip_error", "kq_version", "kq_int4_gemv",
            "kq_moe_workspace_init", "kq_moe_workspace_error", "kq_moe_router_topk", "kq_moe_gate_up_swiglu",
            "kq_moe_down_combine", "kq_moe_block", "kq_moe_block_path", "kq_moe_block_noalloc",
            "kq_moe_unfused_workspace_size",
-           "kq_moe_block_unfused", "kq_vq_quantize_workspace_size", "kq_vq_quantize")
+           "kq_moe_block_unfused", "kq_vq_quantize_workspace_size", "kq_vq_quantize",
+           "kq_kv_write", "kq_kv_read", "kq_kv_attn_workspace_size", "kq_kv_attn")
 
 
 class KQError(RuntimeError):
@@ -50,6 +51,31 @@ class MoEDesc(C.Structure):
 
     def as_dict(self):
         return {f: getattr(self, f) for f, _ in self._fields_}
+
+
+class _KVCacheC(C.Structure):
+    """kq_kv_cache."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_exp", C.c_void_p), ("v_exp", C.c_void_p),
+                ("type", C.c_uint32), ("n_pages", C.c_uint32), ("page", C.c_uint32),
+                ("block", C.c_uint32), ("heads", C.c_uint32), ("head_dim", C.c_uint32)]
+
+
+class _KVBatchC(C.Structure):
+    """kq_kv_batch."""
+    _fields_ = [("pages", C.c_void_p), ("kv_len", C.c_void_p), ("q_start", C.c_void_p),
+                ("n_seq", C.c_uint32), ("max_pages", C.c_uint32), ("max_q", C.c_uint32),
+                ("n_rows", C.c_uint32), ("max_len", C.c_uint32)]
+
+
+class _KVRowsC(C.Structure):
+    """kq_kv_rows."""
+    _fields_ = [("p", C.c_void_p), ("row", C.c_int64), ("head", C.c_int64)]
+
+
+class _KVAttnC(C.Structure):
+    """kq_kv_attn_desc."""
+    _fields_ = [("q_heads", C.c_uint32), ("scale", C.c_float), ("causal", C.c_uint32),
+                ("window", C.c_uint32), ("sinks", C.c_void_p)]
 
 
 _lib = None
@@ -102,10 +128,17 @@ def lib():
         L.kq_vq_quantize_workspace_size.restype = sz
         L.kq_vq_quantize.argtypes = [vp, i32, u32, u32, u32, u32, u32, u32, C.c_uint64, vp, vp,
                                      vp, vp, sz, vp]
+        pc, pb, pr = C.POINTER(_KVCacheC), C.POINTER(_KVBatchC), C.POINTER(_KVRowsC)
+        L.kq_kv_write.argtypes = [pc, pb, pr, pr, i32, vp]
+        L.kq_kv_read.argtypes = [pc, pb, pr, pr, i32, vp]
+        L.kq_kv_attn_workspace_size.argtypes = [pc, pb, u32]
+        L.kq_kv_attn_workspace_size.restype = sz
+        L.kq_kv_attn.argtypes = [pc, pb, C.POINTER(_KVAttnC), pr, pr, i32, vp, vp, sz, vp]
         for name in EXPORTS:
             if name not in ("kq_status_str", "kq_last_hip_error", "kq_version",
                             "kq_moe_default_desc", "kq_moe_workspace_size",
-                            "kq_moe_unfused_workspace_size", "kq_vq_quantize_workspace_size"):
+                            "kq_moe_unfused_workspace_size", "kq_vq_quantize_workspace_size",
+                            "kq_kv_attn_workspace_size"):
                 getattr(L, name).restype = i32
         _lib = L
     return _lib
@@ -357,3 +390,153 @@ def moe_block_unfused(pool, desc, R, x, idx, wgt, H, y, ws, ws_bytes, batch=1, x
                                       _dt(y), _ptr(ws), ws_bytes, C.byref(n), _stream(stream)),
            "kq_moe_block_unfused")
     return n.value
+
+
+# ---------------------------------------------------------------------------
+# 8-bit key/value cache, and the attention that reads it
+# ---------------------------------------------------------------------------
+KV_I8, KV_E4M3 = 0, 1  # kq_kv_type
+
+
+def _need(ok, what):
+    if not ok:
+        raise ValueError(what)
+
+
+def _here(t, dtype, shape, what):
+    """t: a contiguous tensor of this type and shape on the current device."""
+    _need(t.dtype == dtype and tuple(t.shape) == tuple(shape) and t.is_contiguous(),
+          f"{what}: a contiguous {dtype} tensor {tuple(shape)}, not {t.dtype} {tuple(t.shape)}")
+
+
+class KVCache:
+    """kq_kv_cache over four contiguous tensors, kept alive with it:
+
+    k [n_pages][heads][page][head_dim] and v [n_pages][heads][page/16][head_dim][16]
+    of torch.int8 or torch.float8_e4m3fn, k_exp and v_exp uint8
+    [n_pages][heads][page/block]: a code c stands for c * 2^(exp - 127)."""
+
+    def __init__(self, k, v, k_exp, v_exp):
+        import torch
+        types = {torch.int8: KV_I8, torch.float8_e4m3fn: KV_E4M3}
+        _need(k.dtype in types, f"k: int8 or float8_e4m3fn, not {k.dtype}")
+        _need(k.dim() == 4 and k_exp.dim() == 3, "k: [n_pages][heads][page][head_dim], "
+              "k_exp: [n_pages][heads][page/block]")
+        n, heads, page, dim = k.shape
+        blocks = k_exp.shape[2]
+        _need(blocks and page % blocks == 0 and page % 16 == 0, "k_exp: [n_pages][heads][page/block]")
+        _here(k, k.dtype, k.shape, "k")
+        _here(v, k.dtype, (n, heads, page // 16, dim, 16), "v")
+        _here(k_exp, torch.uint8, (n, heads, blocks), "k_exp")
+        _here(v_exp, torch.uint8, (n, heads, blocks), "v_exp")
+        _need(len({t.device for t in (k, v, k_exp, v_exp)}) == 1, "the cache's tensors are on one device")
+        self.k, self.v, self.k_exp, self.v_exp = k, v, k_exp, v_exp
+        self.device = k.get_device()
+        self.heads, self.head_dim, self.page, self.block = heads, dim, page, page // blocks
+        self._c = _KVCacheC(k.data_ptr(), v.data_ptr(), k_exp.data_ptr(), v_exp.data_ptr(), types[k.dtype],
+                            n, page, page // blocks, heads, dim)
+        self._ref = C.byref(self._c)
+
+
+def kv_cache(n_pages, heads, head_dim, page=16, block=16, dtype=None, device=None):
+    """A new KVCache of zeros (dtype: torch.int8, the default, or torch.float8_e4m3fn)."""
+    import torch
+    _need(page % 16 == 0 and block > 0 and page % block == 0, "page: a multiple of block and of 16")
+    dtype, device = dtype or torch.int8, device or "cuda"
+    codes = [torch.zeros(s, dtype=torch.int8, device=device).view(dtype)
+             for s in ((n_pages, heads, page, head_dim), (n_pages, heads, page // 16, head_dim, 16))]
+    exps = [torch.full((n_pages, heads, page // block), 63, dtype=torch.uint8, device=device)
+            for _ in range(2)]
+    return KVCache(*codes, *exps)
+
+
+class KVBatch:
+    """kq_kv_batch: the sequences of a step, as every layer's calls take them.
+
+    pages int32 [n_seq][max_pages], kv_len int32 [n_seq] (the step's tokens
+    included), q_start int32 [n_seq + 1] or None (max_q rows each); max_len and
+    max_q are the host's bounds. The tensors may be refilled between calls."""
+
+    def __init__(self, pages, kv_len, max_len, q_start=None, max_q=1):
+        import torch
+        _need(pages.dim() == 2 and kv_len.dim() == 1, "pages: [n_seq][max_pages], kv_len: [n_seq]")
+        n = kv_len.shape[0]
+        _here(pages, torch.int32, (n, pages.shape[1]), "pages")
+        _here(kv_len, torch.int32, (n,), "kv_len")
+        if q_start is not None:
+            _here(q_start, torch.int32, (n + 1,), "q_start")
+        _need(0 <= max_len < 2**32 and 0 <= max_q < 2**32, "max_len, max_q: 32-bit")
+        _need(len({t.device for t in (pages, kv_len, q_start) if t is not None}) == 1,
+              "the batch's tensors are on one device")
+        self.pages, self.kv_len, self.q_start = pages, kv_len, q_start
+        self.device, self.n_seq, self.max_q, self.max_len = pages.get_device(), n, max_q, max_len
+        self._args = (_ptr(pages), _ptr(kv_len), _ptr(q_start), n, pages.shape[1], max_q)
+
+    def _c(self, rows):
+        return _KVBatchC(*self._args, rows, self.max_len)
+
+
+def _kv_rows(t, heads, dim, rows, dtype, what):
+    _need(t.dim() == 3 and t.shape[0] == rows and t.shape[1] == heads and t.shape[2] == dim,
+          f"{what}: [{rows}][{heads}][{dim}], not {tuple(t.shape)}")
+    _need(t.dtype == dtype, f"{what}: {dtype}, not {t.dtype}")
+    row, head, one = t.stride()
+    _need(one == 1, f"{what}: its last dimension is contiguous")
+    return _KVRowsC(t.data_ptr(), row, head)
+
+
+def _kv_device(cache, batch, *tensors):
+    """Refuses tensors of another device than the current one, whose stream the call takes."""
+    import torch
+    d = torch.cuda.current_device()
+    _need(cache.device == d and batch.device == d and all(t is None or t.get_device() == d for t in tensors),
+          f"every tensor of the call is on the current device ({d})")
+
+
+def _kv_move(name, cache, batch, k, v, stream):
+    _kv_device(cache, batch, k, v)
+    rows = k.shape[0]
+    a = _kv_rows(k, cache.heads, cache.head_dim, rows, k.dtype, "k")
+    b = _kv_rows(v, cache.heads, cache.head_dim, rows, k.dtype, "v")
+    f = lib().kq_kv_write if name == "kq_kv_write" else lib().kq_kv_read
+    _check(f(cache._ref, C.byref(batch._c(rows)), C.byref(a), C.byref(b), _dt(k), _stream(stream)), name)
+
+
+def kv_write(cache, batch, k, v, stream=None):
+    """The newest tokens' keys and values [n_rows][heads][head_dim] (float16 or
+    bfloat16, any row and head strides) into the cache."""
+    _kv_move("kq_kv_write", cache, batch, k, v, stream)
+
+
+def kv_read(cache, batch, k, v, stream=None):
+    """The batch's newest tokens out of the cache into k and v
+    [n_rows][heads][head_dim] (float16, bfloat16 or float32)."""
+    _kv_move("kq_kv_read", cache, batch, k, v, stream)
+
+
+def kv_attn_workspace_size(cache, batch, q_heads):
+    n = lib().kq_kv_attn_workspace_size(cache._ref, C.byref(batch._c(batch.n_seq * batch.max_q)), q_heads)
+    if n == 0:
+        raise KQError(KQ_EINVAL, "kq_kv_attn_workspace_size")
+    return n
+
+
+def kv_attn(cache, batch, q, out, ws, ws_bytes, scale=None, causal=True, window=0, sinks=None, lse=None,
+            stream=None):
+    """Attention of the rows q [n_rows][q_heads][head_dim] over their sequences in
+    the cache, into out (float16 or bfloat16 both). scale: None is
+    1 / sqrt(head_dim). window > 0: a row sees its own and the window - 1 tokens
+    before. sinks: float32 [q_heads]. lse: float32 [n_rows][q_heads], written."""
+    import torch
+    _kv_device(cache, batch, q, out, sinks, lse)
+    rows, q_heads = q.shape[0], q.shape[1]
+    a = _kv_rows(q, q_heads, cache.head_dim, rows, q.dtype, "q")
+    b = _kv_rows(out, q_heads, cache.head_dim, rows, q.dtype, "out")
+    if sinks is not None:
+        _here(sinks, torch.float32, (q_heads,), "sinks")
+    if lse is not None:
+        _here(lse, torch.float32, (rows, q_heads), "lse")
+    _need(0 <= window < 2**32, "window: 32-bit")
+    d = _KVAttnC(q_heads, cache.head_dim ** -0.5 if scale is None else scale, bool(causal), window, _ptr(sinks))
+    _check(lib().kq_kv_attn(cache._ref, C.byref(batch._c(rows)), C.byref(d), C.byref(a), C.byref(b), _dt(q),
+                            _ptr(lse), _ptr(ws), ws_bytes, _stream(stream)), "kq_kv_attn")

@@ -1,0 +1,201 @@
+"""The key/value cache's calls on the CPU: what the host refuses before any
+launch, and the oracle's own codes."""
+import ctypes as C
+
+import numpy as np
+import pytest
+import torch
+
+from kernels_amd import kq
+from tests import _kv
+
+FAKE = 0x10000
+
+
+def cache_c(**kw):
+    a = dict(k=FAKE, v=FAKE, k_exp=FAKE, v_exp=FAKE, type=kq.KV_I8, n_pages=64, page=16, block=16, heads=8, head_dim=128)
+    a.update(kw)
+    return kq._KVCacheC(**a)
+
+
+def batch_c(**kw):
+    a = dict(pages=FAKE, kv_len=FAKE, q_start=FAKE, n_seq=2, max_pages=8, max_q=3, n_rows=6, max_len=100)
+    a.update(kw)
+    return kq._KVBatchC(**a)
+
+
+def rows_c(**kw):
+    a = dict(p=FAKE, row=1024, head=128)
+    a.update(kw)
+    return kq._KVRowsC(**a)
+
+
+def attn_c(**kw):
+    a = dict(q_heads=32, scale=0.1, causal=1, window=0, sinks=None)
+    a.update(kw)
+    return kq._KVAttnC(**a)
+
+
+def write(c=None, b=None, K=None, V=None, dt=kq.F16, read=False):
+    f = kq.lib().kq_kv_read if read else kq.lib().kq_kv_write
+    return f(C.byref(c or cache_c()), C.byref(b or batch_c()), C.byref(K or rows_c()), C.byref(V or rows_c()), dt, None)
+
+
+def size(c=None, b=None, q_heads=32):
+    return kq.lib().kq_kv_attn_workspace_size(C.byref(c or cache_c()), C.byref(b or batch_c()), q_heads)
+
+
+def attn(c=None, b=None, d=None, Q=None, O=None, dt=kq.F16, lse=None, ws=FAKE, n=1 << 30):
+    return kq.lib().kq_kv_attn(C.byref(c or cache_c()), C.byref(b or batch_c()), C.byref(d or attn_c()),
+                               C.byref(Q or rows_c(row=4096)), C.byref(O or rows_c(row=4096)), dt, lse, ws, n, None)
+
+
+BAD_CACHE = [
+    (dict(type=2), kq.KQ_EUNSUPPORTED), (dict(head_dim=80), kq.KQ_EUNSUPPORTED), (dict(head_dim=0), kq.KQ_EUNSUPPORTED),
+    (dict(head_dim=512), kq.KQ_EUNSUPPORTED), (dict(block=8), kq.KQ_EINVAL), (dict(block=48, page=48), kq.KQ_EINVAL),
+    (dict(block=512, page=512), kq.KQ_EINVAL), (dict(block=32), kq.KQ_EINVAL), (dict(page=24), kq.KQ_EINVAL),
+    (dict(page=8192), kq.KQ_EINVAL), (dict(page=0), kq.KQ_EINVAL), (dict(heads=0), kq.KQ_EINVAL),
+    (dict(heads=1025), kq.KQ_EINVAL), (dict(n_pages=0), kq.KQ_EINVAL), (dict(n_pages=1 << 31), kq.KQ_EINVAL)]
+BAD_CACHE_P = [(dict(k=None), kq.KQ_ENULL), (dict(v=None), kq.KQ_ENULL), (dict(k_exp=None), kq.KQ_ENULL),
+               (dict(v_exp=None), kq.KQ_ENULL), (dict(k=FAKE + 8), kq.KQ_EALIGN), (dict(v=FAKE + 1), kq.KQ_EALIGN)]
+BAD_BATCH = [
+    (dict(n_seq=0), kq.KQ_EINVAL), (dict(n_seq=65536), kq.KQ_EINVAL), (dict(max_pages=0), kq.KQ_EINVAL),
+    (dict(max_q=0), kq.KQ_EINVAL), (dict(max_len=0), kq.KQ_EINVAL), (dict(max_len=0x7FFF0000), kq.KQ_EINVAL),
+    (dict(n_rows=0x80000000), kq.KQ_EINVAL), (dict(max_q=0x80000000), kq.KQ_EINVAL),
+    (dict(q_start=None, n_rows=5), kq.KQ_EINVAL)]
+BAD_BATCH_P = [(dict(pages=None), kq.KQ_ENULL), (dict(kv_len=None), kq.KQ_ENULL), (dict(pages=FAKE + 2), kq.KQ_EALIGN),
+               (dict(kv_len=FAKE + 1), kq.KQ_EALIGN), (dict(q_start=FAKE + 2), kq.KQ_EALIGN)]
+
+
+@pytest.mark.parametrize("kw,status", BAD_CACHE + BAD_CACHE_P)
+def test_bad_cache(kw, status):
+    c = cache_c(**kw)
+    assert write(c) == write(c, read=True) == attn(c) == status
+
+
+@pytest.mark.parametrize("kw,status", BAD_BATCH + BAD_BATCH_P)
+def test_bad_batch(kw, status):
+    b = batch_c(**kw)
+    assert write(b=b) == write(b=b, read=True) == attn(b=b) == status
+
+
+@pytest.mark.parametrize("kw,status", [
+    (dict(p=None), kq.KQ_ENULL), (dict(p=FAKE + 8), kq.KQ_EALIGN), (dict(row=-1024), kq.KQ_EINVAL),
+    (dict(head=-128), kq.KQ_EINVAL), (dict(row=1028), kq.KQ_EINVAL), (dict(head=132), kq.KQ_EINVAL)])
+def test_bad_rows(kw, status):
+    r = rows_c(**kw)
+    assert write(K=r) == write(V=r) == write(K=r, read=True) == write(V=r, read=True) == status
+    r = rows_c(**dict(dict(row=4096), **kw))
+    assert attn(Q=r) == attn(O=r) == status
+
+
+@pytest.mark.parametrize("kw", [dict(row=0), dict(head=0), dict(row=120), dict(head=64)])
+def test_overlapping_outputs_are_refused(kw):
+    r = rows_c(**kw)
+    assert write(K=r, read=True) == write(V=r, read=True) == attn(O=r) == kq.KQ_EINVAL
+
+
+def test_types():
+    assert write(dt=kq.F32) == kq.KQ_EUNSUPPORTED
+    assert write(dt=3) == write(dt=3, read=True) == kq.KQ_EUNSUPPORTED
+    assert attn(dt=kq.F32) == kq.KQ_EUNSUPPORTED
+
+
+@pytest.mark.parametrize("kw", [dict(q_heads=0), dict(q_heads=12), dict(q_heads=8 * 65), dict(scale=float("nan")),
+                                dict(scale=float("inf")), dict(causal=0, window=5)])
+def test_bad_attention(kw):
+    assert attn(d=attn_c(**kw)) == kq.KQ_EINVAL
+
+
+def test_null_structs():
+    L = kq.lib()
+    c, b, r, d = cache_c(), batch_c(), rows_c(row=4096), attn_c()
+    assert L.kq_kv_write(None, C.byref(b), C.byref(r), C.byref(r), 0, None) == kq.KQ_ENULL
+    assert L.kq_kv_read(C.byref(c), None, C.byref(r), C.byref(r), 0, None) == kq.KQ_ENULL
+    assert L.kq_kv_write(C.byref(c), C.byref(b), None, C.byref(r), 0, None) == kq.KQ_ENULL
+    assert L.kq_kv_attn(C.byref(c), C.byref(b), None, C.byref(r), C.byref(r), 0, None, FAKE, 1 << 30, None) == kq.KQ_ENULL
+    assert L.kq_kv_attn(C.byref(c), C.byref(b), C.byref(d), C.byref(r), None, 0, None, FAKE, 1 << 30, None) == kq.KQ_ENULL
+    assert L.kq_kv_attn_workspace_size(None, C.byref(b), 32) == 0
+
+
+def test_attention_pointers_and_workspace():
+    assert attn(lse=FAKE + 2) == attn(d=attn_c(sinks=FAKE + 1)) == kq.KQ_EALIGN
+    b = batch_c(max_len=20000, max_pages=2000)
+    n = size(b=b)
+    assert n > 256
+    assert attn(b=b, n=n - 1) == attn(b=b, ws=None) == kq.KQ_EWORKSPACE
+    assert attn(b=b, ws=FAKE + 64, n=n) == kq.KQ_EALIGN
+
+
+def test_workspace_size_refuses_what_the_call_refuses():
+    for kw, _ in BAD_CACHE:
+        assert size(cache_c(**kw)) == 0
+    for kw, _ in BAD_BATCH:
+        assert size(b=batch_c(**kw)) == 0
+    assert size(q_heads=0) == size(q_heads=12) == size(q_heads=8 * 65) == 0
+    assert size() >= 256
+
+
+def test_launches_too_large():
+    b = batch_c(n_seq=65535, max_q=0x7FFEFFFF, n_rows=0x7FFEFFFF)
+    assert write(cache_c(heads=1024), b, rows_c(), rows_c()) == kq.KQ_EUNSUPPORTED
+    assert write(cache_c(heads=1024), b, rows_c(row=1 << 17), rows_c(row=1 << 17), read=True) == kq.KQ_EUNSUPPORTED
+    assert attn(b=b, n=(1 << 63)) == kq.KQ_EUNSUPPORTED
+
+
+def test_python_tensors():
+    c = kq.kv_cache(4, 2, 64, page=32, block=16, device="cpu")
+    assert (c.page, c.block, c.heads, c.head_dim) == (32, 16, 2, 64)
+    e = kq.kv_cache(4, 2, 96, dtype=torch.float8_e4m3fn, device="cpu")
+    assert e._c.type == kq.KV_E4M3
+    with pytest.raises(ValueError):
+        kq.KVCache(c.k.float(), c.v, c.k_exp, c.v_exp)
+    with pytest.raises(ValueError):
+        kq.KVCache(c.k, c.v.transpose(3, 4), c.k_exp, c.v_exp)
+    with pytest.raises(ValueError):
+        kq.KVCache(c.k, c.v, c.k_exp[:, :, :1], c.v_exp)
+    with pytest.raises(ValueError):
+        kq.KVCache(c.k, c.v, c.k_exp.int(), c.v_exp)
+    with pytest.raises(ValueError):
+        kq.kv_cache(4, 2, 64, page=16, block=32, device="cpu")
+    pages, n = torch.zeros((2, 4), dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+    kq.KVBatch(pages, n, 10)
+    for bad in ((pages.long(), n), (pages.t(), n), (pages, n.long()), (pages[:1], n)):
+        with pytest.raises(ValueError):
+            kq.KVBatch(*bad, 10)
+    with pytest.raises(ValueError):
+        kq.KVBatch(pages, n, 10, q_start=n)
+    with pytest.raises(ValueError):
+        kq.KVBatch(pages, n, -1)
+    b = kq.KVBatch(pages, n, 10)
+    for shape in ((3, 2, 32), (3, 1, 64), (4, 2, 64)):
+        with pytest.raises(ValueError):
+            kq._kv_rows(torch.zeros(shape), 2, 64, 3, torch.float32, "k")
+    with pytest.raises(ValueError):
+        kq._kv_rows(torch.zeros((3, 64, 2)).transpose(1, 2), 2, 64, 3, torch.float32, "k")
+    with pytest.raises(kq.KQError):
+        kq.kv_attn_workspace_size(c, b, 3)
+
+
+@pytest.mark.parametrize("kind", ["i8", "e4m3"])
+def test_oracle_codes(kind):
+    """The oracle's rounding, against torch's conversions on the CPU and halfway values."""
+    codes = np.arange(256, dtype=np.uint8)
+    values = _kv.decode(codes, kind)
+    fine = np.isfinite(values) & (values != 0) & (np.abs(values) <= _kv.LARGEST[kind])
+    assert np.array_equal(_kv.encode(values[fine], kind), codes[fine])
+    rng = np.random.default_rng(0)
+    y = np.concatenate([rng.normal(0, 0.3 * _kv.LARGEST[kind], 5000), rng.normal(0, 0.01, 5000), (np.sort(values[fine])[1:] + np.sort(values[fine])[:-1]) / 2])
+    y = y.astype(np.float32)
+    t = torch.from_numpy(y).clamp(-_kv.LARGEST[kind], _kv.LARGEST[kind])
+    want = t.round().to(torch.int8).view(torch.uint8) if kind == "i8" else t.to(torch.float8_e4m3fn).view(torch.uint8)
+    assert np.array_equal(_kv.decode(_kv.encode(y.astype(np.float64), kind), kind), _kv.decode(want.numpy(), kind))
+
+
+def test_oracle_exponents():
+    for kind in ("i8", "e4m3"):
+        big = _kv.LARGEST[kind]
+        assert _kv.exponent(0.0, kind) == -64
+        assert _kv.exponent(big, kind) == 0 and _kv.exponent(np.nextafter(big, 1e9), kind) == 1
+        assert _kv.exponent(big / 2, kind) == -1
+        assert _kv.exponent(3.3e38, kind) == _kv.MAX_EXP[kind]
