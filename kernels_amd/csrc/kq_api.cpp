@@ -214,11 +214,6 @@ bool kv_blocks_fit(const kq_kv_cache* c, const kq_kv_batch* b, uint32_t unit) {
     return ((uint64_t)(b->max_q / unit) + 2) * ((2 * c->heads + 3) / 4) < 0x7FFFFFFFull;
 }
 
-bool kv_attn_fits(const kq_kv_cache* c, const kq_kv_batch* b, uint32_t q_heads, const kq::kv::Plan& p) {
-    return (uint64_t)b->n_seq * p.tiles * c->heads < 0x7FFFFFFFull / p.splits &&
-           (uint64_t)b->n_seq * b->max_q < 0x7FFFFFFFull / q_heads;
-}
-
 kq_status check_kv_heads(const kq_kv_cache* c, uint32_t q_heads) {
     return q_heads == 0 || q_heads % c->heads || q_heads / c->heads > 64 ? KQ_EINVAL : KQ_OK;
 }
@@ -620,8 +615,10 @@ kq_status kq_kv_read(const kq_kv_cache* cache, const kq_kv_batch* batch, const k
 
 size_t kq_kv_attn_workspace_size(const kq_kv_cache* cache, const kq_kv_batch* batch, uint32_t q_heads) {
     if (check_kv(cache, batch) != KQ_OK || check_kv_heads(cache, q_heads) != KQ_OK) return 0;
-    const size_t n = kq::kv_attn_ws_bytes(kv_cache(*cache), kv_batch(*batch), cache->head_dim, q_heads / cache->heads);
-    return n > 256 ? (n + 255) / 256 * 256 : 256;
+    const kq::kv::Batch b = kv_batch(*batch);
+    const uint32_t group = q_heads / cache->heads;
+    if (!kq::kv_attn_fits(kv_cache(*cache), b, group)) return 0;
+    return kq::kv_attn_ws_bytes(kv_cache(*cache), b, cache->head_dim, group);
 }
 
 kq_status kq_kv_attn(const kq_kv_cache* cache, const kq_kv_batch* batch, const kq_kv_attn_desc* d,
@@ -643,12 +640,11 @@ kq_status kq_kv_attn(const kq_kv_cache* cache, const kq_kv_batch* batch, const k
     const kq::kv::Batch b = kv_batch(*batch);
     const uint32_t group = d->q_heads / cache->heads;
     const uint32_t window = d->window < batch->max_len ? d->window : 0;  // as wide as all there is: none
-    const kq::kv::Plan p = kq::kv_attn_plan(c, b, group, window);
-    if (!kv_attn_fits(cache, batch, d->q_heads, p)) return KQ_EUNSUPPORTED;
-    if (!ws || ws_bytes < kq_kv_attn_workspace_size(cache, batch, d->q_heads)) return KQ_EWORKSPACE;
+    if (!kq::kv_attn_fits(c, b, group)) return KQ_EUNSUPPORTED;
+    if (!ws || ws_bytes < kq::kv_attn_ws_bytes(c, b, cache->head_dim, group)) return KQ_EWORKSPACE;
     if (!aligned(ws, 256)) return KQ_EALIGN;
     const kq::kv::Attn a = {d->scale * 1.4426950408889634f, group, d->causal != 0, window, d->sinks, lse};
-    return hip_status(kq::launch_kv_attn(c, b, cache->head_dim, (int)cache->type, a, p, kv_rows(*Q), kv_rows(*O),
+    return hip_status(kq::launch_kv_attn(c, b, cache->head_dim, (int)cache->type, a, kv_rows(*Q), kv_rows(*O),
                                          dtype == KQ_BF16, ws, reinterpret_cast<hipStream_t>(stream)));
 }
 

@@ -175,17 +175,19 @@ struct Rows {
     void* p;
     int64_t row, head;
 };
-// What a call of the attention asks for, and its launch plan.
+// What a call of the attention asks for.
 struct Attn {
     float scale_log2;  // scale * log2(e)
     uint32_t group, causal, window;
     const float* sinks;
     float* lse;
 };
-struct Plan {
-    uint32_t tiles;   // row tiles of a sequence and head
+// Launch of the kernel for many rows.
+struct RowPlan {
+    uint32_t rows;    // of a tile: 32 a wave
+    uint32_t tiles;   // of a sequence and head
     uint32_t chunk;   // tokens of a split, a multiple of 64
-    uint32_t splits;  // at most, of a row tile
+    uint32_t splits;  // at most, of a tile
 };
 template <int N>
 struct Int {
@@ -209,9 +211,21 @@ hipError_t launch_kv_write(const kv::Cache& c, const kv::Batch& b, uint32_t D, i
                            const kv::Rows& V, bool bf, hipStream_t s);
 hipError_t launch_kv_read(const kv::Cache& c, const kv::Batch& b, uint32_t D, int type, const kv::Rows& K,
                           const kv::Rows& V, kq_dtype f, hipStream_t s);
-size_t kv_attn_ws_bytes(const kv::Cache& c, const kv::Batch& b, uint32_t D, uint32_t group);  // of any window
-kv::Plan kv_attn_plan(const kv::Cache& c, const kv::Batch& b, uint32_t group, uint32_t window);
+namespace kv {
+// The kernel for many rows, heads D wide (kq_kv_rows_<D>.hip).
+template <int D>
+hipError_t launch_rows(int type, const Cache& c, const Batch& b, const Attn& a, const RowPlan& p, const Rows& Q,
+                       const Rows& O, bool bf, float* ws, hipStream_t s);
+template <> hipError_t launch_rows<64>(int, const Cache&, const Batch&, const Attn&, const RowPlan&, const Rows&, const Rows&, bool, float*, hipStream_t);
+template <> hipError_t launch_rows<96>(int, const Cache&, const Batch&, const Attn&, const RowPlan&, const Rows&, const Rows&, bool, float*, hipStream_t);
+template <> hipError_t launch_rows<128>(int, const Cache&, const Batch&, const Attn&, const RowPlan&, const Rows&, const Rows&, bool, float*, hipStream_t);
+template <> hipError_t launch_rows<192>(int, const Cache&, const Batch&, const Attn&, const RowPlan&, const Rows&, const Rows&, bool, float*, hipStream_t);
+template <> hipError_t launch_rows<256>(int, const Cache&, const Batch&, const Attn&, const RowPlan&, const Rows&, const Rows&, bool, float*, hipStream_t);
+}  // namespace kv
+// Workspace of a call with any window; whether its launches can be made.
+size_t kv_attn_ws_bytes(const kv::Cache& c, const kv::Batch& b, uint32_t D, uint32_t group);
+bool kv_attn_fits(const kv::Cache& c, const kv::Batch& b, uint32_t group);
 hipError_t launch_kv_attn(const kv::Cache& c, const kv::Batch& b, uint32_t D, int type, const kv::Attn& a,
-                          const kv::Plan& p, const kv::Rows& Q, const kv::Rows& O, bool bf, void* ws, hipStream_t s);
+                          const kv::Rows& Q, const kv::Rows& O, bool bf, void* ws, hipStream_t s);
 
 }  // namespace kq

@@ -20,11 +20,13 @@ namespace kq {
 namespace kv {
 
 constexpr int kTile = 64;      // tokens a wave takes at a time
+constexpr int kUnit = 256;     // tokens of a unit of work: a tile of each of four waves
 constexpr int kLift = 14;      // probabilities are scaled by 2^14: the fp16 ones stay normal down to 2^-28 of the largest
-constexpr int kSegment = 8192;  // tokens whose page ids a workgroup holds at a time
+constexpr int kIds = 4096;     // page ids that a workgroup holds at a time
+constexpr int kScan = 1024;    // most sequences whose lengths a workgroup adds up
 constexpr float kLowest = -3.0e38f;  // running maximum before any token
 
-// Tokens that a row tile sees: [lo, hi), lo a multiple of 64.
+// Tokens that rows row .. row + rows - 1 of a sequence and head see: [lo, hi), lo a multiple of 64.
 struct Span {
     int lo, hi;
 };
@@ -37,8 +39,9 @@ __device__ __forceinline__ Span span_of(const Seq& s, const Attn& a, int row, in
     }
     return v;
 }
-__device__ __forceinline__ int splits_of(const Span& v, int chunk) {
-    return v.hi > v.lo ? (v.hi - v.lo + chunk - 1) / chunk : 0;
+
+__device__ __forceinline__ int row_splits(const Span& v, int chunk) {
+    return v.hi > v.lo ? (v.hi - v.lo - 1) / chunk + 1 : 0;
 }
 
 // Of a value in lanes l, l ^ 16, l ^ 32, l ^ 48: one step of its largest or sum. (A bit cast of an
@@ -92,250 +95,428 @@ __device__ __forceinline__ float finish(const Attn& a, float m, float l, int row
     return y;
 }
 
-// One workgroup: a row tile of 16 rows, one split of its tokens, four waves that take
-// 64 tokens in turn and join their sums at the end.
+// The power of two that brings a row's largest bf16 magnitude (bits m) into [2^14, 2^15); an infinity or
+// NaN makes its row NaN anyway.
+__device__ __forceinline__ int bf_lift(uint32_t m) {
+    return m >= 0x7F80u ? 0 : min(max(14 - ((int)(m >> 7) - 127), -126), 126);
+}
+__device__ __forceinline__ f16x8 bf_f16x8(u32x4 raw, float up) {
+    f16x8 q;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        q[2 * j] = (_Float16)(bf2f((uint16_t)(raw[j] & 0xFFFF)) * up);
+        q[2 * j + 1] = (_Float16)(bf2f((uint16_t)(raw[j] >> 16)) * up);
+    }
+    return q;
+}
+
+// A row's query as the second operand of S^T, in fp16: 16 columns a lane of each 64, 8 of a
+// last 32. bf16 rows go through a power of two; returns what undoes it.
+template <int D>
+__device__ __forceinline__ float load_q(const Rows& Q, bool there, int row, uint32_t head, int g, int bf,
+                                        f16x8 (&q)[D / 32]) {
+    constexpr int C64 = D / 64;
+    u32x4 raw[D / 32];
+    const uint16_t* const x =
+        static_cast<const uint16_t*>(Q.p) + (there ? (int64_t)row * Q.row + (int64_t)head * Q.head : 0);
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) {
+        const int d = i < 2 * C64 ? i / 2 * 64 + g * 16 + i % 2 * 8 : C64 * 64 + g * 8;
+        raw[i] = there ? *reinterpret_cast<const u32x4*>(x + d) : u32x4{};
+    }
+    if (!bf) {
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) q[i] = __builtin_bit_cast(f16x8, raw[i]);
+        return 1.0f;
+    }
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) m = max(m, max(raw[i][j] & 0x7FFFu, raw[i][j] >> 16 & 0x7FFFu));
+    const int e = bf_lift(across_rows_max(m));
+    const float up = pow2f(e);
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) q[i] = bf_f16x8(raw[i], up);
+    return pow2f(-e);
+}
+
+// ---- the work of a call of few rows, shared out evenly
+//
+// A sequence and head of u = ceil(tokens / kUnit) units (one at least, for its outputs) is a
+// row of work; all rows' units in order of sequence and head are cut into W equal shares, one
+// for each workgroup, however the lengths differ. A row that a cut goes through leaves partial
+// sums: a share's first piece, if it continues a row, in slot 2k, a last piece that begins a row
+// and does not end it in slot 2k + 1 (k the workgroup); kv_join_k adds the row's parts up.
+__device__ __forceinline__ int units_of(const Seq& s, const Span& v) {
+    return s.n == 0 ? 0 : max((v.hi - v.lo + kUnit - 1) / kUnit, 1);
+}
+
+struct Share {
+    int seq;
+    uint32_t head;
+    int unit;      // first unit, within its row
+    int units;     // in all
+    uint64_t at;   // of the first unit, among all
+    uint64_t total;
+    uint32_t wgs;  // shares
+};
+
+__device__ __forceinline__ int prefix64(int v, int lane) {  // inclusive sum over the wave
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const int w = __shfl_up(v, d);
+        v += lane >= d ? w : 0;
+    }
+    return v;
+}
+
+// lds: kScan + 1 + 8 ints. Every thread gets the same.
+__device__ Share share_of(const Cache& c, const Batch& b, const Attn& a, bool balanced, int* lds) {
+    const int tid = threadIdx.x;
+    Share w = {0, 0, 0, 0, 0, 0, gridDim.x};
+    if (!balanced) {  // one row each
+        w.seq = (int)(blockIdx.x / c.heads);
+        w.head = blockIdx.x % c.heads;
+        const Seq s = sequence(b, c.page_log2, w.seq);
+        w.units = units_of(s, span_of(s, a, 0, 16));
+        w.total = w.units;
+        w.wgs = 1;
+        return w;
+    }
+    uint32_t u, before = 0;
+    if (b.n_seq == 1) {
+        const Seq s = sequence(b, c.page_log2, 0);
+        u = (uint32_t)units_of(s, span_of(s, a, 0, 16));
+        w.total = (uint64_t)u * c.heads;
+    } else {
+        int* const sums = lds + kScan + 1;
+        int base = 0;
+        for (uint32_t i0 = 0; i0 < b.n_seq; i0 += 256) {
+            int mine = 0;
+            if (i0 + tid < b.n_seq) {
+                const Seq s = sequence(b, c.page_log2, i0 + tid);
+                mine = units_of(s, span_of(s, a, 0, 16));
+            }
+            const int up = prefix64(mine, tid & 63);
+            if ((tid & 63) == 63) sums[tid >> 6] = up;
+            __syncthreads();
+            int wave_base = base;
+            for (int i = 0; i < tid >> 6; ++i) wave_base += sums[i];
+            if (i0 + tid < b.n_seq) lds[i0 + tid] = wave_base + up - mine;
+            base += sums[0] + sums[1] + sums[2] + sums[3];
+            __syncthreads();
+        }
+        if (tid == 0) lds[b.n_seq] = base;
+        w.total = (uint64_t)(uint32_t)base * c.heads;
+    }
+    if (w.total < w.wgs) w.wgs = (uint32_t)w.total;
+    if (blockIdx.x >= w.wgs) return w;
+    w.at = w.total * blockIdx.x / w.wgs;
+    w.units = (int)(w.total * (blockIdx.x + 1) / w.wgs - w.at);
+    if (b.n_seq > 1) {
+        int* const found = lds + kScan + 5;
+        __syncthreads();
+        for (uint32_t i = tid; i < b.n_seq; i += 256) {
+            const uint64_t from = (uint64_t)(uint32_t)lds[i] * c.heads, to = (uint64_t)(uint32_t)lds[i + 1] * c.heads;
+            if (from <= w.at && w.at < to) {
+                found[0] = (int)i;
+                found[1] = lds[i];
+                found[2] = lds[i + 1] - lds[i];
+            }
+        }
+        __syncthreads();
+        w.seq = found[0];
+        before = (uint32_t)found[1];
+        u = (uint32_t)found[2];
+        __syncthreads();
+    }
+    const uint64_t in = w.at - (uint64_t)before * c.heads;
+    w.head = (uint32_t)(in / u);
+    w.unit = (int)(in % u);
+    return w;
+}
+
+// A row that is cut, by its first part's workgroup; parts 0: that workgroup begins none.
+struct Cut {
+    int seq, head, parts, pad;
+};
+// The partial results of slot i: [16][D] sums, then [16] (m, l).
+template <int D>
+__device__ __forceinline__ float* slot_of(float* ws, uint32_t cuts, uint32_t i) {
+    return ws + cuts * 4 + (uint64_t)i * (16 * (D + 2));
+}
+
+// Few rows: at most 16 (tokens x heads of a group) a sequence and head. Four waves take 64 tokens
+// of a piece in turn and join their sums at its end. What bounds it is the stream of codes:
+// a wave asks for its next keys as soon as the present ones are multiplied, and for its
+// next values after the product with the present ones, so that most of 16 KiB a wave
+// (128 wide) is always on its way.
 template <int D, int TYPE>
-__global__ __launch_bounds__(256, 2) void kv_attn_k(Cache c, Batch b, Attn a, Plan p, Rows Q, Rows O, int bf,
-                                                    float* ws) {
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_attn_k(Cache c, Batch b, Attn a, int balanced, Rows Q,
+                                                                   Rows O, int bf, float* ws) {
     constexpr int C64 = D / 64, kHalf = D % 64 ? 1 : 0;  // 64-column pieces of a key, and a 32-column one
     constexpr int kPad = D + 4;
     __shared__ __attribute__((aligned(16))) float o_lds[4 * 16 * kPad];
     __shared__ float m_lds[4][16], l_lds[4][16];
-    __shared__ int ids[kSegment / 16 + 1];
+    static_assert(sizeof(o_lds) >= kIds * sizeof(int) && kIds >= kScan + 9, "page ids, sums of lengths");
+    int* const ids = reinterpret_cast<int*>(o_lds);  // page ids of the piece, until the waves join
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 15, g = lane >> 4;
-    uint32_t id = blockIdx.x;
-    const uint32_t h = id % c.heads;
-    id /= c.heads;
-    const uint32_t tile = id % p.tiles;
-    id /= p.tiles;
-    const uint32_t split = id % p.splits, seq = id / p.splits;
-    const Seq s = sequence(b, c.page_log2, seq);
-    const int row0 = (int)tile * 16, rows = s.n * (int)a.group;
-    if (row0 >= rows) return;
-    const Span sp = span_of(s, a, row0, 16);
-    const int n_splits = splits_of(sp, (int)p.chunk);
-    if ((int)split >= max(n_splits, 1)) return;
-    const int lo = sp.lo + (int)(split * p.chunk), hi = (int)min((int64_t)sp.hi, (int64_t)lo + p.chunk);
+    const uint32_t q_heads = c.heads * a.group;
 
-    const int32_t* const table = b.pages + (uint64_t)seq * b.max_pages;
-
-    // this lane's row
-    const int row = row0 + r, tok = row / (int)a.group;
-    const uint32_t head = h * a.group + (uint32_t)(row % (int)a.group), q_heads = c.heads * a.group;
-    const bool there = row < rows;
-    const int pos = s.len - s.n + tok;
-    const int sees_hi = a.causal ? pos + 1 : s.len, sees_lo = a.window ? pos + 1 - (int)a.window : 0;
-
-    // Q as the second operand of S^T, in fp16; bf16 rows go through a power of two
-    f16x8 q[D / 32];
-    float q_scale = a.scale_log2;
-    {
-        u32x4 raw[D / 32];
-        const uint16_t* const x = static_cast<const uint16_t*>(Q.p) +
-                                  (there ? (int64_t)(s.row0 + tok) * Q.row + (int64_t)head * Q.head : 0);
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i) {
-            const int d = i < 2 * C64 ? i / 2 * 64 + g * 16 + i % 2 * 8 : C64 * 64 + g * 8;
-            raw[i] = there ? *reinterpret_cast<const u32x4*>(x + d) : u32x4{};
+    const Share share = share_of(c, b, a, balanced, ids);
+    Cut* const cuts = reinterpret_cast<Cut*>(ws);
+    if (balanced && tid == 0) cuts[blockIdx.x].parts = 0;
+    int left = share.units, unit = share.unit;
+    int seq = share.seq;
+    uint32_t h = share.head;
+    uint64_t at = share.at;
+    while (left > 0) {
+        const Seq s = sequence(b, c.page_log2, (uint32_t)seq);
+        const Span sp = span_of(s, a, 0, 16);
+        const int units = units_of(s, sp), mine = min(left, units - unit);
+        if (mine <= 0) {  // a sequence without rows
+            ++seq;
+            continue;
         }
-        if (bf) {
-            uint32_t m = 0;
+        const int rows = s.n * (int)a.group;
+        const int lo = sp.lo + unit * kUnit, hi = (int)min((int64_t)sp.hi, (int64_t)lo + (int64_t)mine * kUnit);
+        const int32_t* const table = b.pages + (uint64_t)seq * b.max_pages;
+
+        // this lane's row
+        const int row = r, tok = row / (int)a.group;
+        const uint32_t head = h * a.group + (uint32_t)(row % (int)a.group);
+        const bool there = row < rows;
+        const int pos = s.len - s.n + tok;
+        const int sees_hi = min(a.causal ? pos + 1 : s.len, hi), sees_lo = a.window ? pos + 1 - (int)a.window : 0;
+
+        f16x8 q[D / 32];
+        const float q_scale = a.scale_log2 * load_q<D>(Q, there, s.row0 + tok, head, g, bf, q);
+
+        float m = kLowest, l = 0.0f;  // of the row; l: this lane's tokens alone
+        f32x4 o[D / 16] = {};
+        int page0 = 0;
+        u32x4 kw[4 * C64 + 1], vw[D / 16];
+        u32x2 kx[4];  // the 32-column pieces
+        int ke = 0, ve = 0, pv = 0;
+        // Codes of the wave's 64 tokens from t0 on: the lane's row of K operand t, and its columns of V
+        // with the exponents of its 16 tokens.
+        auto page_at = [&](int t) { return ids[(min(t, hi - 1) >> c.page_log2) - page0]; };
+        auto load_k = [&](int t0) {
+            const int tk = t0 + 16 * (r >> 2);
+            const uint8_t* const kp = c.k + code_offset(c, D, max(page_at(tk), 0), h, tk) + (r & 3) * D;
 #pragma unroll
-            for (int i = 0; i < D / 32; ++i)
+            for (int t = 0; t < 4; ++t) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) m = max(m, max(raw[i][j] & 0x7FFFu, raw[i][j] >> 16 & 0x7FFFu));
-            m = across_rows_max(m);
-            // largest magnitude into [2^14, 2^15); an infinity or NaN makes its row NaN anyway
-            const int e = m >= 0x7F80u ? 0 : min(max(14 - ((int)(m >> 7) - 127), -126), 126);
-            q_scale *= pow2f(-e);
-            const float up = pow2f(e);
+                for (int i = 0; i < C64; ++i) kw[t * C64 + i] = *reinterpret_cast<const u32x4*>(kp + t * 4 * D + i * 64 + g * 16);
+                if constexpr (kHalf) kx[t] = *reinterpret_cast<const u32x2*>(kp + t * 4 * D + C64 * 64 + g * 8);
+            }
+        };
+        auto load_v = [&](int t0) {
+            const int tv = t0 + 16 * g;
+            pv = page_at(tv);
+            const uint64_t eo = exp_offset(c, max(pv, 0), h, tv);
+            ke = c.k_exp[eo];
+            ve = c.v_exp[eo];
+            const uint8_t* const vp = c.v + code_offset(c, D, max(pv, 0), h, tv) + r * 16;
 #pragma unroll
-            for (int i = 0; i < D / 32; ++i)
+            for (int i = 0; i < D / 16; ++i) vw[i] = *reinterpret_cast<const u32x4*>(vp + i * 256);
+        };
+        auto step = [&](int t0, auto more) {
+            f32x4 st[4];
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                st[t] = f32x4{0, 0, 0, 0};
+#pragma unroll
+                for (int i = 0; i < C64; ++i) {
+                    const u32x4 w = kw[t * C64 + i];
+                    st[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes_f16x8<TYPE>(w.x, w.y), q[2 * i], st[t], 0, 0, 0);
+                    st[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes_f16x8<TYPE>(w.z, w.w), q[2 * i + 1], st[t], 0, 0, 0);
+                }
+                if constexpr (kHalf)
+                    st[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes_f16x8<TYPE>(kx[t].x, kx[t].y), q[2 * C64], st[t], 0, 0, 0);
+            }
+            __builtin_amdgcn_sched_barrier(0);  // into the registers just read, not beside them
+            if constexpr (decltype(more)::value) load_k(t0 + 4 * kTile);
+            __builtin_amdgcn_sched_barrier(0);
+
+            const int tv = t0 + 16 * g;
+            const float f = q_scale * pow2f(min(max(ke - 127, -126), 127)), ev = (float)(ve - 127);
+            float x[16], top = m;
+            // tokens in sight of the row, of the lane's 16
+            const int from = sees_lo - tv, to = pv < 0 ? 0 : sees_hi - tv;
+            if (__all(from <= 0 && to >= 16)) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) x[i] = __builtin_fmaf(st[i / 4][i % 4], f, ev);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    x[i] = i < from || i >= to ? -__builtin_inff() : __builtin_fmaf(st[i / 4][i % 4], f, ev);
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) top = fmaxf(top, x[i]);
+            top = across_rows_maxf(top);
+            if (__any(top > m)) {
+                const float fade = __builtin_amdgcn_exp2f(m - top);
+                m = top;
+                l *= fade;
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i) o[i] *= fade;
+            }
+            float sum = 0.0f;
+            f16x8 w[2];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float y = __builtin_amdgcn_exp2f(x[i] - (m - kLift));
+                sum += y;
+                w[i / 8][i % 8] = (_Float16)y;
+            }
+            l += sum * pow2f(min(max(127 - ve, -126), 127));
+            if (t0 + kTile > hi || __any(pv < 0)) {
+                // bytes of tokens that no length covers may hold anything, NaN among it
+                const int valid = pv < 0 ? 0 : min(max(hi - tv, 0), 16);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    q[i][2 * j] = (_Float16)(bf2f((uint16_t)(raw[i][j] & 0xFFFF)) * up);
-                    q[i][2 * j + 1] = (_Float16)(bf2f((uint16_t)(raw[i][j] >> 16)) * up);
-                }
-        } else {
+                    const int n = min(max(valid - 4 * j, 0), 4);
+                    const uint32_t keep = n == 4 ? 0xFFFFFFFFu : (1u << 8 * n) - 1;
 #pragma unroll
-            for (int i = 0; i < D / 32; ++i) q[i] = __builtin_bit_cast(f16x8, raw[i]);
-        }
-    }
-
-    float m = kLowest, l = 0.0f;  // of the row; l: this lane's tokens alone
-    f32x4 o[D / 16] = {};
-    int page0 = 0;
-    for (int base = lo; base < hi; base += 4 * kTile) {
-        if (!((base - lo) % kSegment)) {  // the page ids of the next tokens
+                    for (int i = 0; i < D / 16; ++i) vw[i][j] &= keep;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) {
+                o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes_f16x8<TYPE>(vw[i].x, vw[i].y), w[0], o[i], 0, 0, 0);
+                o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes_f16x8<TYPE>(vw[i].z, vw[i].w), w[1], o[i], 0, 0, 0);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            if constexpr (decltype(more)::value) load_v(t0 + 4 * kTile);
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        // the piece, or as much of it as there is room for page ids
+        const int most = ((kIds - 1) << c.page_log2) & ~(kUnit - 1);
+        for (int from = lo; from < hi;) {
+            const int to = hi - from > most ? from + most : hi;
             __syncthreads();
-            page0 = base >> c.page_log2;
-            const int pages = ((min(hi, base + kSegment) - 1) >> c.page_log2) - page0 + 1;
+            page0 = from >> c.page_log2;
+            const int pages = ((to - 1) >> c.page_log2) - page0 + 1;
             for (int i = tid; i < pages; i += 256) {
                 const int v = table[page0 + i];
                 ids[i] = (uint32_t)v < c.n_pages ? v : -1;
             }
             __syncthreads();
-        }
-        const int t0 = base + wave * kTile;
-        if (t0 >= hi) continue;
-        // the lane's blocks: of V and the scores, and of K
-        const int tv = t0 + 16 * g, tk = t0 + 16 * (r >> 2);
-        const int last = hi - 1;
-        const int pv = ids[(min(tv, last) >> c.page_log2) - page0], pk = ids[(min(tk, last) >> c.page_log2) - page0];
-        const uint8_t* const kp = c.k + code_offset(c, D, max(pk, 0), h, tk) + (r & 3) * D;
-        const uint8_t* const vp = c.v + code_offset(c, D, max(pv, 0), h, tv) + r * 16;
-        const uint64_t eo = exp_offset(c, max(pv, 0), h, tv);
-        const int ke = (int)c.k_exp[eo] - 127, ve = (int)c.v_exp[eo] - 127;
-
-        f32x4 st[4];
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            st[t] = f32x4{0, 0, 0, 0};
-#pragma unroll
-            for (int i = 0; i < C64; ++i) {
-                const u32x4 w = *reinterpret_cast<const u32x4*>(kp + t * 4 * D + i * 64 + g * 16);
-                st[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes_f16x8<TYPE>(w.x, w.y), q[2 * i], st[t], 0, 0, 0);
-                st[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes_f16x8<TYPE>(w.z, w.w), q[2 * i + 1], st[t], 0, 0, 0);
+            int t0 = from + wave * kTile;
+            if (t0 < to) {
+                load_k(t0);
+                load_v(t0);
+                for (; t0 < to - kUnit; t0 += kUnit) step(t0, Int<1>());
+                step(t0, Int<0>());
             }
-            if constexpr (kHalf) {
-                const u32x2 w = *reinterpret_cast<const u32x2*>(kp + t * 4 * D + C64 * 64 + g * 8);
-                st[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes_f16x8<TYPE>(w.x, w.y), q[2 * C64], st[t], 0, 0, 0);
-            }
+            from = to;
         }
 
-        const float f = q_scale * pow2f(min(max(ke, -126), 127)), ev = (float)ve;
-        float x[16], top = kLowest;
-        // tokens in sight of the row, of the lane's 16
-        const int from = sees_lo - tv, to = pv < 0 ? 0 : min(sees_hi, hi) - tv;
-        const bool all = from <= 0 && to >= 16;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            x[i] = __builtin_fmaf(st[i / 4][i % 4], f, ev);
-            if (!all && (i < from || i >= to)) x[i] = -__builtin_inff();
-            top = fmaxf(top, x[i]);
+        // join the waves
+        l = across_rows_sum(l);
+        __syncthreads();
+        if (g == 0) {
+            m_lds[wave][r] = m;
+            l_lds[wave][r] = l;
         }
-        top = fmaxf(across_rows_maxf(top), m);
-        const float fade = __builtin_amdgcn_exp2f(m - top);
-        m = top;
-        float sum = 0.0f;
-        f16x8 w[2];
+        __syncthreads();
+        {
+            float top = m_lds[0][r];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const float y = __builtin_amdgcn_exp2f(x[i] - (m - kLift));
-            sum += y;
-            w[i / 8][i % 8] = (_Float16)y;
+            for (int w = 1; w < 4; ++w) top = fmaxf(top, m_lds[w][r]);
+            const float fade = __builtin_amdgcn_exp2f(m - top);
+            float* const to = o_lds + (wave * 16 + r) * kPad;
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) *reinterpret_cast<f32x4*>(to + i * 16 + g * 4) = o[i] * fade;
         }
-        l = l * fade + sum * pow2f(min(max(-ve, -126), 127));
-        // bytes of tokens that no length covers may hold anything, NaN among it
-        const int valid = pv < 0 ? 0 : min(max(hi - tv, 0), 16);
+        __syncthreads();
+        const bool whole = mine == units;
+        float* const part = slot_of<D>(ws, gridDim.x, 2 * blockIdx.x + (unit == 0));
+        for (int i = tid; i < rows * (D / 4); i += 256) {
+            const int rr = i / (D / 4), d = i % (D / 4) * 4;
+            f32x4 y = *reinterpret_cast<const f32x4*>(o_lds + rr * kPad + d);
+            float top = m_lds[0][rr];
 #pragma unroll
-        for (int i = 0; i < D / 16; ++i) {
-            u32x4 v = *reinterpret_cast<const u32x4*>(vp + i * 256);
-            if (valid < 16) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int n = min(max(valid - 4 * j, 0), 4);
-                    v[j] = n == 4 ? v[j] : v[j] & ((1u << 8 * n) - 1);
-                }
+            for (int w = 1; w < 4; ++w) {
+                y += *reinterpret_cast<const f32x4*>(o_lds + (w * 16 + rr) * kPad + d);
+                top = fmaxf(top, m_lds[w][rr]);
             }
-            o[i] *= fade;
-            o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes_f16x8<TYPE>(v.x, v.y), w[0], o[i], 0, 0, 0);
-            o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes_f16x8<TYPE>(v.z, v.w), w[1], o[i], 0, 0, 0);
-        }
-    }
-
-    // join the waves
-    l = across_rows_sum(l);
-    if (g == 0) {
-        m_lds[wave][r] = m;
-        l_lds[wave][r] = l;
-    }
-    __syncthreads();
-    {
-        float top = m_lds[0][r];
+            float sum = 0.0f;
 #pragma unroll
-        for (int w = 1; w < 4; ++w) top = fmaxf(top, m_lds[w][r]);
-        const float fade = __builtin_amdgcn_exp2f(m - top);
-        float* const to = o_lds + (wave * 16 + r) * kPad;
-#pragma unroll
-        for (int i = 0; i < D / 16; ++i) *reinterpret_cast<f32x4*>(to + i * 16 + g * 4) = o[i] * fade;
-    }
-    __syncthreads();
-    for (int i = tid; i < 16 * (D / 4); i += 256) {
-        const int rr = i / (D / 4), d = i % (D / 4) * 4, my_row = row0 + rr;
-        if (my_row >= rows) break;
-        f32x4 y = *reinterpret_cast<const f32x4*>(o_lds + rr * kPad + d);
-        float top = m_lds[0][rr];
-#pragma unroll
-        for (int w = 1; w < 4; ++w) {
-            y += *reinterpret_cast<const f32x4*>(o_lds + (w * 16 + rr) * kPad + d);
-            top = fmaxf(top, m_lds[w][rr]);
-        }
-        float sum = 0.0f;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) sum += l_lds[w][rr] * __builtin_amdgcn_exp2f(m_lds[w][rr] - top);
-        const uint32_t hd = h * a.group + (uint32_t)(my_row % (int)a.group);
-        const int at = s.row0 + my_row / (int)a.group;
-        if (n_splits <= 1) {
-            store4(O, at, hd, d, y * finish(a, top, sum, at, hd, q_heads, d == 0), bf);
-        } else {
-            // [row][split]: D sums, then m and l
-            float* const part = ws + ((((uint64_t)seq * p.splits + split) * p.tiles + tile) * c.heads + h) * (16 * (D + 2)) + rr * D;
-            *reinterpret_cast<f32x4*>(part + d) = y;
-            if (d == 0) {
-                float* const ml = part - rr * D + 16 * D + rr * 2;
-                ml[0] = top;
-                ml[1] = sum;
+            for (int w = 0; w < 4; ++w) sum += l_lds[w][rr] * __builtin_amdgcn_exp2f(m_lds[w][rr] - top);
+            if (whole) {
+                const uint32_t hd = h * a.group + (uint32_t)(rr % (int)a.group);
+                const int out = s.row0 + rr / (int)a.group;
+                store4(O, out, hd, d, y * finish(a, top, sum, out, hd, q_heads, d == 0), bf);
+            } else {
+                *reinterpret_cast<f32x4*>(part + rr * D + d) = y;
+                if (d == 0) *reinterpret_cast<float2*>(part + 16 * D + rr * 2) = make_float2(top, sum);
             }
         }
+        if (!whole && unit == 0 && tid == 0) {
+            // its last unit's workgroup: shares begin at floor(k total / wgs)
+            const uint64_t end = at + (uint64_t)units;
+            const int last = (int)((end * share.wgs - 1) / share.total);
+            cuts[blockIdx.x] = {seq, (int)h, last - (int)blockIdx.x + 1, 0};
+        }
+        left -= mine;
+        at += (uint64_t)mine;
+        unit = 0;
+        if (++h == c.heads) h = 0, ++seq;
     }
 }
 
-// Joins the splits of one row and query head: four waves take every fourth split.
-template <int D>
-__global__ __launch_bounds__(256) void kv_join_k(Cache c, Batch b, Attn a, Plan p, Rows O, int bf, const float* ws) {
-    __shared__ __attribute__((aligned(16))) float o_lds[4][D];
-    __shared__ float l_lds[4];
-    const uint32_t q_heads = c.heads * a.group, head = blockIdx.x % q_heads, h = head / a.group;
-    const uint32_t j = blockIdx.x / q_heads % b.max_q, seq = blockIdx.x / q_heads / b.max_q;
-    const Seq s = sequence(b, c.page_log2, seq);
-    if ((int)j >= s.n) return;
-    const int row = (int)(j * a.group + head % a.group), tile = row / 16;
-    const int n = splits_of(span_of(s, a, tile * 16, 16), (int)p.chunk);
-    if (n <= 1) return;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    constexpr int kPart = 16 * (D + 2);
-    const float* const first = ws + (((uint64_t)seq * p.splits * p.tiles + tile) * c.heads + h) * kPart;
-    const uint64_t step = (uint64_t)p.tiles * c.heads * kPart;
-    float m = kLowest;
-    for (int i = lane; i < n; i += 64) m = fmaxf(m, first[i * step + 16 * D + row % 16 * 2]);
+// Adds up the n parts of a row in one wave: sums(i) and ml(i) are part i's sums and (m, l).
+template <int D, class Sums, class Ml>
+__device__ __forceinline__ void join_row(const Attn& a, int n, Sums sums, Ml ml_of, const Rows& O, int bf, int at,
+                                         uint32_t head, uint32_t q_heads) {
+    constexpr int N = (D + 63) / 64;
+    const int lane = threadIdx.x & 63;
+    float m = kLowest, l = 0.0f, o[N] = {};
+    for (int i0 = 0; i0 < n; i0 += 64) {
+        const int here = min(n - i0, 64);
+        float2 ml = make_float2(kLowest, 0.0f);
+        if (lane < here) ml = *reinterpret_cast<const float2*>(ml_of(i0 + lane));
+        float top = fmaxf(m, ml.x);
 #pragma unroll
-    for (int i = 1; i < 64; i *= 2) m = fmaxf(m, __shfl_xor(m, i));
-    float l = 0.0f, o[(D + 63) / 64] = {};
-    for (int i = wave; i < n; i += 4) {
-        const float* const part = first + i * step;
-        const float f = __builtin_amdgcn_exp2f(part[16 * D + row % 16 * 2] - m);
-        l += part[16 * D + row % 16 * 2 + 1] * f;
+        for (int d = 1; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
+        const float fade = __builtin_amdgcn_exp2f(m - top), f = __builtin_amdgcn_exp2f(ml.x - top);
+        m = top;
+        l = l * fade + wave_sum(ml.y * f);
 #pragma unroll
-        for (int k = 0; k < (D + 63) / 64; ++k)
-            if (k * 64 + lane < D) o[k] += part[row % 16 * D + k * 64 + lane] * f;
-    }
+        for (int k = 0; k < N; ++k) o[k] *= fade;
+#pragma unroll 8
+        for (int i = 0; i < here; ++i) {
+            const float fi = __shfl(f, i);
+            const float* const from = sums(i0 + i);
 #pragma unroll
-    for (int k = 0; k < (D + 63) / 64; ++k)
-        if (k * 64 + lane < D) o_lds[wave][k * 64 + lane] = o[k];
-    if (lane == 0) l_lds[wave] = l;
-    __syncthreads();
-    if ((int)threadIdx.x < D / 4) {
-        const int d = (int)threadIdx.x * 4, at = s.row0 + (int)j;
-        f32x4 y = {0, 0, 0, 0};
-        l = 0.0f;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            y += *reinterpret_cast<const f32x4*>(&o_lds[w][d]);
-            l += l_lds[w];
+            for (int k = 0; k < N; ++k)
+                if (D % 64 == 0 || k * 64 + lane < D) o[k] += from[k * 64 + lane] * fi;
         }
-        store4(O, at, head, d, y * finish(a, m, l, at, head, q_heads, d == 0), bf);
     }
+    const float y = finish(a, m, l, at, head, q_heads, lane == 0);
+    uint16_t* const to = static_cast<uint16_t*>(O.p) + (int64_t)at * O.row + (int64_t)head * O.head;
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+        if (D % 64 == 0 || k * 64 + lane < D)
+            to[k * 64 + lane] = (uint16_t)(bf ? pair16<1>(o[k] * y, 0.0f) : pair16<0>(o[k] * y, 0.0f));
+}
+
+// The cut rows of kv_attn_k: a wave takes one of the 16 (token, head) rows.
+template <int D>
+__global__ __launch_bounds__(256) void kv_join_k(Cache c, Batch b, Attn a, uint32_t wgs, Rows O, int bf, float* ws) {
+    const Cut cut = reinterpret_cast<const Cut*>(ws)[blockIdx.x];
+    if (cut.parts == 0) return;
+    const Seq s = sequence(b, c.page_log2, (uint32_t)cut.seq);
+    const int row = (int)(blockIdx.y * 4 + (threadIdx.x >> 6));
+    if (row >= s.n * (int)a.group) return;
+    // part 0 begins the row, the others continue it: slots 2k + 1, then 2 (k + i)
+    auto part = [&](int i) { return slot_of<D>(ws, wgs, 2 * (blockIdx.x + i) + (i == 0)); };
+    join_row<D>(a, cut.parts, [&](int i) { return part(i) + row * D; }, [&](int i) { return part(i) + 16 * D + row * 2; },
+                O, bf, s.row0 + row / (int)a.group, (uint32_t)cut.head * a.group + (uint32_t)(row % (int)a.group),
+                c.heads * a.group);
 }
 
 }  // namespace kv
