@@ -182,9 +182,28 @@ struct Attn {
     const float* sinks;
     float* lse;
 };
+// Launch of the kernel for few rows.
+struct FewPlan {
+    uint32_t sixteens;  // of rows of a sequence and head: 1 to few_most(head_dim)
+    uint32_t wgs;
+    uint32_t balanced;  // equal shares of all units; else a sequence and head each
+    uint32_t start;     // units that the beginning of a sequence and head is priced at
+    uint32_t by_row;    // cuts are by sequence and head
+    uint32_t cuts;      // descriptors of cuts in the workspace
+};
+// Rows that its registers hold, in sixteens, and the waves of a SIMD they allow.
+constexpr uint32_t few_most(uint32_t D) { return D <= 96 ? 4 : D == 128 ? 3 : D == 192 ? 2 : 1; }
+constexpr uint32_t few_waves(uint32_t D, uint32_t R) {
+    return D == 64 ? (R <= 3 ? 2 : 1) : D <= 128 ? (R <= 2 ? 2 : 1) : D == 192 && R == 1 ? 2 : 1;
+}
+// Rows of a tile of the kernel for many rows, at most.
+#ifndef KV_ROWMOST
+#define KV_ROWMOST (D == 96 || D == 128 ? 256 : 128)
+#endif
+constexpr uint32_t row_most(uint32_t D) { return KV_ROWMOST; }
 // Launch of the kernel for many rows.
 struct RowPlan {
-    uint32_t rows;    // of a tile: 32 a wave
+    uint32_t rows;    // of a tile: 128 or 256, 32 a wave
     uint32_t tiles;   // of a sequence and head
     uint32_t chunk;   // tokens of a split, a multiple of 64
     uint32_t splits;  // at most, of a tile
@@ -212,15 +231,14 @@ hipError_t launch_kv_write(const kv::Cache& c, const kv::Batch& b, uint32_t D, i
 hipError_t launch_kv_read(const kv::Cache& c, const kv::Batch& b, uint32_t D, int type, const kv::Rows& K,
                           const kv::Rows& V, kq_dtype f, hipStream_t s);
 namespace kv {
-// The kernel for many rows, heads D wide (kq_kv_rows_<D>.hip).
+// The kernels, heads D wide (kq_kv_attn_<D>.hip).
 template <int D>
-hipError_t launch_rows(int type, const Cache& c, const Batch& b, const Attn& a, const RowPlan& p, const Rows& Q,
-                       const Rows& O, bool bf, float* ws, hipStream_t s);
-template <> hipError_t launch_rows<64>(int, const Cache&, const Batch&, const Attn&, const RowPlan&, const Rows&, const Rows&, bool, float*, hipStream_t);
-template <> hipError_t launch_rows<96>(int, const Cache&, const Batch&, const Attn&, const RowPlan&, const Rows&, const Rows&, bool, float*, hipStream_t);
-template <> hipError_t launch_rows<128>(int, const Cache&, const Batch&, const Attn&, const RowPlan&, const Rows&, const Rows&, bool, float*, hipStream_t);
-template <> hipError_t launch_rows<192>(int, const Cache&, const Batch&, const Attn&, const RowPlan&, const Rows&, const Rows&, bool, float*, hipStream_t);
-template <> hipError_t launch_rows<256>(int, const Cache&, const Batch&, const Attn&, const RowPlan&, const Rows&, const Rows&, bool, float*, hipStream_t);
+struct AttnKernels {
+    static hipError_t few(int type, const Cache& c, const Batch& b, const Attn& a, const FewPlan& p, const Rows& Q,
+                          const Rows& O, bool bf, float* ws, hipStream_t s);
+    static hipError_t rows(int type, const Cache& c, const Batch& b, const Attn& a, const RowPlan& p, const Rows& Q,
+                           const Rows& O, bool bf, float* ws, hipStream_t s);
+};
 }  // namespace kv
 // Workspace of a call with any window; whether its launches can be made.
 size_t kv_attn_ws_bytes(const kv::Cache& c, const kv::Batch& b, uint32_t D, uint32_t group);

@@ -1,12 +1,8 @@
-// kq_kv_attn.hip -- attention over the 8-bit key/value cache (kq_kv_attn): launch
-// plans, and the launches of the kernel for few rows.
+// kq_kv_attn.hip -- attention over the 8-bit key/value cache (kq_kv_attn): which
+// kernel a call runs, and its launch plan.
 #include <algorithm>
 
 #include "kq_kv_attn_kernel.h"
-
-#ifndef KV_WGS
-#define KV_WGS 2
-#endif
 
 namespace kq {
 namespace kv {
@@ -19,45 +15,41 @@ uint64_t longest_span(const Batch& b, uint64_t rows, uint32_t window) {
     return window ? std::min<uint64_t>(b.max_len, (uint64_t)window + rows - 1 + kTile - 1) : b.max_len;
 }
 
-// Few rows: the kernel of kq_kv_attn_kernel.h.
-bool few(const Batch& b, uint32_t group) { return (uint64_t)b.max_q * group <= 16; }
+// Few rows, as many as the registers of kv_few_k hold: a cache's codes are read once for all of them.
+bool few(const Batch& b, uint32_t D, uint32_t group) { return (uint64_t)b.max_q * group <= 16 * few_most(D); }
 
-// Its workgroups: all that the device holds at once (their registers allow two a compute unit, one
-// at 256 columns), or one for each unit or row of work where there is less, or where
-// the sequences are too many to add up their lengths in each workgroup.
-struct FewPlan {
-    uint32_t wgs;
-    bool balanced, join;
-};
-FewPlan few_plan(const Cache& c, const Batch& b, uint32_t D, uint32_t window) {
-    FewPlan p;
-    const uint64_t units = ceil_div(longest_span(b, 16, window), kUnit), rows = (uint64_t)b.n_seq * c.heads;
-    p.balanced = b.n_seq <= kScan && b.n_seq * units < 0x7FFFFFFF;
-    p.wgs = (uint32_t)(p.balanced ? std::min<uint64_t>((uint64_t)cu_count() * (D == 256 ? 1 : KV_WGS), rows * units) : rows);
-    p.join = p.balanced && units > 1;
+// Its workgroups: all that the device holds at once, or one for each unit of work where there
+// is less; one for each row of work where those are a unit long or the sequences too
+// many to add up their lengths in each workgroup.
+FewPlan few_plan(const Cache& c, const Batch& b, uint32_t D, uint32_t group, uint32_t window) {
+    FewPlan p = {};
+    p.sixteens = (uint32_t)ceil_div((uint64_t)b.max_q * group, 16);
+    const uint64_t units = ceil_div(longest_span(b, 16 * p.sixteens, window), kUnit), rows = (uint64_t)b.n_seq * c.heads;
+    p.balanced = units > 1 && b.n_seq <= kScan && b.n_seq * (units + 1) < 0x7FFFFFFF;
+    if (!p.balanced) {
+        p.wgs = (uint32_t)rows;
+        return p;
+    }
+    const uint64_t fit = (uint64_t)cu_count() * few_waves(D, p.sixteens);
+    p.wgs = (uint32_t)std::min<uint64_t>(fit, rows * units);
+    p.start = b.n_seq > 1 && rows * units >= 4 * fit;
+    p.by_row = rows <= p.wgs;
+    p.cuts = p.by_row ? (uint32_t)rows : p.wgs;
     return p;
 }
-size_t few_ws_bytes(const FewPlan& p, uint32_t D) {
-    return p.balanced ? (size_t)p.wgs * (sizeof(Cut) + 2 * 16 * (D + 2) * 4) : 0;
-}
-
-template <int D, int TYPE>
-hipError_t few_d(const Cache& c, const Batch& b, const Attn& a, const FewPlan& p, const Rows& Q, const Rows& O, bool bf,
-                 float* ws, hipStream_t s) {
-    kv_attn_k<D, TYPE><<<p.wgs, 256, 0, s>>>(c, b, a, p.balanced, Q, O, bf, ws);
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess || !p.join) return e;
-    kv_join_k<D><<<dim3(p.wgs, (b.max_q * a.group + 3) / 4), 256, 0, s>>>(c, b, a, p.wgs, O, bf, ws);
-    return hipGetLastError();
+// Of any window: descriptors and slots of the widest launch.
+size_t few_ws_bytes(const Cache& c, const Batch& b, uint32_t D, uint32_t group) {
+    const FewPlan p = few_plan(c, b, D, group, 0);
+    return p.balanced ? (size_t)p.wgs * (sizeof(Cut) + 2 * 16 * p.sixteens * (D + 2) * 4) : 0;
 }
 
 uint64_t row_splits_wanted(const Cache& c, const Batch& b, const RowPlan& p) {
     return ceil_div((uint64_t)cu_count() * (p.rows == 256 ? 1 : 2), (uint64_t)b.n_seq * p.tiles * c.heads);
 }
-RowPlan row_plan(const Cache& c, const Batch& b, uint32_t group, uint32_t window) {
+RowPlan row_plan(const Cache& c, const Batch& b, uint32_t D, uint32_t group, uint32_t window) {
     RowPlan p;
     const uint64_t rows = (uint64_t)b.max_q * group;
-    p.rows = rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
+    p.rows = rows <= 128 ? 128 : row_most(D);
     p.tiles = (uint32_t)ceil_div(rows, p.rows);
     const uint64_t longest = longest_span(b, p.rows, window);
     p.chunk = (uint32_t)std::max<uint64_t>(ceil_div(ceil_div(longest, row_splits_wanted(c, b, p)), kTile) * kTile, kUnit);
@@ -66,7 +58,7 @@ RowPlan row_plan(const Cache& c, const Batch& b, uint32_t group, uint32_t window
 }
 // Of any window: a split has kUnit tokens at least.
 size_t row_ws_bytes(const Cache& c, const Batch& b, uint32_t group, uint32_t D) {
-    const RowPlan p = row_plan(c, b, group, 0);
+    const RowPlan p = row_plan(c, b, D, group, 0);
     const uint64_t splits = std::min(row_splits_wanted(c, b, p), ceil_div(b.max_len, kUnit));
     return splits > 1 ? (size_t)b.n_seq * splits * p.tiles * c.heads * p.rows * (D + 2) * 4 : 0;
 }
@@ -75,7 +67,7 @@ size_t row_ws_bytes(const Cache& c, const Batch& b, uint32_t group, uint32_t D) 
 }  // namespace kv
 
 size_t kv_attn_ws_bytes(const kv::Cache& c, const kv::Batch& b, uint32_t D, uint32_t group) {
-    const size_t n = kv::few(b, group) ? kv::few_ws_bytes(kv::few_plan(c, b, D, 0), D) : kv::row_ws_bytes(c, b, group, D);
+    const size_t n = kv::few(b, D, group) ? kv::few_ws_bytes(c, b, D, group) : kv::row_ws_bytes(c, b, group, D);
     return n > 256 ? (n + 255) / 256 * 256 : 256;
 }
 
@@ -86,20 +78,12 @@ bool kv_attn_fits(const kv::Cache& c, const kv::Batch& b, uint32_t group) {
 hipError_t launch_kv_attn(const kv::Cache& c, const kv::Batch& b, uint32_t D, int type, const kv::Attn& a,
                           const kv::Rows& Q, const kv::Rows& O, bool bf, void* ws, hipStream_t s) {
     float* const w = static_cast<float*>(ws);
-    if (kv::few(b, a.group)) {
-        const kv::FewPlan p = kv::few_plan(c, b, D, a.window);
-        return kv::by_dim(D, type, [&](auto d, auto t) {
-            return kv::few_d<decltype(d)::value, decltype(t)::value>(c, b, a, p, Q, O, bf, w, s);
-        });
-    }
-    const kv::RowPlan p = kv::row_plan(c, b, a.group, a.window);
-    switch (D) {
-        case 64: return kv::launch_rows<64>(type, c, b, a, p, Q, O, bf, w, s);
-        case 96: return kv::launch_rows<96>(type, c, b, a, p, Q, O, bf, w, s);
-        case 128: return kv::launch_rows<128>(type, c, b, a, p, Q, O, bf, w, s);
-        case 192: return kv::launch_rows<192>(type, c, b, a, p, Q, O, bf, w, s);
-        default: return kv::launch_rows<256>(type, c, b, a, p, Q, O, bf, w, s);
-    }
+    return kv::by_dim(D, type, [&](auto d, auto) {
+        constexpr int N = decltype(d)::value;
+        return kv::few(b, D, a.group)
+                   ? kv::AttnKernels<N>::few(type, c, b, a, kv::few_plan(c, b, D, a.group, a.window), Q, O, bf, w, s)
+                   : kv::AttnKernels<N>::rows(type, c, b, a, kv::row_plan(c, b, D, a.group, a.window), Q, O, bf, w, s);
+    });
 }
 
 }  // namespace kq

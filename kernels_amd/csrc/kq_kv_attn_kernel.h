@@ -110,10 +110,16 @@ __device__ __forceinline__ f16x8 bf_f16x8(u32x4 raw, float up) {
     return q;
 }
 
+// Eight elements of q, with the scale's sign: the kernels multiply scores by its size, so that larger
+// scores stay larger.
+__device__ __forceinline__ u32x4 signed16(u32x4 v, float scale) {
+    return v ^ (scale < 0.0f ? 0x80008000u : 0u);
+}
+
 // A row's query as the second operand of S^T, in fp16: 16 columns a lane of each 64, 8 of a
 // last 32. bf16 rows go through a power of two; returns what undoes it.
 template <int D>
-__device__ __forceinline__ float load_q(const Rows& Q, bool there, int row, uint32_t head, int g, int bf,
+__device__ __forceinline__ float load_q(const Rows& Q, bool there, int row, uint32_t head, int g, int bf, float scale,
                                         f16x8 (&q)[D / 32]) {
     constexpr int C64 = D / 64;
     u32x4 raw[D / 32];
@@ -122,7 +128,7 @@ __device__ __forceinline__ float load_q(const Rows& Q, bool there, int row, uint
 #pragma unroll
     for (int i = 0; i < D / 32; ++i) {
         const int d = i < 2 * C64 ? i / 2 * 64 + g * 16 + i % 2 * 8 : C64 * 64 + g * 8;
-        raw[i] = there ? *reinterpret_cast<const u32x4*>(x + d) : u32x4{};
+        raw[i] = there ? signed16(*reinterpret_cast<const u32x4*>(x + d), scale) : u32x4{};
     }
     if (!bf) {
 #pragma unroll
@@ -143,23 +149,25 @@ __device__ __forceinline__ float load_q(const Rows& Q, bool there, int row, uint
 
 // ---- the work of a call of few rows, shared out evenly
 //
-// A sequence and head of u = ceil(tokens / kUnit) units (one at least, for its outputs) is a
-// row of work; all rows' units in order of sequence and head are cut into W equal shares, one
-// for each workgroup, however the lengths differ. A row that a cut goes through leaves partial
-// sums: a share's first piece, if it continues a row, in slot 2k, a last piece that begins a row
-// and does not end it in slot 2k + 1 (k the workgroup); kv_join_k adds the row's parts up.
-__device__ __forceinline__ int units_of(const Seq& s, const Span& v) {
-    return s.n == 0 ? 0 : max((v.hi - v.lo + kUnit - 1) / kUnit, 1);
+// A sequence and head is a row of work of ceil(tokens / kUnit) units, and where p.start is 1 one more at
+// its beginning, the price of beginning it: asking for its length, page ids, query and first codes one
+// after the other takes about as long as 256 tokens. All rows' units in order of sequence and head are cut
+// into equal shares, one for each workgroup, however the lengths differ. A row that a cut goes
+// through leaves partial sums: a share's first piece, if it continues a row, in slot 2k, a last piece that
+// begins a row and does not end it in slot 2k + 1 (k the workgroup); kv_join_k adds the row's parts up.
+__device__ __forceinline__ int units_of(const Seq& s, const Attn& a, int rows, int start) {
+    const Span v = span_of(s, a, 0, rows);
+    return s.n == 0 ? 0 : max((v.hi - v.lo + kUnit - 1) / kUnit, 1) + start;
 }
 
 struct Share {
     int seq;
     uint32_t head;
-    int unit;      // first unit, within its row
-    int units;     // in all
-    uint64_t at;   // of the first unit, among all
+    int unit;        // first unit, within its row
+    int units;       // in all
+    uint64_t at;     // of the first unit, among all
     uint64_t total;
-    uint32_t wgs;  // shares
+    uint32_t wgs;    // shares
 };
 
 __device__ __forceinline__ int prefix64(int v, int lane) {  // inclusive sum over the wave
@@ -171,33 +179,25 @@ __device__ __forceinline__ int prefix64(int v, int lane) {  // inclusive sum ove
     return v;
 }
 
-// lds: kScan + 1 + 8 ints. Every thread gets the same.
-__device__ Share share_of(const Cache& c, const Batch& b, const Attn& a, bool balanced, int* lds) {
+// lds: kScan + 9 ints. Every thread gets the same.
+__device__ inline Share share_of(const Cache& c, const Batch& b, const Attn& a, const FewPlan& p, int rows, int* lds) {
     const int tid = threadIdx.x;
     Share w = {0, 0, 0, 0, 0, 0, gridDim.x};
-    if (!balanced) {  // one row each
+    if (!p.balanced) {  // a whole row each
         w.seq = (int)(blockIdx.x / c.heads);
         w.head = blockIdx.x % c.heads;
-        const Seq s = sequence(b, c.page_log2, w.seq);
-        w.units = units_of(s, span_of(s, a, 0, 16));
-        w.total = w.units;
-        w.wgs = 1;
+        w.units = units_of(sequence(b, c.page_log2, w.seq), a, rows, (int)p.start);
         return w;
     }
     uint32_t u, before = 0;
     if (b.n_seq == 1) {
-        const Seq s = sequence(b, c.page_log2, 0);
-        u = (uint32_t)units_of(s, span_of(s, a, 0, 16));
+        u = (uint32_t)units_of(sequence(b, c.page_log2, 0), a, rows, (int)p.start);
         w.total = (uint64_t)u * c.heads;
     } else {
         int* const sums = lds + kScan + 1;
         int base = 0;
         for (uint32_t i0 = 0; i0 < b.n_seq; i0 += 256) {
-            int mine = 0;
-            if (i0 + tid < b.n_seq) {
-                const Seq s = sequence(b, c.page_log2, i0 + tid);
-                mine = units_of(s, span_of(s, a, 0, 16));
-            }
+            const int mine = i0 + tid < b.n_seq ? units_of(sequence(b, c.page_log2, i0 + tid), a, rows, (int)p.start) : 0;
             const int up = prefix64(mine, tid & 63);
             if ((tid & 63) == 63) sums[tid >> 6] = up;
             __syncthreads();
@@ -237,64 +237,74 @@ __device__ Share share_of(const Cache& c, const Batch& b, const Attn& a, bool ba
     return w;
 }
 
-// A row that is cut, by its first part's workgroup; parts 0: that workgroup begins none.
+// A row of work that is cut: the workgroup of its first part, and how many parts (0: it is whole).
+// By row of work where those are no more than the workgroups, else by workgroup.
 struct Cut {
-    int seq, head, parts, pad;
+    int seq, head, first, parts;
 };
-// The partial results of slot i: [16][D] sums, then [16] (m, l).
-template <int D>
+// The partial results of slot i: [16 R][D] sums, then [16 R] (m, l).
+template <int D, int R>
 __device__ __forceinline__ float* slot_of(float* ws, uint32_t cuts, uint32_t i) {
-    return ws + cuts * 4 + (uint64_t)i * (16 * (D + 2));
+    return ws + cuts * 4 + (uint64_t)i * (16 * R * (D + 2));
 }
 
-// Few rows: at most 16 (tokens x heads of a group) a sequence and head. Four waves take 64 tokens
+// Few rows: at most 16 R (tokens x heads of a group) of a sequence and head. Four waves take 64 tokens
 // of a piece in turn and join their sums at its end. What bounds it is the stream of codes:
 // a wave asks for its next keys as soon as the present ones are multiplied, and for its
 // next values after the product with the present ones, so that most of 16 KiB a wave
 // (128 wide) is always on its way.
-template <int D, int TYPE>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_attn_k(Cache c, Batch b, Attn a, int balanced, Rows Q,
-                                                                   Rows O, int bf, float* ws) {
+template <int D, int TYPE, int R>
+__global__ __launch_bounds__(256, few_waves(D, R)) void kv_few_k(Cache c, Batch b, Attn a, FewPlan p, Rows Q, Rows O,
+                                                                 int bf, float* ws) {
     constexpr int C64 = D / 64, kHalf = D % 64 ? 1 : 0;  // 64-column pieces of a key, and a 32-column one
     constexpr int kPad = D + 4;
     __shared__ __attribute__((aligned(16))) float o_lds[4 * 16 * kPad];
-    __shared__ float m_lds[4][16], l_lds[4][16];
+    __shared__ float m_lds[4][16 * R], l_lds[4][16 * R];
     static_assert(sizeof(o_lds) >= kIds * sizeof(int) && kIds >= kScan + 9, "page ids, sums of lengths");
     int* const ids = reinterpret_cast<int*>(o_lds);  // page ids of the piece, until the waves join
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 15, g = lane >> 4;
     const uint32_t q_heads = c.heads * a.group;
 
-    const Share share = share_of(c, b, a, balanced, ids);
+    const Share share = share_of(c, b, a, p, 16 * R, ids);
     Cut* const cuts = reinterpret_cast<Cut*>(ws);
-    if (balanced && tid == 0) cuts[blockIdx.x].parts = 0;
+    if (p.balanced && !p.by_row && tid == 0) cuts[blockIdx.x].parts = 0;
     int left = share.units, unit = share.unit;
     int seq = share.seq;
     uint32_t h = share.head;
     uint64_t at = share.at;
     while (left > 0) {
         const Seq s = sequence(b, c.page_log2, (uint32_t)seq);
-        const Span sp = span_of(s, a, 0, 16);
-        const int units = units_of(s, sp), mine = min(left, units - unit);
+        const Span sp = span_of(s, a, 0, 16 * R);
+        const int units = units_of(s, a, 16 * R, (int)p.start), mine = min(left, units - unit);
         if (mine <= 0) {  // a sequence without rows
             ++seq;
             continue;
         }
-        const int rows = s.n * (int)a.group;
-        const int lo = sp.lo + unit * kUnit, hi = (int)min((int64_t)sp.hi, (int64_t)lo + (int64_t)mine * kUnit);
+        const int rows = s.n * (int)a.group, tail = (int)p.start;
+        const int lo = sp.lo + max(unit - tail, 0) * kUnit;
+        const int hi = (int)min((int64_t)sp.hi, (int64_t)sp.lo + (int64_t)(unit + mine - tail) * kUnit);
         const int32_t* const table = b.pages + (uint64_t)seq * b.max_pages;
 
-        // this lane's row
-        const int row = r, tok = row / (int)a.group;
-        const uint32_t head = h * a.group + (uint32_t)(row % (int)a.group);
-        const bool there = row < rows;
-        const int pos = s.len - s.n + tok;
-        const int sees_hi = min(a.causal ? pos + 1 : s.len, hi), sees_lo = a.window ? pos + 1 - (int)a.window : 0;
+        // this lane's row of each sixteen
+        f16x8 q[R][D / 32];
+        float q_scale[R], m[R], l[R];  // m, l: of the row; l: this lane's tokens alone
+        int sees_lo[R], sees_hi[R];
+        f32x4 o[R][D / 16];
+#pragma unroll
+        for (int k = 0; k < R; ++k) {
+            const int row = 16 * k + r, tok = row / (int)a.group;
+            const bool there = row < rows;
+            const int pos = s.len - s.n + tok;
+            sees_hi[k] = there ? min(a.causal ? pos + 1 : s.len, hi) : 0;
+            sees_lo[k] = a.window ? pos + 1 - (int)a.window : 0;
+            q_scale[k] = fabsf(a.scale_log2) * load_q<D>(Q, there, s.row0 + tok, h * a.group + (uint32_t)(row % (int)a.group),
+                                                         g, bf, a.scale_log2, q[k]);
+            m[k] = kLowest;
+            l[k] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) o[k][i] = f32x4{0, 0, 0, 0};
+        }
 
-        f16x8 q[D / 32];
-        const float q_scale = a.scale_log2 * load_q<D>(Q, there, s.row0 + tok, head, g, bf, q);
-
-        float m = kLowest, l = 0.0f;  // of the row; l: this lane's tokens alone
-        f32x4 o[D / 16] = {};
         int page0 = 0;
         u32x4 kw[4 * C64 + 1], vw[D / 16];
         u32x2 kx[4];  // the 32-column pieces
@@ -323,55 +333,72 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_attn_k(Cache c, Batc
             for (int i = 0; i < D / 16; ++i) vw[i] = *reinterpret_cast<const u32x4*>(vp + i * 256);
         };
         auto step = [&](int t0, auto more) {
-            f32x4 st[4];
+            f32x4 st[R][4];
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
-                st[t] = f32x4{0, 0, 0, 0};
+#pragma unroll
+                for (int k = 0; k < R; ++k) st[k][t] = f32x4{0, 0, 0, 0};
 #pragma unroll
                 for (int i = 0; i < C64; ++i) {
                     const u32x4 w = kw[t * C64 + i];
-                    st[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes_f16x8<TYPE>(w.x, w.y), q[2 * i], st[t], 0, 0, 0);
-                    st[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes_f16x8<TYPE>(w.z, w.w), q[2 * i + 1], st[t], 0, 0, 0);
+                    const f16x8 x = codes_f16x8<TYPE>(w.x, w.y), y = codes_f16x8<TYPE>(w.z, w.w);
+#pragma unroll
+                    for (int k = 0; k < R; ++k) {
+                        st[k][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, q[k][2 * i], st[k][t], 0, 0, 0);
+                        st[k][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, q[k][2 * i + 1], st[k][t], 0, 0, 0);
+                    }
                 }
-                if constexpr (kHalf)
-                    st[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes_f16x8<TYPE>(kx[t].x, kx[t].y), q[2 * C64], st[t], 0, 0, 0);
+                if constexpr (kHalf) {
+                    const f16x8 x = codes_f16x8<TYPE>(kx[t].x, kx[t].y);
+#pragma unroll
+                    for (int k = 0; k < R; ++k)
+                        st[k][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, q[k][2 * C64], st[k][t], 0, 0, 0);
+                }
             }
             __builtin_amdgcn_sched_barrier(0);  // into the registers just read, not beside them
-            if constexpr (decltype(more)::value) load_k(t0 + 4 * kTile);
+            if constexpr (decltype(more)::value) load_k(t0 + kUnit);
             __builtin_amdgcn_sched_barrier(0);
 
             const int tv = t0 + 16 * g;
-            const float f = q_scale * pow2f(min(max(ke - 127, -126), 127)), ev = (float)(ve - 127);
-            float x[16], top = m;
-            // tokens in sight of the row, of the lane's 16
-            const int from = sees_lo - tv, to = pv < 0 ? 0 : sees_hi - tv;
-            if (__all(from <= 0 && to >= 16)) {
+            const float k_scale = pow2f(min(max(ke - 127, -126), 127)), un_v = pow2f(min(max(127 - ve, -126), 127));
+            f16x8 w[R][2];
 #pragma unroll
-                for (int i = 0; i < 16; ++i) x[i] = __builtin_fmaf(st[i / 4][i % 4], f, ev);
-            } else {
+            for (int k = 0; k < R; ++k) {
+                // t = f s + e with f >= 0: the largest t is the largest s's
+                float f = q_scale[k] * k_scale, e = (float)(ve - 127);
+                // tokens in sight of the row, of the lane's 16
+                const int from = sees_lo[k] - tv, to = pv < 0 ? 0 : sees_hi[k] - tv;
+                if (!__all(from <= 0 && to >= 16)) {
+                    // only the few tiles that need it: nothing of this is computed ahead of the branch
+                    int first = from;
+                    asm volatile("" : "+v"(first));
 #pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    x[i] = i < from || i >= to ? -__builtin_inff() : __builtin_fmaf(st[i / 4][i % 4], f, ev);
+                    for (int i = 0; i < 16; ++i)
+                        st[k][i / 4][i % 4] = i < first || i >= to ? -__builtin_inff() : __builtin_fmaf(st[k][i / 4][i % 4], f, e);
+                    f = 1.0f;
+                    e = 0.0f;
+                }
+                float top = st[k][0][0];
+#pragma unroll
+                for (int i = 1; i < 16; ++i) top = fmaxf(top, st[k][i / 4][i % 4]);
+                top = across_rows_maxf(fmaxf(m[k], __builtin_fmaf(top, f, e)));
+                if (__any(top > m[k])) {
+                    const float fade = __builtin_amdgcn_exp2f(m[k] - top);
+                    m[k] = top;
+                    l[k] *= fade;
+#pragma unroll
+                    for (int i = 0; i < D / 16; ++i) o[k][i] *= fade;
+                }
+                const float down = e - (m[k] - kLift);
+                float sum = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(st[k][i / 4][i % 4], f, down));
+                    sum += y;
+                    w[k][i / 8][i % 8] = (_Float16)y;
+                }
+                l[k] += sum * un_v;
             }
-#pragma unroll
-            for (int i = 0; i < 16; ++i) top = fmaxf(top, x[i]);
-            top = across_rows_maxf(top);
-            if (__any(top > m)) {
-                const float fade = __builtin_amdgcn_exp2f(m - top);
-                m = top;
-                l *= fade;
-#pragma unroll
-                for (int i = 0; i < D / 16; ++i) o[i] *= fade;
-            }
-            float sum = 0.0f;
-            f16x8 w[2];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const float y = __builtin_amdgcn_exp2f(x[i] - (m - kLift));
-                sum += y;
-                w[i / 8][i % 8] = (_Float16)y;
-            }
-            l += sum * pow2f(min(max(127 - ve, -126), 127));
             if (t0 + kTile > hi || __any(pv < 0)) {
                 // bytes of tokens that no length covers may hold anything, NaN among it
                 const int valid = pv < 0 ? 0 : min(max(hi - tv, 0), 16);
@@ -385,11 +412,15 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_attn_k(Cache c, Batc
             }
 #pragma unroll
             for (int i = 0; i < D / 16; ++i) {
-                o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes_f16x8<TYPE>(vw[i].x, vw[i].y), w[0], o[i], 0, 0, 0);
-                o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes_f16x8<TYPE>(vw[i].z, vw[i].w), w[1], o[i], 0, 0, 0);
+                const f16x8 x = codes_f16x8<TYPE>(vw[i].x, vw[i].y), y = codes_f16x8<TYPE>(vw[i].z, vw[i].w);
+#pragma unroll
+                for (int k = 0; k < R; ++k) {
+                    o[k][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, w[k][0], o[k][i], 0, 0, 0);
+                    o[k][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, w[k][1], o[k][i], 0, 0, 0);
+                }
             }
             __builtin_amdgcn_sched_barrier(0);
-            if constexpr (decltype(more)::value) load_v(t0 + 4 * kTile);
+            if constexpr (decltype(more)::value) load_v(t0 + kUnit);
             __builtin_amdgcn_sched_barrier(0);
         };
         // the piece, or as much of it as there is room for page ids
@@ -415,51 +446,57 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_attn_k(Cache c, Batc
         }
 
         // join the waves
-        l = across_rows_sum(l);
+        const bool whole = mine == units;
+        float* const part = slot_of<D, R>(ws, p.cuts, 2 * blockIdx.x + (unit == 0));
         __syncthreads();
-        if (g == 0) {
-            m_lds[wave][r] = m;
-            l_lds[wave][r] = l;
+#pragma unroll
+        for (int k = 0; k < R; ++k) {
+            l[k] = across_rows_sum(l[k]);
+            if (g == 0) {
+                m_lds[wave][16 * k + r] = m[k];
+                l_lds[wave][16 * k + r] = l[k];
+            }
         }
         __syncthreads();
-        {
-            float top = m_lds[0][r];
 #pragma unroll
-            for (int w = 1; w < 4; ++w) top = fmaxf(top, m_lds[w][r]);
-            const float fade = __builtin_amdgcn_exp2f(m - top);
+        for (int k = 0; k < R; ++k) {
+            if (16 * k >= rows) break;
+            float top = m_lds[0][16 * k + r];
+#pragma unroll
+            for (int w = 1; w < 4; ++w) top = fmaxf(top, m_lds[w][16 * k + r]);
+            const float fade = __builtin_amdgcn_exp2f(m[k] - top);
             float* const to = o_lds + (wave * 16 + r) * kPad;
 #pragma unroll
-            for (int i = 0; i < D / 16; ++i) *reinterpret_cast<f32x4*>(to + i * 16 + g * 4) = o[i] * fade;
-        }
-        __syncthreads();
-        const bool whole = mine == units;
-        float* const part = slot_of<D>(ws, gridDim.x, 2 * blockIdx.x + (unit == 0));
-        for (int i = tid; i < rows * (D / 4); i += 256) {
-            const int rr = i / (D / 4), d = i % (D / 4) * 4;
-            f32x4 y = *reinterpret_cast<const f32x4*>(o_lds + rr * kPad + d);
-            float top = m_lds[0][rr];
+            for (int i = 0; i < D / 16; ++i) *reinterpret_cast<f32x4*>(to + i * 16 + g * 4) = o[k][i] * fade;
+            __syncthreads();
+            for (int i = tid; i < min(rows - 16 * k, 16) * (D / 4); i += 256) {
+                const int in = i / (D / 4), row = 16 * k + in, d = i % (D / 4) * 4;
+                f32x4 y = *reinterpret_cast<const f32x4*>(o_lds + in * kPad + d);
+                float best = m_lds[0][row];
 #pragma unroll
-            for (int w = 1; w < 4; ++w) {
-                y += *reinterpret_cast<const f32x4*>(o_lds + (w * 16 + rr) * kPad + d);
-                top = fmaxf(top, m_lds[w][rr]);
-            }
-            float sum = 0.0f;
+                for (int w = 1; w < 4; ++w) {
+                    y += *reinterpret_cast<const f32x4*>(o_lds + (w * 16 + in) * kPad + d);
+                    best = fmaxf(best, m_lds[w][row]);
+                }
+                float sum = 0.0f;
 #pragma unroll
-            for (int w = 0; w < 4; ++w) sum += l_lds[w][rr] * __builtin_amdgcn_exp2f(m_lds[w][rr] - top);
-            if (whole) {
-                const uint32_t hd = h * a.group + (uint32_t)(rr % (int)a.group);
-                const int out = s.row0 + rr / (int)a.group;
-                store4(O, out, hd, d, y * finish(a, top, sum, out, hd, q_heads, d == 0), bf);
-            } else {
-                *reinterpret_cast<f32x4*>(part + rr * D + d) = y;
-                if (d == 0) *reinterpret_cast<float2*>(part + 16 * D + rr * 2) = make_float2(top, sum);
+                for (int w = 0; w < 4; ++w) sum += l_lds[w][row] * __builtin_amdgcn_exp2f(m_lds[w][row] - best);
+                if (whole) {
+                    const uint32_t head = h * a.group + (uint32_t)(row % (int)a.group);
+                    const int out = s.row0 + row / (int)a.group;
+                    store4(O, out, head, d, y * finish(a, best, sum, out, head, q_heads, d == 0), bf);
+                } else {
+                    *reinterpret_cast<f32x4*>(part + row * D + d) = y;
+                    if (d == 0) *reinterpret_cast<float2*>(part + 16 * R * D + row * 2) = make_float2(best, sum);
+                }
             }
+            __syncthreads();
         }
-        if (!whole && unit == 0 && tid == 0) {
-            // its last unit's workgroup: shares begin at floor(k total / wgs)
+        if (unit == 0 && tid == 0 && p.balanced && (p.by_row || !whole)) {
+            // the last unit's workgroup: shares begin at floor(k total / wgs)
             const uint64_t end = at + (uint64_t)units;
-            const int last = (int)((end * share.wgs - 1) / share.total);
-            cuts[blockIdx.x] = {seq, (int)h, last - (int)blockIdx.x + 1, 0};
+            const int parts = whole ? 0 : (int)((end * share.wgs - 1) / share.total) - (int)blockIdx.x + 1;
+            cuts[p.by_row ? (uint32_t)seq * c.heads + h : blockIdx.x] = {seq, (int)h, (int)blockIdx.x, parts};
         }
         left -= mine;
         at += (uint64_t)mine;
@@ -468,17 +505,18 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_attn_k(Cache c, Batc
     }
 }
 
-// Adds up the n parts of a row in one wave: sums(i) and ml(i) are part i's sums and (m, l).
-template <int D, class Sums, class Ml>
-__device__ __forceinline__ void join_row(const Attn& a, int n, Sums sums, Ml ml_of, const Rows& O, int bf, int at,
-                                         uint32_t head, uint32_t q_heads) {
+// Adds up the n parts of a row: sums(i) and ml(i) are part i's sums and (m, l). W waves of a workgroup
+// share the parts (lds: W (D + 2) floats), or one does it alone.
+template <int D, int W, class Sums, class Ml>
+__device__ __forceinline__ void join_row(const Attn& a, int n, Sums sums, Ml ml_of, float* lds, const Rows& O, int bf,
+                                         int at, uint32_t head, uint32_t q_heads) {
     constexpr int N = (D + 63) / 64;
-    const int lane = threadIdx.x & 63;
+    const int lane = threadIdx.x & 63, wave = W > 1 ? threadIdx.x >> 6 : 0;
     float m = kLowest, l = 0.0f, o[N] = {};
-    for (int i0 = 0; i0 < n; i0 += 64) {
-        const int here = min(n - i0, 64);
+    for (int i0 = 0; i0 < n; i0 += 64 * W) {
+        const int here = min((n - i0 - wave + W - 1) / W, 64);  // this wave's: i0 + wave, and every W-th
         float2 ml = make_float2(kLowest, 0.0f);
-        if (lane < here) ml = *reinterpret_cast<const float2*>(ml_of(i0 + lane));
+        if (lane < here) ml = *reinterpret_cast<const float2*>(ml_of(i0 + wave + lane * W));
         float top = fmaxf(m, ml.x);
 #pragma unroll
         for (int d = 1; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
@@ -487,14 +525,39 @@ __device__ __forceinline__ void join_row(const Attn& a, int n, Sums sums, Ml ml_
         l = l * fade + wave_sum(ml.y * f);
 #pragma unroll
         for (int k = 0; k < N; ++k) o[k] *= fade;
-#pragma unroll 8
+#pragma unroll 16
         for (int i = 0; i < here; ++i) {
             const float fi = __shfl(f, i);
-            const float* const from = sums(i0 + i);
+            const float* const from = sums(i0 + wave + i * W);
 #pragma unroll
             for (int k = 0; k < N; ++k)
                 if (D % 64 == 0 || k * 64 + lane < D) o[k] += from[k * 64 + lane] * fi;
         }
+    }
+    if constexpr (W > 1) {
+        float* const ml = lds + W * D;
+        if (lane == 0) ml[2 * wave] = m, ml[2 * wave + 1] = l;
+        __syncthreads();
+        float top = ml[0];
+#pragma unroll
+        for (int w = 1; w < W; ++w) top = fmaxf(top, ml[2 * w]);
+        const float fade = __builtin_amdgcn_exp2f(m - top);
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+            if (D % 64 == 0 || k * 64 + lane < D) lds[wave * D + k * 64 + lane] = o[k] * fade;
+        l = 0.0f;
+#pragma unroll
+        for (int w = 0; w < W; ++w) l += ml[2 * w + 1] * __builtin_amdgcn_exp2f(ml[2 * w] - top);
+        m = top;
+        __syncthreads();
+        if (wave) return;
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+            if (D % 64 == 0 || k * 64 + lane < D) {
+                o[k] = 0.0f;
+#pragma unroll
+                for (int w = 0; w < W; ++w) o[k] += lds[w * D + k * 64 + lane];
+            }
     }
     const float y = finish(a, m, l, at, head, q_heads, lane == 0);
     uint16_t* const to = static_cast<uint16_t*>(O.p) + (int64_t)at * O.row + (int64_t)head * O.head;
@@ -504,19 +567,47 @@ __device__ __forceinline__ void join_row(const Attn& a, int n, Sums sums, Ml ml_
             to[k * 64 + lane] = (uint16_t)(bf ? pair16<1>(o[k] * y, 0.0f) : pair16<0>(o[k] * y, 0.0f));
 }
 
-// The cut rows of kv_attn_k: a wave takes one of the 16 (token, head) rows.
-template <int D>
-__global__ __launch_bounds__(256) void kv_join_k(Cache c, Batch b, Attn a, uint32_t wgs, Rows O, int bf, float* ws) {
+// The cut rows of work of kv_few_k, one of their 16 R (token, head) rows for each W waves.
+template <int D, int R, int W>
+__global__ __launch_bounds__(256) void kv_join_k(Cache c, Batch b, Attn a, FewPlan p, Rows O, int bf, float* ws) {
+    __shared__ float lds[W > 1 ? W * (D + 2) : 1];
+    const int row = (int)(W > 1 ? blockIdx.y : blockIdx.y * 4 + (threadIdx.x >> 6));
+    // by row of work: a sequence without rows has written nothing
+    if (p.by_row && sequence(b, c.page_log2, blockIdx.x / c.heads).n == 0) return;
     const Cut cut = reinterpret_cast<const Cut*>(ws)[blockIdx.x];
     if (cut.parts == 0) return;
     const Seq s = sequence(b, c.page_log2, (uint32_t)cut.seq);
-    const int row = (int)(blockIdx.y * 4 + (threadIdx.x >> 6));
     if (row >= s.n * (int)a.group) return;
-    // part 0 begins the row, the others continue it: slots 2k + 1, then 2 (k + i)
-    auto part = [&](int i) { return slot_of<D>(ws, wgs, 2 * (blockIdx.x + i) + (i == 0)); };
-    join_row<D>(a, cut.parts, [&](int i) { return part(i) + row * D; }, [&](int i) { return part(i) + 16 * D + row * 2; },
-                O, bf, s.row0 + row / (int)a.group, (uint32_t)cut.head * a.group + (uint32_t)(row % (int)a.group),
-                c.heads * a.group);
+    // part 0 begins the row of work, the others continue it: slots 2k + 1, then 2 (k + i)
+    auto part = [&](int i) { return slot_of<D, R>(ws, p.cuts, 2 * (cut.first + i) + (i == 0)); };
+    join_row<D, W>(a, cut.parts, [&](int i) { return part(i) + row * D; },
+                   [&](int i) { return part(i) + 16 * R * D + row * 2; }, lds, O, bf, s.row0 + row / (int)a.group,
+                   (uint32_t)cut.head * a.group + (uint32_t)(row % (int)a.group), c.heads * a.group);
+}
+
+template <int D, int TYPE, int R>
+hipError_t few_r(const Cache& c, const Batch& b, const Attn& a, const FewPlan& p, const Rows& Q, const Rows& O, bool bf,
+                 float* ws, hipStream_t s) {
+    kv_few_k<D, TYPE, R><<<p.wgs, 256, 0, s>>>(c, b, a, p, Q, O, bf, ws);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess || !p.balanced) return e;
+    const uint32_t rows = b.max_q * a.group;
+    // many parts a row of work: four waves for each of its rows
+    if (p.wgs >= 8 * p.cuts) kv_join_k<D, R, 4><<<dim3(p.cuts, rows), 256, 0, s>>>(c, b, a, p, O, bf, ws);
+    else kv_join_k<D, R, 1><<<dim3(p.cuts, (rows + 3) / 4), 256, 0, s>>>(c, b, a, p, O, bf, ws);
+    return hipGetLastError();
+}
+
+template <int D, int TYPE>
+hipError_t few_d(const Cache& c, const Batch& b, const Attn& a, const FewPlan& p, const Rows& Q, const Rows& O, bool bf,
+                 float* ws, hipStream_t s) {
+    if constexpr (few_most(D) > 3)
+        if (p.sixteens == 4) return few_r<D, TYPE, 4>(c, b, a, p, Q, O, bf, ws, s);
+    if constexpr (few_most(D) > 2)
+        if (p.sixteens == 3) return few_r<D, TYPE, 3>(c, b, a, p, Q, O, bf, ws, s);
+    if constexpr (few_most(D) > 1)
+        if (p.sixteens == 2) return few_r<D, TYPE, 2>(c, b, a, p, Q, O, bf, ws, s);
+    return few_r<D, TYPE, 1>(c, b, a, p, Q, O, bf, ws, s);
 }
 
 }  // namespace kv

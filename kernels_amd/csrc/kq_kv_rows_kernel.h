@@ -1,5 +1,5 @@
 // kq_kv_rows_kernel.h -- attention over the 8-bit cache, many rows: the kernel of
-// kq_kv_rows_*.hip, for prompts and for more than 16 rows a sequence and head.
+// kq_kv_attn_<D>.hip for prompts and for more than 16 rows a sequence and head.
 //
 // A workgroup of NW waves takes 32 NW rows (query tokens x the heads of a group) of a sequence
 // and head, 64 tokens at a time. The tokens' codes become fp16 once for all its waves, in
@@ -59,13 +59,14 @@ __global__ __launch_bounds__(64 * NW, D >= 192 ? 1 : 2) void kv_rows_k(Cache c, 
 
     // Q as the second operand: 8 of each 16 columns
     f16x8 q[D / 16];
-    float q_scale = a.scale_log2;
+    float q_scale = fabsf(a.scale_log2);
     {
         u32x4 raw[D / 16];
         const uint16_t* const x = static_cast<const uint16_t*>(Q.p) +
                                   (there ? (int64_t)(s.row0 + tok) * Q.row + (int64_t)head * Q.head : 0);
 #pragma unroll
-        for (int i = 0; i < D / 16; ++i) raw[i] = there ? *reinterpret_cast<const u32x4*>(x + i * 16 + g * 8) : u32x4{};
+        for (int i = 0; i < D / 16; ++i)
+            raw[i] = there ? signed16(*reinterpret_cast<const u32x4*>(x + i * 16 + g * 8), a.scale_log2) : u32x4{};
         if (bf) {
             uint32_t top = 0;
 #pragma unroll
@@ -162,28 +163,34 @@ __global__ __launch_bounds__(64 * NW, D >= 192 ? 1 : 2) void kv_rows_k(Cache c, 
                     *reinterpret_cast<const f16x8*>(in.k + ((2 * i + g) * 65 + u * 32 + n) * 8), q[i], st[u], 0, 0, 0);
         }
         const int k0 = in.exps[g], k1 = in.exps[2 + g], v0 = in.exps[4 + g], v1 = in.exps[6 + g];
-        const float f[2] = {q_scale * pow2f(min(max(k0 - 127, -126), 127)), q_scale * pow2f(min(max(k1 - 127, -126), 127))};
-        const float ev[2] = {(float)(v0 - 127), (float)(v1 - 127)};
-        float top = m;
-        if (__all(t0 + 64 <= sees_hi && t0 >= sees_lo && k0 >= 0 && k1 >= 0)) {
+        // t = f s + e with f >= 0: the largest t of a block is its largest s's
+        float f[2] = {q_scale * pow2f(min(max(k0 - 127, -126), 127)), q_scale * pow2f(min(max(k1 - 127, -126), 127))};
+        float e[2] = {(float)(v0 - 127), (float)(v1 - 127)};
+        if (!__all(t0 + 64 <= sees_hi && t0 >= sees_lo && k0 >= 0 && k1 >= 0)) {
+            // only the few tiles that need it: nothing of this is computed ahead of the branch
+            int first = sees_lo - t0 - 16 * g;
+            asm volatile("" : "+v"(first));
+            const int end = first + sees_hi - sees_lo;
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) st[u][i] = __builtin_fmaf(st[u][i], f[u], ev[u]);
-        } else {
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
+            for (int u = 0; u < 2; ++u) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    const int t = t0 + 32 * u + 16 * g + i;
-                    st[u][i] = t < sees_lo || t >= sees_hi || (u ? k1 : k0) < 0 ? -__builtin_inff()
-                                                                               : __builtin_fmaf(st[u][i], f[u], ev[u]);
+                    const int t = 32 * u + i;
+                    st[u][i] = t < first || t >= end || (u ? k1 : k0) < 0 ? -__builtin_inff()
+                                                                         : __builtin_fmaf(st[u][i], f[u], e[u]);
                 }
+                f[u] = 1.0f;
+                e[u] = 0.0f;
+            }
         }
+        float top = m;
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+        for (int u = 0; u < 2; ++u) {
+            float most = st[u][0];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) top = fmaxf(top, st[u][i]);
+            for (int i = 1; i < 16; ++i) most = fmaxf(most, st[u][i]);
+            top = fmaxf(top, __builtin_fmaf(most, f[u], e[u]));
+        }
         {
             float x, y;
             swapped<true>(top, x, y);
@@ -196,14 +203,14 @@ __global__ __launch_bounds__(64 * NW, D >= 192 ? 1 : 2) void kv_rows_k(Cache c, 
 #pragma unroll
             for (int i = 0; i < D / 32; ++i) o[i] *= fade;
         }
-        const float down = m - kLift;
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
+            const float down = e[u] - (m - kLift);
             f16x8 w[2];
             float sum = 0.0f;
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                const float y = __builtin_amdgcn_exp2f(st[u][i] - down);
+                const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(st[u][i], f[u], down));
                 sum += y;
                 w[i / 8][i % 8] = (_Float16)y;
             }
@@ -275,19 +282,19 @@ __global__ __launch_bounds__(256) void kv_rows_join_k(Cache c, Batch b, Attn a, 
     const uint64_t size = (uint64_t)RT * (D + 2);
     const float* const first = ws + (((uint64_t)seq * p.splits * p.tiles + tile) * c.heads + h) * size;
     const uint64_t step = (uint64_t)p.tiles * c.heads * size;
-    join_row<D>(a, n, [&](int i) { return first + i * step + in * D; },
-                [&](int i) { return first + i * step + RT * D + in * 2; }, O, bf, s.row0 + (int)j, head, q_heads);
+    join_row<D, 1>(a, n, [&](int i) { return first + i * step + in * D; },
+                   [&](int i) { return first + i * step + RT * D + in * 2; }, nullptr, O, bf, s.row0 + (int)j, head, q_heads);
 }
 
 template <int D, int TYPE>
 hipError_t rows_d(const Cache& c, const Batch& b, const Attn& a, const RowPlan& p, const Rows& Q, const Rows& O, bool bf,
                   float* ws, hipStream_t s) {
     const uint32_t wgs = b.n_seq * p.splits * p.tiles * c.heads;
-    switch (p.rows) {
-        case 32: kv_rows_k<D, TYPE, 1><<<wgs, 64, 0, s>>>(c, b, a, p, Q, O, bf, ws); break;
-        case 64: kv_rows_k<D, TYPE, 2><<<wgs, 128, 0, s>>>(c, b, a, p, Q, O, bf, ws); break;
-        case 128: kv_rows_k<D, TYPE, 4><<<wgs, 256, 0, s>>>(c, b, a, p, Q, O, bf, ws); break;
-        default: kv_rows_k<D, TYPE, 8><<<wgs, 512, 0, s>>>(c, b, a, p, Q, O, bf, ws); break;
+    if constexpr (row_most(D) > 128) {
+        if (p.rows > 128) kv_rows_k<D, TYPE, 8><<<wgs, 512, 0, s>>>(c, b, a, p, Q, O, bf, ws);
+        else kv_rows_k<D, TYPE, 4><<<wgs, 256, 0, s>>>(c, b, a, p, Q, O, bf, ws);
+    } else {
+        kv_rows_k<D, TYPE, 4><<<wgs, 256, 0, s>>>(c, b, a, p, Q, O, bf, ws);
     }
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.splits == 1) return e;
