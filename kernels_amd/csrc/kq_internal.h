@@ -182,13 +182,18 @@ struct Attn {
     const float* sinks;
     float* lse;
 };
-// Launch of the kernel for few rows.
+// Launch of the kernel for few rows. A row of work is a sequence and head.
 struct FewPlan {
+    enum Mode : uint32_t {
+        kRows,    // a workgroup each
+        kParts,   // rows of work in equal parts, a workgroup each
+        kShares,  // all of it in equal shares, whatever rows they begin and end in
+    };
     uint32_t sixteens;  // of rows of a sequence and head: 1 to few_most(head_dim)
     uint32_t wgs;
-    uint32_t balanced;  // equal shares of all units; else a sequence and head each
-    uint32_t start;     // units that the beginning of a sequence and head is priced at
-    uint32_t by_row;    // cuts are by sequence and head
+    uint32_t mode;
+    uint32_t start;     // units that the beginning of a row of work is priced at
+    uint32_t by_row;    // cuts are by row of work
     uint32_t cuts;      // descriptors of cuts in the workspace
 };
 // Rows that its registers hold, in sixteens, and the waves of a SIMD they allow.

@@ -20,19 +20,21 @@ bool few(const Batch& b, uint32_t D, uint32_t group) { return (uint64_t)b.max_q 
 
 // Its workgroups: all that the device holds at once, or one for each unit of work where there
 // is less; one for each row of work where those are a unit long or the sequences too
-// many to add up their lengths in each workgroup.
+// many to add up their lengths in each workgroup. Where there are workgroups enough each takes a
+// part of one row of work: the beginning of another costs it about as long as 256 tokens do.
 FewPlan few_plan(const Cache& c, const Batch& b, uint32_t D, uint32_t group, uint32_t window) {
     FewPlan p = {};
     p.sixteens = (uint32_t)ceil_div((uint64_t)b.max_q * group, 16);
     const uint64_t units = ceil_div(longest_span(b, 16 * p.sixteens, window), kUnit), rows = (uint64_t)b.n_seq * c.heads;
-    p.balanced = units > 1 && b.n_seq <= kScan && b.n_seq * (units + 1) < 0x7FFFFFFF;
-    if (!p.balanced) {
+    if (units <= 1 || b.n_seq > kScan || b.n_seq * (units + 1) >= 0x7FFFFFFF) {
+        p.mode = FewPlan::kRows;
         p.wgs = (uint32_t)rows;
         return p;
     }
     const uint64_t fit = (uint64_t)cu_count() * few_waves(D, p.sixteens);
     p.wgs = (uint32_t)std::min<uint64_t>(fit, rows * units);
-    p.start = b.n_seq > 1 && rows * units >= 4 * fit;
+    p.mode = 2 * rows <= p.wgs ? FewPlan::kParts : FewPlan::kShares;
+    p.start = p.mode == FewPlan::kShares && rows * units >= 4 * fit;
     p.by_row = rows <= p.wgs;
     p.cuts = p.by_row ? (uint32_t)rows : p.wgs;
     return p;
@@ -40,7 +42,7 @@ FewPlan few_plan(const Cache& c, const Batch& b, uint32_t D, uint32_t group, uin
 // Of any window: descriptors and slots of the widest launch.
 size_t few_ws_bytes(const Cache& c, const Batch& b, uint32_t D, uint32_t group) {
     const FewPlan p = few_plan(c, b, D, group, 0);
-    return p.balanced ? (size_t)p.wgs * (sizeof(Cut) + 2 * 16 * p.sixteens * (D + 2) * 4) : 0;
+    return p.mode == FewPlan::kRows ? 0 : (size_t)p.wgs * (sizeof(Cut) + 2 * 16 * p.sixteens * (D + 2) * 4);
 }
 
 uint64_t row_splits_wanted(const Cache& c, const Batch& b, const RowPlan& p) {

@@ -149,12 +149,15 @@ __device__ __forceinline__ float load_q(const Rows& Q, bool there, int row, uint
 
 // ---- the work of a call of few rows, shared out evenly
 //
-// A sequence and head is a row of work of ceil(tokens / kUnit) units, and where p.start is 1 one more at
+// A row of work (a sequence and head) is ceil(tokens / kUnit) units, and where p.start is 1 one more at
 // its beginning, the price of beginning it: asking for its length, page ids, query and first codes one
-// after the other takes about as long as 256 tokens. All rows' units in order of sequence and head are cut
-// into equal shares, one for each workgroup, however the lengths differ. A row that a cut goes
-// through leaves partial sums: a share's first piece, if it continues a row, in slot 2k, a last piece that
-// begins a row and does not end it in slot 2k + 1 (k the workgroup); kv_join_k adds the row's parts up.
+// after the other takes about as long as 256 tokens.
+// kParts: rows of work are cut into parts of at most c units, with the smallest c that gives no more parts
+// than workgroups (or near it). kShares: all rows' units in order of sequence and head are cut
+// into equal shares, one for each workgroup, however the lengths differ.
+// A row of work that a cut goes through leaves partial sums: a workgroup's first piece, if it continues a
+// row, in slot 2k, a last piece that begins a row and does not end it in slot 2k + 1 (k the workgroup);
+// kv_join_k adds the row's parts up.
 __device__ __forceinline__ int units_of(const Seq& s, const Attn& a, int rows, int start) {
     const Span v = span_of(s, a, 0, rows);
     return s.n == 0 ? 0 : max((v.hi - v.lo + kUnit - 1) / kUnit, 1) + start;
@@ -163,9 +166,10 @@ __device__ __forceinline__ int units_of(const Seq& s, const Attn& a, int rows, i
 struct Share {
     int seq;
     uint32_t head;
-    int unit;        // first unit, within its row
+    int unit;        // first unit, within its row of work
     int units;       // in all
-    uint64_t at;     // of the first unit, among all
+    int parts;       // of its row of work (kParts)
+    uint64_t at;     // of the first unit, among all (kShares)
     uint64_t total;
     uint32_t wgs;    // shares
 };
@@ -179,61 +183,85 @@ __device__ __forceinline__ int prefix64(int v, int lane) {  // inclusive sum ove
     return v;
 }
 
-// lds: kScan + 9 ints. Every thread gets the same.
+// What this workgroup does; each wave works it out for itself from the units of all sequences.
+// lds: kScan ints.
 __device__ inline Share share_of(const Cache& c, const Batch& b, const Attn& a, const FewPlan& p, int rows, int* lds) {
-    const int tid = threadIdx.x;
-    Share w = {0, 0, 0, 0, 0, 0, gridDim.x};
-    if (!p.balanced) {  // a whole row each
+    const int lane = threadIdx.x & 63, n = (int)b.n_seq;
+    Share w = {0, 0, 0, 0, 1, 0, 0, gridDim.x};
+    if (p.mode == FewPlan::kRows) {
         w.seq = (int)(blockIdx.x / c.heads);
         w.head = blockIdx.x % c.heads;
         w.units = units_of(sequence(b, c.page_log2, w.seq), a, rows, (int)p.start);
         return w;
     }
-    uint32_t u, before = 0;
-    if (b.n_seq == 1) {
-        u = (uint32_t)units_of(sequence(b, c.page_log2, 0), a, rows, (int)p.start);
-        w.total = (uint64_t)u * c.heads;
+    int u0;  // of sequence `lane`
+    if (n <= 64) {
+        u0 = lane < n ? units_of(sequence(b, c.page_log2, lane), a, rows, (int)p.start) : 0;
     } else {
-        int* const sums = lds + kScan + 1;
-        int base = 0;
-        for (uint32_t i0 = 0; i0 < b.n_seq; i0 += 256) {
-            const int mine = i0 + tid < b.n_seq ? units_of(sequence(b, c.page_log2, i0 + tid), a, rows, (int)p.start) : 0;
-            const int up = prefix64(mine, tid & 63);
-            if ((tid & 63) == 63) sums[tid >> 6] = up;
-            __syncthreads();
-            int wave_base = base;
-            for (int i = 0; i < tid >> 6; ++i) wave_base += sums[i];
-            if (i0 + tid < b.n_seq) lds[i0 + tid] = wave_base + up - mine;
-            base += sums[0] + sums[1] + sums[2] + sums[3];
-            __syncthreads();
-        }
-        if (tid == 0) lds[b.n_seq] = base;
-        w.total = (uint64_t)(uint32_t)base * c.heads;
+        for (int i = threadIdx.x; i < n; i += 256) lds[i] = units_of(sequence(b, c.page_log2, i), a, rows, (int)p.start);
+        __syncthreads();
+        u0 = lds[lane];
     }
+    // sum over all sequences of f(units)
+    auto sum = [&](auto f) {
+        int v = 0;
+        for (int i = lane; i < n; i += 64) v += f(i < 64 ? u0 : lds[i]);
+        return (uint64_t)(uint32_t)__builtin_amdgcn_readlane(prefix64(v, lane), 63);
+    };
+    // the sequence i with sum_{j < i} f <= x < sum_{j <= i} f; x becomes what is left, u its units
+    auto find = [&](uint32_t& x, int& u, auto f) {
+        int before = 0;
+        for (int i0 = 0; i0 < n; i0 += 64) {
+            const int mine = i0 + lane < n ? i0 ? lds[i0 + lane] : u0 : 0, v = f(mine);
+            const int up = prefix64(v, lane) + before;
+            const uint64_t hit = __ballot((uint32_t)(up - v) <= x && x < (uint32_t)up);
+            if (hit) {
+                const int l = __ffsll((unsigned long long)hit) - 1;
+                x -= (uint32_t)__builtin_amdgcn_readlane(up - v, l);
+                u = __builtin_amdgcn_readlane(mine, l);
+                return i0 + l;
+            }
+            before = __builtin_amdgcn_readlane(up, 63);
+        }
+        return 0;
+    };
+    const uint64_t all = sum([](int u) { return u; });
+    if (all == 0) return w;
+    int u = 0;
+    if (p.mode == FewPlan::kParts) {
+        // c from the mean on; the last is enough for any lengths: sum ceil(u / c) <= sum u / c + rows of work
+        const uint32_t most = gridDim.x / c.heads;
+        uint32_t size = (uint32_t)((all + most - 1) / most), count = 0;
+        for (int tries = 0; tries < 4; ++tries, ++size) {
+            count = (uint32_t)sum([&](int v) { return (int)(((uint32_t)v + size - 1) / size); });
+            if (count <= most) break;
+        }
+        if (count > most) {
+            size = max(size, (uint32_t)((all + most - n - 1) / (most - n)));
+            count = (uint32_t)sum([&](int v) { return (int)(((uint32_t)v + size - 1) / size); });
+        }
+        if (blockIdx.x >= count * c.heads) return w;
+        // parts in order of head, then sequence
+        w.head = blockIdx.x / count;
+        uint32_t x = blockIdx.x % count;
+        w.seq = find(x, u, [&](int v) { return (int)(((uint32_t)v + size - 1) / size); });
+        w.parts = (int)(((uint32_t)u + size - 1) / size);
+        w.unit = (int)((uint64_t)x * u / w.parts);
+        w.units = (int)((uint64_t)(x + 1) * u / w.parts) - w.unit;
+        return w;
+    }
+    w.total = all * c.heads;
     if (w.total < w.wgs) w.wgs = (uint32_t)w.total;
     if (blockIdx.x >= w.wgs) return w;
     w.at = w.total * blockIdx.x / w.wgs;
     w.units = (int)(w.total * (blockIdx.x + 1) / w.wgs - w.at);
-    if (b.n_seq > 1) {
-        int* const found = lds + kScan + 5;
-        __syncthreads();
-        for (uint32_t i = tid; i < b.n_seq; i += 256) {
-            const uint64_t from = (uint64_t)(uint32_t)lds[i] * c.heads, to = (uint64_t)(uint32_t)lds[i + 1] * c.heads;
-            if (from <= w.at && w.at < to) {
-                found[0] = (int)i;
-                found[1] = lds[i];
-                found[2] = lds[i + 1] - lds[i];
-            }
-        }
-        __syncthreads();
-        w.seq = found[0];
-        before = (uint32_t)found[1];
-        u = (uint32_t)found[2];
-        __syncthreads();
-    }
-    const uint64_t in = w.at - (uint64_t)before * c.heads;
-    w.head = (uint32_t)(in / u);
-    w.unit = (int)(in % u);
+    // in order of sequence, then head
+    uint32_t x = (uint32_t)(w.at / c.heads);
+    const uint32_t odd = (uint32_t)(w.at % c.heads);
+    w.seq = find(x, u, [](int v) { return v; });
+    const uint64_t in = (uint64_t)x * c.heads + odd;
+    w.head = (uint32_t)(in / (uint32_t)u);
+    w.unit = (int)(in % (uint32_t)u);
     return w;
 }
 
@@ -258,21 +286,23 @@ __global__ __launch_bounds__(256, few_waves(D, R)) void kv_few_k(Cache c, Batch 
                                                                  int bf, float* ws) {
     constexpr int C64 = D / 64, kHalf = D % 64 ? 1 : 0;  // 64-column pieces of a key, and a 32-column one
     constexpr int kPad = D + 4;
-    __shared__ __attribute__((aligned(16))) float o_lds[4 * 16 * kPad];
+    __shared__ __attribute__((aligned(16))) float o_lds[4 * 16 * R * kPad];
     __shared__ float m_lds[4][16 * R], l_lds[4][16 * R];
-    static_assert(sizeof(o_lds) >= kIds * sizeof(int) && kIds >= kScan + 9, "page ids, sums of lengths");
+    static_assert(sizeof(o_lds) >= kIds * sizeof(int) && kIds >= kScan, "page ids, units of the sequences");
     int* const ids = reinterpret_cast<int*>(o_lds);  // page ids of the piece, until the waves join
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 15, g = lane >> 4;
     const uint32_t q_heads = c.heads * a.group;
 
     const Share share = share_of(c, b, a, p, 16 * R, ids);
     Cut* const cuts = reinterpret_cast<Cut*>(ws);
-    if (p.balanced && !p.by_row && tid == 0) cuts[blockIdx.x].parts = 0;
+    if (p.mode == FewPlan::kShares && !p.by_row && tid == 0) cuts[blockIdx.x].parts = 0;
     int left = share.units, unit = share.unit;
     int seq = share.seq;
     uint32_t h = share.head;
     uint64_t at = share.at;
     while (left > 0) {
+        seq = __builtin_amdgcn_readfirstlane(seq);
+        h = (uint32_t)__builtin_amdgcn_readfirstlane((int)h);
         const Seq s = sequence(b, c.page_log2, (uint32_t)seq);
         const Span sp = span_of(s, a, 0, 16 * R);
         const int units = units_of(s, a, 16 * R, (int)p.start), mine = min(left, units - unit);
@@ -318,8 +348,8 @@ __global__ __launch_bounds__(256, few_waves(D, R)) void kv_few_k(Cache c, Batch 
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
 #pragma unroll
-                for (int i = 0; i < C64; ++i) kw[t * C64 + i] = *reinterpret_cast<const u32x4*>(kp + t * 4 * D + i * 64 + g * 16);
-                if constexpr (kHalf) kx[t] = *reinterpret_cast<const u32x2*>(kp + t * 4 * D + C64 * 64 + g * 8);
+                for (int i = 0; i < C64; ++i) kw[t * C64 + i] = ldg_nt(reinterpret_cast<const u32x4*>(kp + t * 4 * D + i * 64 + g * 16));
+                if constexpr (kHalf) kx[t] = ldg_nt(reinterpret_cast<const u32x2*>(kp + t * 4 * D + C64 * 64 + g * 8));
             }
         };
         auto load_v = [&](int t0) {
@@ -330,7 +360,7 @@ __global__ __launch_bounds__(256, few_waves(D, R)) void kv_few_k(Cache c, Batch 
             ve = c.v_exp[eo];
             const uint8_t* const vp = c.v + code_offset(c, D, max(pv, 0), h, tv) + r * 16;
 #pragma unroll
-            for (int i = 0; i < D / 16; ++i) vw[i] = *reinterpret_cast<const u32x4*>(vp + i * 256);
+            for (int i = 0; i < D / 16; ++i) vw[i] = ldg_nt(reinterpret_cast<const u32x4*>(vp + i * 256));
         };
         auto step = [&](int t0, auto more) {
             f32x4 st[R][4];
@@ -460,44 +490,43 @@ __global__ __launch_bounds__(256, few_waves(D, R)) void kv_few_k(Cache c, Batch 
         __syncthreads();
 #pragma unroll
         for (int k = 0; k < R; ++k) {
-            if (16 * k >= rows) break;
             float top = m_lds[0][16 * k + r];
 #pragma unroll
             for (int w = 1; w < 4; ++w) top = fmaxf(top, m_lds[w][16 * k + r]);
             const float fade = __builtin_amdgcn_exp2f(m[k] - top);
-            float* const to = o_lds + (wave * 16 + r) * kPad;
+            float* const to = o_lds + ((wave * R + k) * 16 + r) * kPad;
 #pragma unroll
             for (int i = 0; i < D / 16; ++i) *reinterpret_cast<f32x4*>(to + i * 16 + g * 4) = o[k][i] * fade;
-            __syncthreads();
-            for (int i = tid; i < min(rows - 16 * k, 16) * (D / 4); i += 256) {
-                const int in = i / (D / 4), row = 16 * k + in, d = i % (D / 4) * 4;
-                f32x4 y = *reinterpret_cast<const f32x4*>(o_lds + in * kPad + d);
-                float best = m_lds[0][row];
+        }
+        __syncthreads();
+        for (int i = tid; i < rows * (D / 4); i += 256) {
+            const int row = i / (D / 4), d = i % (D / 4) * 4;
+            f32x4 y = *reinterpret_cast<const f32x4*>(o_lds + row * kPad + d);
+            float best = m_lds[0][row];
 #pragma unroll
-                for (int w = 1; w < 4; ++w) {
-                    y += *reinterpret_cast<const f32x4*>(o_lds + (w * 16 + in) * kPad + d);
-                    best = fmaxf(best, m_lds[w][row]);
-                }
-                float sum = 0.0f;
-#pragma unroll
-                for (int w = 0; w < 4; ++w) sum += l_lds[w][row] * __builtin_amdgcn_exp2f(m_lds[w][row] - best);
-                if (whole) {
-                    const uint32_t head = h * a.group + (uint32_t)(row % (int)a.group);
-                    const int out = s.row0 + row / (int)a.group;
-                    store4(O, out, head, d, y * finish(a, best, sum, out, head, q_heads, d == 0), bf);
-                } else {
-                    *reinterpret_cast<f32x4*>(part + row * D + d) = y;
-                    if (d == 0) *reinterpret_cast<float2*>(part + 16 * R * D + row * 2) = make_float2(best, sum);
-                }
+            for (int w = 1; w < 4; ++w) {
+                y += *reinterpret_cast<const f32x4*>(o_lds + (w * 16 * R + row) * kPad + d);
+                best = fmaxf(best, m_lds[w][row]);
             }
-            __syncthreads();
+            float sum = 0.0f;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) sum += l_lds[w][row] * __builtin_amdgcn_exp2f(m_lds[w][row] - best);
+            if (whole) {
+                const uint32_t head = h * a.group + (uint32_t)(row % (int)a.group);
+                const int out = s.row0 + row / (int)a.group;
+                store4(O, out, head, d, y * finish(a, best, sum, out, head, q_heads, d == 0), bf);
+            } else {
+                *reinterpret_cast<f32x4*>(part + row * D + d) = y;
+                if (d == 0) *reinterpret_cast<float2*>(part + 16 * R * D + row * 2) = make_float2(best, sum);
+            }
         }
-        if (unit == 0 && tid == 0 && p.balanced && (p.by_row || !whole)) {
-            // the last unit's workgroup: shares begin at floor(k total / wgs)
-            const uint64_t end = at + (uint64_t)units;
-            const int parts = whole ? 0 : (int)((end * share.wgs - 1) / share.total) - (int)blockIdx.x + 1;
-            cuts[p.by_row ? (uint32_t)seq * c.heads + h : blockIdx.x] = {seq, (int)h, (int)blockIdx.x, parts};
+        if (unit == 0 && tid == 0 && p.mode != FewPlan::kRows && (p.by_row || !whole)) {
+            int parts = share.parts;
+            if (p.mode == FewPlan::kShares)  // the last unit's workgroup: shares begin at floor(k total / wgs)
+                parts = (int)(((at + (uint64_t)units) * share.wgs - 1) / share.total) - (int)blockIdx.x + 1;
+            cuts[p.by_row ? (uint32_t)seq * c.heads + h : blockIdx.x] = {seq, (int)h, (int)blockIdx.x, whole ? 0 : parts};
         }
+        __syncthreads();
         left -= mine;
         at += (uint64_t)mine;
         unit = 0;
@@ -513,26 +542,35 @@ __device__ __forceinline__ void join_row(const Attn& a, int n, Sums sums, Ml ml_
     constexpr int N = (D + 63) / 64;
     const int lane = threadIdx.x & 63, wave = W > 1 ? threadIdx.x >> 6 : 0;
     float m = kLowest, l = 0.0f, o[N] = {};
-    for (int i0 = 0; i0 < n; i0 += 64 * W) {
-        const int here = min((n - i0 - wave + W - 1) / W, 64);  // this wave's: i0 + wave, and every W-th
+    for (int i0 = 0; i0 < n; i0 += 16 * W) {
+        const int here = min((n - i0 - wave + W - 1) / W, 16);  // this wave's: i0 + wave, and every W-th
+        // the sums are asked for along with what scales them
+        float v[16][N];
         float2 ml = make_float2(kLowest, 0.0f);
         if (lane < here) ml = *reinterpret_cast<const float2*>(ml_of(i0 + wave + lane * W));
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            if (i < here) {
+                const float* const from = sums(i0 + wave + i * W);
+#pragma unroll
+                for (int k = 0; k < N; ++k) v[i][k] = D % 64 == 0 || k * 64 + lane < D ? from[k * 64 + lane] : 0.0f;
+            }
         float top = fmaxf(m, ml.x);
 #pragma unroll
-        for (int d = 1; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
+        for (int d = 1; d < 16; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
+        top = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, top)));
         const float fade = __builtin_amdgcn_exp2f(m - top), f = __builtin_amdgcn_exp2f(ml.x - top);
         m = top;
         l = l * fade + wave_sum(ml.y * f);
 #pragma unroll
         for (int k = 0; k < N; ++k) o[k] *= fade;
-#pragma unroll 16
-        for (int i = 0; i < here; ++i) {
-            const float fi = __shfl(f, i);
-            const float* const from = sums(i0 + wave + i * W);
 #pragma unroll
-            for (int k = 0; k < N; ++k)
-                if (D % 64 == 0 || k * 64 + lane < D) o[k] += from[k * 64 + lane] * fi;
-        }
+        for (int i = 0; i < 16; ++i)
+            if (i < here) {
+                const float fi = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), i));
+#pragma unroll
+                for (int k = 0; k < N; ++k) o[k] += v[i][k] * fi;
+            }
     }
     if constexpr (W > 1) {
         float* const ml = lds + W * D;
@@ -573,10 +611,11 @@ __global__ __launch_bounds__(256) void kv_join_k(Cache c, Batch b, Attn a, FewPl
     __shared__ float lds[W > 1 ? W * (D + 2) : 1];
     const int row = (int)(W > 1 ? blockIdx.y : blockIdx.y * 4 + (threadIdx.x >> 6));
     // by row of work: a sequence without rows has written nothing
-    if (p.by_row && sequence(b, c.page_log2, blockIdx.x / c.heads).n == 0) return;
     const Cut cut = reinterpret_cast<const Cut*>(ws)[blockIdx.x];
+    const Seq own = sequence(b, c.page_log2, p.by_row ? blockIdx.x / c.heads : 0);
+    if (p.by_row && own.n == 0) return;
     if (cut.parts == 0) return;
-    const Seq s = sequence(b, c.page_log2, (uint32_t)cut.seq);
+    const Seq s = p.by_row ? own : sequence(b, c.page_log2, (uint32_t)cut.seq);
     if (row >= s.n * (int)a.group) return;
     // part 0 begins the row of work, the others continue it: slots 2k + 1, then 2 (k + i)
     auto part = [&](int i) { return slot_of<D, R>(ws, p.cuts, 2 * (cut.first + i) + (i == 0)); };
@@ -590,7 +629,7 @@ hipError_t few_r(const Cache& c, const Batch& b, const Attn& a, const FewPlan& p
                  float* ws, hipStream_t s) {
     kv_few_k<D, TYPE, R><<<p.wgs, 256, 0, s>>>(c, b, a, p, Q, O, bf, ws);
     const hipError_t e = hipGetLastError();
-    if (e != hipSuccess || !p.balanced) return e;
+    if (e != hipSuccess || p.mode == FewPlan::kRows) return e;
     const uint32_t rows = b.max_q * a.group;
     // many parts a row of work: four waves for each of its rows
     if (p.wgs >= 8 * p.cuts) kv_join_k<D, R, 4><<<dim3(p.cuts, rows), 256, 0, s>>>(c, b, a, p, O, bf, ws);
