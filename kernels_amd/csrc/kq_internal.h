@@ -185,22 +185,21 @@ struct Attn {
 // Launch of the kernel for few rows. A row of work is a sequence and head.
 struct FewPlan {
     enum Mode : uint32_t {
-        kRows,    // a workgroup each
-        kParts,   // rows of work in equal parts, a workgroup each
+        kRows,    // a group each
+        kParts,   // rows of work in equal parts, a group each
         kShares,  // all of it in equal shares, whatever rows they begin and end in
     };
-    uint32_t sixteens;  // of rows of a sequence and head: 1 to few_most(head_dim)
-    uint32_t wgs;
+    uint32_t sixteens;  // rows of a workgroup, in sixteens: 1 or 2
+    uint32_t tiles;     // workgroups that take the same tokens for other rows
+    uint32_t groups;    // of such workgroups
     uint32_t mode;
-    uint32_t start;     // units that the beginning of a row of work is priced at
+    uint32_t start;     // units (of 64 tokens) that the beginning of a row of work is priced at
     uint32_t by_row;    // cuts are by row of work
     uint32_t cuts;      // descriptors of cuts in the workspace
 };
-// Rows that its registers hold, in sixteens, and the waves of a SIMD they allow.
-constexpr uint32_t few_most(uint32_t D) { return D <= 96 ? 4 : D == 128 ? 3 : D == 192 ? 2 : 1; }
-constexpr uint32_t few_waves(uint32_t D, uint32_t R) {
-    return D == 64 ? (R <= 3 ? 2 : 1) : D <= 128 ? (R <= 2 ? 2 : 1) : D == 192 && R == 1 ? 2 : 1;
-}
+// Sixteens of rows that its registers hold, and the waves of a SIMD they allow then.
+constexpr uint32_t few_sixteens(uint32_t D) { return D <= 128 ? 2 : 1; }
+constexpr uint32_t few_waves(uint32_t D) { return D == 256 ? 1 : 2; }
 // Rows of a tile of the kernel for many rows, at most.
 #ifndef KV_ROWMOST
 #define KV_ROWMOST (D == 96 || D == 128 ? 256 : 128)

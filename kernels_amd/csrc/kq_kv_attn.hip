@@ -15,34 +15,37 @@ uint64_t longest_span(const Batch& b, uint64_t rows, uint32_t window) {
     return window ? std::min<uint64_t>(b.max_len, (uint64_t)window + rows - 1 + kTile - 1) : b.max_len;
 }
 
-// Few rows, as many as the registers of kv_few_k hold: a cache's codes are read once for all of them.
-bool few(const Batch& b, uint32_t D, uint32_t group) { return (uint64_t)b.max_q * group <= 16 * few_most(D); }
+// Few rows: up to 64, in tiles of 16 or 32. The workgroups of a group read the same codes, which one
+// L2 keeps for all of them.
+bool few(const Batch& b, uint32_t group) { return (uint64_t)b.max_q * group <= 64; }
 
-// Its workgroups: all that the device holds at once, or one for each unit of work where there
-// is less; one for each row of work where those are a unit long or the sequences too
-// many to add up their lengths in each workgroup. Where there are workgroups enough each takes a
-// part of one row of work: the beginning of another costs it about as long as 256 tokens do.
+// Their groups: all that the device holds at once, or one for each 256 tokens where there is less. Where
+// there are enough of them each takes a part of one row of work, for the beginning of another
+// costs it about as long as 256 tokens do. One for each row of work where those are short, or the
+// sequences too many to add up their lengths in each workgroup.
 FewPlan few_plan(const Cache& c, const Batch& b, uint32_t D, uint32_t group, uint32_t window) {
     FewPlan p = {};
-    p.sixteens = (uint32_t)ceil_div((uint64_t)b.max_q * group, 16);
-    const uint64_t units = ceil_div(longest_span(b, 16 * p.sixteens, window), kUnit), rows = (uint64_t)b.n_seq * c.heads;
-    if (units <= 1 || b.n_seq > kScan || b.n_seq * (units + 1) >= 0x7FFFFFFF) {
+    const uint32_t q_rows = b.max_q * group;
+    p.sixteens = q_rows <= 16 ? 1 : few_sixteens(D);
+    p.tiles = (uint32_t)ceil_div(q_rows, 16 * p.sixteens);
+    const uint64_t longest = longest_span(b, q_rows, window), rounds = ceil_div(longest, kRound);
+    const uint64_t rows = (uint64_t)b.n_seq * c.heads, fit = (uint64_t)cu_count() * few_waves(D) / p.tiles;
+    p.groups = (uint32_t)std::min<uint64_t>(fit, rows * rounds);
+    p.mode = 2 * rows <= p.groups ? FewPlan::kParts : FewPlan::kShares;
+    if (rounds <= (p.mode == FewPlan::kShares ? 4 : 1) || b.n_seq > kScan || b.n_seq * (ceil_div(longest, kTile) + 4) >= 0x7FFFFFFF) {
         p.mode = FewPlan::kRows;
-        p.wgs = (uint32_t)rows;
+        p.groups = (uint32_t)rows;
         return p;
     }
-    const uint64_t fit = (uint64_t)cu_count() * few_waves(D, p.sixteens);
-    p.wgs = (uint32_t)std::min<uint64_t>(fit, rows * units);
-    p.mode = 2 * rows <= p.wgs ? FewPlan::kParts : FewPlan::kShares;
-    p.start = p.mode == FewPlan::kShares && rows * units >= 4 * fit;
-    p.by_row = rows <= p.wgs;
-    p.cuts = p.by_row ? (uint32_t)rows : p.wgs;
+    p.start = p.mode == FewPlan::kShares && rows * rounds >= 4 * fit ? kRound / kTile : 0;
+    p.by_row = rows <= p.groups;
+    p.cuts = p.by_row ? (uint32_t)rows : p.groups;
     return p;
 }
 // Of any window: descriptors and slots of the widest launch.
 size_t few_ws_bytes(const Cache& c, const Batch& b, uint32_t D, uint32_t group) {
     const FewPlan p = few_plan(c, b, D, group, 0);
-    return p.mode == FewPlan::kRows ? 0 : (size_t)p.wgs * (sizeof(Cut) + 2 * 16 * p.sixteens * (D + 2) * 4);
+    return p.mode == FewPlan::kRows ? 0 : (size_t)p.groups * (sizeof(Cut) + 2 * p.tiles * 16 * p.sixteens * (D + 2) * 4);
 }
 
 uint64_t row_splits_wanted(const Cache& c, const Batch& b, const RowPlan& p) {
@@ -54,14 +57,14 @@ RowPlan row_plan(const Cache& c, const Batch& b, uint32_t D, uint32_t group, uin
     p.rows = rows <= 128 ? 128 : row_most(D);
     p.tiles = (uint32_t)ceil_div(rows, p.rows);
     const uint64_t longest = longest_span(b, p.rows, window);
-    p.chunk = (uint32_t)std::max<uint64_t>(ceil_div(ceil_div(longest, row_splits_wanted(c, b, p)), kTile) * kTile, kUnit);
+    p.chunk = (uint32_t)std::max<uint64_t>(ceil_div(ceil_div(longest, row_splits_wanted(c, b, p)), kTile) * kTile, kRound);
     p.splits = (uint32_t)ceil_div(longest, p.chunk);
     return p;
 }
-// Of any window: a split has kUnit tokens at least.
+// Of any window: a split has kRound tokens at least.
 size_t row_ws_bytes(const Cache& c, const Batch& b, uint32_t group, uint32_t D) {
     const RowPlan p = row_plan(c, b, D, group, 0);
-    const uint64_t splits = std::min(row_splits_wanted(c, b, p), ceil_div(b.max_len, kUnit));
+    const uint64_t splits = std::min(row_splits_wanted(c, b, p), ceil_div(b.max_len, kRound));
     return splits > 1 ? (size_t)b.n_seq * splits * p.tiles * c.heads * p.rows * (D + 2) * 4 : 0;
 }
 
@@ -69,7 +72,7 @@ size_t row_ws_bytes(const Cache& c, const Batch& b, uint32_t group, uint32_t D) 
 }  // namespace kv
 
 size_t kv_attn_ws_bytes(const kv::Cache& c, const kv::Batch& b, uint32_t D, uint32_t group) {
-    const size_t n = kv::few(b, D, group) ? kv::few_ws_bytes(c, b, D, group) : kv::row_ws_bytes(c, b, group, D);
+    const size_t n = kv::few(b, group) ? kv::few_ws_bytes(c, b, D, group) : kv::row_ws_bytes(c, b, group, D);
     return n > 256 ? (n + 255) / 256 * 256 : 256;
 }
 
@@ -82,7 +85,7 @@ hipError_t launch_kv_attn(const kv::Cache& c, const kv::Batch& b, uint32_t D, in
     float* const w = static_cast<float*>(ws);
     return kv::by_dim(D, type, [&](auto d, auto) {
         constexpr int N = decltype(d)::value;
-        return kv::few(b, D, a.group)
+        return kv::few(b, a.group)
                    ? kv::AttnKernels<N>::few(type, c, b, a, kv::few_plan(c, b, D, a.group, a.window), Q, O, bf, w, s)
                    : kv::AttnKernels<N>::rows(type, c, b, a, kv::row_plan(c, b, D, a.group, a.window), Q, O, bf, w, s);
     });

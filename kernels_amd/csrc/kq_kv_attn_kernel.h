@@ -20,7 +20,7 @@ namespace kq {
 namespace kv {
 
 constexpr int kTile = 64;      // tokens a wave takes at a time
-constexpr int kUnit = 256;     // tokens of a unit of work: a tile of each of four waves
+constexpr int kRound = 256;    // ... and four waves do
 constexpr int kLift = 14;      // probabilities are scaled by 2^14: the fp16 ones stay normal down to 2^-28 of the largest
 constexpr int kIds = 4096;     // page ids that a workgroup holds at a time
 constexpr int kScan = 1024;    // most sequences whose lengths a workgroup adds up
@@ -149,18 +149,18 @@ __device__ __forceinline__ float load_q(const Rows& Q, bool there, int row, uint
 
 // ---- the work of a call of few rows, shared out evenly
 //
-// A row of work (a sequence and head) is ceil(tokens / kUnit) units, and where p.start is 1 one more at
-// its beginning, the price of beginning it: asking for its length, page ids, query and first codes one
-// after the other takes about as long as 256 tokens.
-// kParts: rows of work are cut into parts of at most c units, with the smallest c that gives no more parts
-// than workgroups (or near it). kShares: all rows' units in order of sequence and head are cut
-// into equal shares, one for each workgroup, however the lengths differ.
-// A row of work that a cut goes through leaves partial sums: a workgroup's first piece, if it continues a
-// row, in slot 2k, a last piece that begins a row and does not end it in slot 2k + 1 (k the workgroup);
+// A row of work (a sequence and head) is ceil(tokens / kTile) units, and p.start more at its beginning, the
+// price of beginning it: asking for its length, page ids, query and first codes one after
+// the other takes about as long as kRound tokens.
+// kParts: rows of work are cut into parts of at most c units (a round's, at least), with the smallest c that
+// gives no more parts than groups (or near it). kShares: all rows' units in order of sequence and head are cut
+// into equal shares, one for each group, however the lengths differ.
+// A row of work that a cut goes through leaves partial sums: a group's first piece, if it continues a
+// row, in slot 2k, a last piece that begins a row and does not end it in slot 2k + 1 (k the group);
 // kv_join_k adds the row's parts up.
 __device__ __forceinline__ int units_of(const Seq& s, const Attn& a, int rows, int start) {
     const Span v = span_of(s, a, 0, rows);
-    return s.n == 0 ? 0 : max((v.hi - v.lo + kUnit - 1) / kUnit, 1) + start;
+    return s.n == 0 ? 0 : max((v.hi - v.lo + kTile - 1) / kTile, 1) + start;
 }
 
 struct Share {
@@ -171,7 +171,7 @@ struct Share {
     int parts;       // of its row of work (kParts)
     uint64_t at;     // of the first unit, among all (kShares)
     uint64_t total;
-    uint32_t wgs;    // shares
+    uint32_t groups; // that have some
 };
 
 __device__ __forceinline__ int prefix64(int v, int lane) {  // inclusive sum over the wave
@@ -183,14 +183,16 @@ __device__ __forceinline__ int prefix64(int v, int lane) {  // inclusive sum ove
     return v;
 }
 
-// What this workgroup does; each wave works it out for itself from the units of all sequences.
+// What group k does; each wave works it out for itself from the units of all sequences.
 // lds: kScan ints.
-__device__ inline Share share_of(const Cache& c, const Batch& b, const Attn& a, const FewPlan& p, int rows, int* lds) {
+__device__ inline Share share_of(const Cache& c, const Batch& b, const Attn& a, const FewPlan& p, uint32_t k, int rows,
+                                 int* lds) {
     const int lane = threadIdx.x & 63, n = (int)b.n_seq;
-    Share w = {0, 0, 0, 0, 1, 0, 0, gridDim.x};
+    Share w = {0, 0, 0, 0, 1, 0, 0, p.groups};
+    if (k >= p.groups) return w;
     if (p.mode == FewPlan::kRows) {
-        w.seq = (int)(blockIdx.x / c.heads);
-        w.head = blockIdx.x % c.heads;
+        w.seq = (int)(k / c.heads);
+        w.head = k % c.heads;
         w.units = units_of(sequence(b, c.page_log2, w.seq), a, rows, (int)p.start);
         return w;
     }
@@ -230,8 +232,8 @@ __device__ inline Share share_of(const Cache& c, const Batch& b, const Attn& a, 
     int u = 0;
     if (p.mode == FewPlan::kParts) {
         // c from the mean on; the last is enough for any lengths: sum ceil(u / c) <= sum u / c + rows of work
-        const uint32_t most = gridDim.x / c.heads;
-        uint32_t size = (uint32_t)((all + most - 1) / most), count = 0;
+        const uint32_t most = p.groups / c.heads;
+        uint32_t size = max((uint32_t)((all + most - 1) / most), (uint32_t)(kRound / kTile)), count = 0;
         for (int tries = 0; tries < 4; ++tries, ++size) {
             count = (uint32_t)sum([&](int v) { return (int)(((uint32_t)v + size - 1) / size); });
             if (count <= most) break;
@@ -240,10 +242,10 @@ __device__ inline Share share_of(const Cache& c, const Batch& b, const Attn& a, 
             size = max(size, (uint32_t)((all + most - n - 1) / (most - n)));
             count = (uint32_t)sum([&](int v) { return (int)(((uint32_t)v + size - 1) / size); });
         }
-        if (blockIdx.x >= count * c.heads) return w;
+        if (k >= count * c.heads) return w;
         // parts in order of head, then sequence
-        w.head = blockIdx.x / count;
-        uint32_t x = blockIdx.x % count;
+        w.head = k / count;
+        uint32_t x = k % count;
         w.seq = find(x, u, [&](int v) { return (int)(((uint32_t)v + size - 1) / size); });
         w.parts = (int)(((uint32_t)u + size - 1) / size);
         w.unit = (int)((uint64_t)x * u / w.parts);
@@ -251,10 +253,10 @@ __device__ inline Share share_of(const Cache& c, const Batch& b, const Attn& a, 
         return w;
     }
     w.total = all * c.heads;
-    if (w.total < w.wgs) w.wgs = (uint32_t)w.total;
-    if (blockIdx.x >= w.wgs) return w;
-    w.at = w.total * blockIdx.x / w.wgs;
-    w.units = (int)(w.total * (blockIdx.x + 1) / w.wgs - w.at);
+    if (w.total < w.groups) w.groups = (uint32_t)w.total;
+    if (k >= w.groups) return w;
+    w.at = w.total * k / w.groups;
+    w.units = (int)(w.total * (k + 1) / w.groups - w.at);
     // in order of sequence, then head
     uint32_t x = (uint32_t)(w.at / c.heads);
     const uint32_t odd = (uint32_t)(w.at % c.heads);
@@ -265,25 +267,25 @@ __device__ inline Share share_of(const Cache& c, const Batch& b, const Attn& a, 
     return w;
 }
 
-// A row of work that is cut: the workgroup of its first part, and how many parts (0: it is whole).
-// By row of work where those are no more than the workgroups, else by workgroup.
+// A row of work that is cut: the group of its first part, and how many parts (0: it is whole).
+// By row of work where those are no more than the groups, else by group.
 struct Cut {
     int seq, head, first, parts;
 };
-// The partial results of slot i: [16 R][D] sums, then [16 R] (m, l).
+// The partial results of slot i and row tile t: [16 R][D] sums, then [16 R] (m, l).
 template <int D, int R>
-__device__ __forceinline__ float* slot_of(float* ws, uint32_t cuts, uint32_t i) {
-    return ws + cuts * 4 + (uint64_t)i * (16 * R * (D + 2));
+__device__ __forceinline__ float* slot_of(float* ws, const FewPlan& p, uint32_t i, uint32_t t) {
+    return ws + p.cuts * 4 + ((uint64_t)i * p.tiles + t) * (16 * R * (D + 2));
 }
 
-// Few rows: at most 16 R (tokens x heads of a group) of a sequence and head. Four waves take 64 tokens
+// Few rows (tokens x heads of a group) of a sequence and head, 16 R a workgroup. Four waves take 64 tokens
 // of a piece in turn and join their sums at its end. What bounds it is the stream of codes:
 // a wave asks for its next keys as soon as the present ones are multiplied, and for its
 // next values after the product with the present ones, so that most of 16 KiB a wave
 // (128 wide) is always on its way.
 template <int D, int TYPE, int R>
-__global__ __launch_bounds__(256, few_waves(D, R)) void kv_few_k(Cache c, Batch b, Attn a, FewPlan p, Rows Q, Rows O,
-                                                                 int bf, float* ws) {
+__global__ __launch_bounds__(256, few_waves(D)) void kv_few_k(Cache c, Batch b, Attn a, FewPlan p, Rows Q, Rows O, int bf,
+                                                              float* ws) {
     constexpr int C64 = D / 64, kHalf = D % 64 ? 1 : 0;  // 64-column pieces of a key, and a 32-column one
     constexpr int kPad = D + 4;
     __shared__ __attribute__((aligned(16))) float o_lds[4 * 16 * R * kPad];
@@ -293,9 +295,12 @@ __global__ __launch_bounds__(256, few_waves(D, R)) void kv_few_k(Cache c, Batch 
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 15, g = lane >> 4;
     const uint32_t q_heads = c.heads * a.group;
 
-    const Share share = share_of(c, b, a, p, 16 * R, ids);
+    // the workgroups of a group side by side in one of eight XCDs: 8 groups' first tiles, their second, ...
+    const uint32_t group = blockIdx.x / (8 * p.tiles) * 8 + blockIdx.x % 8, tile = blockIdx.x / 8 % p.tiles;
+    const int all_rows = (int)(b.max_q * a.group), row0 = (int)tile * 16 * R;
+    const Share share = share_of(c, b, a, p, group, all_rows, ids);
     Cut* const cuts = reinterpret_cast<Cut*>(ws);
-    if (p.mode == FewPlan::kShares && !p.by_row && tid == 0) cuts[blockIdx.x].parts = 0;
+    if (p.mode == FewPlan::kShares && !p.by_row && group < p.groups && tile == 0 && tid == 0) cuts[group].parts = 0;
     int left = share.units, unit = share.unit;
     int seq = share.seq;
     uint32_t h = share.head;
@@ -304,229 +309,231 @@ __global__ __launch_bounds__(256, few_waves(D, R)) void kv_few_k(Cache c, Batch 
         seq = __builtin_amdgcn_readfirstlane(seq);
         h = (uint32_t)__builtin_amdgcn_readfirstlane((int)h);
         const Seq s = sequence(b, c.page_log2, (uint32_t)seq);
-        const Span sp = span_of(s, a, 0, 16 * R);
-        const int units = units_of(s, a, 16 * R, (int)p.start), mine = min(left, units - unit);
+        const Span sp = span_of(s, a, 0, all_rows);  // the same for all row tiles
+        const int units = units_of(s, a, all_rows, (int)p.start), mine = min(left, units - unit);
         if (mine <= 0) {  // a sequence without rows
             ++seq;
             continue;
         }
-        const int rows = s.n * (int)a.group, tail = (int)p.start;
-        const int lo = sp.lo + max(unit - tail, 0) * kUnit;
-        const int hi = (int)min((int64_t)sp.hi, (int64_t)sp.lo + (int64_t)(unit + mine - tail) * kUnit);
+        const int rows = s.n * (int)a.group - row0, tail = (int)p.start;  // from this tile on
+        const int lo = sp.lo + max(unit - tail, 0) * kTile;
+        const int hi = (int)min((int64_t)sp.hi, (int64_t)sp.lo + (int64_t)max(unit + mine - tail, 0) * kTile);
         const int32_t* const table = b.pages + (uint64_t)seq * b.max_pages;
 
-        // this lane's row of each sixteen
-        f16x8 q[R][D / 32];
-        float q_scale[R], m[R], l[R];  // m, l: of the row; l: this lane's tokens alone
-        int sees_lo[R], sees_hi[R];
-        f32x4 o[R][D / 16];
-#pragma unroll
-        for (int k = 0; k < R; ++k) {
-            const int row = 16 * k + r, tok = row / (int)a.group;
-            const bool there = row < rows;
-            const int pos = s.len - s.n + tok;
-            sees_hi[k] = there ? min(a.causal ? pos + 1 : s.len, hi) : 0;
-            sees_lo[k] = a.window ? pos + 1 - (int)a.window : 0;
-            q_scale[k] = fabsf(a.scale_log2) * load_q<D>(Q, there, s.row0 + tok, h * a.group + (uint32_t)(row % (int)a.group),
-                                                         g, bf, a.scale_log2, q[k]);
-            m[k] = kLowest;
-            l[k] = 0.0f;
-#pragma unroll
-            for (int i = 0; i < D / 16; ++i) o[k][i] = f32x4{0, 0, 0, 0};
-        }
-
-        int page0 = 0;
-        u32x4 kw[4 * C64 + 1], vw[D / 16];
-        u32x2 kx[4];  // the 32-column pieces
-        int ke = 0, ve = 0, pv = 0;
-        // Codes of the wave's 64 tokens from t0 on: the lane's row of K operand t, and its columns of V
-        // with the exponents of its 16 tokens.
-        auto page_at = [&](int t) { return ids[(min(t, hi - 1) >> c.page_log2) - page0]; };
-        auto load_k = [&](int t0) {
-            const int tk = t0 + 16 * (r >> 2);
-            const uint8_t* const kp = c.k + code_offset(c, D, max(page_at(tk), 0), h, tk) + (r & 3) * D;
-#pragma unroll
-            for (int t = 0; t < 4; ++t) {
-#pragma unroll
-                for (int i = 0; i < C64; ++i) kw[t * C64 + i] = ldg_nt(reinterpret_cast<const u32x4*>(kp + t * 4 * D + i * 64 + g * 16));
-                if constexpr (kHalf) kx[t] = ldg_nt(reinterpret_cast<const u32x2*>(kp + t * 4 * D + C64 * 64 + g * 8));
-            }
-        };
-        auto load_v = [&](int t0) {
-            const int tv = t0 + 16 * g;
-            pv = page_at(tv);
-            const uint64_t eo = exp_offset(c, max(pv, 0), h, tv);
-            ke = c.k_exp[eo];
-            ve = c.v_exp[eo];
-            const uint8_t* const vp = c.v + code_offset(c, D, max(pv, 0), h, tv) + r * 16;
-#pragma unroll
-            for (int i = 0; i < D / 16; ++i) vw[i] = ldg_nt(reinterpret_cast<const u32x4*>(vp + i * 256));
-        };
-        auto step = [&](int t0, auto more) {
-            f32x4 st[R][4];
-#pragma unroll
-            for (int t = 0; t < 4; ++t) {
-#pragma unroll
-                for (int k = 0; k < R; ++k) st[k][t] = f32x4{0, 0, 0, 0};
-#pragma unroll
-                for (int i = 0; i < C64; ++i) {
-                    const u32x4 w = kw[t * C64 + i];
-                    const f16x8 x = codes_f16x8<TYPE>(w.x, w.y), y = codes_f16x8<TYPE>(w.z, w.w);
-#pragma unroll
-                    for (int k = 0; k < R; ++k) {
-                        st[k][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, q[k][2 * i], st[k][t], 0, 0, 0);
-                        st[k][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, q[k][2 * i + 1], st[k][t], 0, 0, 0);
-                    }
-                }
-                if constexpr (kHalf) {
-                    const f16x8 x = codes_f16x8<TYPE>(kx[t].x, kx[t].y);
-#pragma unroll
-                    for (int k = 0; k < R; ++k)
-                        st[k][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, q[k][2 * C64], st[k][t], 0, 0, 0);
-                }
-            }
-            __builtin_amdgcn_sched_barrier(0);  // into the registers just read, not beside them
-            if constexpr (decltype(more)::value) load_k(t0 + kUnit);
-            __builtin_amdgcn_sched_barrier(0);
-
-            const int tv = t0 + 16 * g;
-            const float k_scale = pow2f(min(max(ke - 127, -126), 127)), un_v = pow2f(min(max(127 - ve, -126), 127));
-            f16x8 w[R][2];
+        if (rows > 0) {
+            // this lane's row of each sixteen
+            f16x8 q[R][D / 32];
+            float q_scale[R], m[R], l[R];  // m, l: of the row; l: this lane's tokens alone
+            int sees_lo[R], sees_hi[R];
+            f32x4 o[R][D / 16];
 #pragma unroll
             for (int k = 0; k < R; ++k) {
-                // t = f s + e with f >= 0: the largest t is the largest s's
-                float f = q_scale[k] * k_scale, e = (float)(ve - 127);
-                // tokens in sight of the row, of the lane's 16
-                const int from = sees_lo[k] - tv, to = pv < 0 ? 0 : sees_hi[k] - tv;
-                if (!__all(from <= 0 && to >= 16)) {
-                    // only the few tiles that need it: nothing of this is computed ahead of the branch
-                    int first = from;
-                    asm volatile("" : "+v"(first));
+                const int row = row0 + 16 * k + r, tok = row / (int)a.group;
+                const bool there = 16 * k + r < rows;
+                const int pos = s.len - s.n + tok;
+                sees_hi[k] = there ? min(a.causal ? pos + 1 : s.len, hi) : 0;
+                sees_lo[k] = a.window ? pos + 1 - (int)a.window : 0;
+                q_scale[k] = fabsf(a.scale_log2) * load_q<D>(Q, there, s.row0 + tok, h * a.group + (uint32_t)(row % (int)a.group),
+                                                             g, bf, a.scale_log2, q[k]);
+                m[k] = kLowest;
+                l[k] = 0.0f;
 #pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        st[k][i / 4][i % 4] = i < first || i >= to ? -__builtin_inff() : __builtin_fmaf(st[k][i / 4][i % 4], f, e);
-                    f = 1.0f;
-                    e = 0.0f;
-                }
-                float top = st[k][0][0];
-#pragma unroll
-                for (int i = 1; i < 16; ++i) top = fmaxf(top, st[k][i / 4][i % 4]);
-                top = across_rows_maxf(fmaxf(m[k], __builtin_fmaf(top, f, e)));
-                if (__any(top > m[k])) {
-                    const float fade = __builtin_amdgcn_exp2f(m[k] - top);
-                    m[k] = top;
-                    l[k] *= fade;
-#pragma unroll
-                    for (int i = 0; i < D / 16; ++i) o[k][i] *= fade;
-                }
-                const float down = e - (m[k] - kLift);
-                float sum = 0.0f;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(st[k][i / 4][i % 4], f, down));
-                    sum += y;
-                    w[k][i / 8][i % 8] = (_Float16)y;
-                }
-                l[k] += sum * un_v;
+                for (int i = 0; i < D / 16; ++i) o[k][i] = f32x4{0, 0, 0, 0};
             }
-            if (t0 + kTile > hi || __any(pv < 0)) {
-                // bytes of tokens that no length covers may hold anything, NaN among it
-                const int valid = pv < 0 ? 0 : min(max(hi - tv, 0), 16);
+
+            int page0 = 0;
+            u32x4 kw[4 * C64 + 1], vw[D / 16];
+            u32x2 kx[4];  // the 32-column pieces
+            int ke = 0, ve = 0, pv = 0;
+            // Codes of the wave's 64 tokens from t0 on: the lane's row of K operand t, and its columns of V
+            // with the exponents of its 16 tokens.
+            auto page_at = [&](int t) { return ids[(min(t, hi - 1) >> c.page_log2) - page0]; };
+            auto load_k = [&](int t0) {
+                const int tk = t0 + 16 * (r >> 2);
+                const uint8_t* const kp = c.k + code_offset(c, D, max(page_at(tk), 0), h, tk) + (r & 3) * D;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int n = min(max(valid - 4 * j, 0), 4);
-                    const uint32_t keep = n == 4 ? 0xFFFFFFFFu : (1u << 8 * n) - 1;
+                for (int t = 0; t < 4; ++t) {
 #pragma unroll
-                    for (int i = 0; i < D / 16; ++i) vw[i][j] &= keep;
+                    for (int i = 0; i < C64; ++i) kw[t * C64 + i] = ldg_nt(reinterpret_cast<const u32x4*>(kp + t * 4 * D + i * 64 + g * 16));
+                    if constexpr (kHalf) kx[t] = ldg_nt(reinterpret_cast<const u32x2*>(kp + t * 4 * D + C64 * 64 + g * 8));
                 }
-            }
+            };
+            auto load_v = [&](int t0) {
+                const int tv = t0 + 16 * g;
+                pv = page_at(tv);
+                const uint64_t eo = exp_offset(c, max(pv, 0), h, tv);
+                ke = c.k_exp[eo];
+                ve = c.v_exp[eo];
+                const uint8_t* const vp = c.v + code_offset(c, D, max(pv, 0), h, tv) + r * 16;
 #pragma unroll
-            for (int i = 0; i < D / 16; ++i) {
-                const f16x8 x = codes_f16x8<TYPE>(vw[i].x, vw[i].y), y = codes_f16x8<TYPE>(vw[i].z, vw[i].w);
+                for (int i = 0; i < D / 16; ++i) vw[i] = ldg_nt(reinterpret_cast<const u32x4*>(vp + i * 256));
+            };
+            auto step = [&](int t0, auto more) {
+                f32x4 st[R][4];
+#pragma unroll
+                for (int t = 0; t < 4; ++t) {
+#pragma unroll
+                    for (int k = 0; k < R; ++k) st[k][t] = f32x4{0, 0, 0, 0};
+#pragma unroll
+                    for (int i = 0; i < C64; ++i) {
+                        const u32x4 w = kw[t * C64 + i];
+                        const f16x8 x = codes_f16x8<TYPE>(w.x, w.y), y = codes_f16x8<TYPE>(w.z, w.w);
+#pragma unroll
+                        for (int k = 0; k < R; ++k) {
+                            st[k][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, q[k][2 * i], st[k][t], 0, 0, 0);
+                            st[k][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, q[k][2 * i + 1], st[k][t], 0, 0, 0);
+                        }
+                    }
+                    if constexpr (kHalf) {
+                        const f16x8 x = codes_f16x8<TYPE>(kx[t].x, kx[t].y);
+#pragma unroll
+                        for (int k = 0; k < R; ++k)
+                            st[k][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, q[k][2 * C64], st[k][t], 0, 0, 0);
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);  // into the registers just read, not beside them
+                if constexpr (decltype(more)::value) load_k(t0 + kRound);
+                __builtin_amdgcn_sched_barrier(0);
+
+                const int tv = t0 + 16 * g;
+                const float k_scale = pow2f(min(max(ke - 127, -126), 127)), un_v = pow2f(min(max(127 - ve, -126), 127));
+                f16x8 w[R][2];
 #pragma unroll
                 for (int k = 0; k < R; ++k) {
-                    o[k][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, w[k][0], o[k][i], 0, 0, 0);
-                    o[k][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, w[k][1], o[k][i], 0, 0, 0);
+                    // t = f s + e with f >= 0: the largest t is the largest s's
+                    float f = q_scale[k] * k_scale, e = (float)(ve - 127);
+                    // tokens in sight of the row, of the lane's 16
+                    const int from = sees_lo[k] - tv, to = pv < 0 ? 0 : sees_hi[k] - tv;
+                    if (!__all(from <= 0 && to >= 16)) {
+                        // only the few tiles that need it: nothing of this is computed ahead of the branch
+                        int first = from;
+                        asm volatile("" : "+v"(first));
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            st[k][i / 4][i % 4] = i < first || i >= to ? -__builtin_inff() : __builtin_fmaf(st[k][i / 4][i % 4], f, e);
+                        f = 1.0f;
+                        e = 0.0f;
+                    }
+                    float top = st[k][0][0];
+#pragma unroll
+                    for (int i = 1; i < 16; ++i) top = fmaxf(top, st[k][i / 4][i % 4]);
+                    top = across_rows_maxf(fmaxf(m[k], __builtin_fmaf(top, f, e)));
+                    if (__any(top > m[k])) {
+                        const float fade = __builtin_amdgcn_exp2f(m[k] - top);
+                        m[k] = top;
+                        l[k] *= fade;
+#pragma unroll
+                        for (int i = 0; i < D / 16; ++i) o[k][i] *= fade;
+                    }
+                    const float down = e - (m[k] - kLift);
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(st[k][i / 4][i % 4], f, down));
+                        sum += y;
+                        w[k][i / 8][i % 8] = (_Float16)y;
+                    }
+                    l[k] += sum * un_v;
+                }
+                if (t0 + kTile > hi || __any(pv < 0)) {
+                    // bytes of tokens that no length covers may hold anything, NaN among it
+                    const int valid = pv < 0 ? 0 : min(max(hi - tv, 0), 16);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int n = min(max(valid - 4 * j, 0), 4);
+                        const uint32_t keep = n == 4 ? 0xFFFFFFFFu : (1u << 8 * n) - 1;
+#pragma unroll
+                        for (int i = 0; i < D / 16; ++i) vw[i][j] &= keep;
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i) {
+                    const f16x8 x = codes_f16x8<TYPE>(vw[i].x, vw[i].y), y = codes_f16x8<TYPE>(vw[i].z, vw[i].w);
+#pragma unroll
+                    for (int k = 0; k < R; ++k) {
+                        o[k][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, w[k][0], o[k][i], 0, 0, 0);
+                        o[k][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, w[k][1], o[k][i], 0, 0, 0);
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                if constexpr (decltype(more)::value) load_v(t0 + kRound);
+                __builtin_amdgcn_sched_barrier(0);
+            };
+            // the piece, or as much of it as there is room for page ids
+            const int most = ((kIds - 1) << c.page_log2) & ~(kRound - 1);
+            for (int from = lo; from < hi;) {
+                const int to = hi - from > most ? from + most : hi;
+                __syncthreads();
+                page0 = from >> c.page_log2;
+                const int pages = ((to - 1) >> c.page_log2) - page0 + 1;
+                for (int i = tid; i < pages; i += 256) {
+                    const int v = table[page0 + i];
+                    ids[i] = (uint32_t)v < c.n_pages ? v : -1;
+                }
+                __syncthreads();
+                int t0 = from + wave * kTile;
+                if (t0 < to) {
+                    load_k(t0);
+                    load_v(t0);
+                    for (; t0 < to - kRound; t0 += kRound) step(t0, Int<1>());
+                    step(t0, Int<0>());
+                }
+                from = to;
+            }
+
+            // join the waves
+            const bool whole = mine == units;
+            float* const part = slot_of<D, R>(ws, p, 2 * group + (unit == 0), tile);
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < R; ++k) {
+                l[k] = across_rows_sum(l[k]);
+                if (g == 0) {
+                    m_lds[wave][16 * k + r] = m[k];
+                    l_lds[wave][16 * k + r] = l[k];
                 }
             }
-            __builtin_amdgcn_sched_barrier(0);
-            if constexpr (decltype(more)::value) load_v(t0 + kUnit);
-            __builtin_amdgcn_sched_barrier(0);
-        };
-        // the piece, or as much of it as there is room for page ids
-        const int most = ((kIds - 1) << c.page_log2) & ~(kUnit - 1);
-        for (int from = lo; from < hi;) {
-            const int to = hi - from > most ? from + most : hi;
             __syncthreads();
-            page0 = from >> c.page_log2;
-            const int pages = ((to - 1) >> c.page_log2) - page0 + 1;
-            for (int i = tid; i < pages; i += 256) {
-                const int v = table[page0 + i];
-                ids[i] = (uint32_t)v < c.n_pages ? v : -1;
+#pragma unroll
+            for (int k = 0; k < R; ++k) {
+                float top = m_lds[0][16 * k + r];
+#pragma unroll
+                for (int w = 1; w < 4; ++w) top = fmaxf(top, m_lds[w][16 * k + r]);
+                const float fade = __builtin_amdgcn_exp2f(m[k] - top);
+                float* const to = o_lds + ((wave * R + k) * 16 + r) * kPad;
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i) *reinterpret_cast<f32x4*>(to + i * 16 + g * 4) = o[k][i] * fade;
             }
             __syncthreads();
-            int t0 = from + wave * kTile;
-            if (t0 < to) {
-                load_k(t0);
-                load_v(t0);
-                for (; t0 < to - kUnit; t0 += kUnit) step(t0, Int<1>());
-                step(t0, Int<0>());
+            for (int i = tid; i < min(rows, 16 * R) * (D / 4); i += 256) {
+                const int row = i / (D / 4), d = i % (D / 4) * 4;
+                f32x4 y = *reinterpret_cast<const f32x4*>(o_lds + row * kPad + d);
+                float best = m_lds[0][row];
+#pragma unroll
+                for (int w = 1; w < 4; ++w) {
+                    y += *reinterpret_cast<const f32x4*>(o_lds + (w * 16 * R + row) * kPad + d);
+                    best = fmaxf(best, m_lds[w][row]);
+                }
+                float sum = 0.0f;
+#pragma unroll
+                for (int w = 0; w < 4; ++w) sum += l_lds[w][row] * __builtin_amdgcn_exp2f(m_lds[w][row] - best);
+                if (whole) {
+                    const uint32_t head = h * a.group + (uint32_t)((row0 + row) % (int)a.group);
+                    const int out = s.row0 + (row0 + row) / (int)a.group;
+                    store4(O, out, head, d, y * finish(a, best, sum, out, head, q_heads, d == 0), bf);
+                } else {
+                    *reinterpret_cast<f32x4*>(part + row * D + d) = y;
+                    if (d == 0) *reinterpret_cast<float2*>(part + 16 * R * D + row * 2) = make_float2(best, sum);
+                }
             }
-            from = to;
+            __syncthreads();
         }
-
-        // join the waves
-        const bool whole = mine == units;
-        float* const part = slot_of<D, R>(ws, p.cuts, 2 * blockIdx.x + (unit == 0));
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < R; ++k) {
-            l[k] = across_rows_sum(l[k]);
-            if (g == 0) {
-                m_lds[wave][16 * k + r] = m[k];
-                l_lds[wave][16 * k + r] = l[k];
-            }
-        }
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < R; ++k) {
-            float top = m_lds[0][16 * k + r];
-#pragma unroll
-            for (int w = 1; w < 4; ++w) top = fmaxf(top, m_lds[w][16 * k + r]);
-            const float fade = __builtin_amdgcn_exp2f(m[k] - top);
-            float* const to = o_lds + ((wave * R + k) * 16 + r) * kPad;
-#pragma unroll
-            for (int i = 0; i < D / 16; ++i) *reinterpret_cast<f32x4*>(to + i * 16 + g * 4) = o[k][i] * fade;
-        }
-        __syncthreads();
-        for (int i = tid; i < rows * (D / 4); i += 256) {
-            const int row = i / (D / 4), d = i % (D / 4) * 4;
-            f32x4 y = *reinterpret_cast<const f32x4*>(o_lds + row * kPad + d);
-            float best = m_lds[0][row];
-#pragma unroll
-            for (int w = 1; w < 4; ++w) {
-                y += *reinterpret_cast<const f32x4*>(o_lds + (w * 16 * R + row) * kPad + d);
-                best = fmaxf(best, m_lds[w][row]);
-            }
-            float sum = 0.0f;
-#pragma unroll
-            for (int w = 0; w < 4; ++w) sum += l_lds[w][row] * __builtin_amdgcn_exp2f(m_lds[w][row] - best);
-            if (whole) {
-                const uint32_t head = h * a.group + (uint32_t)(row % (int)a.group);
-                const int out = s.row0 + row / (int)a.group;
-                store4(O, out, head, d, y * finish(a, best, sum, out, head, q_heads, d == 0), bf);
-            } else {
-                *reinterpret_cast<f32x4*>(part + row * D + d) = y;
-                if (d == 0) *reinterpret_cast<float2*>(part + 16 * R * D + row * 2) = make_float2(best, sum);
-            }
-        }
-        if (unit == 0 && tid == 0 && p.mode != FewPlan::kRows && (p.by_row || !whole)) {
+        if (unit == 0 && tile == 0 && tid == 0 && p.mode != FewPlan::kRows && (p.by_row || mine < units)) {
             int parts = share.parts;
-            if (p.mode == FewPlan::kShares)  // the last unit's workgroup: shares begin at floor(k total / wgs)
-                parts = (int)(((at + (uint64_t)units) * share.wgs - 1) / share.total) - (int)blockIdx.x + 1;
-            cuts[p.by_row ? (uint32_t)seq * c.heads + h : blockIdx.x] = {seq, (int)h, (int)blockIdx.x, whole ? 0 : parts};
+            if (p.mode == FewPlan::kShares)  // the last unit's group: shares begin at floor(k total / groups)
+                parts = (int)(((at + (uint64_t)units) * share.groups - 1) / share.total) - (int)group + 1;
+            cuts[p.by_row ? (uint32_t)seq * c.heads + h : group] = {seq, (int)h, (int)group, mine == units ? 0 : parts};
         }
-        __syncthreads();
         left -= mine;
         at += (uint64_t)mine;
         unit = 0;
@@ -605,7 +612,7 @@ __device__ __forceinline__ void join_row(const Attn& a, int n, Sums sums, Ml ml_
             to[k * 64 + lane] = (uint16_t)(bf ? pair16<1>(o[k] * y, 0.0f) : pair16<0>(o[k] * y, 0.0f));
 }
 
-// The cut rows of work of kv_few_k, one of their 16 R (token, head) rows for each W waves.
+// The cut rows of work of kv_few_k, one of their (token, head) rows for each W waves.
 template <int D, int R, int W>
 __global__ __launch_bounds__(256) void kv_join_k(Cache c, Batch b, Attn a, FewPlan p, Rows O, int bf, float* ws) {
     __shared__ float lds[W > 1 ? W * (D + 2) : 1];
@@ -618,21 +625,22 @@ __global__ __launch_bounds__(256) void kv_join_k(Cache c, Batch b, Attn a, FewPl
     const Seq s = p.by_row ? own : sequence(b, c.page_log2, (uint32_t)cut.seq);
     if (row >= s.n * (int)a.group) return;
     // part 0 begins the row of work, the others continue it: slots 2k + 1, then 2 (k + i)
-    auto part = [&](int i) { return slot_of<D, R>(ws, p.cuts, 2 * (cut.first + i) + (i == 0)); };
-    join_row<D, W>(a, cut.parts, [&](int i) { return part(i) + row * D; },
-                   [&](int i) { return part(i) + 16 * R * D + row * 2; }, lds, O, bf, s.row0 + row / (int)a.group,
+    const int in = row % (16 * R);
+    auto part = [&](int i) { return slot_of<D, R>(ws, p, 2 * (cut.first + i) + (i == 0), (uint32_t)(row / (16 * R))); };
+    join_row<D, W>(a, cut.parts, [&](int i) { return part(i) + in * D; },
+                   [&](int i) { return part(i) + 16 * R * D + in * 2; }, lds, O, bf, s.row0 + row / (int)a.group,
                    (uint32_t)cut.head * a.group + (uint32_t)(row % (int)a.group), c.heads * a.group);
 }
 
 template <int D, int TYPE, int R>
 hipError_t few_r(const Cache& c, const Batch& b, const Attn& a, const FewPlan& p, const Rows& Q, const Rows& O, bool bf,
                  float* ws, hipStream_t s) {
-    kv_few_k<D, TYPE, R><<<p.wgs, 256, 0, s>>>(c, b, a, p, Q, O, bf, ws);
+    kv_few_k<D, TYPE, R><<<(p.groups + 7) / 8 * 8 * p.tiles, 256, 0, s>>>(c, b, a, p, Q, O, bf, ws);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.mode == FewPlan::kRows) return e;
     const uint32_t rows = b.max_q * a.group;
     // many parts a row of work: four waves for each of its rows
-    if (p.wgs >= 8 * p.cuts) kv_join_k<D, R, 4><<<dim3(p.cuts, rows), 256, 0, s>>>(c, b, a, p, O, bf, ws);
+    if (p.groups >= 8 * p.cuts) kv_join_k<D, R, 4><<<dim3(p.cuts, rows), 256, 0, s>>>(c, b, a, p, O, bf, ws);
     else kv_join_k<D, R, 1><<<dim3(p.cuts, (rows + 3) / 4), 256, 0, s>>>(c, b, a, p, O, bf, ws);
     return hipGetLastError();
 }
@@ -640,11 +648,7 @@ hipError_t few_r(const Cache& c, const Batch& b, const Attn& a, const FewPlan& p
 template <int D, int TYPE>
 hipError_t few_d(const Cache& c, const Batch& b, const Attn& a, const FewPlan& p, const Rows& Q, const Rows& O, bool bf,
                  float* ws, hipStream_t s) {
-    if constexpr (few_most(D) > 3)
-        if (p.sixteens == 4) return few_r<D, TYPE, 4>(c, b, a, p, Q, O, bf, ws, s);
-    if constexpr (few_most(D) > 2)
-        if (p.sixteens == 3) return few_r<D, TYPE, 3>(c, b, a, p, Q, O, bf, ws, s);
-    if constexpr (few_most(D) > 1)
+    if constexpr (few_sixteens(D) > 1)
         if (p.sixteens == 2) return few_r<D, TYPE, 2>(c, b, a, p, Q, O, bf, ws, s);
     return few_r<D, TYPE, 1>(c, b, a, p, Q, O, bf, ws, s);
 }

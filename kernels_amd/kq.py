@@ -404,9 +404,9 @@ def _need(ok, what):
 
 
 def _here(t, dtype, shape, what):
-    """t: a contiguous tensor of this type and shape on the current device."""
-    _need(t.dtype == dtype and tuple(t.shape) == tuple(shape) and t.is_contiguous(),
-          f"{what}: a contiguous {dtype} tensor {tuple(shape)}, not {t.dtype} {tuple(t.shape)}")
+    """t: a contiguous tensor of this type and shape."""
+    if t.dtype != dtype or t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{what}: a contiguous {dtype} tensor {tuple(shape)}, not {t.dtype} {tuple(t.shape)}")
 
 
 class KVCache:
@@ -433,6 +433,7 @@ class KVCache:
         self.k, self.v, self.k_exp, self.v_exp = k, v, k_exp, v_exp
         self.device = k.get_device()
         self.heads, self.head_dim, self.page, self.block = heads, dim, page, page // blocks
+        self.scale = dim ** -0.5
         self._c = _KVCacheC(k.data_ptr(), v.data_ptr(), k_exp.data_ptr(), v_exp.data_ptr(), types[k.dtype],
                             n, page, page // blocks, heads, dim)
         self._ref = C.byref(self._c)
@@ -476,42 +477,49 @@ class KVBatch:
         return _KVBatchC(*self._args, rows, self.max_len)
 
 
-def _kv_rows(t, heads, dim, rows, dtype, what):
-    _need(t.dim() == 3 and t.shape[0] == rows and t.shape[1] == heads and t.shape[2] == dim,
-          f"{what}: [{rows}][{heads}][{dim}], not {tuple(t.shape)}")
-    _need(t.dtype == dtype, f"{what}: {dtype}, not {t.dtype}")
+def _kv_rows(t, shape, dtype, what):
+    """kq_kv_rows of a tensor of this shape [rows][heads][head_dim] and type."""
+    if t.shape != shape or t.dtype != dtype:
+        raise ValueError(f"{what}: a {dtype} tensor {tuple(shape)}, not {t.dtype} {tuple(t.shape)}")
     row, head, one = t.stride()
-    _need(one == 1, f"{what}: its last dimension is contiguous")
+    if one != 1:
+        raise ValueError(f"{what}: contiguous in its last dimension, not strides {t.stride()}")
     return _KVRowsC(t.data_ptr(), row, head)
 
 
-def _kv_device(cache, batch, *tensors):
-    """Refuses tensors of another device than the current one, whose stream the call takes."""
-    import torch
-    d = torch.cuda.current_device()
-    _need(cache.device == d and batch.device == d and all(t is None or t.get_device() == d for t in tensors),
-          f"every tensor of the call is on the current device ({d})")
+def _kv_call(cache, batch, stream, *tensors):
+    """The call's stream; refuses tensors of another device than the current one, whose stream it is."""
+    s = _stream(stream)
+    if _current is None:
+        _stream(None)
+    d = _current[1]()
+    if cache.device != d or batch.device != d:
+        raise ValueError(f"the cache and the batch are on the current device ({d})")
+    for t in tensors:
+        if t is not None and t.get_device() != d:
+            raise ValueError(f"every tensor of the call is on the current device ({d})")
+    return s
 
 
-def _kv_move(name, cache, batch, k, v, stream):
-    _kv_device(cache, batch, k, v)
-    rows = k.shape[0]
-    a = _kv_rows(k, cache.heads, cache.head_dim, rows, k.dtype, "k")
-    b = _kv_rows(v, cache.heads, cache.head_dim, rows, k.dtype, "v")
-    f = lib().kq_kv_write if name == "kq_kv_write" else lib().kq_kv_read
-    _check(f(cache._ref, C.byref(batch._c(rows)), C.byref(a), C.byref(b), _dt(k), _stream(stream)), name)
+def _kv_move(f, where, cache, batch, k, v, stream):
+    s = _kv_call(cache, batch, stream, k, v)
+    shape, dtype = k.shape, k.dtype
+    if len(shape) != 3 or shape[1] != cache.heads or shape[2] != cache.head_dim:
+        raise ValueError(f"k: [n_rows][{cache.heads}][{cache.head_dim}], not {tuple(shape)}")
+    a, b = _kv_rows(k, shape, dtype, "k"), _kv_rows(v, shape, dtype, "v")
+    _check(f(cache._ref, C.byref(batch._c(shape[0])), C.byref(a), C.byref(b), _dt(k), s), where)
 
 
 def kv_write(cache, batch, k, v, stream=None):
     """The newest tokens' keys and values [n_rows][heads][head_dim] (float16 or
     bfloat16, any row and head strides) into the cache."""
-    _kv_move("kq_kv_write", cache, batch, k, v, stream)
+    _kv_move(lib().kq_kv_write, "kq_kv_write", cache, batch, k, v, stream)
 
 
 def kv_read(cache, batch, k, v, stream=None):
     """The batch's newest tokens out of the cache into k and v
     [n_rows][heads][head_dim] (float16, bfloat16 or float32)."""
-    _kv_move("kq_kv_read", cache, batch, k, v, stream)
+    _kv_move(lib().kq_kv_read, "kq_kv_read", cache, batch, k, v, stream)
 
 
 def kv_attn_workspace_size(cache, batch, q_heads):
@@ -527,16 +535,18 @@ def kv_attn(cache, batch, q, out, ws, ws_bytes, scale=None, causal=True, window=
     the cache, into out (float16 or bfloat16 both). scale: None is
     1 / sqrt(head_dim). window > 0: a row sees its own and the window - 1 tokens
     before. sinks: float32 [q_heads]. lse: float32 [n_rows][q_heads], written."""
-    import torch
-    _kv_device(cache, batch, q, out, sinks, lse)
-    rows, q_heads = q.shape[0], q.shape[1]
-    a = _kv_rows(q, q_heads, cache.head_dim, rows, q.dtype, "q")
-    b = _kv_rows(out, q_heads, cache.head_dim, rows, q.dtype, "out")
-    if sinks is not None:
-        _here(sinks, torch.float32, (q_heads,), "sinks")
-    if lse is not None:
-        _here(lse, torch.float32, (rows, q_heads), "lse")
-    _need(0 <= window < 2**32, "window: 32-bit")
-    d = _KVAttnC(q_heads, cache.head_dim ** -0.5 if scale is None else scale, bool(causal), window, _ptr(sinks))
+    s = _kv_call(cache, batch, stream, q, out, sinks, lse)
+    shape, dtype = q.shape, q.dtype
+    if len(shape) != 3 or shape[2] != cache.head_dim:
+        raise ValueError(f"q: [n_rows][q_heads][{cache.head_dim}], not {tuple(shape)}")
+    rows, q_heads, _ = shape
+    a, b = _kv_rows(q, shape, dtype, "q"), _kv_rows(out, shape, dtype, "out")
+    if sinks is not None and (_dt(sinks) != F32 or sinks.shape != (q_heads,) or not sinks.is_contiguous()):
+        raise ValueError(f"sinks: a contiguous float32 tensor [{q_heads}]")
+    if lse is not None and (_dt(lse) != F32 or lse.shape != (rows, q_heads) or not lse.is_contiguous()):
+        raise ValueError(f"lse: a contiguous float32 tensor [{rows}][{q_heads}]")
+    if not 0 <= window < 2**32:
+        raise ValueError("window: 32-bit")
+    d = _KVAttnC(q_heads, cache.scale if scale is None else scale, causal, window, _ptr(sinks))
     _check(lib().kq_kv_attn(cache._ref, C.byref(batch._c(rows)), C.byref(d), C.byref(a), C.byref(b), _dt(q),
-                            _ptr(lse), _ptr(ws), ws_bytes, _stream(stream)), "kq_kv_attn")
+                            _ptr(lse), _ptr(ws), ws_bytes, s), "kq_kv_attn")

@@ -168,11 +168,13 @@ def test_python_tensors():
     with pytest.raises(ValueError):
         kq.KVBatch(pages, n, -1)
     b = kq.KVBatch(pages, n, 10)
-    for shape in ((3, 2, 32), (3, 1, 64), (4, 2, 64)):
+    for shape in ((3, 2, 32), (3, 1, 64), (4, 2, 64), (3, 64), (3, 2, 64, 1)):
         with pytest.raises(ValueError):
-            kq._kv_rows(torch.zeros(shape), 2, 64, 3, torch.float32, "k")
+            kq._kv_rows(torch.zeros(shape), (3, 2, 64), torch.float32, "k")
     with pytest.raises(ValueError):
-        kq._kv_rows(torch.zeros((3, 64, 2)).transpose(1, 2), 2, 64, 3, torch.float32, "k")
+        kq._kv_rows(torch.zeros((3, 2, 64)), (3, 2, 64), torch.float16, "k")
+    with pytest.raises(ValueError):
+        kq._kv_rows(torch.zeros((3, 64, 2)).transpose(1, 2), (3, 2, 64), torch.float32, "k")
     with pytest.raises(kq.KQError):
         kq.kv_attn_workspace_size(c, b, 3)
 
