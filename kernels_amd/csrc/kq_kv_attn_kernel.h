@@ -147,6 +147,11 @@ __device__ __forceinline__ float load_q(const Rows& Q, bool there, int row, uint
     return pow2f(-e);
 }
 
+template <bool ONCE, class T>
+__device__ __forceinline__ T load_codes(const T* p) {
+    return ONCE ? ldg_nt(p) : *p;
+}
+
 // ---- the work of a call of few rows, shared out evenly
 //
 // A row of work (a sequence and head) is ceil(tokens / kTile) units, and p.start more at its beginning, the
@@ -282,8 +287,10 @@ __device__ __forceinline__ float* slot_of(float* ws, const FewPlan& p, uint32_t 
 // of a piece in turn and join their sums at its end. What bounds it is the stream of codes:
 // a wave asks for its next keys as soon as the present ones are multiplied, and for its
 // next values after the product with the present ones, so that most of 16 KiB a wave
-// (128 wide) is always on its way.
-template <int D, int TYPE, int R>
+// (128 wide) is always on its way. ONCE: no other workgroup reads the codes, and they are loaded past the
+// caches' other lines (64 sequences of 2486 tokens 69 us without, 64 with); with two row tiles to
+// share them that costs more than it saves (28 us without, 31 with).
+template <int D, int TYPE, int R, bool ONCE>
 __global__ __launch_bounds__(256, few_waves(D)) void kv_few_k(Cache c, Batch b, Attn a, FewPlan p, Rows Q, Rows O, int bf,
                                                               float* ws) {
     constexpr int C64 = D / 64, kHalf = D % 64 ? 1 : 0;  // 64-column pieces of a key, and a 32-column one
@@ -354,8 +361,8 @@ __global__ __launch_bounds__(256, few_waves(D)) void kv_few_k(Cache c, Batch b, 
 #pragma unroll
                 for (int t = 0; t < 4; ++t) {
 #pragma unroll
-                    for (int i = 0; i < C64; ++i) kw[t * C64 + i] = ldg_nt(reinterpret_cast<const u32x4*>(kp + t * 4 * D + i * 64 + g * 16));
-                    if constexpr (kHalf) kx[t] = ldg_nt(reinterpret_cast<const u32x2*>(kp + t * 4 * D + C64 * 64 + g * 8));
+                    for (int i = 0; i < C64; ++i) kw[t * C64 + i] = load_codes<ONCE>(reinterpret_cast<const u32x4*>(kp + t * 4 * D + i * 64 + g * 16));
+                    if constexpr (kHalf) kx[t] = load_codes<ONCE>(reinterpret_cast<const u32x2*>(kp + t * 4 * D + C64 * 64 + g * 8));
                 }
             };
             auto load_v = [&](int t0) {
@@ -366,31 +373,26 @@ __global__ __launch_bounds__(256, few_waves(D)) void kv_few_k(Cache c, Batch b, 
                 ve = c.v_exp[eo];
                 const uint8_t* const vp = c.v + code_offset(c, D, max(pv, 0), h, tv) + r * 16;
 #pragma unroll
-                for (int i = 0; i < D / 16; ++i) vw[i] = ldg_nt(reinterpret_cast<const u32x4*>(vp + i * 256));
+                for (int i = 0; i < D / 16; ++i) vw[i] = load_codes<ONCE>(reinterpret_cast<const u32x4*>(vp + i * 256));
             };
             auto step = [&](int t0, auto more) {
+                // products on the same sums stand apart: each waits for the one before
                 f32x4 st[R][4];
 #pragma unroll
-                for (int t = 0; t < 4; ++t) {
+                for (int t = 0; t < 4; ++t)
 #pragma unroll
                     for (int k = 0; k < R; ++k) st[k][t] = f32x4{0, 0, 0, 0};
 #pragma unroll
-                    for (int i = 0; i < C64; ++i) {
-                        const u32x4 w = kw[t * C64 + i];
-                        const f16x8 x = codes_f16x8<TYPE>(w.x, w.y), y = codes_f16x8<TYPE>(w.z, w.w);
+                for (int i = 0; i < 2 * C64 + kHalf; ++i)
 #pragma unroll
-                        for (int k = 0; k < R; ++k) {
-                            st[k][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, q[k][2 * i], st[k][t], 0, 0, 0);
-                            st[k][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, q[k][2 * i + 1], st[k][t], 0, 0, 0);
-                        }
-                    }
-                    if constexpr (kHalf) {
-                        const f16x8 x = codes_f16x8<TYPE>(kx[t].x, kx[t].y);
+                    for (int t = 0; t < 4; ++t) {
+                        const u32x4 w = kw[t * C64 + min(i / 2, C64 - 1)];
+                        const f16x8 x = i == 2 * C64 ? codes_f16x8<TYPE>(kx[t].x, kx[t].y)
+                                        : i % 2      ? codes_f16x8<TYPE>(w.z, w.w)
+                                                     : codes_f16x8<TYPE>(w.x, w.y);
 #pragma unroll
-                        for (int k = 0; k < R; ++k)
-                            st[k][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, q[k][2 * C64], st[k][t], 0, 0, 0);
+                        for (int k = 0; k < R; ++k) st[k][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, q[k][i], st[k][t], 0, 0, 0);
                     }
-                }
                 __builtin_amdgcn_sched_barrier(0);  // into the registers just read, not beside them
                 if constexpr (decltype(more)::value) load_k(t0 + kRound);
                 __builtin_amdgcn_sched_barrier(0);
@@ -447,14 +449,15 @@ __global__ __launch_bounds__(256, few_waves(D)) void kv_few_k(Cache c, Batch b, 
                     }
                 }
 #pragma unroll
-                for (int i = 0; i < D / 16; ++i) {
-                    const f16x8 x = codes_f16x8<TYPE>(vw[i].x, vw[i].y), y = codes_f16x8<TYPE>(vw[i].z, vw[i].w);
+                for (int i0 = 0; i0 < D / 16; i0 += 4)
 #pragma unroll
-                    for (int k = 0; k < R; ++k) {
-                        o[k][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, w[k][0], o[k][i], 0, 0, 0);
-                        o[k][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(y, w[k][1], o[k][i], 0, 0, 0);
-                    }
-                }
+                    for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+                        for (int i = i0; i < i0 + 4 && i < D / 16; ++i) {
+                            const f16x8 x = hh ? codes_f16x8<TYPE>(vw[i].z, vw[i].w) : codes_f16x8<TYPE>(vw[i].x, vw[i].y);
+#pragma unroll
+                            for (int k = 0; k < R; ++k) o[k][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, w[k][hh], o[k][i], 0, 0, 0);
+                        }
                 __builtin_amdgcn_sched_barrier(0);
                 if constexpr (decltype(more)::value) load_v(t0 + kRound);
                 __builtin_amdgcn_sched_barrier(0);
@@ -635,7 +638,9 @@ __global__ __launch_bounds__(256) void kv_join_k(Cache c, Batch b, Attn a, FewPl
 template <int D, int TYPE, int R>
 hipError_t few_r(const Cache& c, const Batch& b, const Attn& a, const FewPlan& p, const Rows& Q, const Rows& O, bool bf,
                  float* ws, hipStream_t s) {
-    kv_few_k<D, TYPE, R><<<(p.groups + 7) / 8 * 8 * p.tiles, 256, 0, s>>>(c, b, a, p, Q, O, bf, ws);
+    const uint32_t wgs = (p.groups + 7) / 8 * 8 * p.tiles;
+    if (p.tiles == 1) kv_few_k<D, TYPE, R, true><<<wgs, 256, 0, s>>>(c, b, a, p, Q, O, bf, ws);
+    else if constexpr (R == few_sixteens(D)) kv_few_k<D, TYPE, R, false><<<wgs, 256, 0, s>>>(c, b, a, p, Q, O, bf, ws);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.mode == FewPlan::kRows) return e;
     const uint32_t rows = b.max_q * a.group;
