@@ -487,7 +487,8 @@ kq_status kq_kv_read(const kq_kv_cache* cache, const kq_kv_batch* batch, const k
  * Scores, softmax and sums are fp32. The products run in fp16 on exact
  * codes: bf16 queries are scaled to fp16 by a power of two for each row, which
  * keeps every bit down to 2^-28 of the row's largest; probabilities are
- * rounded to fp16, scaled so that 2^-28 of the row's largest is still normal.
+ * rounded to fp16 (subnormal from 2^-25 of the row's largest down; smaller
+ * than 2^-36 of it they are lost, in O alone).
  * ws: kq_kv_attn_workspace_size bytes, 256-byte aligned, no initialisation and
  * nothing kept in it between calls: a range of it for the partial results of
  * sequences that are split among workgroups. Calls that share one must be

@@ -643,7 +643,8 @@ kq_status kq_kv_attn(const kq_kv_cache* cache, const kq_kv_batch* batch, const k
     if (!kq::kv_attn_fits(c, b, group)) return KQ_EUNSUPPORTED;
     if (!ws || ws_bytes < kq::kv_attn_ws_bytes(c, b, cache->head_dim, group)) return KQ_EWORKSPACE;
     if (!aligned(ws, 256)) return KQ_EALIGN;
-    const kq::kv::Attn a = {d->scale * 1.4426950408889634f, group, d->causal != 0, window, d->sinks, lse};
+    const kq::kv::Attn a = {d->scale * 1.4426950408889634f, group, d->causal != 0, window,
+                             (65536 + group - 1) / group, d->sinks, lse};
     return hip_status(kq::launch_kv_attn(c, b, cache->head_dim, (int)cache->type, a, kv_rows(*Q), kv_rows(*O),
                                          dtype == KQ_BF16, ws, reinterpret_cast<hipStream_t>(stream)));
 }

@@ -179,6 +179,7 @@ struct Rows {
 struct Attn {
     float scale_log2;  // scale * log2(e)
     uint32_t group, causal, window;
+    uint32_t group_inv;  // 2^16 / group, rounded up
     const float* sinks;
     float* lse;
 };

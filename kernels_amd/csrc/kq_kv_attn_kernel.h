@@ -21,10 +21,15 @@ namespace kv {
 
 constexpr int kTile = 64;      // tokens a wave takes at a time
 constexpr int kRound = 256;    // ... and four waves do
-constexpr int kLift = 14;      // probabilities are scaled by 2^14: the fp16 ones stay normal down to 2^-28 of the largest
+// A row's sums go by a reference m that its largest t exceeds by kSlack at most: it moves, and the sums with
+// it, only where it would be by more (with every new maximum the sums of 32 rows moved in most
+// tiles of 64 tokens). Probabilities are scaled by 2^kLift, so that the fp16 ones lie below 2^15 and stay
+// normal down to 2^-25 of the reference.
+constexpr int kLift = 11;
+constexpr float kSlack = 4.0f;
 constexpr int kIds = 4096;     // page ids that a workgroup holds at a time
 constexpr int kScan = 1024;    // most sequences whose lengths a workgroup adds up
-constexpr float kLowest = -3.0e38f;  // running maximum before any token
+constexpr float kLowest = -3.0e38f;  // reference before any token
 
 // Tokens that rows row .. row + rows - 1 of a sequence and head see: [lo, hi), lo a multiple of 64.
 struct Span {
@@ -147,6 +152,9 @@ __device__ __forceinline__ float load_q(const Rows& Q, bool there, int row, uint
     return pow2f(-e);
 }
 
+// Token of one of the few rows: row / group by a multiplication, exact below 64 x 64.
+__device__ __forceinline__ int token_of(const Attn& a, int row) { return (int)((uint32_t)row * a.group_inv >> 16); }
+
 template <bool ONCE, class T>
 __device__ __forceinline__ T load_codes(const T* p) {
     return ONCE ? ldg_nt(p) : *p;
@@ -253,22 +261,29 @@ __device__ inline Share share_of(const Cache& c, const Batch& b, const Attn& a, 
         uint32_t x = k % count;
         w.seq = find(x, u, [&](int v) { return (int)(((uint32_t)v + size - 1) / size); });
         w.parts = (int)(((uint32_t)u + size - 1) / size);
-        w.unit = (int)((uint64_t)x * u / w.parts);
-        w.units = (int)((uint64_t)(x + 1) * u / w.parts) - w.unit;
+        // the first u % parts of them are a unit longer
+        const int each = u / w.parts, more = u - each * w.parts;
+        w.unit = (int)x * each + min((int)x, more);
+        w.units = each + ((int)x < more);
         return w;
     }
     w.total = all * c.heads;
     if (w.total < w.groups) w.groups = (uint32_t)w.total;
     if (k >= w.groups) return w;
-    w.at = w.total * k / w.groups;
-    w.units = (int)(w.total * (k + 1) / w.groups - w.at);
+    if (w.total < 0xFFFFFFFFu / w.groups) {  // short divisions where they do
+        w.at = (uint32_t)w.total * k / w.groups;
+        w.units = (int)((uint32_t)w.total * (k + 1) / w.groups - (uint32_t)w.at);
+    } else {
+        w.at = w.total * k / w.groups;
+        w.units = (int)(w.total * (k + 1) / w.groups - w.at);
+    }
     // in order of sequence, then head
-    uint32_t x = (uint32_t)(w.at / c.heads);
-    const uint32_t odd = (uint32_t)(w.at % c.heads);
+    uint32_t x = (uint32_t)(w.total <= 0xFFFFFFFFu ? (uint32_t)w.at / c.heads : w.at / c.heads);
+    const uint32_t odd = (uint32_t)(w.at - (uint64_t)x * c.heads);
     w.seq = find(x, u, [](int v) { return v; });
     const uint64_t in = (uint64_t)x * c.heads + odd;
-    w.head = (uint32_t)(in / (uint32_t)u);
-    w.unit = (int)(in % (uint32_t)u);
+    w.head = (uint32_t)(in <= 0xFFFFFFFFu ? (uint32_t)in / (uint32_t)u : in / (uint32_t)u);
+    w.unit = (int)(in - (uint64_t)w.head * (uint32_t)u);
     return w;
 }
 
@@ -335,12 +350,12 @@ __global__ __launch_bounds__(256, few_waves(D)) void kv_few_k(Cache c, Batch b, 
             f32x4 o[R][D / 16];
 #pragma unroll
             for (int k = 0; k < R; ++k) {
-                const int row = row0 + 16 * k + r, tok = row / (int)a.group;
+                const int row = row0 + 16 * k + r, tok = token_of(a, row);
                 const bool there = 16 * k + r < rows;
                 const int pos = s.len - s.n + tok;
                 sees_hi[k] = there ? min(a.causal ? pos + 1 : s.len, hi) : 0;
                 sees_lo[k] = a.window ? pos + 1 - (int)a.window : 0;
-                q_scale[k] = fabsf(a.scale_log2) * load_q<D>(Q, there, s.row0 + tok, h * a.group + (uint32_t)(row % (int)a.group),
+                q_scale[k] = fabsf(a.scale_log2) * load_q<D>(Q, there, s.row0 + tok, h * a.group + (uint32_t)(row - tok * (int)a.group),
                                                              g, bf, a.scale_log2, q[k]);
                 m[k] = kLowest;
                 l[k] = 0.0f;
@@ -420,7 +435,7 @@ __global__ __launch_bounds__(256, few_waves(D)) void kv_few_k(Cache c, Batch b, 
 #pragma unroll
                     for (int i = 1; i < 16; ++i) top = fmaxf(top, st[k][i / 4][i % 4]);
                     top = across_rows_maxf(fmaxf(m[k], __builtin_fmaf(top, f, e)));
-                    if (__any(top > m[k])) {
+                    if (__any(top > m[k] + kSlack)) {
                         const float fade = __builtin_amdgcn_exp2f(m[k] - top);
                         m[k] = top;
                         l[k] *= fade;
@@ -521,8 +536,8 @@ __global__ __launch_bounds__(256, few_waves(D)) void kv_few_k(Cache c, Batch b, 
 #pragma unroll
                 for (int w = 0; w < 4; ++w) sum += l_lds[w][row] * __builtin_amdgcn_exp2f(m_lds[w][row] - best);
                 if (whole) {
-                    const uint32_t head = h * a.group + (uint32_t)((row0 + row) % (int)a.group);
-                    const int out = s.row0 + (row0 + row) / (int)a.group;
+                    const int tok = token_of(a, row0 + row), out = s.row0 + tok;
+                    const uint32_t head = h * a.group + (uint32_t)(row0 + row - tok * (int)a.group);
                     store4(O, out, head, d, y * finish(a, best, sum, out, head, q_heads, d == 0), bf);
                 } else {
                     *reinterpret_cast<f32x4*>(part + row * D + d) = y;

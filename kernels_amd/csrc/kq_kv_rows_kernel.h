@@ -87,6 +87,7 @@ __global__ __launch_bounds__(64 * NW, D >= 192 ? 1 : 2) void kv_rows_k(Cache c, 
 
     int page0 = 0, page1 = 0;  // ids holds the table's [page0, page1)
     u32x4 kc[kEach], vc[kEach];
+    int valid[kEach];  // tokens of the piece's block that there are
     int ex = 0;
     auto page_at = [&](int t) { return ids[(min(t, hi - 1) >> c.page_log2) - page0]; };
     // Tokens t0 .. t0 + 63 on their way into registers.
@@ -106,11 +107,14 @@ __global__ __launch_bounds__(64 * NW, D >= 192 ? 1 : 2) void kv_rows_k(Cache c, 
         for (int e = 0; e < kEach; ++e) {
             const int i = tid + e * T;
             if (kPieces % T == 0 || i < kPieces) {
-                const int tk = t0 + i / (D / 16);
-                kc[e] = *reinterpret_cast<const u32x4*>(c.k + code_offset(c, D, max(page_at(tk), 0), h, tk) + (tk & 15) * D +
-                                                        i % (D / 16) * 16);
-                const int tv = t0 + i / D * 16;
-                vc[e] = *reinterpret_cast<const u32x4*>(c.v + code_offset(c, D, max(page_at(tv), 0), h, tv) + i % D * 16);
+                // 16-byte piece i % D of block i / D, of K and of V; the block is the wave's, but for 96 columns
+                const int in = i / D * 16, t = t0 + (D % 64 ? in : __builtin_amdgcn_readfirstlane(in));
+                int page = page_at(t);
+                if (D % 64 == 0) page = __builtin_amdgcn_readfirstlane(page);
+                const uint64_t off = code_offset(c, D, max(page, 0), h, t);
+                kc[e] = *reinterpret_cast<const u32x4*>(c.k + off + i % D * 16);
+                vc[e] = *reinterpret_cast<const u32x4*>(c.v + off + i % D * 16);
+                valid[e] = page < 0 ? 0 : hi - t;
             }
         }
         if (tid < 8) {
@@ -120,7 +124,7 @@ __global__ __launch_bounds__(64 * NW, D >= 192 ? 1 : 2) void kv_rows_k(Cache c, 
         }
     };
     // ... and out of them.
-    auto store = [&](int t0, RowTile<D>& to) {
+    auto store = [&](RowTile<D>& to) {
 #pragma unroll
         for (int e = 0; e < kEach; ++e) {
             const int i = tid + e * T;
@@ -131,14 +135,12 @@ __global__ __launch_bounds__(64 * NW, D >= 192 ? 1 : 2) void kv_rows_k(Cache c, 
                 _Float16* const k = to.k + (2 * col * 65 + place) * 8;
                 *reinterpret_cast<f16x8*>(k) = codes_f16x8<TYPE>(kc[e].x, kc[e].y);
                 *reinterpret_cast<f16x8*>(k + 65 * 8) = codes_f16x8<TYPE>(kc[e].z, kc[e].w);
-                const int tv = t0 + i / D * 16;
                 // bytes of tokens that no length covers, or of no page, may hold anything, NaN among it
-                if (tv + 16 > hi || page_at(tv) < 0) {
-                    const int valid = page_at(tv) < 0 ? 0 : max(hi - tv, 0);
+                if (valid[e] < 16) {
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        const int m = min(max(valid - 4 * j, 0), 4);
-                        vc[e][j] = m == 4 ? vc[e][j] : vc[e][j] & ((1u << 8 * m) - 1);
+                        const int keep = min(max(valid[e] - 4 * j, 0), 4);
+                        vc[e][j] = keep == 4 ? vc[e][j] : vc[e][j] & ((1u << 8 * keep) - 1);
                     }
                 }
                 _Float16* const v = to.v + (i / D * 2 * D + i % D) * 8;
@@ -196,7 +198,7 @@ __global__ __launch_bounds__(64 * NW, D >= 192 ? 1 : 2) void kv_rows_k(Cache c, 
             swapped<true>(top, x, y);
             top = fmaxf(x, y);
         }
-        if (__any(top > m)) {
+        if (__any(top > m + kSlack)) {
             const float fade = __builtin_amdgcn_exp2f(m - top);
             m = top;
             l *= fade;
@@ -226,14 +228,14 @@ __global__ __launch_bounds__(64 * NW, D >= 192 ? 1 : 2) void kv_rows_k(Cache c, 
 
     if (lo < hi) {
         load(lo);
-        store(lo, tiles[0]);
+        store(tiles[0]);
         if (lo + 64 < hi) load(lo + 64);
         __syncthreads();
         int cur = 0;
         for (int t0 = lo; t0 < hi; t0 += 64, cur ^= 1) {
             compute(t0, tiles[cur]);
             if (t0 + 64 < hi) {
-                store(t0 + 64, tiles[cur ^ 1]);
+                store(tiles[cur ^ 1]);
                 if (t0 + 128 < hi) load(t0 + 128);
             }
             __syncthreads();

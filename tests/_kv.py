@@ -118,17 +118,19 @@ class Cache:
 
 
 def attend(cache, table, length, q, scale, causal=True, window=0, sinks=None):
-    """q float64 [n][q_heads][dim] -> (o, lse, spread, reach): float64 results, sum p |v| and the largest
-    sum |q k| * scale of a row, which the tolerances go by."""
+    """q float64 [n][q_heads][dim] -> (o, lse, spread, reach, codes): float64 results, sum p |v|, the largest
+    sum |q k| * scale of a row, and sum |code of v| * the largest scale of v: what the tolerances go by."""
     n, q_heads, dim = q.shape
     group = q_heads // cache.heads
     seen = [t for t in range(length) if 0 <= table[t // cache.page] < cache.n_pages]
     k = np.zeros((len(seen), cache.heads, dim))
     v = k.copy()
+    ev = np.zeros((len(seen), cache.heads))
     for i, t in enumerate(seen):
         k[i], v[i] = (cache.token(w, table[t // cache.page], t % cache.page) for w in "kv")
+        ev[i] = cache.exps["v"][table[t // cache.page], :, t % cache.page // cache.block].astype(np.float64) - 127
     at = np.array(seen, np.int64)
-    o, spread = np.zeros(q.shape), np.zeros(q.shape)
+    o, spread, codes = np.zeros(q.shape), np.zeros(q.shape), np.zeros(q.shape)
     lse, reach = np.full((n, q_heads), -np.inf), np.zeros((n, q_heads))
     for j in range(n):
         pos = length - n + j
@@ -149,11 +151,13 @@ def attend(cache, table, length, q, scale, causal=True, window=0, sinks=None):
             if len(s):
                 o[j, h] = w @ vv / total
                 spread[j, h] = w @ np.abs(vv) / total
+                e = ev[sees, h // group]
+                codes[j, h] = (np.abs(vv) * 2.0 ** (e.max() - e)[:, None]).sum(0)
                 reach[j, h] = (np.abs(kk) @ np.abs(q[j, h])).max() * abs(scale)
-    return o, lse, spread, reach
+    return o, lse, spread, reach, codes
 
 
-def attend_tolerance(o, lse, spread, reach, dim, eps, tiny):
+def attend_tolerance(o, lse, spread, reach, codes, dim, eps, tiny):
     """How far (out, lse) may be off.
 
     A score is dim exact products summed in 32 bits, then times the scale (itself
@@ -162,9 +166,14 @@ def attend_tolerance(o, lse, spread, reach, dim, eps, tiny):
     exp2 and the sums add a few 2^-23. A probability is then rounded to fp16
     (2^-11 of itself), so out is off by (2^-11 + 4 E) sum p |v|, and by the
     rounding of the result: eps / 2 of it, or half its type's smallest step.
+    fp16 rounds no finer than 2^-24: w = 2^(t - m + 11), t = log2 p + e_v, is off by
+    2^-25 where it is subnormal, and out = sum w code / sum w 2^-e_v by 2^-25 sum
+    |code| / sum w 2^-e_v. The reference m is at most the largest t, whose token
+    alone makes the denominator 2^11 2^-e_v at least: out is off by at most
+    2^-36 sum |code| 2^(largest e_v).
     lse: E, and its own roundings."""
     E = (dim + 16) * 2.0**-24 * (reach + 96.0)
-    out = (2.0**-11 + 4 * E)[..., None] * spread * 1.01 + eps / 2 * np.abs(o) * 1.01 + tiny
+    out = (2.0**-11 + 4 * E)[..., None] * spread * 1.01 + eps / 2 * np.abs(o) * 1.01 + tiny + 2.0**-36 * codes
     with np.errstate(invalid="ignore"):
         size = np.where(np.isfinite(lse), np.abs(lse), 0.0)
     return out, 2 * E + 2.0**-21 * (size + 1.0)
