@@ -7,21 +7,55 @@ namespace kq {
 namespace kv {
 namespace {
 
-// Magnitude bits of both halves of a pair, 0 for infinities and NaN: for finite
-// values they order as the magnitudes do.
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+
+// Magnitude bits of both halves of pairs order as the magnitudes do; from kInf on they are no finite value's.
+template <int BF>
+constexpr uint32_t kInf = BF ? 0x7F80u : 0x7C00u;
+__device__ __forceinline__ uint32_t pair_max(uint32_t pair, uint32_t m) {
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, pair & 0x7FFF7FFFu),
+                                                                  __builtin_bit_cast(u16x2, m)));
+}
+// The larger half, and the same of finite values alone.
+__device__ __forceinline__ uint32_t half_max(uint32_t m) { return max(m & 0xFFFFu, m >> 16); }
 template <int BF>
 __device__ __forceinline__ uint32_t finite_max(uint32_t pair, uint32_t m) {
-    const uint32_t top = BF ? 0x7F80u : 0x7C00u;
     const uint32_t a = pair & 0x7FFFu, b = pair >> 16 & 0x7FFFu;
-    m = max(m, a < top ? a : 0u);
-    return max(m, b < top ? b : 0u);
+    return max(m, max(a < kInf<BF> ? a : 0u, b < kInf<BF> ? b : 0u));
 }
 
-// One wave writes one block of one head's K or V: the largest new magnitude
-// over the wave, the exponent, then the codes.
+// Four codes of a dword anew: the values they stand for times `keep`, rounded.
+template <int TYPE>
+__device__ __forceinline__ uint32_t rounded_anew(uint32_t w, float keep) {
+    float y[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) y[q] = to_range<TYPE>(Code<TYPE>::value(w >> 8 * q & 0xFF), keep);
+    return Code<TYPE>::code2(y[0], y[1]) | Code<TYPE>::code2(y[2], y[3]) << 16;
+}
+// Codes of four values times `scale`. PLAIN: all are finite and within the codes' range as they are.
+// int8: adding 1.5 * 2^23 rounds to nearest even and leaves the integer's low byte in the sum's.
+template <int TYPE, bool PLAIN>
+__device__ __forceinline__ uint32_t four_codes(float a, float b, float c, float d, float scale) {
+    if constexpr (!PLAIN) {
+        return Code<TYPE>::code2(to_range<TYPE>(a, scale), to_range<TYPE>(b, scale)) |
+               Code<TYPE>::code2(to_range<TYPE>(c, scale), to_range<TYPE>(d, scale)) << 16;
+    } else if constexpr (TYPE == KQ_KV_I8) {
+        auto low = [&](float x) { return __builtin_bit_cast(uint32_t, __builtin_fmaf(x, scale, 12582912.0f)); };
+        return __builtin_amdgcn_perm(low(b), low(a), 0x0C0C0400u) | __builtin_amdgcn_perm(low(d), low(c), 0x04000C0Cu);
+    } else {
+        const int w = __builtin_amdgcn_cvt_pk_fp8_f32(a * scale, b * scale, 0, false);
+        return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c * scale, d * scale, w, true);
+    }
+}
+
+// One wave writes one block of one head's K or V: the largest new magnitude over the wave, the
+// exponent, then the codes. Blocks of 16 tokens stay in registers in between (bf16 prefill of 13k
+// tokens, 8 heads of 128: 28-35 us for 82 MB with a second read, 21-27 without); larger ones are read
+// twice, 16 tokens at a time, the second time from a cache.
 template <int D, int TYPE, int BF>
 __global__ __launch_bounds__(256) void kv_write_k(Cache c, Batch b, Rows K, Rows V, uint32_t groups) {
-    const uint32_t lane = threadIdx.x & 63, job = (blockIdx.x % groups) * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
+    const uint32_t job = (blockIdx.x % groups) * 4 + (threadIdx.x >> 6);
     if (job >= 2 * c.heads) return;
     const uint32_t h = job >> 1;
     const bool is_v = job & 1;
@@ -30,150 +64,253 @@ __global__ __launch_bounds__(256) void kv_write_k(Cache c, Batch b, Rows K, Rows
     const int t0 = ((first0 >> c.block_log2) + (int)(blockIdx.x / groups)) << c.block_log2;
     if (s.n == 0 || t0 >= s.len) return;
     const int page = page_of(c, b.pages + (uint64_t)blockIdx.y * b.max_pages, t0);
-    if (page < 0) return;
     const int lo = max(first0 - t0, 0), hi = min(s.len - t0, B);  // the block's new tokens
-    uint8_t* const codes = (is_v ? c.v : c.k) + code_offset(c, D, page, h, t0);
-    uint8_t* const ep = (is_v ? c.v_exp : c.k_exp) + exp_offset(c, page, h, t0);
     const Rows& R = is_v ? V : K;
     const uint16_t* const x = static_cast<const uint16_t*>(R.p) + (int64_t)(s.row0 + t0 - first) * R.row +
                               (int64_t)h * R.head;  // token t0's values
-    // 8 values a lane and step
-    uint32_t m = 0;
-    for (int i = lo * (D / 8) + (int)lane; i < hi * (D / 8); i += 64) {
-        const u32x4 v = *reinterpret_cast<const u32x4*>(x + (int64_t)(i / (D / 8)) * R.row + i % (D / 8) * 8);
+
+    // 16 tokens in registers. K: 8 columns of a token a piece. V: two columns of 16 tokens, or of 8
+    // where that fills the wave.
+    constexpr int NK = D / 32, H = D == 64 ? 2 : 1, TL = 16 / H, NV = (D / 2 * H + 63) / 64;
+    u32x4 xk[NK];
+    uint32_t xv[NV][TL];
+    auto load = [&](int sub) {
+        if (!is_v) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) m = finite_max<BF>(v[j], m);
+            for (int j = 0; j < NK; ++j) {
+                const int i = lane + 64 * j, t = sub + i / (D / 8);
+                xk[j] = t >= lo && t < hi ? *reinterpret_cast<const u32x4*>(x + (int64_t)t * R.row + i % (D / 8) * 8) : u32x4{};
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < NV; ++j)
+#pragma unroll
+                for (int q = 0; q < TL; ++q) {
+                    const int i = lane + 64 * j, t = sub + i / (D / 2) * TL + q;
+                    const bool there = t >= lo && t < hi && (NV * 64 == D / 2 * H || i < D / 2 * H);
+                    xv[j][q] = there ? *reinterpret_cast<const uint32_t*>(x + (int64_t)t * R.row + i % (D / 2) * 2) : 0u;
+                }
+        }
+    };
+    load(lo & ~15);  // on its way while the page id is
+    if (page < 0) return;
+    uint8_t* const codes = (is_v ? c.v : c.k) + code_offset(c, D, page, h, t0);
+    uint8_t* const ep = (is_v ? c.v_exp : c.k_exp) + exp_offset(c, page, h, t0);
+    const int was = lo > 0 ? (int)*ep - 127 : -127;
+    uint32_t m = 0;
+    for (int sub = lo & ~15; sub < hi; sub += 16) {
+        if (sub > lo) load(sub);
+        if (!is_v) {
+#pragma unroll
+            for (int j = 0; j < NK; ++j)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) m = pair_max(xk[j][q], m);
+        } else {
+#pragma unroll
+            for (int j = 0; j < NV; ++j)
+#pragma unroll
+                for (int q = 0; q < TL; ++q) m = pair_max(xv[j][q], m);
+        }
     }
-    m = wave_max(m);
-    int e = block_exponent<TYPE>(elem<BF>(m));
-    float keep = 1.0f;  // what older codes are multiplied by
-    bool grew = false;
-    if (lo > 0) {
-        const int was = (int)*ep - 127;
-        grew = e > was;
-        e = max(e, was);
-        keep = pow2f(max(was - e, -126));
+    m = wave_max(half_max(m));
+    const bool finite = m < kInf<BF>;
+    if (!finite) {  // once more, without infinities and NaN
+        m = 0;
+        for (int sub = lo & ~15; sub < hi; sub += 16) {
+            if (B > 16) load(sub);
+            if (!is_v) {
+#pragma unroll
+                for (int j = 0; j < NK; ++j)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) m = finite_max<BF>(xk[j][q], m);
+            } else {
+#pragma unroll
+                for (int j = 0; j < NV; ++j)
+#pragma unroll
+                    for (int q = 0; q < TL; ++q) m = finite_max<BF>(xv[j][q], m);
+            }
+        }
+        m = wave_max(m);
     }
+    const int wanted = block_exponent<TYPE>(elem<BF>(m));
+    const int e = max(wanted, was);
+    const bool grew = lo > 0 && wanted > was;
+    const float keep = pow2f(max(was - e, -126));  // what older codes are multiplied by
     // a foreign cache may hold any byte: stay within pow2f's range
     const float scale = pow2f(min(max(-e, -126), 127));
     if (lane == 0) *ep = (uint8_t)(e + 127);
-    if (!is_v) {
-        for (int i = (grew ? 0 : lo * (D / 8)) + (int)lane; i < hi * (D / 8); i += 64) {
-            const int t = i / (D / 8);
-            u32x2* const at = reinterpret_cast<u32x2*>(codes + (uint32_t)i * 8);
-            u32x2 out;
-            if (t < lo) {
-                const u32x2 old = *at;
+    auto write = [&](auto plain) {
+        constexpr bool P = decltype(plain)::value;
+        for (int sub = grew ? 0 : lo & ~15; sub < hi; sub += 16) {
+            if (B > 16) load(sub);
+            if (!is_v) {
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    float y[4];
+                for (int j = 0; j < NK; ++j) {
+                    const int i = lane + 64 * j, t = sub + i / (D / 8);
+                    u32x2* const at = reinterpret_cast<u32x2*>(codes + (uint32_t)(sub * D + i * 8));
+                    if (t >= lo && t < hi) {
+                        const u32x4 v = xk[j];
+                        u32x2 w;
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) y[q] = to_range<TYPE>(Code<TYPE>::value(old[j] >> 8 * q & 0xFF), keep);
-                    out[j] = Code<TYPE>::code2(y[0], y[1]) | Code<TYPE>::code2(y[2], y[3]) << 16;
+                        for (int q = 0; q < 2; ++q)
+                            w[q] = four_codes<TYPE, P>(elem<BF>(v[2 * q] & 0xFFFF), elem<BF>(v[2 * q] >> 16),
+                                                       elem<BF>(v[2 * q + 1] & 0xFFFF), elem<BF>(v[2 * q + 1] >> 16), scale);
+                        *at = w;
+                    } else if (t < lo && grew) {
+                        const u32x2 old = *at;
+                        *at = u32x2{rounded_anew<TYPE>(old.x, keep), rounded_anew<TYPE>(old.y, keep)};
+                    }
                 }
-            } else {
-                const u32x4 v = *reinterpret_cast<const u32x4*>(x + (int64_t)t * R.row + i % (D / 8) * 8);
-#pragma unroll
-                for (int j = 0; j < 2; ++j)
-                    out[j] = Code<TYPE>::code2(to_range<TYPE>(elem<BF>(v[2 * j] & 0xFFFF), scale),
-                                               to_range<TYPE>(elem<BF>(v[2 * j] >> 16), scale)) |
-                             Code<TYPE>::code2(to_range<TYPE>(elem<BF>(v[2 * j + 1] & 0xFFFF), scale),
-                                               to_range<TYPE>(elem<BF>(v[2 * j + 1] >> 16), scale)) << 16;
+                continue;
             }
-            *at = out;
-        }
-        return;
-    }
-    // V: two columns of 16 tokens a lane and step, 32 contiguous bytes
-    for (int i = (int)lane; i < (B >> 4) * (D / 2); i += 64) {
-        const int sub = i / (D / 2) * 16, d = i % (D / 2) * 2;
-        if (sub >= hi || (sub + 16 <= lo && !grew)) continue;
-        u32x4* const at = reinterpret_cast<u32x4*>(codes + (uint32_t)sub * D + d * 16);
-        u32x4 col[2] = {};
-        if (lo > sub || hi < sub + 16) {
-            col[0] = at[0];
-            col[1] = at[1];
-        }
 #pragma unroll
-        for (int t = 0; t < 16; ++t) {
-            const uint32_t sh = t % 4 * 8;
-            uint32_t n0, n1;
-            if (sub + t >= hi) continue;
-            if (sub + t < lo) {
-                if (!grew) continue;
-                n0 = Code<TYPE>::code(to_range<TYPE>(Code<TYPE>::value(col[0][t / 4] >> sh & 0xFF), keep));
-                n1 = Code<TYPE>::code(to_range<TYPE>(Code<TYPE>::value(col[1][t / 4] >> sh & 0xFF), keep));
-            } else {
-                const uint32_t v = *reinterpret_cast<const uint32_t*>(x + (int64_t)(sub + t) * R.row + d);
-                n0 = Code<TYPE>::code(to_range<TYPE>(elem<BF>(v & 0xFFFF), scale));
-                n1 = Code<TYPE>::code(to_range<TYPE>(elem<BF>(v >> 16), scale));
+            for (int j = 0; j < NV; ++j) {
+                const int i = lane + 64 * j, t = sub + i / (D / 2) * TL;
+                if (NV * 64 != D / 2 * H && i >= D / 2 * H) continue;
+                uint32_t* const at = reinterpret_cast<uint32_t*>(codes + (uint32_t)(sub * D + i % (D / 2) * 32 + i / (D / 2) * TL));
+                const bool part = t < lo || t + TL > hi;  // older tokens, or none, among them
+                uint32_t out[2][TL / 4];
+#pragma unroll
+                for (int w = 0; w < TL / 4; ++w) {
+                    const uint32_t* const v = xv[j] + 4 * w;
+                    uint32_t col[2] = {four_codes<TYPE, P>(elem<BF>(v[0] & 0xFFFF), elem<BF>(v[1] & 0xFFFF), elem<BF>(v[2] & 0xFFFF),
+                                                           elem<BF>(v[3] & 0xFFFF), scale),
+                                       four_codes<TYPE, P>(elem<BF>(v[0] >> 16), elem<BF>(v[1] >> 16), elem<BF>(v[2] >> 16),
+                                                           elem<BF>(v[3] >> 16), scale)};
+                    if (part) {
+                        // bytes of older tokens stay, or are rounded anew; those behind the last stay
+                        uint32_t fresh = 0, older = 0;
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            fresh |= t + 4 * w + q >= lo && t + 4 * w + q < hi ? 0xFFu << 8 * q : 0u;
+                            older |= t + 4 * w + q < lo ? 0xFFu << 8 * q : 0u;
+                        }
+#pragma unroll
+                        for (int n = 0; n < 2; ++n) {
+                            uint32_t old = at[4 * n + w];
+                            if (grew) old = (rounded_anew<TYPE>(old, keep) & older) | (old & ~older);
+                            col[n] = (col[n] & fresh) | (old & ~fresh);
+                        }
+                    }
+                    out[0][w] = col[0];
+                    out[1][w] = col[1];
+                }
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+                    if constexpr (TL == 16) *reinterpret_cast<u32x4*>(at + 4 * n) = u32x4{out[n][0], out[n][1], out[n][2], out[n][3]};
+                    else *reinterpret_cast<u32x2*>(at + 4 * n) = u32x2{out[n][0], out[n][1]};
             }
-            col[0][t / 4] = (col[0][t / 4] & ~(0xFFu << sh)) | n0 << sh;
-            col[1][t / 4] = (col[1][t / 4] & ~(0xFFu << sh)) | n1 << sh;
         }
-        at[0] = col[0];
-        at[1] = col[1];
-    }
+    };
+    // at the range's end a finite value may still exceed the largest code
+    if (finite && e < Code<TYPE>::kMaxExp) write(Int<1>());
+    else write(Int<0>());
 }
 
-// F: the type of the rows. Eight values to eight consecutive elements, two to two.
+// F: the type of the rows.
 template <int F>
 __device__ __forceinline__ float saturate(float y) {
     const float top = F == KQ_F16 ? 65504.0f : F == KQ_BF16 ? 0x1.FEp127f : 3.402823466e38f;
     return y != y ? y : fminf(fmaxf(y, -top), top);
 }
+// Two, four, eight values to consecutive elements.
+template <int F>
+__device__ __forceinline__ void put2(uint8_t* to, const float (&y)[2]) {
+    if constexpr (F == KQ_F32) *reinterpret_cast<float2*>(to) = make_float2(y[0], y[1]);
+    else *reinterpret_cast<uint32_t*>(to) = pair16<F>(y[0], y[1]);
+}
+template <int F>
+__device__ __forceinline__ void put4(uint8_t* to, const float (&y)[4]) {
+    if constexpr (F == KQ_F32) *reinterpret_cast<f32x4*>(to) = f32x4{y[0], y[1], y[2], y[3]};
+    else *reinterpret_cast<u32x2*>(to) = u32x2{pair16<F>(y[0], y[1]), pair16<F>(y[2], y[3])};
+}
 
-// One wave reads 16 tokens (an aligned 16 of the sequence) of one head's K or V.
-template <int D, int TYPE, int F>
+template <int F>
+__device__ __forceinline__ void put8(uint8_t* to, const float (&y)[8]) {
+    if constexpr (F == KQ_F32) {
+        *reinterpret_cast<f32x4*>(to) = f32x4{y[0], y[1], y[2], y[3]};
+        *reinterpret_cast<f32x4*>(to + 16) = f32x4{y[4], y[5], y[6], y[7]};
+    } else {
+        *reinterpret_cast<u32x4*>(to) = u32x4{pair16<F>(y[0], y[1]), pair16<F>(y[2], y[3]), pair16<F>(y[4], y[5]), pair16<F>(y[6], y[7])};
+    }
+}
+
+// One wave reads SPAN tokens (16 or 64, an aligned span of the sequence) of one head's K or V. What bounds it is
+// the writes: 131k tokens of 8 heads of 128, e4m3 to fp16, 160 us for 805 MB, where a copy of that
+// size reaches 4.9 TB/s.
+template <int D, int TYPE, int F, int SPAN>
 __global__ __launch_bounds__(256) void kv_read_k(Cache c, Batch b, Rows K, Rows V, uint32_t groups) {
-    const uint32_t lane = threadIdx.x & 63, job = (blockIdx.x % groups) * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
+    const uint32_t job = (blockIdx.x % groups) * 4 + (threadIdx.x >> 6);
     if (job >= 2 * c.heads) return;
     const uint32_t h = job >> 1;
     const bool is_v = job & 1;
     const Seq s = sequence(b, c.page_log2, blockIdx.y);
     const int first = s.len - s.n, first0 = max(first, 0);
-    const int t0 = ((first0 >> 4) + (int)(blockIdx.x / groups)) << 4;
+    const int t0 = (first0 / SPAN + (int)(blockIdx.x / groups)) * SPAN;
     if (s.n == 0 || t0 >= s.len) return;
-    const int lo = max(first0 - t0, 0), hi = min(s.len - t0, 16);
-    const int page = page_of(c, b.pages + (uint64_t)blockIdx.y * b.max_pages, t0);
+    const int lo = max(first0 - t0, 0), hi = min(s.len - t0, SPAN);
+    const int32_t* const table = b.pages + (uint64_t)blockIdx.y * b.max_pages;
     const Rows& R = is_v ? V : K;
     constexpr int kSize = F == KQ_F32 ? 4 : 2;
     uint8_t* const out = static_cast<uint8_t*>(R.p) +
                          ((int64_t)(s.row0 + t0 - first) * R.row + (int64_t)h * R.head) * kSize;
     const int64_t pitch = R.row * kSize;
-    const uint64_t off = page < 0 ? 0 : code_offset(c, D, page, h, t0);
-    const uint8_t* const codes = (is_v ? c.v : c.k) + off;
-    float scale = 0.0f;
-    if (page >= 0) {
-        const int e = (int)(is_v ? c.v_exp : c.k_exp)[exp_offset(c, page, h, t0)] - 127;
-        scale = pow2f(max(e, -126));
-    }
-    if (!is_v) {
-        for (int i = lo * (D / 4) + (int)lane; i < hi * (D / 4); i += 64) {
-            const uint32_t w = page < 0 ? 0u : *reinterpret_cast<const uint32_t*>(codes + (uint32_t)i * 4);
-            float y[4];
+    // its 16-token blocks: where their codes are, and their scales; no page: zeros of anything
+    constexpr int N = SPAN / 16, C = N == 1 ? 2 : 4;  // columns of 16 values a lane
+    const uint8_t* from[N];
+    float scales[N];
 #pragma unroll
-            for (int q = 0; q < 4; ++q) y[q] = saturate<F>(Code<TYPE>::value(w >> 8 * q & 0xFF) * scale);
-            uint8_t* const to = out + (i / (D / 4)) * pitch + i % (D / 4) * 4 * kSize;
-            if constexpr (F == KQ_F32) *reinterpret_cast<f32x4*>(to) = f32x4{y[0], y[1], y[2], y[3]};
-            else *reinterpret_cast<u32x2*>(to) = u32x2{pair16<F>(y[0], y[1]), pair16<F>(y[2], y[3])};
+    for (int i = 0; i < N; ++i) {
+        const int t = min(t0 + 16 * i, s.len - 1), page = page_of(c, table, t);
+        from[i] = (is_v ? c.v : c.k) + code_offset(c, D, max(page, 0), h, t);
+        scales[i] = (float)((is_v ? c.v_exp : c.k_exp)[exp_offset(c, max(page, 0), h, t)]);
+        if (page < 0) scales[i] = -1.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) scales[i] = scales[i] < 0.0f ? 0.0f : pow2f(max((int)scales[i] - 127, -126));
+    auto value = [&](uint32_t byte, float scale) { return scale == 0.0f ? 0.0f : saturate<F>(Code<TYPE>::value(byte) * scale); };
+    if (!is_v) {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            if (16 * n + 16 <= lo || 16 * n >= hi) continue;
+            u32x2 w[D / 32];
+#pragma unroll
+            for (int j = 0; j < D / 32; ++j) w[j] = *reinterpret_cast<const u32x2*>(from[n] + (lane + 64 * j) * 8);
+#pragma unroll
+            for (int j = 0; j < D / 32; ++j) {
+                const int i = lane + 64 * j, t = 16 * n + i / (D / 8);  // 8 columns of token t
+                float y[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) y[k] = value(w[j][k / 4] >> k % 4 * 8 & 0xFF, scales[n]);
+                if (t >= lo && t < hi) put8<F>(out + t * pitch + i % (D / 8) * 8 * kSize, y);
+            }
         }
         return;
     }
-    for (int i = (int)lane; i < D / 2; i += 64) {
-        u32x4 col[2] = {};
-        if (page >= 0) {
-            col[0] = *reinterpret_cast<const u32x4*>(codes + i * 32);
-            col[1] = *reinterpret_cast<const u32x4*>(codes + i * 32 + 16);
-        }
 #pragma unroll
-        for (int t = 0; t < 16; ++t) {
-            if (t < lo || t >= hi) continue;
-            const float y0 = saturate<F>(Code<TYPE>::value(col[0][t / 4] >> t % 4 * 8 & 0xFF) * scale);
-            const float y1 = saturate<F>(Code<TYPE>::value(col[1][t / 4] >> t % 4 * 8 & 0xFF) * scale);
-            uint8_t* const to = out + t * pitch + i * 2 * kSize;
-            if constexpr (F == KQ_F32) *reinterpret_cast<float2*>(to) = make_float2(y0, y1);
-            else *reinterpret_cast<uint32_t*>(to) = pair16<F>(y0, y1);
+    for (int j = 0; j < (N * D / C + 63) / 64; ++j) {
+        const int i = lane + 64 * j, n = i / (D / C), t = n * 16, d = i % (D / C) * C;  // C columns of block n
+        if (t + 16 <= lo || t >= hi) continue;  // hi <= SPAN: past the last block too
+        float scale = scales[0];
+        const uint8_t* at = from[0];
+#pragma unroll
+        for (int k = 1; k < N; ++k) {
+            scale = n == k ? scales[k] : scale;
+            at = n == k ? from[k] : at;
+        }
+        at += d * 16;
+        u32x4 w[C];
+#pragma unroll
+        for (int k = 0; k < C; ++k) w[k] = *reinterpret_cast<const u32x4*>(at + k * 16);
+#pragma unroll
+        for (int q = 0; q < 16; ++q) {
+            float y[C];
+#pragma unroll
+            for (int k = 0; k < C; ++k) y[k] = value(w[k][q / 4] >> q % 4 * 8 & 0xFF, scale);
+            if (t + q < lo || t + q >= hi) continue;
+            if constexpr (C == 4) put4<F>(out + (t + q) * pitch + d * kSize, y);
+            else put2<F>(out + (t + q) * pitch + d * kSize, y);
         }
     }
 }
@@ -186,35 +323,42 @@ hipError_t write_d(const Cache& c, const Batch& b, const Rows& K, const Rows& V,
     return hipGetLastError();
 }
 
-template <int D, int TYPE>
+template <int D, int TYPE, int SPAN>
 hipError_t read_d(const Cache& c, const Batch& b, const Rows& K, const Rows& V, kq_dtype f, dim3 grid, uint32_t groups,
                   hipStream_t s) {
-    if (f == KQ_F16) kv_read_k<D, TYPE, KQ_F16><<<grid, 256, 0, s>>>(c, b, K, V, groups);
-    else if (f == KQ_BF16) kv_read_k<D, TYPE, KQ_BF16><<<grid, 256, 0, s>>>(c, b, K, V, groups);
-    else kv_read_k<D, TYPE, KQ_F32><<<grid, 256, 0, s>>>(c, b, K, V, groups);
+    if (f == KQ_F16) kv_read_k<D, TYPE, KQ_F16, SPAN><<<grid, 256, 0, s>>>(c, b, K, V, groups);
+    else if (f == KQ_BF16) kv_read_k<D, TYPE, KQ_BF16, SPAN><<<grid, 256, 0, s>>>(c, b, K, V, groups);
+    else kv_read_k<D, TYPE, KQ_F32, SPAN><<<grid, 256, 0, s>>>(c, b, K, V, groups);
     return hipGetLastError();
 }
 
 }  // namespace
 }  // namespace kv
 
-// The launches of one wave a block: blockIdx.x = the block counted from the
-// sequence's first new one x the groups of four waves of its heads, .y = the sequence.
+// blockIdx.x = the block (write) or span (read), counted from the sequence's first newest token's, x the groups
+// of four waves of its heads; .y = the sequence.
+static uint32_t spans(uint32_t max_q, uint32_t tokens) { return (max_q - 1) / tokens + 1 + (max_q > 1); }
+
 hipError_t launch_kv_write(const kv::Cache& c, const kv::Batch& b, uint32_t D, int type, const kv::Rows& K,
                            const kv::Rows& V, bool bf, hipStream_t s) {
-    const uint32_t blocks = ((b.max_q - 1) >> c.block_log2) + 1 + (b.max_q > 1), groups = (2 * c.heads + 3) / 4;
-    const dim3 grid(blocks * groups, b.n_seq);
+    const uint32_t groups = (2 * c.heads + 3) / 4;
+    const dim3 grid(spans(b.max_q, 1u << c.block_log2) * groups, b.n_seq);
     return kv::by_dim(D, type, [&](auto d, auto t) {
         return kv::write_d<decltype(d)::value, decltype(t)::value>(c, b, K, V, bf, grid, groups, s);
     });
 }
 
+// 16 tokens a wave: the shortest way for a few (a decode step's blocks of 96 sequences 6 us, 9 with 64). 64 where that
+// makes a great many workgroups, most of which may find nothing in ragged batches (24 sequences of up to
+// 6007 tokens, 890 on average: 16 us, 26 with 16); in between 16 is the faster (13k tokens 17 us, 20).
 hipError_t launch_kv_read(const kv::Cache& c, const kv::Batch& b, uint32_t D, int type, const kv::Rows& K,
                           const kv::Rows& V, kq_dtype f, hipStream_t s) {
-    const uint32_t blocks = ((b.max_q - 1) >> 4) + 1 + (b.max_q > 1), groups = (2 * c.heads + 3) / 4;
-    const dim3 grid(blocks * groups, b.n_seq);
+    const uint32_t groups = (2 * c.heads + 3) / 4;
+    const bool wide = (uint64_t)spans(b.max_q, 16) * groups * b.n_seq > 16384;
+    const dim3 grid(spans(b.max_q, wide ? 64 : 16) * groups, b.n_seq);
     return kv::by_dim(D, type, [&](auto d, auto t) {
-        return kv::read_d<decltype(d)::value, decltype(t)::value>(c, b, K, V, f, grid, groups, s);
+        constexpr int N = decltype(d)::value, T = decltype(t)::value;
+        return wide ? kv::read_d<N, T, 64>(c, b, K, V, f, grid, groups, s) : kv::read_d<N, T, 16>(c, b, K, V, f, grid, groups, s);
     });
 }
 

@@ -15,14 +15,17 @@ struct Seq {
 __device__ __forceinline__ Seq sequence(const Batch& b, uint32_t page_log2, uint32_t i) {
     Seq s;
     const uint64_t room = (uint64_t)b.max_pages << page_log2;
-    const int most = (int)(room < b.max_len ? room : b.max_len);
-    s.len = min(max(b.kv_len[i], 0), most);
+    const int most = (int)(room < b.max_len ? room : b.max_len), rows = (int)b.n_rows, max_q = (int)b.max_q;
     if (b.q_start) {
-        s.row0 = min(max(b.q_start[i], 0), (int)b.n_rows);
-        s.n = min(min(max(b.q_start[i + 1], s.row0), (int)b.n_rows) - s.row0, (int)b.max_q);
+        // asked for together: one way to memory, not three
+        const int len = b.kv_len[i], from = b.q_start[i], to = b.q_start[i + 1];
+        s.len = min(max(len, 0), most);
+        s.row0 = min(max(from, 0), rows);
+        s.n = min(min(max(to, s.row0), rows) - s.row0, max_q);
     } else {
-        s.row0 = (int)(i * b.max_q);
-        s.n = (int)b.max_q;
+        s.len = min(max(b.kv_len[i], 0), most);
+        s.row0 = (int)i * max_q;
+        s.n = max_q;
     }
     return s;
 }
