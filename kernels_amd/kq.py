@@ -10,6 +10,7 @@ if the library is missing or a call fails, a KQError is raised.
 """
 import ctypes as C
 import os
+import struct
 from dataclasses import dataclass
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -128,12 +129,12 @@ def lib():
         L.kq_vq_quantize_workspace_size.restype = sz
         L.kq_vq_quantize.argtypes = [vp, i32, u32, u32, u32, u32, u32, u32, C.c_uint64, vp, vp,
                                      vp, vp, sz, vp]
-        pc, pb, pr = C.POINTER(_KVCacheC), C.POINTER(_KVBatchC), C.POINTER(_KVRowsC)
-        L.kq_kv_write.argtypes = [pc, pb, pr, pr, i32, vp]
-        L.kq_kv_read.argtypes = [pc, pb, pr, pr, i32, vp]
-        L.kq_kv_attn_workspace_size.argtypes = [pc, pb, u32]
+        # the structs of the key/value cache's calls: by reference, or packed (bytes)
+        L.kq_kv_write.argtypes = [vp, vp, vp, vp, i32, vp]
+        L.kq_kv_read.argtypes = [vp, vp, vp, vp, i32, vp]
+        L.kq_kv_attn_workspace_size.argtypes = [vp, vp, u32]
         L.kq_kv_attn_workspace_size.restype = sz
-        L.kq_kv_attn.argtypes = [pc, pb, C.POINTER(_KVAttnC), pr, pr, i32, vp, vp, sz, vp]
+        L.kq_kv_attn.argtypes = [vp, vp, vp, vp, vp, i32, vp, vp, sz, vp]
         for name in EXPORTS:
             if name not in ("kq_status_str", "kq_last_hip_error", "kq_version",
                             "kq_moe_default_desc", "kq_moe_workspace_size",
@@ -397,6 +398,10 @@ def moe_block_unfused(pool, desc, R, x, idx, wgt, H, y, ws, ws_bytes, batch=1, x
 # ---------------------------------------------------------------------------
 KV_I8, KV_E4M3 = 0, 1  # kq_kv_type
 
+# kq_kv_batch, kq_kv_rows and kq_kv_attn_desc as bytes: a call makes up to four of them, and a
+# ctypes.Structure costs several times as much
+_pack_batch, _pack_rows, _pack_attn = (struct.Struct("@" + f).pack for f in ("3P5I4x", "Pqq", "If2IP"))
+
 
 def _need(ok, what):
     if not ok:
@@ -471,10 +476,10 @@ class KVBatch:
               "the batch's tensors are on one device")
         self.pages, self.kv_len, self.q_start = pages, kv_len, q_start
         self.device, self.n_seq, self.max_q, self.max_len = pages.get_device(), n, max_q, max_len
-        self._args = (_ptr(pages), _ptr(kv_len), _ptr(q_start), n, pages.shape[1], max_q)
+        self._args = (_ptr(pages), _ptr(kv_len), _ptr(q_start) or 0, n, pages.shape[1], max_q)
 
-    def _c(self, rows):
-        return _KVBatchC(*self._args, rows, self.max_len)
+    def _packed(self, rows):
+        return _pack_batch(*self._args, rows, self.max_len)
 
 
 def _kv_rows(t, shape, dtype, what):
@@ -484,7 +489,7 @@ def _kv_rows(t, shape, dtype, what):
     row, head, one = t.stride()
     if one != 1:
         raise ValueError(f"{what}: contiguous in its last dimension, not strides {t.stride()}")
-    return _KVRowsC(t.data_ptr(), row, head)
+    return _pack_rows(t.data_ptr(), row, head)
 
 
 def _kv_call(cache, batch, stream, *tensors):
@@ -507,7 +512,7 @@ def _kv_move(f, where, cache, batch, k, v, stream):
     if len(shape) != 3 or shape[1] != cache.heads or shape[2] != cache.head_dim:
         raise ValueError(f"k: [n_rows][{cache.heads}][{cache.head_dim}], not {tuple(shape)}")
     a, b = _kv_rows(k, shape, dtype, "k"), _kv_rows(v, shape, dtype, "v")
-    _check(f(cache._ref, C.byref(batch._c(shape[0])), C.byref(a), C.byref(b), _dt(k), s), where)
+    _check(f(cache._ref, batch._packed(shape[0]), a, b, _dt(k), s), where)
 
 
 def kv_write(cache, batch, k, v, stream=None):
@@ -523,7 +528,7 @@ def kv_read(cache, batch, k, v, stream=None):
 
 
 def kv_attn_workspace_size(cache, batch, q_heads):
-    n = lib().kq_kv_attn_workspace_size(cache._ref, C.byref(batch._c(batch.n_seq * batch.max_q)), q_heads)
+    n = lib().kq_kv_attn_workspace_size(cache._ref, batch._packed(batch.n_seq * batch.max_q), q_heads)
     if n == 0:
         raise KQError(KQ_EINVAL, "kq_kv_attn_workspace_size")
     return n
@@ -547,6 +552,6 @@ def kv_attn(cache, batch, q, out, ws, ws_bytes, scale=None, causal=True, window=
         raise ValueError(f"lse: a contiguous float32 tensor [{rows}][{q_heads}]")
     if not 0 <= window < 2**32:
         raise ValueError("window: 32-bit")
-    d = _KVAttnC(q_heads, cache.scale if scale is None else scale, causal, window, _ptr(sinks))
-    _check(lib().kq_kv_attn(cache._ref, C.byref(batch._c(rows)), C.byref(d), C.byref(a), C.byref(b), _dt(q),
+    d = _pack_attn(q_heads, cache.scale if scale is None else scale, bool(causal), window, _ptr(sinks) or 0)
+    _check(lib().kq_kv_attn(cache._ref, batch._packed(rows), d, a, b, _dt(q),
                             _ptr(lse), _ptr(ws), ws_bytes, s), "kq_kv_attn")

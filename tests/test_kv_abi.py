@@ -143,6 +143,13 @@ def test_launches_too_large():
     assert attn(b=b, n=(1 << 63)) == kq.KQ_EUNSUPPORTED
 
 
+def test_packed_structs():
+    """What kq.py passes as bytes is what the C structs hold."""
+    assert bytes(batch_c(pages=1, kv_len=2, q_start=3)) == kq._pack_batch(1, 2, 3, 2, 8, 3, 6, 100)
+    assert bytes(rows_c(p=5, row=-3, head=2**40)) == kq._pack_rows(5, -3, 2**40)
+    assert bytes(attn_c(sinks=9, scale=-0.5, window=7)) == kq._pack_attn(32, -0.5, True, 7, 9)
+
+
 def test_python_tensors():
     c = kq.kv_cache(4, 2, 64, page=32, block=16, device="cpu")
     assert (c.page, c.block, c.heads, c.head_dim) == (32, 16, 2, 64)
