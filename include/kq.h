@@ -423,8 +423,8 @@ typedef struct kq_kv_cache {
  * max_q rows from i * max_q on. They are the last of its kv_len[i] tokens:
  * kv_len counts them, in kq_kv_write too.
  *
- * pages   : int32 [n_seq][max_pages] page ids; what lies behind a sequence's
- *           last token is not read
+ * pages   : int32 [n_seq][max_pages] page ids; those behind a sequence's last
+ *           token may be anything
  * kv_len  : int32 [n_seq], 0 <= kv_len[i] <= max_len
  * q_start : int32 [n_seq + 1], ascending, q_start[n_seq] <= n_rows; or NULL
  * max_q   : at least the most rows of a sequence;  n_rows: the rows of the

@@ -19,12 +19,16 @@ uint64_t longest_span(const Batch& b, uint64_t rows, uint32_t window) {
 // L2 keeps for all of them.
 bool few(const Batch& b, uint32_t group) { return (uint64_t)b.max_q * group <= 64; }
 
-// Their groups: all that the device holds at once, or one for each 256 tokens where there is less. Where
-// there are enough of them each takes a part of one row of work, for the beginning of another
-// costs it about as long as 256 tokens do. One for each row of work where those are short, or the
-// sequences too many to add up their lengths in each workgroup.
+// Their groups: all that the device holds at once (two workgroups a compute unit: three were slower, 73 us
+// against 58 for 64 sequences of 2486 tokens of 8 heads of 128), or one for each 256 tokens where
+// there is less. Where there are enough of them each takes a part of one row of work, for the beginning of
+// another costs it about as long as 384 tokens 128 wide do. One for each row of work where those are
+// short (73 sequences of 100 to 1795 tokens, 16 heads of 64: 30 us, in shares 34; 48 of 200 to
+// 2500, 8 heads of 128: 40 us, in shares 35), or the sequences too many to add up their lengths in
+// each workgroup. In shares the beginning of a row is priced (64 ragged sequences: 94 us without, 73 with).
 FewPlan few_plan(const Cache& c, const Batch& b, uint32_t D, uint32_t group, uint32_t window) {
     FewPlan p = {};
+    const uint32_t start = 768 / D;
     const uint32_t q_rows = b.max_q * group;
     p.sixteens = q_rows <= 16 ? 1 : few_sixteens(D);
     p.tiles = (uint32_t)ceil_div(q_rows, 16 * p.sixteens);
@@ -32,12 +36,12 @@ FewPlan few_plan(const Cache& c, const Batch& b, uint32_t D, uint32_t group, uin
     const uint64_t rows = (uint64_t)b.n_seq * c.heads, fit = (uint64_t)cu_count() * few_waves(D) / p.tiles;
     p.groups = (uint32_t)std::min<uint64_t>(fit, rows * rounds);
     p.mode = 2 * rows <= p.groups ? FewPlan::kParts : FewPlan::kShares;
-    if (rounds <= (p.mode == FewPlan::kShares ? 4 : 1) || b.n_seq > kScan || b.n_seq * (ceil_div(longest, kTile) + 4) >= 0x7FFFFFFF) {
+    if (rounds <= (p.mode == FewPlan::kShares ? 8 : 1) || b.n_seq > kScan || b.n_seq * (ceil_div(longest, kTile) + start) >= 0x7FFFFFFF) {
         p.mode = FewPlan::kRows;
         p.groups = (uint32_t)rows;
         return p;
     }
-    p.start = p.mode == FewPlan::kShares && rows * rounds >= 4 * fit ? kRound / kTile : 0;
+    p.start = p.mode == FewPlan::kShares && rows * rounds >= 4 * fit ? start : 0;
     p.by_row = rows <= p.groups;
     p.cuts = p.by_row ? (uint32_t)rows : p.groups;
     return p;

@@ -164,7 +164,7 @@ __device__ __forceinline__ T load_codes(const T* p) {
 //
 // A row of work (a sequence and head) is ceil(tokens / kTile) units, and p.start more at its beginning, the
 // price of beginning it: asking for its length, page ids, query and first codes one after
-// the other takes about as long as kRound tokens.
+// the other takes about as long as 768 / D units do.
 // kParts: rows of work are cut into parts of at most c units (a round's, at least), with the smallest c that
 // gives no more parts than groups (or near it). kShares: all rows' units in order of sequence and head are cut
 // into equal shares, one for each group, however the lengths differ.
