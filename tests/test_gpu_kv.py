@@ -282,6 +282,33 @@ def test_long_and_bounds_above(gpu):
     attn_case(gpu, [(4000, 70), (3, 1)], 1, 2, 64, max_len=50000, page=64, block=32)
 
 
+def ragged(n, longest, seed, new=1):
+    """n short sequences, empty ones among them, with a few long ones in between."""
+    rng = np.random.default_rng(seed)
+    lens = rng.integers(0, 40, n)
+    lens[rng.integers(0, n, 4)] = rng.integers(longest // 2, longest, 4)
+    lens[n // 3] = longest
+    return [(int(x), int(m)) for x, m in zip(lens, rng.integers(0 if new > 1 else 1, new + 1, n))]
+
+
+# the ways to share out few rows: parts of a row (up to 64 sequences, and more), equal shares (with fewer and more rows
+# of work than workgroups; rows of several tiles; windows), a workgroup a row
+@pytest.mark.parametrize("n,heads,group,longest,new,kw", [
+    (40, 2, 4, 2700, 1, {}), (100, 1, 2, 2700, 1, {}), (70, 1, 16, 2500, 3, dict(kind="e4m3")),
+    (300, 1, 2, 2700, 1, {}), (140, 4, 1, 2400, 1, dict(kind="e4m3", dtype="bf16")), (300, 1, 5, 2300, 5, {}),
+    (150, 2, 9, 2300, 4, dict(dim=128)), (280, 1, 3, 2600, 2, dict(window=2200, sinks=True)), (1100, 1, 2, 2500, 1, {}),
+    (30, 16, 1, 1500, 1, dict(dim=256)), (20, 8, 8, 2100, 8, dict(dim=192))])
+def test_shares(gpu, n, heads, group, longest, new, kw):
+    attn_case(gpu, ragged(n, longest, n), heads, group, **{"dim": 64, "nan": True, "pad": 1, **kw})
+
+
+def test_more_page_ids_than_are_held(gpu):
+    """Sequences longer than the page ids that a workgroup keeps at a time: few rows (a row each, for there are over 1024
+    sequences) and many."""
+    attn_case(gpu, [(1, 1)] * 600 + [(66100, 1)] + [(3, 1)] * 500, 1, 2, 64, max_len=70000)
+    attn_case(gpu, [(17000, 70), (5, 5)], 1, 1, 64, "e4m3", "bf16")
+
+
 @pytest.mark.parametrize("scale", [0.0, -0.3, 1.0])
 def test_scales(gpu, scale):
     attn_case(gpu, [(100, 1), (65, 3)], 2, 2, 64, scale=scale)
