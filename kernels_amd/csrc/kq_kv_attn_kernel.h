@@ -350,10 +350,11 @@ __global__ __launch_bounds__(256, few_waves(D)) void kv_few_k(Cache c, Batch b, 
             f32x4 o[R][D / 16];
 #pragma unroll
             for (int k = 0; k < R; ++k) {
-                const int row = row0 + 16 * k + r, tok = token_of(a, row);
+                // a row that there is not sees what the last one does: it takes no tile off the short way
                 const bool there = 16 * k + r < rows;
+                const int row = there ? row0 + 16 * k + r : row0 + rows - 1, tok = token_of(a, row);
                 const int pos = s.len - s.n + tok;
-                sees_hi[k] = there ? min(a.causal ? pos + 1 : s.len, hi) : 0;
+                sees_hi[k] = min(a.causal ? pos + 1 : s.len, hi);
                 sees_lo[k] = a.window ? pos + 1 - (int)a.window : 0;
                 q_scale[k] = fabsf(a.scale_log2) * load_q<D>(Q, there, s.row0 + tok, h * a.group + (uint32_t)(row - tok * (int)a.group),
                                                              g, bf, a.scale_log2, q[k]);

@@ -51,11 +51,12 @@ __global__ __launch_bounds__(64 * NW, D >= 192 ? 1 : 2) void kv_rows_k(Cache c, 
     const int lo = sp.lo + (int)(split * p.chunk), hi = (int)min((int64_t)sp.hi, (int64_t)lo + p.chunk);
     const int32_t* const table = b.pages + (uint64_t)seq * b.max_pages;
 
-    const int row = row0 + wave * 32 + n, tok = row / (int)a.group;
+    // a row that there is not sees what the last one does: it takes no tile off the short way
+    const int row = min(row0 + wave * 32 + n, rows - 1), tok = row / (int)a.group;
     const uint32_t q_heads = c.heads * a.group, head = h * a.group + (uint32_t)(row % (int)a.group);
-    const bool there = row < rows;
+    const bool there = row0 + wave * 32 + n < rows;
     const int pos = s.len - s.n + tok;
-    const int sees_hi = there ? min(a.causal ? pos + 1 : s.len, hi) : 0, sees_lo = a.window ? pos + 1 - (int)a.window : 0;
+    const int sees_hi = row0 + wave * 32 < rows ? min(a.causal ? pos + 1 : s.len, hi) : 0, sees_lo = a.window ? pos + 1 - (int)a.window : 0;
 
     // Q as the second operand: 8 of each 16 columns
     f16x8 q[D / 16];
