@@ -446,8 +446,9 @@ typedef struct kq_kv_batch {
 } kq_kv_batch;
 
 /* The rows of a tensor [n_rows][heads][head_dim]: element strides of a row and of a
- * head; head_dim is contiguous. Strides are non-negative multiples of 8, the
- * pointer 16-byte aligned (a slice of a fused projection's output is). */
+ * head; head_dim is contiguous. Strides are non-negative multiples of 8 (that of
+ * a single row or head is not looked at), the pointer 16-byte aligned (a slice
+ * of a fused projection's output is). */
 typedef struct kq_kv_rows {
     void* p;
     int64_t row, head;
@@ -489,9 +490,12 @@ kq_status kq_kv_read(const kq_kv_cache* cache, const kq_kv_batch* batch, const k
  * keeps every bit down to 2^-28 of the row's largest; probabilities are
  * rounded to fp16 (subnormal from 2^-25 of the row's largest down; smaller
  * than 2^-36 of it they are lost, in O alone).
- * ws: kq_kv_attn_workspace_size bytes, 256-byte aligned, no initialisation and
- * nothing kept in it between calls: a range of it for the partial results of
- * sequences that are split among workgroups. Calls that share one must be
+ * A cache from elsewhere holds no NaN codes (e4m3 0x7F, 0xFF) below kv_len, or
+ * rows of that sequence and head may be NaN; behind it any bytes do. The
+ * exponents of a sequence and head's values differ by 100 at most.
+ * ws: kq_kv_attn_workspace_size bytes (enough for any window), 256-byte
+ * aligned, no initialisation and nothing kept in it between calls: the partial
+ * results of sequences that are split among workgroups. Calls that share one must be
  * stream-ordered. 0 from kq_kv_attn_workspace_size means invalid arguments.
  * q_heads: a multiple of cache->heads, at most 64 times as many. Results do
  * not change from run to run (no atomics). */

@@ -194,7 +194,8 @@ kq_status check_kv_pointers(const kq_kv_cache* c, const kq_kv_batch* b) {
 
 kq_status check_kv_rows(const kq_kv_rows* r, const kq_kv_batch* b, uint32_t heads, uint32_t D, bool written) {
     if (!r || !r->p) return KQ_ENULL;
-    if (r->row < 0 || r->head < 0 || r->row % 8 || r->head % 8) return KQ_EINVAL;
+    // the stride of a single row or head is never used
+    if ((b->n_rows > 1 && (r->row < 0 || r->row % 8)) || (heads > 1 && (r->head < 0 || r->head % 8))) return KQ_EINVAL;
     // rows and heads that overlap cannot be written
     if (written && ((b->n_rows > 1 && r->row < (int64_t)D) || (heads > 1 && r->head < (int64_t)D))) return KQ_EINVAL;
     return aligned(r->p, 16) ? KQ_OK : KQ_EALIGN;
@@ -641,7 +642,9 @@ kq_status kq_kv_attn(const kq_kv_cache* cache, const kq_kv_batch* batch, const k
     const uint32_t group = d->q_heads / cache->heads;
     const uint32_t window = d->window < batch->max_len ? d->window : 0;  // as wide as all there is: none
     if (!kq::kv_attn_fits(c, b, group)) return KQ_EUNSUPPORTED;
-    if (!ws || ws_bytes < kq::kv_attn_ws_bytes(c, b, cache->head_dim, group)) return KQ_EWORKSPACE;
+    if (!ws || ws_bytes < kq::kv_attn_ws_bytes(c, b, cache->head_dim, group) ||
+        ws_bytes < kq::kv_attn_ws_need(c, b, cache->head_dim, group, window))  // never more than the former
+        return KQ_EWORKSPACE;
     if (!aligned(ws, 256)) return KQ_EALIGN;
     const kq::kv::Attn a = {d->scale * 1.4426950408889634f, group, d->causal != 0, window,
                              (65536 + group - 1) / group, d->sinks, lse};

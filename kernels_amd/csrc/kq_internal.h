@@ -245,7 +245,9 @@ struct AttnKernels {
                            const Rows& O, bool bf, float* ws, hipStream_t s);
 };
 }  // namespace kv
-// Workspace of a call with any window; whether its launches can be made.
+// Bytes of the workspace that a call writes; that no call with another window exceeds; whether the launches
+// can be made.
+size_t kv_attn_ws_need(const kv::Cache& c, const kv::Batch& b, uint32_t D, uint32_t group, uint32_t window);
 size_t kv_attn_ws_bytes(const kv::Cache& c, const kv::Batch& b, uint32_t D, uint32_t group);
 bool kv_attn_fits(const kv::Cache& c, const kv::Batch& b, uint32_t group);
 hipError_t launch_kv_attn(const kv::Cache& c, const kv::Batch& b, uint32_t D, int type, const kv::Attn& a,

@@ -19,13 +19,15 @@ uint64_t longest_span(const Batch& b, uint64_t rows, uint32_t window) {
 // L2 keeps for all of them.
 bool few(const Batch& b, uint32_t group) { return (uint64_t)b.max_q * group <= 64; }
 
-// Their groups: all that the device holds at once (two workgroups a compute unit: three were slower, 73 us
-// against 58 for 64 sequences of 2486 tokens of 8 heads of 128), or one for each 256 tokens where
+// Their groups: all that the device holds at once (two workgroups a compute unit: three were slower, 80 us
+// against 64 for 64 sequences of 2486 tokens of 8 heads of 128), or one for each 256 tokens where
 // there is less. Where there are enough of them each takes a part of one row of work, for the beginning of
-// another costs it about as long as 384 tokens 128 wide do. One for each row of work where those are
-// short (73 sequences of 100 to 1795 tokens, 16 heads of 64: 30 us, in shares 34; 48 of 200 to
-// 2500, 8 heads of 128: 40 us, in shares 35), or the sequences too many to add up their lengths in
-// each workgroup. In shares the beginning of a row is priced (64 ragged sequences: 94 us without, 73 with).
+// another costs it about as long as 384 tokens 128 wide do; in equal shares the beginning of a row is priced
+// (64 ragged sequences: 94 us without, 73 with). One for each row of work where those are short: up to
+// 1024 tokens instead of parts, which a second launch joins (one sequence of 300 tokens 8.2 us a call, in parts
+// 11.0; 1000: 11.2, 11.3; 1500: 14.2, 11.4), up to 2048 instead of shares (73 sequences of 100 to 1795
+// tokens, 16 heads of 64: 30 us, in shares 34; 48 of 200 to 2500, 8 heads of 128: 40 us, in shares
+// 35). So too where the sequences are too many to add up their lengths in each workgroup.
 FewPlan few_plan(const Cache& c, const Batch& b, uint32_t D, uint32_t group, uint32_t window) {
     FewPlan p = {};
     const uint32_t start = 768 / D;
@@ -36,7 +38,7 @@ FewPlan few_plan(const Cache& c, const Batch& b, uint32_t D, uint32_t group, uin
     const uint64_t rows = (uint64_t)b.n_seq * c.heads, fit = (uint64_t)cu_count() * few_waves(D) / p.tiles;
     p.groups = (uint32_t)std::min<uint64_t>(fit, rows * rounds);
     p.mode = 2 * rows <= p.groups ? FewPlan::kParts : FewPlan::kShares;
-    if (rounds <= (p.mode == FewPlan::kShares ? 8 : 1) || b.n_seq > kScan || b.n_seq * (ceil_div(longest, kTile) + start) >= 0x7FFFFFFF) {
+    if (rounds <= (p.mode == FewPlan::kShares ? 8 : 4) || b.n_seq > kScan || b.n_seq * (ceil_div(b.max_len, kTile) + start) >= 0x7FFFFFFF) {
         p.mode = FewPlan::kRows;
         p.groups = (uint32_t)rows;
         return p;
@@ -46,9 +48,8 @@ FewPlan few_plan(const Cache& c, const Batch& b, uint32_t D, uint32_t group, uin
     p.cuts = p.by_row ? (uint32_t)rows : p.groups;
     return p;
 }
-// Of any window: descriptors and slots of the widest launch.
-size_t few_ws_bytes(const Cache& c, const Batch& b, uint32_t D, uint32_t group) {
-    const FewPlan p = few_plan(c, b, D, group, 0);
+// Descriptors and slots.
+size_t few_ws_bytes(const FewPlan& p, uint32_t D) {
     return p.mode == FewPlan::kRows ? 0 : (size_t)p.groups * (sizeof(Cut) + 2 * p.tiles * 16 * p.sixteens * (D + 2) * 4);
 }
 
@@ -65,18 +66,27 @@ RowPlan row_plan(const Cache& c, const Batch& b, uint32_t D, uint32_t group, uin
     p.splits = (uint32_t)ceil_div(longest, p.chunk);
     return p;
 }
-// Of any window: a split has kRound tokens at least.
-size_t row_ws_bytes(const Cache& c, const Batch& b, uint32_t group, uint32_t D) {
-    const RowPlan p = row_plan(c, b, D, group, 0);
-    const uint64_t splits = std::min(row_splits_wanted(c, b, p), ceil_div(b.max_len, kRound));
+size_t row_ws_bytes(const Cache& c, const Batch& b, const RowPlan& p, uint64_t splits, uint32_t D) {
     return splits > 1 ? (size_t)b.n_seq * splits * p.tiles * c.heads * p.rows * (D + 2) * 4 : 0;
 }
 
 }  // namespace
 }  // namespace kv
 
+size_t kv_attn_ws_need(const kv::Cache& c, const kv::Batch& b, uint32_t D, uint32_t group, uint32_t window) {
+    if (kv::few(b, group)) return kv::few_ws_bytes(kv::few_plan(c, b, D, group, window), D);
+    const kv::RowPlan p = kv::row_plan(c, b, D, group, window);
+    return kv::row_ws_bytes(c, b, p, p.splits, D);
+}
+
+// Without a window there are the most groups, and shares or parts wherever there are some with one. Splits
+// are not as orderly: no window makes more than are wanted, nor of less than a round.
 size_t kv_attn_ws_bytes(const kv::Cache& c, const kv::Batch& b, uint32_t D, uint32_t group) {
-    const size_t n = kv::few(b, group) ? kv::few_ws_bytes(c, b, D, group) : kv::row_ws_bytes(c, b, group, D);
+    size_t n = kv_attn_ws_need(c, b, D, group, 0);
+    if (!kv::few(b, group)) {
+        const kv::RowPlan p = kv::row_plan(c, b, D, group, 0);
+        n = kv::row_ws_bytes(c, b, p, std::min(kv::row_splits_wanted(c, b, p), kv::ceil_div(b.max_len, kv::kRound)), D);
+    }
     return n > 256 ? (n + 255) / 256 * 256 : 256;
 }
 

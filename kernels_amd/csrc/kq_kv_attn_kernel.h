@@ -122,9 +122,9 @@ __device__ __forceinline__ u32x4 signed16(u32x4 v, float scale) {
 }
 
 // A row's query as the second operand of S^T, in fp16: 16 columns a lane of each 64, 8 of a
-// last 32. bf16 rows go through a power of two; returns what undoes it.
+// last 32. bf16 rows go through a power of two; returns the exponent that undoes it.
 template <int D>
-__device__ __forceinline__ float load_q(const Rows& Q, bool there, int row, uint32_t head, int g, int bf, float scale,
+__device__ __forceinline__ int load_q(const Rows& Q, bool there, int row, uint32_t head, int g, int bf, float scale,
                                         f16x8 (&q)[D / 32]) {
     constexpr int C64 = D / 64;
     u32x4 raw[D / 32];
@@ -138,7 +138,7 @@ __device__ __forceinline__ float load_q(const Rows& Q, bool there, int row, uint
     if (!bf) {
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) q[i] = __builtin_bit_cast(f16x8, raw[i]);
-        return 1.0f;
+        return 0;
     }
     uint32_t m = 0;
 #pragma unroll
@@ -149,7 +149,7 @@ __device__ __forceinline__ float load_q(const Rows& Q, bool there, int row, uint
     const float up = pow2f(e);
 #pragma unroll
     for (int i = 0; i < D / 32; ++i) q[i] = bf_f16x8(raw[i], up);
-    return pow2f(-e);
+    return -e;
 }
 
 // Token of one of the few rows: row / group by a multiplication, exact below 64 x 64.
@@ -345,8 +345,8 @@ __global__ __launch_bounds__(256, few_waves(D)) void kv_few_k(Cache c, Batch b, 
         if (rows > 0) {
             // this lane's row of each sixteen
             f16x8 q[R][D / 32];
-            float q_scale[R], m[R], l[R];  // m, l: of the row; l: this lane's tokens alone
-            int sees_lo[R], sees_hi[R];
+            float m[R], l[R];  // of the row; l: this lane's tokens alone
+            int q_exp[R], sees_lo[R], sees_hi[R];
             f32x4 o[R][D / 16];
 #pragma unroll
             for (int k = 0; k < R; ++k) {
@@ -356,7 +356,7 @@ __global__ __launch_bounds__(256, few_waves(D)) void kv_few_k(Cache c, Batch b, 
                 const int pos = s.len - s.n + tok;
                 sees_hi[k] = min(a.causal ? pos + 1 : s.len, hi);
                 sees_lo[k] = a.window ? pos + 1 - (int)a.window : 0;
-                q_scale[k] = fabsf(a.scale_log2) * load_q<D>(Q, there, s.row0 + tok, h * a.group + (uint32_t)(row - tok * (int)a.group),
+                q_exp[k] = load_q<D>(Q, there, s.row0 + tok, h * a.group + (uint32_t)(row - tok * (int)a.group),
                                                              g, bf, a.scale_log2, q[k]);
                 m[k] = kLowest;
                 l[k] = 0.0f;
@@ -414,12 +414,12 @@ __global__ __launch_bounds__(256, few_waves(D)) void kv_few_k(Cache c, Batch b, 
                 __builtin_amdgcn_sched_barrier(0);
 
                 const int tv = t0 + 16 * g;
-                const float k_scale = pow2f(min(max(ke - 127, -126), 127)), un_v = pow2f(min(max(127 - ve, -126), 127));
+                const float un_v = pow2f(min(max(127 - ve, -126), 127));
                 f16x8 w[R][2];
 #pragma unroll
                 for (int k = 0; k < R; ++k) {
                     // t = f s + e with f >= 0: the largest t is the largest s's
-                    float f = q_scale[k] * k_scale, e = (float)(ve - 127);
+                    float f = __builtin_ldexpf(fabsf(a.scale_log2), ke - 127 + q_exp[k]), e = (float)(ve - 127);
                     // tokens in sight of the row, of the lane's 16
                     const int from = sees_lo[k] - tv, to = pv < 0 ? 0 : sees_hi[k] - tv;
                     if (!__all(from <= 0 && to >= 16)) {

@@ -60,7 +60,7 @@ __global__ __launch_bounds__(64 * NW, D >= 192 ? 1 : 2) void kv_rows_k(Cache c, 
 
     // Q as the second operand: 8 of each 16 columns
     f16x8 q[D / 16];
-    float q_scale = fabsf(a.scale_log2);
+    int q_exp = 0;  // undoes the power of two of a bf16 row
     {
         u32x4 raw[D / 16];
         const uint16_t* const x = static_cast<const uint16_t*>(Q.p) +
@@ -77,7 +77,7 @@ __global__ __launch_bounds__(64 * NW, D >= 192 ? 1 : 2) void kv_rows_k(Cache c, 
             const auto both = __builtin_amdgcn_permlane32_swap(top, top, false, false);
             const int e = bf_lift(max(both[0], both[1]));
             const float up = pow2f(e);
-            q_scale *= pow2f(-e);
+            q_exp = -e;
 #pragma unroll
             for (int i = 0; i < D / 16; ++i) q[i] = bf_f16x8(raw[i], up);
         } else {
@@ -167,7 +167,8 @@ __global__ __launch_bounds__(64 * NW, D >= 192 ? 1 : 2) void kv_rows_k(Cache c, 
         }
         const int k0 = in.exps[g], k1 = in.exps[2 + g], v0 = in.exps[4 + g], v1 = in.exps[6 + g];
         // t = f s + e with f >= 0: the largest t of a block is its largest s's
-        float f[2] = {q_scale * pow2f(min(max(k0 - 127, -126), 127)), q_scale * pow2f(min(max(k1 - 127, -126), 127))};
+        const float scale = fabsf(a.scale_log2);
+        float f[2] = {__builtin_ldexpf(scale, k0 - 127 + q_exp), __builtin_ldexpf(scale, k1 - 127 + q_exp)};
         float e[2] = {(float)(v0 - 127), (float)(v1 - 127)};
         if (!__all(t0 + 64 <= sees_hi && t0 >= sees_lo && k0 >= 0 && k1 >= 0)) {
             // only the few tiles that need it: nothing of this is computed ahead of the branch

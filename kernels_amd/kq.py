@@ -540,7 +540,7 @@ def kv_attn(cache, batch, q, out, ws, ws_bytes, scale=None, causal=True, window=
     the cache, into out (float16 or bfloat16 both). scale: None is
     1 / sqrt(head_dim). window > 0: a row sees its own and the window - 1 tokens
     before. sinks: float32 [q_heads]. lse: float32 [n_rows][q_heads], written."""
-    s = _kv_call(cache, batch, stream, q, out, sinks, lse)
+    s = _kv_call(cache, batch, stream, q, out, sinks, lse, None if isinstance(ws, int) else ws)
     shape, dtype = q.shape, q.dtype
     if len(shape) != 3 or shape[2] != cache.head_dim:
         raise ValueError(f"q: [n_rows][q_heads][{cache.head_dim}], not {tuple(shape)}")

@@ -327,6 +327,41 @@ def test_query_range(gpu):
     attn_case(gpu, [(100, 1), (65, 3)], 2, 2, 64, dtype="bf16", scale=1e-37, q=huge)
 
 
+def test_tiny_queries_on_huge_keys(gpu):
+    """Queries of about 2^-110 and keys of about 2^110: their products are moderate, though neither factor nor the
+    exponents' product is within float32's reach alone."""
+    rng = np.random.default_rng(12)
+    for n, m in ((70, 1), (200, 90)):
+        b = Batch(gpu, [(n, m)], 16, rng)
+        oracle = _kv.Cache(b.n_pages, 1, 64)
+        oracle.fill(rng)
+        oracle.exps["k"] = (oracle.exps["k"].astype(int) + 110).astype(np.uint8)
+        q, q64 = to(rng.normal(0, 1, (m, 2, 64)) * 2.0**-110, "bf16", gpu)
+        cache, out = upload(oracle, gpu), torch.zeros((m, 2, 64), dtype=torch.bfloat16, device=gpu)
+        ws = torch.empty(kq.kv_attn_workspace_size(cache, b.c, 2), dtype=torch.uint8, device=gpu)
+        kq.kv_attn(cache, b.c, q, out, ws, ws.numel())
+        torch.cuda.synchronize()
+        want = _kv.attend(oracle, b.table[0], n, q64, 64**-0.5)
+        tol, _ = _kv.attend_tolerance(*want, 64, *EPS["bf16"])
+        assert (np.abs(out.double().cpu().numpy() - want[0]) <= tol).all()
+
+
+def test_single_row_of_any_stride(gpu):
+    """One row and one head whose strides are no multiple of 8."""
+    cache = kq.kv_cache(2, 1, 64, device=gpu)
+    b = kq.KVBatch(torch.tensor([[1]], dtype=torch.int32, device=gpu), torch.tensor([1], dtype=torch.int32, device=gpu), 16)
+    x = torch.randn(64, device=gpu).half()
+    row = x.as_strided((1, 1, 64), (3, 5, 1))
+    out = torch.zeros_like(x)
+    kq.kv_write(cache, b, row, row)
+    ws = torch.empty(kq.kv_attn_workspace_size(cache, b, 1), dtype=torch.uint8, device=gpu)
+    kq.kv_attn(cache, b, row, out.as_strided((1, 1, 64), (1, 1, 1)), ws, ws.numel())
+    back = torch.zeros((1, 1, 64), device=gpu)
+    kq.kv_read(cache, b, back, torch.zeros_like(back))
+    torch.cuda.synchronize()
+    assert torch.equal(out.float(), back.view(-1).half().float())  # one token: its value
+
+
 def test_scales_of_blocks_far_apart(gpu):
     """Values whose blocks differ by 2^60 in scale: the large ones have little probability."""
     rng = np.random.default_rng(3)

@@ -89,6 +89,15 @@ def test_bad_rows(kw, status):
     assert attn(Q=r) == attn(O=r) == status
 
 
+def test_strides_of_single_rows_and_heads():
+    """A stride that nothing is reached by is not looked at: such calls are refused for what follows only."""
+    one = batch_c(n_seq=1, n_rows=1, max_q=1)
+    assert write(cache_c(heads=1), one, rows_c(row=3, head=-5), rows_c(row=3, head=-5), dt=kq.F32) == kq.KQ_EUNSUPPORTED
+    assert attn(cache_c(heads=1), one, attn_c(q_heads=1), rows_c(row=1, head=1), rows_c(row=-1, head=0), ws=None) == kq.KQ_EWORKSPACE
+    assert attn(cache_c(heads=1), batch_c(), attn_c(q_heads=1), rows_c(row=1, head=1), rows_c(), ws=None) == kq.KQ_EINVAL
+    assert attn(cache_c(heads=1), one, attn_c(q_heads=2), rows_c(row=1, head=1), rows_c(), ws=None) == kq.KQ_EINVAL
+
+
 @pytest.mark.parametrize("kw", [dict(row=0), dict(head=0), dict(row=120), dict(head=64)])
 def test_overlapping_outputs_are_refused(kw):
     r = rows_c(**kw)
@@ -125,6 +134,36 @@ def test_attention_pointers_and_workspace():
     assert n > 256
     assert attn(b=b, n=n - 1) == attn(b=b, ws=None) == kq.KQ_EWORKSPACE
     assert attn(b=b, ws=FAKE + 64, n=n) == kq.KQ_EALIGN
+
+
+class _Cache(C.Structure):
+    """kq::kv::Cache (kernels_amd/csrc/kq_internal.h)."""
+    _fields_ = [(n, C.c_void_p) for n in ("k", "v", "k_exp", "v_exp")] + [(n, C.c_uint32) for n in ("n_pages", "heads", "page_log2", "block_log2")]
+
+
+def test_workspace_covers_every_window():
+    """What a call writes (libkq's own plan, declared in kq_internal.h) is within what kq_kv_attn_workspace_size said,
+    whatever the window: over sizes where the launch takes its different forms, the largest among them."""
+    need = kq.lib()["_ZN2kq15kv_attn_ws_needERKNS_2kv5CacheERKNS0_5BatchEjjj"]
+    need.restype = C.c_size_t
+    rng = np.random.default_rng(0)
+    some = 0
+    for _ in range(3000):
+        heads, group = int(rng.choice([1, 2, 3, 8, 16, 64])), int(rng.choice([1, 2, 5, 8, 16, 64]))
+        dim, page = int(rng.choice([64, 96, 128, 192, 256])), int(rng.choice([16, 64, 1024]))
+        max_len, n_seq = int(2 ** rng.uniform(0, 31) * 0.99), int(2 ** rng.uniform(0, 14))
+        max_q = int(2 ** rng.uniform(0, rng.choice([3, 12])))
+        if n_seq * max_q * heads * group >= 2**31 - 2**16:
+            continue
+        b = batch_c(n_seq=n_seq, max_q=max_q, n_rows=n_seq * max_q, max_len=max(max_len, 1), max_pages=1 << 20)
+        said = size(cache_c(heads=heads, head_dim=dim, page=page), b, heads * group)
+        assert said > 0
+        c = _Cache(FAKE, FAKE, FAKE, FAKE, 64, heads, page.bit_length() - 1, 4)
+        for window in [0] + [int(2 ** rng.uniform(0, 31)) for _ in range(6)]:
+            n = need(C.byref(c), C.byref(b), C.c_uint32(dim), C.c_uint32(group), C.c_uint32(window))
+            assert n <= said, (heads, group, dim, max_len, n_seq, max_q, window)
+            some += window > 0 and n > 0
+    assert some > 1000
 
 
 def test_workspace_size_refuses_what_the_call_refuses():
