@@ -428,7 +428,8 @@ typedef struct kq_kv_cache {
  * kv_len  : int32 [n_seq], 0 <= kv_len[i] <= max_len
  * q_start : int32 [n_seq + 1], ascending, q_start[n_seq] <= n_rows; or NULL
  * max_q   : at least the most rows of a sequence;  n_rows: the rows of the
- *           arrays (more than the sequences have: the rest is left as it was)
+ *           arrays (more than the sequences have: the rest is left as it was;
+ *           0: the call does nothing)
  * max_len : at least the longest kv_len; both bounds shape the launch
  *
  * pages, kv_len and q_start are device memory and cannot be checked on the

@@ -193,7 +193,9 @@ kq_status check_kv_pointers(const kq_kv_cache* c, const kq_kv_batch* b) {
 }
 
 kq_status check_kv_rows(const kq_kv_rows* r, const kq_kv_batch* b, uint32_t heads, uint32_t D, bool written) {
-    if (!r || !r->p) return KQ_ENULL;
+    if (!r) return KQ_ENULL;
+    if (b->n_rows == 0) return KQ_OK;  // an empty tensor has no address
+    if (!r->p) return KQ_ENULL;
     // the stride of a single row or head is never used
     if ((b->n_rows > 1 && (r->row < 0 || r->row % 8)) || (heads > 1 && (r->head < 0 || r->head % 8))) return KQ_EINVAL;
     // rows and heads that overlap cannot be written
@@ -595,6 +597,7 @@ kq_status kq_kv_write(const kq_kv_cache* cache, const kq_kv_batch* batch, const 
     if (st == KQ_OK) st = check_kv_rows(V, batch, cache->heads, cache->head_dim, false);
     if (st != KQ_OK) return st;
     if (!kv_blocks_fit(cache, batch, cache->block)) return KQ_EUNSUPPORTED;
+    if (batch->n_rows == 0) return KQ_OK;
     return hip_status(kq::launch_kv_write(kv_cache(*cache), kv_batch(*batch), cache->head_dim, (int)cache->type,
                                           kv_rows(*K), kv_rows(*V), dtype == KQ_BF16,
                                           reinterpret_cast<hipStream_t>(stream)));
@@ -610,6 +613,7 @@ kq_status kq_kv_read(const kq_kv_cache* cache, const kq_kv_batch* batch, const k
     if (st == KQ_OK) st = check_kv_rows(V, batch, cache->heads, cache->head_dim, true);
     if (st != KQ_OK) return st;
     if (!kv_blocks_fit(cache, batch, 16)) return KQ_EUNSUPPORTED;
+    if (batch->n_rows == 0) return KQ_OK;
     return hip_status(kq::launch_kv_read(kv_cache(*cache), kv_batch(*batch), cache->head_dim, (int)cache->type,
                                          kv_rows(*K), kv_rows(*V), dtype, reinterpret_cast<hipStream_t>(stream)));
 }
@@ -646,6 +650,7 @@ kq_status kq_kv_attn(const kq_kv_cache* cache, const kq_kv_batch* batch, const k
         ws_bytes < kq::kv_attn_ws_need(c, b, cache->head_dim, group, window))  // never more than the former
         return KQ_EWORKSPACE;
     if (!aligned(ws, 256)) return KQ_EALIGN;
+    if (batch->n_rows == 0) return KQ_OK;
     const kq::kv::Attn a = {d->scale * 1.4426950408889634f, group, d->causal != 0, window,
                              (65536 + group - 1) / group, d->sinks, lse};
     return hip_status(kq::launch_kv_attn(c, b, cache->head_dim, (int)cache->type, a, kv_rows(*Q), kv_rows(*O),

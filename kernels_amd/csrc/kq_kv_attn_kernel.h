@@ -187,13 +187,19 @@ struct Share {
     uint32_t groups; // that have some
 };
 
-__device__ __forceinline__ int prefix64(int v, int lane) {  // inclusive sum over the wave
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const int w = __shfl_up(v, d);
-        v += lane >= d ? w : 0;
-    }
-    return v;
+// Inclusive sum over the wave, in DPP steps (six exchanges through the LDS unit take 0.3 us, and a
+// share takes up to seven sums): 1, 2, 4 and 8 lanes within rows of 16, then the rows before.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int plus_dpp(int v) {
+    return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false);
+}
+__device__ __forceinline__ int prefix64(int v) {
+    v = plus_dpp<0x111, 0xF>(v);
+    v = plus_dpp<0x112, 0xF>(v);
+    v = plus_dpp<0x114, 0xF>(v);
+    v = plus_dpp<0x118, 0xF>(v);
+    v = plus_dpp<0x142, 0xA>(v);
+    return plus_dpp<0x143, 0xC>(v);
 }
 
 // What group k does; each wave works it out for itself from the units of all sequences.
@@ -221,14 +227,14 @@ __device__ inline Share share_of(const Cache& c, const Batch& b, const Attn& a, 
     auto sum = [&](auto f) {
         int v = 0;
         for (int i = lane; i < n; i += 64) v += f(i < 64 ? u0 : lds[i]);
-        return (uint64_t)(uint32_t)__builtin_amdgcn_readlane(prefix64(v, lane), 63);
+        return (uint64_t)(uint32_t)__builtin_amdgcn_readlane(prefix64(v), 63);
     };
     // the sequence i with sum_{j < i} f <= x < sum_{j <= i} f; x becomes what is left, u its units
     auto find = [&](uint32_t& x, int& u, auto f) {
         int before = 0;
         for (int i0 = 0; i0 < n; i0 += 64) {
             const int mine = i0 + lane < n ? i0 ? lds[i0 + lane] : u0 : 0, v = f(mine);
-            const int up = prefix64(v, lane) + before;
+            const int up = prefix64(v) + before;
             const uint64_t hit = __ballot((uint32_t)(up - v) <= x && x < (uint32_t)up);
             if (hit) {
                 const int l = __ffsll((unsigned long long)hit) - 1;

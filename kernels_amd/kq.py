@@ -487,7 +487,7 @@ def _kv_rows(t, shape, dtype, what):
     if t.shape != shape or t.dtype != dtype:
         raise ValueError(f"{what}: a {dtype} tensor {tuple(shape)}, not {t.dtype} {tuple(t.shape)}")
     row, head, one = t.stride()
-    if one != 1:
+    if one != 1 and shape[0]:
         raise ValueError(f"{what}: contiguous in its last dimension, not strides {t.stride()}")
     return _pack_rows(t.data_ptr(), row, head)
 

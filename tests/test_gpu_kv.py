@@ -511,6 +511,24 @@ def test_python_checks(gpu):
             f()
 
 
+def test_most_sequences(gpu):
+    """65535 sequences, of a token each: written, read back and attended to, which gives the value back."""
+    n = 65535
+    cache = kq.kv_cache(n, 1, 64, device=gpu)
+    pages = torch.randperm(n, device=gpu).to(torch.int32).view(n, 1)
+    b = kq.KVBatch(pages, torch.ones(n, dtype=torch.int32, device=gpu), 16)
+    x = torch.randn((n, 3, 64), device=gpu).half()
+    kq.kv_write(cache, b, x[:, 1:2], x[:, 2:])
+    back = torch.zeros((n, 2, 64), device=gpu)
+    kq.kv_read(cache, b, back[:, :1], back[:, 1:])
+    ws = torch.empty(kq.kv_attn_workspace_size(cache, b, 1), dtype=torch.uint8, device=gpu)
+    out = torch.zeros((n, 1, 64), dtype=torch.float16, device=gpu)
+    kq.kv_attn(cache, b, x[:, :1], out, ws, ws.numel())
+    torch.cuda.synchronize()
+    assert torch.equal(out.float(), back[:, 1:])  # int8 times a power of two is fp16
+    assert (back - x[:, 1:].float()).abs().max() <= 0.5 * 2.0**-4  # |x| < 8: steps of 2^-4 at most
+
+
 def test_offsets_beyond_32_bits(gpu):
     """A cache of over 4 GiB of keys: the last pages' tokens."""
     heads, dim, page = 8, 128, 256

@@ -98,6 +98,15 @@ def test_strides_of_single_rows_and_heads():
     assert attn(cache_c(heads=1), one, attn_c(q_heads=2), rows_c(row=1, head=1), rows_c(), ws=None) == kq.KQ_EINVAL
 
 
+def test_no_rows():
+    """A call of no rows, whose tensors have no address, is checked and does nothing."""
+    none, r = batch_c(n_rows=0), rows_c(p=None)
+    assert write(b=none, K=r, V=r) == write(b=none, K=r, V=r, read=True) == attn(b=none, Q=r, O=r) == kq.KQ_OK
+    assert write(cache_c(type=3), none, r, r) == attn(b=none, Q=r, O=r, dt=kq.F32) == kq.KQ_EUNSUPPORTED
+    assert attn(b=none, Q=r, O=r, ws=None) == kq.KQ_EWORKSPACE
+    assert write(b=batch_c(n_rows=0, q_start=None), K=r, V=r) == kq.KQ_EINVAL
+
+
 @pytest.mark.parametrize("kw", [dict(row=0), dict(head=0), dict(row=120), dict(head=64)])
 def test_overlapping_outputs_are_refused(kw):
     r = rows_c(**kw)
