@@ -91,12 +91,20 @@ __device__ __forceinline__ float finish(const Attn& a, float m, float l, int row
                                         bool write_lse) {
     float total = l == 0.0f ? -__builtin_inff() : __builtin_amdgcn_logf(l) + (m - kLift);  // log2
     float y = l == 0.0f ? 0.0f : 1.0f / l;
+    float lse = total * 0.69314718f;
     if (a.sinks) {
-        const float own = total, sink = a.sinks[head] * 1.44269504f, top = fmaxf(own, sink);
-        total = top + __builtin_amdgcn_logf(__builtin_amdgcn_exp2f(own - top) + __builtin_amdgcn_exp2f(sink - top));
-        y *= __builtin_amdgcn_exp2f(own - total);
+        const float own = total, given = a.sinks[head], sink = given * 1.44269504f, top = fmaxf(own, sink);
+        // no token in sight and a sink of (about) -inf, or a sink that takes all; a NaN stays one
+        if (__builtin_isinf(top) && own == own) {
+            lse = given;
+            y = 0.0f;
+        } else {
+            total = top + __builtin_amdgcn_logf(__builtin_amdgcn_exp2f(own - top) + __builtin_amdgcn_exp2f(sink - top));
+            lse = total * 0.69314718f;
+            y *= __builtin_amdgcn_exp2f(own - total);
+        }
     }
-    if (a.lse && write_lse) a.lse[(int64_t)row * q_heads + head] = total * 0.69314718f;
+    if (a.lse && write_lse) a.lse[(int64_t)row * q_heads + head] = lse;
     return y;
 }
 

@@ -143,7 +143,8 @@ def attend(cache, table, length, q, scale, causal=True, window=0, sinks=None):
             kk, vv = k[sees, h // group], v[sees, h // group]
             s = kk @ q[j, h] * scale
             m = max([s.max() if len(s) else -np.inf, sinks[h] if sinks is not None else -np.inf])
-            if m == -np.inf:
+            if np.isinf(m):  # nothing in sight, or a sink that takes all
+                lse[j, h] = m
                 continue
             w = np.exp(s - m)
             total = w.sum() + (np.exp(sinks[h] - m) if sinks is not None else 0.0)

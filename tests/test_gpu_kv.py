@@ -195,7 +195,7 @@ def attn_case(gpu, seqs, heads, group, dim, kind="i8", dtype="f16", page=16, blo
     cache = upload(oracle, gpu)
     q_heads = heads * group
     qt, q64 = to(rng.normal(0, 1, (b.rows, q_heads, dim)) * np.exp(rng.normal(0, 0.7, (b.rows, q_heads, 1))) if q is None else q(b, q_heads), dtype, gpu)
-    s = rng.normal(0, 3, q_heads).astype(np.float32) if sinks else None
+    s = rng.normal(0, 3, q_heads).astype(np.float32) if sinks is True else np.float32(sinks) if sinks else None
     out = torch.full((b.rows, q_heads, dim), 7.0, dtype=DTYPES[dtype], device=gpu)
     ls = torch.full((b.rows, q_heads), 7.0, device=gpu) if lse else None
     n = kq.kv_attn_workspace_size(cache, b.c, q_heads)
@@ -218,8 +218,8 @@ def attn_case(gpu, seqs, heads, group, dim, kind="i8", dtype="f16", page=16, blo
         assert np.isfinite(got).all() and (off <= tol).all(), (i, float(np.nanmax(off / tol)), np.argwhere(~(off <= tol))[:3].tolist())
         if lse:
             have = ls[rows].double().cpu().numpy()
-            none = np.isneginf(want[1])
-            assert np.array_equal(np.isneginf(have), none)
+            none = np.isinf(want[1])
+            assert np.array_equal(np.isinf(have), none) and np.array_equal(have[none], want[1][none])
             off = np.abs(have[~none] - want[1][~none])
             assert (off <= tol_lse[~none]).all(), (i, np.nanmax(off / tol_lse[~none]))
     assert (out[b.starts[-1]:] == 7.0).all() and (ls is None or (ls[b.starts[-1]:] == 7.0).all()), "rows behind the last sequence"
@@ -314,6 +314,12 @@ def test_scales(gpu, scale):
     attn_case(gpu, [(100, 1), (65, 3)], 2, 2, 64, scale=scale)
 
 
+@pytest.mark.parametrize("seqs,window", [([(0, 1), (1, 1), (70, 1), (2, 3)], 0), ([(1, 1), (5000, 1), (0, 1)], 0), ([(300, 1), (90, 40), (0, 20)], 7)])
+def test_sinks_without_bounds(gpu, seqs, window):
+    """A sink of -inf is none, also for a row that sees nothing; one of inf leaves nothing of the values."""
+    attn_case(gpu, seqs, 2, 4, 128, window=window, sinks=[-np.inf, np.inf, 0.5, -np.inf, np.inf, -3e38, -np.inf, 3e38])
+
+
 def test_query_range(gpu):
     """Queries from the smallest to the largest of bf16 (with a scale that keeps the scores moderate), and rows of zeros."""
     def tiny(b, q_heads):
@@ -402,6 +408,11 @@ def test_nan_and_infinite_queries_stay_in_their_row(gpu):
         bad[1, 2] = bad[3, 0] = True
         assert torch.isnan(out[bad]).all() and torch.equal(out[~bad], clean[~bad])
         assert torch.isnan(lse[bad]).all() and torch.isfinite(lse[~bad]).all()
+        for sink in (-float("inf"), float("inf")):  # none; or one that takes all
+            kq.kv_attn(cache, b.c, q, out, ws, ws.numel(), sinks=torch.full((4,), sink, device=gpu), lse=lse)
+            torch.cuda.synchronize()
+            assert torch.isnan(out[bad]).all() and torch.equal(out[~bad], clean[~bad] if sink < 0 else torch.zeros_like(clean[~bad]))
+            assert torch.isnan(lse[bad]).all()
 
 
 def test_pages_that_are_none(gpu):
