@@ -214,7 +214,7 @@ kq::kv::Rows kv_rows(const kq_kv_rows& r) { return {r.p, r.row, r.head}; }
 
 // Workgroups of a launch over the `unit`-token blocks of max_q tokens (grid.x).
 bool kv_blocks_fit(const kq_kv_cache* c, const kq_kv_batch* b, uint32_t unit) {
-    return ((uint64_t)(b->max_q / unit) + 2) * ((2 * c->heads + 3) / 4) < 0x7FFFFFFFull;
+    return ((uint64_t)(b->max_q / unit) + 2) * ((2 * c->heads + 3) / 4) <= kq::kv::kMostGroups;
 }
 
 kq_status check_kv_heads(const kq_kv_cache* c, uint32_t q_heads) {
@@ -622,7 +622,7 @@ size_t kq_kv_attn_workspace_size(const kq_kv_cache* cache, const kq_kv_batch* ba
     if (check_kv(cache, batch) != KQ_OK || check_kv_heads(cache, q_heads) != KQ_OK) return 0;
     const kq::kv::Batch b = kv_batch(*batch);
     const uint32_t group = q_heads / cache->heads;
-    if (!kq::kv_attn_fits(kv_cache(*cache), b, group)) return 0;
+    if (!kq::kv_attn_fits(kv_cache(*cache), b, cache->head_dim, group)) return 0;
     return kq::kv_attn_ws_bytes(kv_cache(*cache), b, cache->head_dim, group);
 }
 
@@ -636,7 +636,8 @@ kq_status kq_kv_attn(const kq_kv_cache* cache, const kq_kv_batch* batch, const k
     if (!(dtype == KQ_F16 || dtype == KQ_BF16)) return KQ_EUNSUPPORTED;
     st = check_kv_heads(cache, d->q_heads);
     if (st != KQ_OK) return st;
-    if (!(d->scale - d->scale == 0.0f) || (d->window && !d->causal)) return KQ_EINVAL;
+    const float scale_log2 = d->scale * 1.4426950408889634f;
+    if (!(scale_log2 - scale_log2 == 0.0f) || (d->window && !d->causal)) return KQ_EINVAL;
     st = check_kv_rows(Q, batch, d->q_heads, cache->head_dim, false);
     if (st == KQ_OK) st = check_kv_rows(O, batch, d->q_heads, cache->head_dim, true);
     if (st != KQ_OK) return st;
@@ -645,13 +646,13 @@ kq_status kq_kv_attn(const kq_kv_cache* cache, const kq_kv_batch* batch, const k
     const kq::kv::Batch b = kv_batch(*batch);
     const uint32_t group = d->q_heads / cache->heads;
     const uint32_t window = d->window < batch->max_len ? d->window : 0;  // as wide as all there is: none
-    if (!kq::kv_attn_fits(c, b, group)) return KQ_EUNSUPPORTED;
+    if (!kq::kv_attn_fits(c, b, cache->head_dim, group)) return KQ_EUNSUPPORTED;
     if (!ws || ws_bytes < kq::kv_attn_ws_bytes(c, b, cache->head_dim, group) ||
         ws_bytes < kq::kv_attn_ws_need(c, b, cache->head_dim, group, window))  // never more than the former
         return KQ_EWORKSPACE;
     if (!aligned(ws, 256)) return KQ_EALIGN;
     if (batch->n_rows == 0) return KQ_OK;
-    const kq::kv::Attn a = {d->scale * 1.4426950408889634f, group, d->causal != 0, window,
+    const kq::kv::Attn a = {scale_log2, group, d->causal != 0, window,
                              (65536 + group - 1) / group, d->sinks, lse};
     return hip_status(kq::launch_kv_attn(c, b, cache->head_dim, (int)cache->type, a, kv_rows(*Q), kv_rows(*O),
                                          dtype == KQ_BF16, ws, reinterpret_cast<hipStream_t>(stream)));

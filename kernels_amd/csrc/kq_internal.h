@@ -175,6 +175,8 @@ struct Rows {
     void* p;
     int64_t row, head;
 };
+// Workgroups of 256 threads that a launch can have: HIP counts its threads in 32 bits.
+constexpr uint64_t kMostGroups = (1ull << 24) - 1;
 // What a call of the attention asks for.
 struct Attn {
     float scale_log2;  // scale * log2(e)
@@ -201,11 +203,12 @@ struct FewPlan {
 // Sixteens of rows that its registers hold, and the waves of a SIMD they allow then.
 constexpr uint32_t few_sixteens(uint32_t D) { return D <= 128 ? 2 : 1; }
 constexpr uint32_t few_waves(uint32_t D) { return D == 256 ? 1 : 2; }
-// Rows of a tile of the kernel for many rows, at most.
-#ifndef KV_ROWMOST
-#define KV_ROWMOST (D == 96 || D == 128 ? 256 : 128)
-#endif
-constexpr uint32_t row_most(uint32_t D) { return KV_ROWMOST; }
+// Rows of a tile of the kernel for many rows, at most. 256 rows read a tile's codes half
+// as often: at 128 wide 615 us against 691 (a chunk of 2048 tokens behind 30000, 32 heads
+// over 8). At 64 wide the tile's products are too short for eight waves to share (a prefill
+// of 4096: 200 us against 174 with 128 rows), and at 192 and 256 a wave's output does not
+// leave the registers for two waves of a SIMD.
+constexpr uint32_t row_most(uint32_t D) { return D == 96 || D == 128 ? 256 : 128; }
 // Launch of the kernel for many rows.
 struct RowPlan {
     uint32_t rows;    // of a tile: 128 or 256, 32 a wave
@@ -249,7 +252,7 @@ struct AttnKernels {
 // can be made.
 size_t kv_attn_ws_need(const kv::Cache& c, const kv::Batch& b, uint32_t D, uint32_t group, uint32_t window);
 size_t kv_attn_ws_bytes(const kv::Cache& c, const kv::Batch& b, uint32_t D, uint32_t group);
-bool kv_attn_fits(const kv::Cache& c, const kv::Batch& b, uint32_t group);
+bool kv_attn_fits(const kv::Cache& c, const kv::Batch& b, uint32_t D, uint32_t group);
 hipError_t launch_kv_attn(const kv::Cache& c, const kv::Batch& b, uint32_t D, int type, const kv::Attn& a,
                           const kv::Rows& Q, const kv::Rows& O, bool bf, void* ws, hipStream_t s);
 

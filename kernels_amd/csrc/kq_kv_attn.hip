@@ -90,8 +90,13 @@ size_t kv_attn_ws_bytes(const kv::Cache& c, const kv::Batch& b, uint32_t D, uint
     return n > 256 ? (n + 255) / 256 * 256 : 256;
 }
 
-bool kv_attn_fits(const kv::Cache& c, const kv::Batch& b, uint32_t group) {
-    return (uint64_t)b.n_seq * b.max_q * c.heads * group < 0x7FFF0000ull;
+bool kv_attn_fits(const kv::Cache& c, const kv::Batch& b, uint32_t D, uint32_t group) {
+    if ((uint64_t)b.n_seq * b.max_q * c.heads * group >= 0x7FFF0000ull) return false;
+    // Shares, parts and splits are made of few rows of work, and are few.
+    const uint64_t rows = (uint64_t)b.n_seq * c.heads;
+    if (kv::few(b, group)) return (rows + 7) / 8 * 8 * kv::few_plan(c, b, D, group, 0).tiles <= kv::kMostGroups;
+    const kv::RowPlan p = kv::row_plan(c, b, D, group, 0);
+    return rows * p.tiles * (p.rows / 128) <= kv::kMostGroups;
 }
 
 hipError_t launch_kv_attn(const kv::Cache& c, const kv::Batch& b, uint32_t D, int type, const kv::Attn& a,

@@ -61,8 +61,10 @@ __global__ __launch_bounds__(256) void kv_write_k(Cache c, Batch b, Rows K, Rows
     const bool is_v = job & 1;
     const Seq s = sequence(b, c.page_log2, blockIdx.y);
     const int first = s.len - s.n, first0 = max(first, 0), B = 1 << c.block_log2;
-    const int t0 = ((first0 >> c.block_log2) + (int)(blockIdx.x / groups)) << c.block_log2;
-    if (s.n == 0 || t0 >= s.len) return;
+    // unsigned: blocks behind a sequence of nearly 2^31 tokens pass 31 bits
+    const uint32_t t0u = (((uint32_t)first0 >> c.block_log2) + blockIdx.x / groups) << c.block_log2;
+    if (s.n == 0 || t0u >= (uint32_t)s.len) return;
+    const int t0 = (int)t0u;
     const int page = page_of(c, b.pages + (uint64_t)blockIdx.y * b.max_pages, t0);
     const int lo = max(first0 - t0, 0), hi = min(s.len - t0, B);  // the block's new tokens
     const Rows& R = is_v ? V : K;
@@ -247,8 +249,9 @@ __global__ __launch_bounds__(256) void kv_read_k(Cache c, Batch b, Rows K, Rows 
     const bool is_v = job & 1;
     const Seq s = sequence(b, c.page_log2, blockIdx.y);
     const int first = s.len - s.n, first0 = max(first, 0);
-    const int t0 = (first0 / SPAN + (int)(blockIdx.x / groups)) * SPAN;
-    if (s.n == 0 || t0 >= s.len) return;
+    const uint32_t t0u = ((uint32_t)first0 / SPAN + blockIdx.x / groups) * SPAN;  // unsigned, as in kv_write_k
+    if (s.n == 0 || t0u >= (uint32_t)s.len) return;
+    const int t0 = (int)t0u;
     const int lo = max(first0 - t0, 0), hi = min(s.len - t0, SPAN);
     const int32_t* const table = b.pages + (uint64_t)blockIdx.y * b.max_pages;
     const Rows& R = is_v ? V : K;

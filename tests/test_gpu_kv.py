@@ -540,6 +540,32 @@ def test_most_sequences(gpu):
     assert (back - x[:, 1:].float()).abs().max() <= 0.5 * 2.0**-4  # |x| < 8: steps of 2^-4 at most
 
 
+@pytest.mark.parametrize("max_q", [1, 1 << 20, 100 << 20])
+def test_longest_sequence(gpu, max_q):
+    """The newest tokens of a sequence of nearly 2^31, all of whose pages are the same one: written and read back, whatever
+    the bound on their number, with which blocks behind it would be counted past 2^31."""
+    page, longest, new = 4096, 0x7FFEFFFF, 40
+    cache = kq.kv_cache(3, 1, 64, page=page, block=16, device=gpu)
+    table = torch.ones((1, -(-longest // page)), dtype=torch.int32, device=gpu)
+    length, new = torch.tensor([longest], dtype=torch.int32, device=gpu), min(new, max_q)
+    start = torch.tensor([0, new], dtype=torch.int32, device=gpu)
+    b = kq.KVBatch(table, length, longest, q_start=start, max_q=max_q)
+    x = torch.randn((new, 2, 64), device=gpu).half()
+    before = [t.view(torch.int8).clone() for t in (cache.k, cache.v, cache.k_exp, cache.v_exp)]
+    print(f"max_q {max_q}", flush=True)
+    kq.kv_write(cache, b, x[:, :1], x[:, 1:])
+    back = torch.zeros((new + 1, 2, 64), device=gpu)
+    kq.kv_read(cache, b, back[:, :1], back[:, 1:])
+    torch.cuda.synchronize()
+    assert (back[:new] - x.float()).abs().max() <= 0.5 * 2.0**-4 and (back[new] == 0).all()  # |x| < 8
+    last = (longest - 1) % page
+    for t, old in zip((cache.k, cache.v, cache.k_exp, cache.v_exp), before):
+        t = t.view(torch.int8)
+        assert torch.equal(t[0], old[0]) and torch.equal(t[2], old[2])
+    same = cache.k.view(torch.int8)[1, 0] == before[0][1, 0]
+    assert same[:last - new + 1].all() and same[last + 1:].all()
+
+
 def test_offsets_beyond_32_bits(gpu):
     """A cache of over 4 GiB of keys: the last pages' tokens."""
     heads, dim, page = 8, 128, 256

@@ -191,6 +191,38 @@ def test_launches_too_large():
     assert attn(b=b, n=(1 << 63)) == kq.KQ_EUNSUPPORTED
 
 
+@pytest.mark.parametrize("n_seq,max_q,heads,group,dim,groups", [
+    # rows of work, by the tiles of 16 or 32 rows of each (up to 64 rows) ...
+    (16384, 1, 1024, 1, 64, 1 << 24), (65535, 1, 256, 64, 192, 65535 * 256 * 4), (32768, 2, 512, 16, 256, 2 << 24),
+    # ... or by the 128s of rows
+    (4096, 65, 1024, 2, 128, 2 << 22), (12000, 129, 1024, 1, 128, 12000 * 1024 * 2), (12000, 129, 1024, 1, 64, 12000 * 1024 * 2),
+    (1 << 12, 250000, 1, 1, 96, 977 * 2 << 12)])
+def test_launch_limits_of_the_attention(n_seq, max_q, heads, group, dim, groups):
+    """2^24 workgroups of 256 threads, which HIP can't launch, are refused; a sixteenth of them is not."""
+    q = rows_c(row=heads * group * dim, head=dim)
+    for part in (1, 16):
+        assert n_seq * max_q * heads * group // part < 2**31 - 2**16
+        refused = groups // part >= 1 << 24
+        b = batch_c(n_seq=n_seq // part, max_q=max_q, n_rows=0)
+        c, d = cache_c(heads=heads, head_dim=dim), attn_c(q_heads=heads * group)
+        assert (size(c, b, heads * group) == 0) == refused
+        assert attn(c, b, d, q, q, n=1 << 62) == (kq.KQ_EUNSUPPORTED if refused else kq.KQ_OK)
+
+
+@pytest.mark.parametrize("read,block", [(False, 16), (False, 256), (True, 256)])
+def test_launch_limits_of_writing_and_reading(read, block):
+    unit = 16 if read else block
+    most = ((1 << 24) - 1) // 2 - 2  # blocks of 2 workgroups each: four heads' K and V
+    for blocks, status in ((most, kq.KQ_OK), (most + 1, kq.KQ_EUNSUPPORTED)):
+        b = batch_c(n_seq=1, max_q=min(blocks * unit, 2**31 - 2**17), n_rows=0)
+        if b.max_q == blocks * unit:
+            assert write(cache_c(heads=4, page=256, block=block), b, read=read) == status
+
+
+def test_scale_whose_log2_is_no_number():
+    assert attn(d=attn_c(scale=3e38)) == attn(d=attn_c(scale=-3e38)) == kq.KQ_EINVAL
+
+
 def test_packed_structs():
     """What kq.py passes as bytes is what the C structs hold."""
     assert bytes(batch_c(pages=1, kv_len=2, q_start=3)) == kq._pack_batch(1, 2, 3, 2, 8, 3, 6, 100)
