@@ -55,7 +55,7 @@ __device__ __forceinline__ uint32_t four_codes(float a, float b, float c, float 
 template <int D, int TYPE, int BF>
 __global__ __launch_bounds__(256) void kv_write_k(Cache c, Batch b, Rows K, Rows V, uint32_t groups) {
     const int lane = threadIdx.x & 63;
-    const uint32_t job = (blockIdx.x % groups) * 4 + (threadIdx.x >> 6);
+    const uint32_t job = (blockIdx.x % groups) * 4 + (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     if (job >= 2 * c.heads) return;
     const uint32_t h = job >> 1;
     const bool is_v = job & 1;
@@ -76,7 +76,9 @@ __global__ __launch_bounds__(256) void kv_write_k(Cache c, Batch b, Rows K, Rows
     constexpr int NK = D / 32, H = D == 64 ? 2 : 1, TL = 16 / H, NV = (D / 2 * H + 63) / 64;
     u32x4 xk[NK];
     uint32_t xv[NV][TL];
-    auto load = [&](int sub) {
+    // (inlined by force: of functions of their own, which the compiler makes of the two at 192 and 256 wide, the
+    // values' registers go through memory; 13k tokens of 8 heads of 256 written and read 64 us, 143 so)
+    auto load = [&](int sub) __attribute__((always_inline)) {
         if (!is_v) {
 #pragma unroll
             for (int j = 0; j < NK; ++j) {
@@ -141,7 +143,7 @@ __global__ __launch_bounds__(256) void kv_write_k(Cache c, Batch b, Rows K, Rows
     // a foreign cache may hold any byte: stay within pow2f's range
     const float scale = pow2f(min(max(-e, -126), 127));
     if (lane == 0) *ep = (uint8_t)(e + 127);
-    auto write = [&](auto plain) {
+    auto write = [&](auto plain) __attribute__((always_inline)) {
         constexpr bool P = decltype(plain)::value;
         for (int sub = grew ? 0 : lo & ~15; sub < hi; sub += 16) {
             if (B > 16) load(sub);
@@ -243,7 +245,7 @@ __device__ __forceinline__ void put8(uint8_t* to, const float (&y)[8]) {
 template <int D, int TYPE, int F, int SPAN>
 __global__ __launch_bounds__(256) void kv_read_k(Cache c, Batch b, Rows K, Rows V, uint32_t groups) {
     const int lane = threadIdx.x & 63;
-    const uint32_t job = (blockIdx.x % groups) * 4 + (threadIdx.x >> 6);
+    const uint32_t job = (blockIdx.x % groups) * 4 + (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     if (job >= 2 * c.heads) return;
     const uint32_t h = job >> 1;
     const bool is_v = job & 1;
