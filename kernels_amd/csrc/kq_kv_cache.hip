@@ -262,20 +262,22 @@ __global__ __launch_bounds__(256) void kv_read_k(Cache c, Batch b, Rows K, Rows 
     uint8_t* const out = static_cast<uint8_t*>(R.p) +
                          ((int64_t)(s.row0 + t0 - first) * R.row + (int64_t)h * R.head) * kSize;
     const int64_t pitch = R.row * kSize;
-    // its 16-token blocks: where their codes are, and their scales; no page: zeros of anything
+    // its 16-token blocks: where their codes are, and their exponents; no page: zeros of anything
     constexpr int N = SPAN / 16, C = N == 1 ? 2 : 4;  // columns of 16 values a lane
+    constexpr int kNone = -1;
     const uint8_t* from[N];
-    float scales[N];
+    int exps[N];  // bytes
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         const int t = min(t0 + 16 * i, s.len - 1), page = page_of(c, table, t);
         from[i] = (is_v ? c.v : c.k) + code_offset(c, D, max(page, 0), h, t);
-        scales[i] = (float)((is_v ? c.v_exp : c.k_exp)[exp_offset(c, max(page, 0), h, t)]);
-        if (page < 0) scales[i] = -1.0f;
+        exps[i] = (is_v ? c.v_exp : c.k_exp)[exp_offset(c, max(page, 0), h, t)];
+        if (page < 0) exps[i] = kNone;
     }
-#pragma unroll
-    for (int i = 0; i < N; ++i) scales[i] = scales[i] < 0.0f ? 0.0f : pow2f(max((int)scales[i] - 127, -126));
-    auto value = [&](uint32_t byte, float scale) { return scale == 0.0f ? 0.0f : saturate<F>(Code<TYPE>::value(byte) * scale); };
+    // not times 2^(e - 127), which is no normal float at bytes 0 and 255
+    auto value = [&](uint32_t byte, int e) {
+        return e == kNone ? 0.0f : saturate<F>(__builtin_ldexpf(Code<TYPE>::value(byte), e - 127));
+    };
     if (!is_v) {
 #pragma unroll
         for (int n = 0; n < N; ++n) {
@@ -288,7 +290,7 @@ __global__ __launch_bounds__(256) void kv_read_k(Cache c, Batch b, Rows K, Rows 
                 const int i = lane + 64 * j, t = 16 * n + i / (D / 8);  // 8 columns of token t
                 float y[8];
 #pragma unroll
-                for (int k = 0; k < 8; ++k) y[k] = value(w[j][k / 4] >> k % 4 * 8 & 0xFF, scales[n]);
+                for (int k = 0; k < 8; ++k) y[k] = value(w[j][k / 4] >> k % 4 * 8 & 0xFF, exps[n]);
                 if (t >= lo && t < hi) put8<F>(out + t * pitch + i % (D / 8) * 8 * kSize, y);
             }
         }
@@ -298,11 +300,11 @@ __global__ __launch_bounds__(256) void kv_read_k(Cache c, Batch b, Rows K, Rows 
     for (int j = 0; j < (N * D / C + 63) / 64; ++j) {
         const int i = lane + 64 * j, n = i / (D / C), t = n * 16, d = i % (D / C) * C;  // C columns of block n
         if (t + 16 <= lo || t >= hi) continue;  // hi <= SPAN: past the last block too
-        float scale = scales[0];
+        int e = exps[0];
         const uint8_t* at = from[0];
 #pragma unroll
         for (int k = 1; k < N; ++k) {
-            scale = n == k ? scales[k] : scale;
+            e = n == k ? exps[k] : e;
             at = n == k ? from[k] : at;
         }
         at += d * 16;
@@ -313,7 +315,7 @@ __global__ __launch_bounds__(256) void kv_read_k(Cache c, Batch b, Rows K, Rows 
         for (int q = 0; q < 16; ++q) {
             float y[C];
 #pragma unroll
-            for (int k = 0; k < C; ++k) y[k] = value(w[k][q / 4] >> q % 4 * 8 & 0xFF, scale);
+            for (int k = 0; k < C; ++k) y[k] = value(w[k][q / 4] >> q % 4 * 8 & 0xFF, e);
             if (t + q < lo || t + q >= hi) continue;
             if constexpr (C == 4) put4<F>(out + (t + q) * pitch + d * kSize, y);
             else put2<F>(out + (t + q) * pitch + d * kSize, y);
