@@ -141,8 +141,8 @@ __global__ __launch_bounds__(256) void kv_write_k(Cache c, Batch b, Rows K, Rows
     const int e = max(wanted, was);
     const bool grew = lo > 0 && wanted > was;
     const float keep = pow2f(max(was - e, -126));  // what older codes are multiplied by
-    // a foreign cache may hold any byte: stay within pow2f's range
-    const float scale = pow2f(min(max(-e, -126), 127));
+    // e >= kMinExp; up to 128 where a cache from elsewhere holds such a byte: a subnormal scale, exact too
+    const float scale = __builtin_ldexpf(1.0f, -e);
     if (lane == 0) *ep = (uint8_t)(e + 127);
     auto write = [&](auto plain) __attribute__((always_inline)) {
         constexpr bool P = decltype(plain)::value;

@@ -38,3 +38,28 @@ def test_read(gpu, dim, kind, out):
             bad = (have != want).nonzero()
             first = tuple(bad[0].tolist()) if len(bad) else None
             assert first is None, (w, i, first, have[first].item(), want[first].item(), len(bad))
+
+
+@pytest.mark.parametrize("kind", ["i8", "e4m3"])
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("dim,block", [(64, 16), (128, 32)])
+def test_write(gpu, dim, block, dtype, kind):
+    """Tokens appended to blocks of any byte: the byte stays where it is the larger, and the new codes are x / 2^(byte - 127)."""
+    rng = np.random.default_rng(dim)
+    was = (0, 1, 10, 62, 63, 64, 127, 190, 246, 248, 252, 253, 254, 255)
+    seqs = [(block + 9, 4)] * len(was)
+    b = Batch(gpu, seqs, block, rng)
+    oracle = _kv.Cache(b.n_pages, 1, dim, block, block, kind)
+    oracle.fill(rng)
+    for i, e in enumerate(was):
+        for w in "kv":
+            oracle.exps[w][b.table[i, 1]] = e
+    cache = upload(oracle, gpu)
+    size = 3.3e38 if dtype == "bf16" else 6e4
+    x = {w: to(np.sign(rng.normal(0, 1, (b.rows, 1, dim))) * size * 2.0 ** -rng.integers(0, 9, (b.rows, 1, dim)), dtype, gpu) for w in "kv"}
+    kq.kv_write(cache, b.c, x["k"][0], x["v"][0])
+    torch.cuda.synchronize()
+    for w in "kv":
+        for i, (n, m) in enumerate(seqs):
+            oracle.write(w, x[w][1][b.starts[i]:b.starts[i + 1]], b.table[i], n, m)
+    same_cache(cache, oracle)
