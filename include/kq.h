@@ -496,7 +496,8 @@ kq_status kq_kv_read(const kq_kv_cache* cache, const kq_kv_batch* batch, const k
  * than 2^-36 of it they are lost, in O alone).
  * A cache from elsewhere holds no NaN codes (e4m3 0x7F, 0xFF) below kv_len, or
  * rows of that sequence and head may be NaN; behind it any bytes do. The
- * exponents of a sequence and head's values differ by 100 at most.
+ * exponents of a sequence and head's V, of all its blocks below kv_len, differ
+ * by 100 at most, wherever in 0 .. 255 they lie.
  * ws: kq_kv_attn_workspace_size bytes (enough for any window), 256-byte
  * aligned, no initialisation and nothing kept in it between calls: the partial
  * results of sequences that are split among workgroups. Calls that share one must be

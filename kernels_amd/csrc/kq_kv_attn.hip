@@ -50,7 +50,7 @@ FewPlan few_plan(const Cache& c, const Batch& b, uint32_t D, uint32_t group, uin
 }
 // Descriptors and slots.
 size_t few_ws_bytes(const FewPlan& p, uint32_t D) {
-    return p.mode == FewPlan::kRows ? 0 : (size_t)p.groups * (sizeof(Cut) + 2 * p.tiles * 16 * p.sixteens * (D + 2) * 4);
+    return p.mode == FewPlan::kRows ? 0 : (size_t)p.groups * (sizeof(Cut) + 2 * p.tiles * 16 * p.sixteens * (D + kRowSum) * 4);
 }
 
 uint64_t row_splits_wanted(const Cache& c, const Batch& b, const RowPlan& p) {
@@ -67,7 +67,7 @@ RowPlan row_plan(const Cache& c, const Batch& b, uint32_t D, uint32_t group, uin
     return p;
 }
 size_t row_ws_bytes(const Cache& c, const Batch& b, const RowPlan& p, uint64_t splits, uint32_t D) {
-    return splits > 1 ? (size_t)b.n_seq * splits * p.tiles * c.heads * p.rows * (D + 2) * 4 : 0;
+    return splits > 1 ? (size_t)b.n_seq * splits * p.tiles * c.heads * p.rows * (D + kRowSum) * 4 : 0;
 }
 
 }  // namespace

@@ -12,7 +12,8 @@
 //         (k place 8g + j <-> token 16g + 8h + j), and the matching V operand is
 //         the 16 bytes that hold column d of the lane's 16 tokens.
 // With t_p = log2(e) s_p + e_v(p), the probabilities and V's scale are one number
-// w_p = 2^(t_p - m); the denominator is the sum of w_p 2^-e_v(p).
+// w_p = 2^(t_p - m); the denominator is the sum of w_p 2^-e_v(p), kept times a power of two
+// where float32's range asks for it.
 #pragma once
 #include "kq_kv_device.h"
 
@@ -30,6 +31,27 @@ constexpr float kSlack = 4.0f;
 constexpr int kIds = 4096;     // page ids that a workgroup holds at a time
 constexpr int kScan = 1024;    // most sequences whose lengths a workgroup adds up
 constexpr float kLowest = -3.0e38f;  // reference before any token
+
+// The denominator's terms w 2^(127 - byte), of V's bytes, lie between 2^11 2^-128 and 2^15 2^127, which float32 does not
+// hold: a wave keeps their sums l times 2^(base - 127), the base a byte. It is 127, and moves, l with it, only where a
+// block's byte is more than 64 below it (2^31 such tokens' sum is finite) or more than 110 above (a term of the row's largest
+// is normal): never for bytes from 63 to 237, and to 64 or 145 at most. What that costs: up to 1% (131071 tokens, 64 / 8
+// heads of 128: 56.9 us in a graph, 56.7 without; a prefill of 4 prompts, 64 wide: 167, 167), but 3% for many short
+// sequences 64 wide, whose kernel goes from 126 to 130 registers (73 of 100 to 1795 tokens: 28.4 us, 27.5 without).
+constexpr int kBase = 127;
+__device__ __forceinline__ bool base_far(int base, int byte) { return (uint32_t)(base + 110 - byte) > 174u; }
+// The base that suits the bytes low .. high of the wave's lanes (which differ by 100 at most).
+__device__ __forceinline__ int base_near(int base, int low, int high) {
+    low = (int)~wave_max(~(uint32_t)low);
+    high = (int)wave_max((uint32_t)high);
+    return __builtin_amdgcn_readfirstlane(min(max(base, high - 110), low + 64));
+}
+// What a row's parts are joined by.
+struct alignas(16) RowSum {
+    float m, l;
+    int base, unused;
+};
+constexpr int kRowSum = sizeof(RowSum) / sizeof(float);
 
 // Tokens that rows row .. row + rows - 1 of a sequence and head see: [lo, hi), lo a multiple of 64.
 struct Span {
@@ -86,10 +108,10 @@ __device__ __forceinline__ void store4(const Rows& O, int row, uint32_t head, in
 }
 
 // The last step of a row: joins the sink, writes lse, and returns what the row's sums are
-// multiplied by. m and l as the waves keep them: l = sum 2^(s log2e + kLift - m).
-__device__ __forceinline__ float finish(const Attn& a, float m, float l, int row, uint32_t head, uint32_t q_heads,
+// multiplied by, before 2^(base - 127). m, l and base as the waves keep them: l = 2^(base - 127) sum 2^(s log2e + kLift - m).
+__device__ __forceinline__ float finish(const Attn& a, float m, float l, int base, int row, uint32_t head, uint32_t q_heads,
                                         bool write_lse) {
-    float total = l == 0.0f ? -__builtin_inff() : __builtin_amdgcn_logf(l) + (m - kLift);  // log2
+    float total = l == 0.0f ? -__builtin_inff() : __builtin_amdgcn_logf(l) + (m - kLift) - (float)(base - 127);  // log2
     float y = l == 0.0f ? 0.0f : 1.0f / l;
     float lse = total * 0.69314718f;
     if (a.sinks) {
@@ -105,6 +127,12 @@ __device__ __forceinline__ float finish(const Attn& a, float m, float l, int row
         }
     }
     if (a.lse && write_lse) a.lse[(int64_t)row * q_heads + head] = lse;
+    return y;
+}
+
+__device__ __forceinline__ f32x4 from_base(f32x4 y, int base) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] = __builtin_ldexpf(y[i], base - 127);
     return y;
 }
 
@@ -306,10 +334,10 @@ __device__ inline Share share_of(const Cache& c, const Batch& b, const Attn& a, 
 struct Cut {
     int seq, head, first, parts;
 };
-// The partial results of slot i and row tile t: [16 R][D] sums, then [16 R] (m, l).
+// The partial results of slot i and row tile t: [16 R][D] sums, then [16 R] of RowSum.
 template <int D, int R>
 __device__ __forceinline__ float* slot_of(float* ws, const FewPlan& p, uint32_t i, uint32_t t) {
-    return ws + p.cuts * 4 + ((uint64_t)i * p.tiles + t) * (16 * R * (D + 2));
+    return ws + p.cuts * 4 + ((uint64_t)i * p.tiles + t) * (16 * R * (D + kRowSum));
 }
 
 // Few rows (tokens x heads of a group) of a sequence and head, 16 R a workgroup. Four waves take 64 tokens
@@ -326,6 +354,7 @@ __global__ __launch_bounds__(256, few_waves(D)) void kv_few_k(Cache c, Batch b, 
     constexpr int kPad = D + 4;
     __shared__ __attribute__((aligned(16))) float o_lds[4 * 16 * R * kPad];
     __shared__ float m_lds[4][16 * R], l_lds[4][16 * R];
+    __shared__ int base_lds[4];
     static_assert(sizeof(o_lds) >= kIds * sizeof(int) && kIds >= kScan, "page ids, units of the sequences");
     int* const ids = reinterpret_cast<int*>(o_lds);  // page ids of the piece, until the waves join
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 15, g = lane >> 4;
@@ -360,7 +389,7 @@ __global__ __launch_bounds__(256, few_waves(D)) void kv_few_k(Cache c, Batch b, 
             // this lane's row of each sixteen
             f16x8 q[R][D / 32];
             float m[R], l[R];  // of the row; l: this lane's tokens alone
-            int q_exp[R], sees_lo[R], sees_hi[R];
+            int q_exp[R], sees_lo[R], sees_hi[R], base = kBase;
             f32x4 o[R][D / 16];
 #pragma unroll
             for (int k = 0; k < R; ++k) {
@@ -428,7 +457,16 @@ __global__ __launch_bounds__(256, few_waves(D)) void kv_few_k(Cache c, Batch b, 
                 __builtin_amdgcn_sched_barrier(0);
 
                 const int tv = t0 + 16 * g;
-                const float un_v = pow2f(min(max(127 - ve, -126), 127));
+                const bool part = t0 + kTile > hi || __any(pv < 0);  // blocks among them that hold anything
+                int byte = ve;
+                if (part && (tv >= hi || pv < 0)) byte = kBase;
+                if (__any(base_far(base, byte))) {
+                    const int to = base_near(base, byte, byte);
+#pragma unroll
+                    for (int k = 0; k < R; ++k) l[k] = __builtin_ldexpf(l[k], to - base);
+                    base = to;
+                }
+                const float un_v = pow2f(base - byte);
                 f16x8 w[R][2];
 #pragma unroll
                 for (int k = 0; k < R; ++k) {
@@ -467,7 +505,7 @@ __global__ __launch_bounds__(256, few_waves(D)) void kv_few_k(Cache c, Batch b, 
                     }
                     l[k] += sum * un_v;
                 }
-                if (t0 + kTile > hi || __any(pv < 0)) {
+                if (part) {
                     // bytes of tokens that no length covers may hold anything, NaN among it
                     const int valid = pv < 0 ? 0 : min(max(hi - tv, 0), 16);
 #pragma unroll
@@ -526,6 +564,7 @@ __global__ __launch_bounds__(256, few_waves(D)) void kv_few_k(Cache c, Batch b, 
                     l_lds[wave][16 * k + r] = l[k];
                 }
             }
+            if (lane == 0) base_lds[wave] = base;
             __syncthreads();
 #pragma unroll
             for (int k = 0; k < R; ++k) {
@@ -538,6 +577,7 @@ __global__ __launch_bounds__(256, few_waves(D)) void kv_few_k(Cache c, Batch b, 
                 for (int i = 0; i < D / 16; ++i) *reinterpret_cast<f32x4*>(to + i * 16 + g * 4) = o[k][i] * fade;
             }
             __syncthreads();
+            const int one = min(min(base_lds[0], base_lds[1]), min(base_lds[2], base_lds[3]));
             for (int i = tid; i < min(rows, 16 * R) * (D / 4); i += 256) {
                 const int row = i / (D / 4), d = i % (D / 4) * 4;
                 f32x4 y = *reinterpret_cast<const f32x4*>(o_lds + row * kPad + d);
@@ -549,14 +589,14 @@ __global__ __launch_bounds__(256, few_waves(D)) void kv_few_k(Cache c, Batch b, 
                 }
                 float sum = 0.0f;
 #pragma unroll
-                for (int w = 0; w < 4; ++w) sum += l_lds[w][row] * __builtin_amdgcn_exp2f(m_lds[w][row] - best);
+                for (int w = 0; w < 4; ++w) sum += __builtin_ldexpf(l_lds[w][row], one - base_lds[w]) * __builtin_amdgcn_exp2f(m_lds[w][row] - best);
                 if (whole) {
                     const int tok = token_of(a, row0 + row), out = s.row0 + tok;
                     const uint32_t head = h * a.group + (uint32_t)(row0 + row - tok * (int)a.group);
-                    store4(O, out, head, d, y * finish(a, best, sum, out, head, q_heads, d == 0), bf);
+                    store4(O, out, head, d, from_base(y * finish(a, best, sum, one, out, head, q_heads, d == 0), one), bf);
                 } else {
                     *reinterpret_cast<f32x4*>(part + row * D + d) = y;
-                    if (d == 0) *reinterpret_cast<float2*>(part + 16 * R * D + row * 2) = make_float2(best, sum);
+                    if (d == 0) *reinterpret_cast<RowSum*>(part + 16 * R * D + row * kRowSum) = {best, sum, one, 0};
                 }
             }
             __syncthreads();
@@ -574,20 +614,21 @@ __global__ __launch_bounds__(256, few_waves(D)) void kv_few_k(Cache c, Batch b, 
     }
 }
 
-// Adds up the n parts of a row: sums(i) and ml(i) are part i's sums and (m, l). W waves of a workgroup
-// share the parts (lds: W (D + 2) floats), or one does it alone.
-template <int D, int W, class Sums, class Ml>
-__device__ __forceinline__ void join_row(const Attn& a, int n, Sums sums, Ml ml_of, float* lds, const Rows& O, int bf,
+// Adds up the n parts of a row: sums(i) and row_sum(i) are part i's sums and RowSum. W waves of a workgroup
+// share the parts (lds: W (D + kRowSum) floats), or one does it alone.
+template <int D, int W, class Sums, class Of>
+__device__ __forceinline__ void join_row(const Attn& a, int n, Sums sums, Of row_sum, float* lds, const Rows& O, int bf,
                                          int at, uint32_t head, uint32_t q_heads) {
     constexpr int N = (D + 63) / 64;
-    const int lane = threadIdx.x & 63, wave = W > 1 ? threadIdx.x >> 6 : 0;
+    const int lane = threadIdx.x & 63, wave = W > 1 ? __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)) : 0;
     float m = kLowest, l = 0.0f, o[N] = {};
+    int base = kBase;
     for (int i0 = 0; i0 < n; i0 += 16 * W) {
         const int here = min((n - i0 - wave + W - 1) / W, 16);  // this wave's: i0 + wave, and every W-th
         // the sums are asked for along with what scales them
         float v[16][N];
-        float2 ml = make_float2(kLowest, 0.0f);
-        if (lane < here) ml = *reinterpret_cast<const float2*>(ml_of(i0 + wave + lane * W));
+        RowSum own = {kLowest, 0.0f, kBase, 0};
+        if (lane < here) own = *reinterpret_cast<const RowSum*>(row_sum(i0 + wave + lane * W));
 #pragma unroll
         for (int i = 0; i < 16; ++i)
             if (i < here) {
@@ -595,13 +636,15 @@ __device__ __forceinline__ void join_row(const Attn& a, int n, Sums sums, Ml ml_
 #pragma unroll
                 for (int k = 0; k < N; ++k) v[i][k] = D % 64 == 0 || k * 64 + lane < D ? from[k * 64 + lane] : 0.0f;
             }
-        float top = fmaxf(m, ml.x);
+        float top = fmaxf(m, own.m);
 #pragma unroll
         for (int d = 1; d < 16; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
         top = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, top)));
-        const float fade = __builtin_amdgcn_exp2f(m - top), f = __builtin_amdgcn_exp2f(ml.x - top);
+        const int one = min(base, __builtin_amdgcn_readfirstlane((int)~wave_max(~(uint32_t)own.base)));
+        const float fade = __builtin_amdgcn_exp2f(m - top), f = __builtin_amdgcn_exp2f(own.m - top);
         m = top;
-        l = l * fade + wave_sum(ml.y * f);
+        l = __builtin_ldexpf(l, one - base) * fade + wave_sum(__builtin_ldexpf(own.l, one - own.base) * f);
+        base = one;
 #pragma unroll
         for (int k = 0; k < N; ++k) o[k] *= fade;
 #pragma unroll
@@ -613,19 +656,23 @@ __device__ __forceinline__ void join_row(const Attn& a, int n, Sums sums, Ml ml_
             }
     }
     if constexpr (W > 1) {
-        float* const ml = lds + W * D;
-        if (lane == 0) ml[2 * wave] = m, ml[2 * wave + 1] = l;
+        RowSum* const all = reinterpret_cast<RowSum*>(lds + W * D);
+        if (lane == 0) all[wave] = {m, l, base, 0};
         __syncthreads();
-        float top = ml[0];
+        float top = all[0].m;
+        base = all[0].base;
 #pragma unroll
-        for (int w = 1; w < W; ++w) top = fmaxf(top, ml[2 * w]);
+        for (int w = 1; w < W; ++w) {
+            top = fmaxf(top, all[w].m);
+            base = min(base, all[w].base);
+        }
         const float fade = __builtin_amdgcn_exp2f(m - top);
 #pragma unroll
         for (int k = 0; k < N; ++k)
             if (D % 64 == 0 || k * 64 + lane < D) lds[wave * D + k * 64 + lane] = o[k] * fade;
         l = 0.0f;
 #pragma unroll
-        for (int w = 0; w < W; ++w) l += ml[2 * w + 1] * __builtin_amdgcn_exp2f(ml[2 * w] - top);
+        for (int w = 0; w < W; ++w) l += __builtin_ldexpf(all[w].l, base - all[w].base) * __builtin_amdgcn_exp2f(all[w].m - top);
         m = top;
         __syncthreads();
         if (wave) return;
@@ -637,19 +684,21 @@ __device__ __forceinline__ void join_row(const Attn& a, int n, Sums sums, Ml ml_
                 for (int w = 0; w < W; ++w) o[k] += lds[w * D + k * 64 + lane];
             }
     }
-    const float y = finish(a, m, l, at, head, q_heads, lane == 0);
+    const float y = finish(a, m, l, base, at, head, q_heads, lane == 0);
     uint16_t* const to = static_cast<uint16_t*>(O.p) + (int64_t)at * O.row + (int64_t)head * O.head;
 #pragma unroll
     for (int k = 0; k < N; ++k)
-        if (D % 64 == 0 || k * 64 + lane < D)
-            to[k * 64 + lane] = (uint16_t)(bf ? pair16<1>(o[k] * y, 0.0f) : pair16<0>(o[k] * y, 0.0f));
+        if (D % 64 == 0 || k * 64 + lane < D) {
+            const float v = __builtin_ldexpf(o[k] * y, base - 127);
+            to[k * 64 + lane] = (uint16_t)(bf ? pair16<1>(v, 0.0f) : pair16<0>(v, 0.0f));
+        }
 }
 
 // The cut rows of work of kv_few_k, one of their (token, head) rows for each W waves.
 template <int D, int R, int W>
 __global__ __launch_bounds__(256) void kv_join_k(Cache c, Batch b, Attn a, FewPlan p, Rows O, int bf, float* ws) {
-    __shared__ float lds[W > 1 ? W * (D + 2) : 1];
-    const int row = (int)(W > 1 ? blockIdx.y : blockIdx.y * 4 + (threadIdx.x >> 6));
+    __shared__ __attribute__((aligned(16))) float lds[W > 1 ? W * (D + kRowSum) : 1];
+    const int row = W > 1 ? (int)blockIdx.y : (int)blockIdx.y * 4 + __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     // by row of work: a sequence without rows has written nothing
     const Cut cut = reinterpret_cast<const Cut*>(ws)[blockIdx.x];
     const Seq own = sequence(b, c.page_log2, p.by_row ? blockIdx.x / c.heads : 0);
@@ -661,7 +710,7 @@ __global__ __launch_bounds__(256) void kv_join_k(Cache c, Batch b, Attn a, FewPl
     const int in = row % (16 * R);
     auto part = [&](int i) { return slot_of<D, R>(ws, p, 2 * (cut.first + i) + (i == 0), (uint32_t)(row / (16 * R))); };
     join_row<D, W>(a, cut.parts, [&](int i) { return part(i) + in * D; },
-                   [&](int i) { return part(i) + 16 * R * D + in * 2; }, lds, O, bf, s.row0 + row / (int)a.group,
+                   [&](int i) { return part(i) + 16 * R * D + in * kRowSum; }, lds, O, bf, s.row0 + row / (int)a.group,
                    (uint32_t)cut.head * a.group + (uint32_t)(row % (int)a.group), c.heads * a.group);
 }
 

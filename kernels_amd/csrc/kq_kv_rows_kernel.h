@@ -23,7 +23,7 @@ template <int D>
 struct RowTile {
     _Float16 k[D / 8 * 65 * 8];
     _Float16 v[8 * D * 8];
-    int exps[8];  // exponent bytes of the four 16-token blocks: K's (-1: no page), V's
+    int exps[8];  // exponent bytes of the four 16-token blocks: K's (-1: no page), V's (kBase: no page or token)
 };
 
 template <int D, int TYPE, int NW>
@@ -121,7 +121,7 @@ __global__ __launch_bounds__(64 * NW, D >= 192 ? 1 : 2) void kv_rows_k(Cache c, 
         if (tid < 8) {
             const int t = t0 + (tid & 3) * 16, page = page_at(t);
             const uint64_t at = exp_offset(c, max(page, 0), h, t);
-            ex = tid < 4 ? page < 0 ? -1 : (int)c.k_exp[at] : (int)c.v_exp[at];
+            ex = tid < 4 ? page < 0 ? -1 : (int)c.k_exp[at] : page < 0 || t >= hi ? kBase : (int)c.v_exp[at];
         }
     };
     // ... and out of them.
@@ -153,6 +153,7 @@ __global__ __launch_bounds__(64 * NW, D >= 192 ? 1 : 2) void kv_rows_k(Cache c, 
     };
 
     float m = kLowest, l = 0.0f;
+    int base = kBase;  // of l
     f32x16v o[D / 32] = {};
     auto compute = [&](int t0, const RowTile<D>& in) {
         if (!__any(t0 < sees_hi && t0 + 64 > sees_lo)) return;  // no token of it in sight of the wave
@@ -207,6 +208,11 @@ __global__ __launch_bounds__(64 * NW, D >= 192 ? 1 : 2) void kv_rows_k(Cache c, 
 #pragma unroll
             for (int i = 0; i < D / 32; ++i) o[i] *= fade;
         }
+        if (__any(base_far(base, v0) || base_far(base, v1))) {
+            const int to = base_near(base, min(v0, v1), max(v0, v1));
+            l = __builtin_ldexpf(l, to - base);
+            base = to;
+        }
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             const float down = e[u] - (m - kLift);
@@ -218,7 +224,7 @@ __global__ __launch_bounds__(64 * NW, D >= 192 ? 1 : 2) void kv_rows_k(Cache c, 
                 sum += y;
                 w[i / 8][i % 8] = (_Float16)y;
             }
-            l += sum * pow2f(min(max(127 - (u ? v1 : v0), -126), 127));
+            l += sum * pow2f(base - (u ? v1 : v0));
 #pragma unroll
             for (int hh = 0; hh < 2; ++hh)
 #pragma unroll
@@ -252,15 +258,15 @@ __global__ __launch_bounds__(64 * NW, D >= 192 ? 1 : 2) void kv_rows_k(Cache c, 
     }
     const int at = s.row0 + tok;
     if (n_splits <= 1) {
-        const float y = finish(a, m, l, at, head, q_heads, g == 0);
+        const float y = finish(a, m, l, base, at, head, q_heads, g == 0);
 #pragma unroll
         for (int i = 0; i < D / 32; ++i)
 #pragma unroll
             for (int j = 0; j < 4; ++j)
                 store4(O, at, head, i * 32 + j * 8 + g * 4,
-                       f32x4{o[i][4 * j] * y, o[i][4 * j + 1] * y, o[i][4 * j + 2] * y, o[i][4 * j + 3] * y}, bf);
+                       from_base(f32x4{o[i][4 * j] * y, o[i][4 * j + 1] * y, o[i][4 * j + 2] * y, o[i][4 * j + 3] * y}, base), bf);
     } else {
-        float* const part = ws + ((((uint64_t)seq * p.splits + split) * p.tiles + tile) * c.heads + h) * (RT * (D + 2));
+        float* const part = ws + ((((uint64_t)seq * p.splits + split) * p.tiles + tile) * c.heads + h) * (RT * (D + kRowSum));
         float* const to = part + (row - row0) * D;
 #pragma unroll
         for (int i = 0; i < D / 32; ++i)
@@ -268,14 +274,14 @@ __global__ __launch_bounds__(64 * NW, D >= 192 ? 1 : 2) void kv_rows_k(Cache c, 
             for (int j = 0; j < 4; ++j)
                 *reinterpret_cast<f32x4*>(to + i * 32 + j * 8 + g * 4) =
                     f32x4{o[i][4 * j], o[i][4 * j + 1], o[i][4 * j + 2], o[i][4 * j + 3]};
-        if (g == 0) *reinterpret_cast<float2*>(part + RT * D + (row - row0) * 2) = make_float2(m, l);
+        if (g == 0) *reinterpret_cast<RowSum*>(part + RT * D + (row - row0) * kRowSum) = {m, l, base, 0};
     }
 }
 
 // Adds up the splits of kv_rows_k: a wave takes one (token, query head).
 template <int D>
 __global__ __launch_bounds__(256) void kv_rows_join_k(Cache c, Batch b, Attn a, RowPlan p, Rows O, int bf, const float* ws) {
-    const uint32_t q_heads = c.heads * a.group, id = blockIdx.x * 4 + (threadIdx.x >> 6);
+    const uint32_t q_heads = c.heads * a.group, id = blockIdx.x * 4 + (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const uint32_t head = id % q_heads, h = head / a.group, j = id / q_heads % b.max_q, seq = id / q_heads / b.max_q;
     if (seq >= b.n_seq) return;
     const Seq s = sequence(b, c.page_log2, seq);
@@ -283,11 +289,11 @@ __global__ __launch_bounds__(256) void kv_rows_join_k(Cache c, Batch b, Attn a, 
     const int RT = (int)p.rows, row = (int)(j * a.group + head % a.group), tile = row / RT, in = row % RT;
     const int n = row_splits(span_of(s, a, tile * RT, RT), (int)p.chunk);
     if (n <= 1) return;
-    const uint64_t size = (uint64_t)RT * (D + 2);
+    const uint64_t size = (uint64_t)RT * (D + kRowSum);
     const float* const first = ws + (((uint64_t)seq * p.splits * p.tiles + tile) * c.heads + h) * size;
     const uint64_t step = (uint64_t)p.tiles * c.heads * size;
     join_row<D, 1>(a, n, [&](int i) { return first + i * step + in * D; },
-                   [&](int i) { return first + i * step + RT * D + in * 2; }, nullptr, O, bf, s.row0 + (int)j, head, q_heads);
+                   [&](int i) { return first + i * step + RT * D + in * kRowSum; }, nullptr, O, bf, s.row0 + (int)j, head, q_heads);
 }
 
 template <int D, int TYPE>

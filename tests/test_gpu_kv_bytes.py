@@ -63,3 +63,58 @@ def test_write(gpu, dim, block, dtype, kind):
         for i, (n, m) in enumerate(seqs):
             oracle.write(w, x[w][1][b.starts[i]:b.starts[i + 1]], b.table[i], n, m)
     same_cache(cache, oracle)
+
+
+# few rows: a row of work each, in parts (joined by four waves or one), in equal shares; many rows: whole, in splits
+FORMS = [([(70, 1), (1, 1), (0, 1), (33, 3)], 2, 4), ([(1500, 1), (100, 1), (0, 1)], 1, 2), ([(2300, 2), (700, 1)], 8, 16),
+         ([(2600, 1)] + [(30, 1)] * 300, 1, 2), ([(64, 64), (90, 40), (0, 20), (200, 1)], 1, 3), ([(2000, 70), (5, 5)], 1, 2)]
+
+
+def attend(gpu, seqs, heads, group, dim, kind, dtype, exps, sinks=False, window=0):
+    """kq_kv_attn where exps(rng, shape) are V's bytes, against the oracle. Its tolerance's 96 for the exponents and
+    the lift (in steps of 2^-24 times dim + 16) is 160 here: |byte - 127| <= 128, and |m| no more than that and the scores."""
+    rng = np.random.default_rng(dim + group)
+    b = Batch(gpu, seqs, 16, rng)
+    oracle = _kv.Cache(b.n_pages, heads, dim, kind=kind)
+    oracle.fill(rng)
+    oracle.exps["v"] = exps(rng, oracle.exps["v"].shape).astype(np.uint8)
+    cache = upload(oracle, gpu)
+    q_heads = heads * group
+    q, q64 = to(rng.normal(0, 1, (b.rows, q_heads, dim)), dtype, gpu)
+    s = rng.normal(0, 3, q_heads).astype(np.float32) if sinks else None
+    out, lse = torch.full((b.rows, q_heads, dim), 7.0, dtype=DTYPES[dtype], device=gpu), torch.full((b.rows, q_heads), 7.0, device=gpu)
+    n = kq.kv_attn_workspace_size(cache, b.c, q_heads)
+    ws = torch.empty(n, dtype=torch.uint8, device=gpu)
+    kq.kv_attn(cache, b.c, q, out, ws, n, window=window, sinks=None if s is None else torch.from_numpy(s).to(gpu), lse=lse)
+    torch.cuda.synchronize()
+    eps, tiny = EPS[dtype]
+    top = torch.finfo(DTYPES[dtype]).max
+    for i, (length, m) in enumerate(seqs):
+        rows = slice(b.starts[i], b.starts[i + 1])
+        want = _kv.attend(oracle, b.table[i], length, q64[rows], dim**-0.5, True, window, s)
+        tol, tol_lse = _kv.attend_tolerance(*want[:3], want[3] + 64.0, want[4], dim, eps, tiny)
+        have, none = lse[rows].double().cpu().numpy(), np.isinf(want[1])
+        assert np.array_equal(np.isinf(have), none) and np.array_equal(have[none], want[1][none]), (i, have[:2], want[1][:2])
+        off = np.abs(have[~none] - want[1][~none])
+        assert (off <= tol_lse[~none]).all(), (i, float(off.max()))
+        got = out[rows].double().cpu().numpy()
+        # off by its tolerance at most, or infinite where that reaches beyond the type's largest value
+        over = np.isinf(got) & (np.sign(got) * want[0] + tol >= top)
+        bad = np.argwhere(~((np.abs(got - want[0]) <= tol) | over))
+        assert not len(bad), (i, bad[0].tolist(), got[tuple(bad[0])], want[0][tuple(bad[0])], tol[tuple(bad[0])], len(bad))
+
+
+@pytest.mark.parametrize("seqs,heads,group", FORMS)
+@pytest.mark.parametrize("byte", [0, 1, 10, 18, 62, 200, 244, 255])
+def test_attention(gpu, byte, seqs, heads, group):
+    attend(gpu, seqs, heads, group, 64, "e4m3" if byte % 2 else "i8", "bf16", lambda rng, shape: np.full(shape, byte), sinks=byte in (10, 200))
+
+
+@pytest.mark.parametrize("dim,kind,dtype", [(64, "i8", "bf16"), (96, "e4m3", "bf16"), (128, "i8", "bf16"), (128, "e4m3", "f16"), (192, "i8", "f16"), (256, "e4m3", "bf16")])
+@pytest.mark.parametrize("low", [0, 60, 155])
+def test_attention_over_bytes_that_differ(gpu, low, dim, kind, dtype):
+    """Bytes of a head that differ by up to 100, in any order, growing and falling."""
+    for j, (seqs, heads, group) in enumerate(FORMS):
+        if j % 2 == low // 60 % 2:
+            orders = (lambda rng, shape: low + rng.integers(0, 101, shape), lambda rng, shape: low + np.arange(np.prod(shape)).reshape(shape) % 101)
+            attend(gpu, seqs, heads, group, dim, kind, dtype, orders[j // 2 % 2], sinks=j == 1, window=37 if j == 4 else 0)
