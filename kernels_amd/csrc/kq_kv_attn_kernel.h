@@ -157,6 +157,11 @@ __device__ __forceinline__ u32x4 signed16(u32x4 v, float scale) {
     return v ^ (scale < 0.0f ? 0x80008000u : 0u);
 }
 
+// What sums of products are multiplied by for scores in log2: finite, so that keys of zero give zeros whatever their byte.
+__device__ __forceinline__ float score_factor(const Attn& a, int byte, int q_exp) {
+    return fminf(__builtin_ldexpf(fabsf(a.scale_log2), byte - 127 + q_exp), 3.402823466e38f);
+}
+
 // A row's query as the second operand of S^T, in fp16: 16 columns a lane of each 64, 8 of a
 // last 32. bf16 rows go through a power of two; returns the exponent that undoes it.
 template <int D>
@@ -471,7 +476,7 @@ __global__ __launch_bounds__(256, few_waves(D)) void kv_few_k(Cache c, Batch b, 
 #pragma unroll
                 for (int k = 0; k < R; ++k) {
                     // t = f s + e with f >= 0: the largest t is the largest s's
-                    float f = __builtin_ldexpf(fabsf(a.scale_log2), ke - 127 + q_exp[k]), e = (float)(ve - 127);
+                    float f = score_factor(a, ke, q_exp[k]), e = (float)(ve - 127);
                     // tokens in sight of the row, of the lane's 16
                     const int from = sees_lo[k] - tv, to = pv < 0 ? 0 : sees_hi[k] - tv;
                     if (!__all(from <= 0 && to >= 16)) {

@@ -168,8 +168,7 @@ __global__ __launch_bounds__(64 * NW, D >= 192 ? 1 : 2) void kv_rows_k(Cache c, 
         }
         const int k0 = in.exps[g], k1 = in.exps[2 + g], v0 = in.exps[4 + g], v1 = in.exps[6 + g];
         // t = f s + e with f >= 0: the largest t of a block is its largest s's
-        const float scale = fabsf(a.scale_log2);
-        float f[2] = {__builtin_ldexpf(scale, k0 - 127 + q_exp), __builtin_ldexpf(scale, k1 - 127 + q_exp)};
+        float f[2] = {score_factor(a, k0, q_exp), score_factor(a, k1, q_exp)};
         float e[2] = {(float)(v0 - 127), (float)(v1 - 127)};
         if (!__all(t0 + 64 <= sees_hi && t0 >= sees_lo && k0 >= 0 && k1 >= 0)) {
             // only the few tiles that need it: nothing of this is computed ahead of the branch

@@ -118,3 +118,27 @@ def test_attention_over_bytes_that_differ(gpu, low, dim, kind, dtype):
         if j % 2 == low // 60 % 2:
             orders = (lambda rng, shape: low + rng.integers(0, 101, shape), lambda rng, shape: low + np.arange(np.prod(shape)).reshape(shape) % 101)
             attend(gpu, seqs, heads, group, dim, kind, dtype, orders[j // 2 % 2], sinks=j == 1, window=37 if j == 4 else 0)
+
+
+@pytest.mark.parametrize("seqs", [[(70, 1), (1, 1)], [(1500, 1)], [(80, 70)]])
+@pytest.mark.parametrize("dtype,size,scale,byte", [("f16", 1.0, 2.0, 255), ("bf16", 1.0, 40.0, 255), ("bf16", 1e38, 0.1, 150)])
+def test_keys_of_zero(gpu, dtype, size, scale, byte, seqs):
+    """Zero codes are zeros, also where 2^(byte - 127) times the scale, or what a row of large queries goes by, is beyond
+    float32's largest: every token has the same probability, 1 / n, and lse is log n."""
+    rng = np.random.default_rng(byte)
+    b = Batch(gpu, seqs, 16, rng)
+    oracle = _kv.Cache(b.n_pages, 1, 64)
+    oracle.fill(rng)
+    oracle.codes["k"][:], oracle.exps["k"][:] = 0, byte
+    cache = upload(oracle, gpu)
+    q, q64 = to(np.clip(rng.normal(0, size, (b.rows, 2, 64)), -3e38, 3e38), dtype, gpu)  # finite
+    out, lse = torch.full((b.rows, 2, 64), 7.0, dtype=DTYPES[dtype], device=gpu), torch.full((b.rows, 2), 7.0, device=gpu)
+    ws = torch.empty(kq.kv_attn_workspace_size(cache, b.c, 2), dtype=torch.uint8, device=gpu)
+    kq.kv_attn(cache, b.c, q, out, ws, ws.numel(), scale=scale, lse=lse)
+    torch.cuda.synchronize()
+    for i, (n, m) in enumerate(seqs):
+        rows = slice(b.starts[i], b.starts[i + 1])
+        want = _kv.attend(oracle, b.table[i], n, q64[rows], scale)
+        tol, tol_lse = _kv.attend_tolerance(*want, 64, *EPS[dtype])
+        assert (np.abs(out[rows].double().cpu().numpy() - want[0]) <= tol).all()
+        assert (np.abs(lse[rows].double().cpu().numpy() - want[1]) <= tol_lse).all()
