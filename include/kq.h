@@ -452,7 +452,8 @@ typedef struct kq_kv_batch {
 /* The rows of a tensor [n_rows][heads][head_dim]: element strides of a row and of a
  * head; head_dim is contiguous. Strides are non-negative multiples of 8 (that of
  * a single row or head is not looked at), the pointer 16-byte aligned (a slice
- * of a fused projection's output is). */
+ * of a fused projection's output is). Where a call writes them, no two rows or
+ * heads share elements (else KQ_EINVAL), nor two of the call's tensors. */
 typedef struct kq_kv_rows {
     void* p;
     int64_t row, head;

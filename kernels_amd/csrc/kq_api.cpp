@@ -11,6 +11,7 @@
 #include <atomic>
 #include <cstdint>
 #include <cstring>
+#include <utility>
 
 #include "kq.h"
 #include "kq_internal.h"
@@ -192,6 +193,19 @@ kq_status check_kv_pointers(const kq_kv_cache* c, const kq_kv_batch* b) {
     return KQ_OK;
 }
 
+// Whether some of n rows and m heads, D wide, share elements; strides of several are D at least. A row and a head step
+// that meet go in opposite directions: |i row - j head| < D.
+bool rows_meet(uint64_t n, uint64_t m, uint64_t row, uint64_t head, uint32_t D) {
+    if (n < m) std::swap(n, m), std::swap(row, head);
+    typedef unsigned __int128 wide;
+    if ((wide)row >= (wide)head * (m - 1) + D || (wide)head >= (wide)row * (n - 1) + D) return false;  // rows of heads, heads of rows
+    for (uint64_t j = 1; j < m; ++j) {
+        const wide at = (wide)head * j, i = at / row, in = at % row;
+        if ((i >= 1 && i < n && in < D) || (i + 1 < n && row - in < D)) return true;
+    }
+    return false;
+}
+
 kq_status check_kv_rows(const kq_kv_rows* r, const kq_kv_batch* b, uint32_t heads, uint32_t D, bool written) {
     if (!r) return KQ_ENULL;
     if (b->n_rows == 0) return KQ_OK;  // an empty tensor has no address
@@ -200,6 +214,7 @@ kq_status check_kv_rows(const kq_kv_rows* r, const kq_kv_batch* b, uint32_t head
     if ((b->n_rows > 1 && (r->row < 0 || r->row % 8)) || (heads > 1 && (r->head < 0 || r->head % 8))) return KQ_EINVAL;
     // rows and heads that overlap cannot be written
     if (written && ((b->n_rows > 1 && r->row < (int64_t)D) || (heads > 1 && r->head < (int64_t)D))) return KQ_EINVAL;
+    if (written && b->n_rows > 1 && heads > 1 && rows_meet(b->n_rows, heads, (uint64_t)r->row, (uint64_t)r->head, D)) return KQ_EINVAL;
     return aligned(r->p, 16) ? KQ_OK : KQ_EALIGN;
 }
 

@@ -288,3 +288,24 @@ def test_oracle_exponents():
         assert _kv.exponent(big, kind) == 0 and _kv.exponent(np.nextafter(big, 1e9), kind) == 1
         assert _kv.exponent(big / 2, kind) == -1
         assert _kv.exponent(3.3e38, kind) == _kv.MAX_EXP[kind]
+
+
+@pytest.mark.parametrize("rows,heads,row,head,overlap", [
+    (6, 32, 128, 128, True), (2, 2, 128, 128, True), (6, 32, 31 * 128, 128, True), (6, 32, 32 * 128 - 8, 128, True),
+    (6, 32, 128, 5 * 128, True), (6, 32, 128, 6 * 128 - 8, True), (3, 4, 3 * 128, 2 * 128, True), (4, 3, 2 * 128, 3 * 128, True),
+    (2**20, 2, 128, 2**20 * 128 - 8, True), (65535, 32, 8 * 1001, 8 * 1003, True), (2, 32, 2**62, 2**61, True),
+    (6, 32, 32 * 128, 128, False), (6, 32, 128, 6 * 128, False), (6, 32, 40 * 128, 128, False), (2, 2, 3 * 128, 2 * 128, False),
+    (1, 32, 0, 128, False), (2, 32, 2**62, 2**40, False), (2**20, 2, 128, 2**20 * 128, False), (6, 1, 128, 0, False)])
+def test_rows_and_heads_that_meet(rows, heads, row, head, overlap):
+    """Outputs whose rows and heads share elements are refused, whichever of the strides is the larger; those that lie
+    between one another without sharing any are not."""
+    # by search, where there are few enough
+    if rows * heads <= 4096 and max(row, head) < 2**40:
+        at = np.sort((np.arange(rows)[:, None] * row + np.arange(heads) * head).reshape(-1))
+        assert (np.diff(at).min() < 128) == overlap
+    b, r = batch_c(n_seq=1, max_q=1, n_rows=rows), rows_c(row=row, head=head)
+    q = rows_c(row=0, head=0)
+    assert attn(cache_c(heads=1), b, attn_c(q_heads=heads), q, r, ws=None) == (kq.KQ_EINVAL if overlap else kq.KQ_EWORKSPACE)
+    if overlap:
+        c, fine = cache_c(heads=heads), rows_c(row=2**30, head=128)
+        assert write(c, b, r, fine, read=True) == write(c, b, fine, r, read=True) == kq.KQ_EINVAL
