@@ -528,7 +528,8 @@ def kv_read(cache, batch, k, v, stream=None):
 
 
 def kv_attn_workspace_size(cache, batch, q_heads):
-    n = lib().kq_kv_attn_workspace_size(cache._ref, batch._packed(batch.n_seq * batch.max_q), q_heads)
+    rows = 0 if batch.q_start is not None else min(batch.n_seq * batch.max_q, 2**32 - 1)  # with q_start any number
+    n = lib().kq_kv_attn_workspace_size(cache._ref, batch._packed(rows), q_heads)
     if n == 0:
         raise KQError(KQ_EINVAL, "kq_kv_attn_workspace_size")
     return n

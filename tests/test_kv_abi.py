@@ -309,3 +309,14 @@ def test_rows_and_heads_that_meet(rows, heads, row, head, overlap):
     if overlap:
         c, fine = cache_c(heads=heads), rows_c(row=2**30, head=128)
         assert write(c, b, r, fine, read=True) == write(c, b, fine, r, read=True) == kq.KQ_EINVAL
+
+
+@pytest.mark.parametrize("starts", [False, True])
+def test_python_workspace_size_of_bounds_too_large(starts):
+    """n_seq * max_q beyond 32 bits: refused like any bounds that no launch can have."""
+    n = 65535
+    c, length = kq.kv_cache(4, 1, 64, device="cpu"), torch.zeros(n, dtype=torch.int32)
+    b = kq.KVBatch(torch.zeros((n, 1), dtype=torch.int32), length, 16, max_q=1 << 17,
+                   q_start=torch.zeros(n + 1, dtype=torch.int32) if starts else None)
+    with pytest.raises(kq.KQError):
+        kq.kv_attn_workspace_size(c, b, 1)
