@@ -320,3 +320,14 @@ def test_python_workspace_size_of_bounds_too_large(starts):
                    q_start=torch.zeros(n + 1, dtype=torch.int32) if starts else None)
     with pytest.raises(kq.KQError):
         kq.kv_attn_workspace_size(c, b, 1)
+
+
+@pytest.mark.parametrize("read,block", [(False, 16), (False, 64), (False, 256), (True, 16), (True, 256)])
+def test_launch_limits_of_many_heads(read, block):
+    """Blocks of 512 workgroups each (1024 heads' K and V): few enough tokens for blocks of 256 too."""
+    unit = 16 if read else block
+    most = ((1 << 24) - 1) // 512 - 2
+    for blocks, status in ((most, kq.KQ_OK), (most + 1, kq.KQ_EUNSUPPORTED)):
+        b = batch_c(n_seq=1, max_q=blocks * unit, n_rows=0)
+        assert b.max_q < 0x7FFF0000
+        assert write(cache_c(heads=1024, page=256, block=block), b, read=read) == status
