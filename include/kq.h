@@ -438,10 +438,14 @@ typedef struct kq_kv_cache {
  * page id outside [0, n_pages) are left out -- not written, not attended to,
  * read as zeros.
  * Constraints: 1 <= n_seq <= 65535; max_q, max_pages, max_len >= 1; max_len, n_rows
- * < 2^31 - 2^16; q_start NULL: n_seq * max_q <= n_rows. KQ_EUNSUPPORTED where the bounds ask for more than a
- * launch can have: 2^24 workgroups (max_q / block * heads / 2 in kq_kv_write, max_q / 16 * heads / 2 in
- * kq_kv_read, n_seq * heads for each 128 of max_q * q_heads / heads in kq_kv_attn), or n_seq * max_q *
- * q_heads of 2^31 - 2^16 in kq_kv_attn. */
+ * < 2^31 - 2^16; q_start NULL: n_seq * max_q <= n_rows. KQ_EUNSUPPORTED where the
+ * bounds ask for more than a launch can have, 2^24 workgroups:
+ *   kq_kv_write, kq_kv_read: (max_q / block + 2) * ceil(heads / 2), block 16 in kq_kv_read
+ *   kq_kv_attn, with rows = max_q * q_heads / heads: n_seq * heads, rounded up to
+ *     a multiple of 8, for each 32 rows (each 16 where rows <= 16 or head_dim is
+ *     192 or 256) if rows <= 64; beyond, n_seq * heads for each 128 rows (two for
+ *     each 256 where head_dim is 96 or 128 and rows > 128)
+ * and in kq_kv_attn for n_seq * max_q * q_heads of 2^31 - 2^16. */
 typedef struct kq_kv_batch {
     const int32_t* pages;
     const int32_t* kv_len;

@@ -331,3 +331,25 @@ def test_launch_limits_of_many_heads(read, block):
         b = batch_c(n_seq=1, max_q=blocks * unit, n_rows=0)
         assert b.max_q < 0x7FFF0000
         assert write(cache_c(heads=1024, page=256, block=block), b, read=read) == status
+
+
+def test_launch_limits_as_documented():
+    """kq_kv_attn_workspace_size refuses what include/kq.h says, over random bounds beside the limits."""
+    rng = np.random.default_rng(1)
+    seen = set()
+    for _ in range(20000):
+        n_seq, heads, group = int(2 ** rng.uniform(0, 16)) - 1 or 1, int(2 ** rng.uniform(0, 10)), int(rng.choice([1, 3, 8, 40, 64]))
+        dim, max_q = int(rng.choice([64, 96, 128, 192, 256])), int(2 ** rng.uniform(0, rng.choice([2, 8, 20])))
+        rows = max_q * group
+        if rows <= 64:
+            each = 16 if rows <= 16 or dim in (192, 256) else 32
+            groups = -(-n_seq * heads // 8) * 8 * -(-rows // each)
+        elif dim in (96, 128) and rows > 128:
+            groups = n_seq * heads * -(-rows // 256) * 2
+        else:
+            groups = n_seq * heads * -(-rows // 128)
+        refused = groups >= 1 << 24 or n_seq * max_q * heads * group >= 2**31 - 2**16
+        b = batch_c(n_seq=n_seq, max_q=max_q, n_rows=0)
+        assert (size(cache_c(heads=heads, head_dim=dim), b, heads * group) == 0) == refused, (n_seq, heads, group, dim, max_q)
+        seen.add((refused, rows <= 64))
+    assert len(seen) == 4
