@@ -508,7 +508,10 @@ kq_status kq_kv_read(const kq_kv_cache* cache, const kq_kv_batch* batch, const k
  * results of sequences that are split among workgroups. Calls that share one must be
  * stream-ordered. 0 from kq_kv_attn_workspace_size means invalid arguments.
  * q_heads: a multiple of cache->heads, at most 64 times as many. Results do
- * not change from run to run (no atomics). */
+ * not change from run to run (no atomics).
+ * A batch whose max_q * q_heads / heads is over 64 runs the kernel for many rows
+ * throughout. Sequences of few rows over long contexts are slow in it: give them
+ * a call of their own (KQ_OK either way; slices of one batch's arrays do). */
 typedef struct kq_kv_attn_desc {
     uint32_t q_heads;
     float scale;
