@@ -323,6 +323,10 @@ __global__ __launch_bounds__(256) void kv_read_k(Cache c, Batch b, Rows K, Rows 
     }
 }
 
+// blockIdx.x = the block (write) or span (read), counted from the sequence's first newest token's, x the groups
+// of four waves of its heads; .y = the sequence.
+uint32_t spans(uint32_t max_q, uint32_t tokens) { return (max_q - 1) / tokens + 1 + (max_q > 1); }
+
 template <int D, int TYPE>
 hipError_t write_d(const Cache& c, const Batch& b, const Rows& K, const Rows& V, bool bf, dim3 grid, uint32_t groups,
                    hipStream_t s) {
@@ -331,42 +335,53 @@ hipError_t write_d(const Cache& c, const Batch& b, const Rows& K, const Rows& V,
     return hipGetLastError();
 }
 
-template <int D, int TYPE, int SPAN>
-hipError_t read_d(const Cache& c, const Batch& b, const Rows& K, const Rows& V, kq_dtype f, dim3 grid, uint32_t groups,
-                  hipStream_t s) {
-    if (f == KQ_F16) kv_read_k<D, TYPE, KQ_F16, SPAN><<<grid, 256, 0, s>>>(c, b, K, V, groups);
-    else if (f == KQ_BF16) kv_read_k<D, TYPE, KQ_BF16, SPAN><<<grid, 256, 0, s>>>(c, b, K, V, groups);
-    else kv_read_k<D, TYPE, KQ_F32, SPAN><<<grid, 256, 0, s>>>(c, b, K, V, groups);
+// Workgroups of 16 tokens a wave beyond which 64 a wave are the faster: fewer workgroups then find nothing in ragged batches,
+// and two heads of 64 fill a wave's loads better. A wave of the widest heads, or one that writes fp32, has enough to do with
+// 16. Graph replays in us, 16 and 64 tokens a wave; 8 heads, int8 to bf16 and lengths spread by their logarithm unless said:
+//   64 wide   one of 70001 (e4m3 to fp16) 67, 56 (17508 workgroups); 64 of 10-4000 57, 43 (64512); 200 of 10-900 51, 54 (46400);
+//             one of 9001 18, 18 (2260)
+//   96        64 of 10-8000 112, 97 (128512); 64 of 10-4000 63, 66 (64512)
+//   128       64 of 10-8000 129, 109 (128512); 64 of 10-4000 73, 71 (64512); 200 of 10-900 66, 86 (46400)
+//   192, 256  64 of 10-8000 170, 159 and 201, 208; 64 of 10-4000 97, 103 and 116, 132
+//   to fp32   64 wide: 64 of 10-8000 119, 104, of 10-4000 68, 73; 128 wide: 177, 203 and 102, 133
+constexpr uint64_t kNeverWide = ~0ull;
+constexpr uint64_t wide_beyond(uint32_t D, kq_dtype f) {
+    if (D == 64) return f == KQ_F32 ? 65536 : 16384;
+    return D <= 128 && f != KQ_F32 ? 65536 : kNeverWide;
+}
+
+template <int D, int TYPE, kq_dtype F>
+hipError_t read_f(const Cache& c, const Batch& b, const Rows& K, const Rows& V, hipStream_t s) {
+    const uint32_t groups = (2 * c.heads + 3) / 4;
+    const uint32_t narrow = spans(b.max_q, 16) * groups;
+    if constexpr (wide_beyond(D, F) != kNeverWide)
+        if ((uint64_t)narrow * b.n_seq > wide_beyond(D, F)) {
+            kv_read_k<D, TYPE, F, 64><<<dim3(spans(b.max_q, 64) * groups, b.n_seq), 256, 0, s>>>(c, b, K, V, groups);
+            return hipGetLastError();
+        }
+    kv_read_k<D, TYPE, F, 16><<<dim3(narrow, b.n_seq), 256, 0, s>>>(c, b, K, V, groups);
     return hipGetLastError();
 }
 
 }  // namespace
 }  // namespace kv
 
-// blockIdx.x = the block (write) or span (read), counted from the sequence's first newest token's, x the groups
-// of four waves of its heads; .y = the sequence.
-static uint32_t spans(uint32_t max_q, uint32_t tokens) { return (max_q - 1) / tokens + 1 + (max_q > 1); }
-
 hipError_t launch_kv_write(const kv::Cache& c, const kv::Batch& b, uint32_t D, int type, const kv::Rows& K,
                            const kv::Rows& V, bool bf, hipStream_t s) {
     const uint32_t groups = (2 * c.heads + 3) / 4;
-    const dim3 grid(spans(b.max_q, 1u << c.block_log2) * groups, b.n_seq);
+    const dim3 grid(kv::spans(b.max_q, 1u << c.block_log2) * groups, b.n_seq);
     return kv::by_dim(D, type, [&](auto d, auto t) {
         return kv::write_d<decltype(d)::value, decltype(t)::value>(c, b, K, V, bf, grid, groups, s);
     });
 }
 
-// 16 tokens a wave: the shortest way for a few (a decode step's blocks of 96 sequences 6 us, 9 with 64). 64 where that
-// makes a great many workgroups, most of which may find nothing in ragged batches (24 sequences of up to
-// 6007 tokens, 890 on average: 16 us, 26 with 16); in between 16 is the faster (13k tokens 17 us, 20).
 hipError_t launch_kv_read(const kv::Cache& c, const kv::Batch& b, uint32_t D, int type, const kv::Rows& K,
                           const kv::Rows& V, kq_dtype f, hipStream_t s) {
-    const uint32_t groups = (2 * c.heads + 3) / 4;
-    const bool wide = (uint64_t)spans(b.max_q, 16) * groups * b.n_seq > 16384;
-    const dim3 grid(spans(b.max_q, wide ? 64 : 16) * groups, b.n_seq);
     return kv::by_dim(D, type, [&](auto d, auto t) {
         constexpr int N = decltype(d)::value, T = decltype(t)::value;
-        return wide ? kv::read_d<N, T, 64>(c, b, K, V, f, grid, groups, s) : kv::read_d<N, T, 16>(c, b, K, V, f, grid, groups, s);
+        return f == KQ_F16    ? kv::read_f<N, T, KQ_F16>(c, b, K, V, s)
+               : f == KQ_BF16 ? kv::read_f<N, T, KQ_BF16>(c, b, K, V, s)
+                              : kv::read_f<N, T, KQ_F32>(c, b, K, V, s);
     });
 }
 

@@ -22,13 +22,17 @@ def test_write_and_read(gpu, dim, heads, page, block, kind, dtype):
 @pytest.mark.parametrize("dim,kind,heads,page,block", [(64, "e4m3", 1, 16, 16), (96, "i8", 2, 32, 32), (96, "e4m3", 3, 16, 16), (128, "i8", 2, 64, 64),
                                                        (128, "e4m3", 1, 16, 16), (192, "i8", 2, 16, 16), (192, "e4m3", 1, 128, 32), (256, "i8", 1, 64, 16), (256, "e4m3", 2, 16, 16)])
 def test_wide_reads(gpu, dim, kind, heads, page, block, out):
-    """64 tokens a wave: beyond 16384 workgroups of 16. Ragged lengths, whole sequences and parts of them, rows at negative
+    """Beyond 16384 workgroups of 16 tokens a wave, where heads of 64 are read by 64. Ragged lengths, whole sequences and parts of them, rows at negative
     positions, nothing at all."""
     rng = np.random.default_rng(dim)
     seqs = [(int(n), int(m)) for n, m in zip(rng.integers(0, 90, 520), rng.integers(0, 100, 520))]
     seqs[3], seqs[100], seqs[519] = (700, 700), (699, 530), (641, 641)
     b = kv.Batch(gpu, seqs, page, rng, pad=2)
     assert ((b.max_q - 1) // 16 + 2) * ((2 * heads + 3) // 4) * len(seqs) > 16384
+    read_check(gpu, rng, b, dim, kind, heads, page, block, out)
+
+
+def read_check(gpu, rng, b, dim, kind, heads, page, block, out):
     oracle = _kv.Cache(b.n_pages, heads, dim, page, block, kind)
     oracle.fill(rng)
     cache = kv.upload(oracle, gpu)
@@ -39,11 +43,23 @@ def test_wide_reads(gpu, dim, kind, heads, page, block, out):
     for w in "kv":
         have = got[w].cpu()
         assert (have[b.starts[-1]:] == 7.0).all(), "rows behind the last sequence"
-        for i, (n, m) in enumerate(seqs):
+        for i, (n, m) in enumerate(b.seqs):
             rows = have[b.starts[i]:b.starts[i + 1]]
             want = torch.from_numpy(oracle.read(w, b.table[i], n, m)).clamp(-top, top).float().to(kv.DTYPES[out])
             there = torch.arange(m) >= m - n
             assert torch.equal(rows[there], want[there]) and (rows[~there] == 7.0).all(), (w, i)
+
+
+@pytest.mark.parametrize("dim,kind,heads,page,block,out", [(64, "i8", 2, 16, 16, "f32"), (96, "i8", 2, 32, 32, "bf16"), (96, "e4m3", 1, 16, 16, "f16"),
+                                                           (128, "e4m3", 2, 16, 16, "bf16"), (128, "i8", 1, 64, 64, "f16"), (192, "i8", 1, 16, 16, "bf16")])
+def test_wider_reads(gpu, dim, kind, heads, page, block, out):
+    """Beyond 65536 workgroups of 16 tokens, where heads of 96 and 128 and fp32 values of 64 are read by 64 too."""
+    rng = np.random.default_rng(dim)
+    seqs = [(int(n), int(m)) for n, m in zip(rng.integers(0, 70, 520), rng.integers(0, 80, 520))]
+    seqs[7], seqs[200], seqs[519] = (2200, 2200), (2111, 700), (70, 70)
+    b = kv.Batch(gpu, seqs, page, rng, pad=2)
+    assert ((b.max_q - 1) // 16 + 2) * ((2 * heads + 3) // 4) * len(seqs) > 65536
+    read_check(gpu, rng, b, dim, kind, heads, page, block, out)
 
 
 class Guarded:
