@@ -1,8 +1,8 @@
 // kq_kv_attn_kernel.h -- attention over the 8-bit cache, few rows: the wave
 // kernel of kq_kv_attn.hip.
 //
-// A wave takes 64 tokens at a time against 16 rows (query tokens x the heads of a
-// group) of one sequence and head. Both products are 16x16x32 fp16 MFMAs on
+// A wave takes 64 tokens at a time against 16 or 32 rows (query tokens x the heads of a
+// group) of one sequence and head, of up to 64. Both products are 16x16x32 fp16 MFMAs on
 // transposed results, so that nothing moves between lanes:
 //   S^T = K Q^T: lane (r = lane % 16, g = lane / 16) receives tokens 4g..4g+3 of a
 //         16-token operand, for row r. Which tokens stand in an operand is
@@ -136,8 +136,8 @@ __device__ __forceinline__ f32x4 from_base(f32x4 y, int base) {
     return y;
 }
 
-// The power of two that brings a row's largest bf16 magnitude (bits m) into [2^14, 2^15); an infinity or
-// NaN makes its row NaN anyway.
+// The power of two that brings a row's largest bf16 magnitude (bits m) into [2^14, 2^15). Of rows with an infinity or a
+// NaN none helps: their scores are infinite or NaN.
 __device__ __forceinline__ int bf_lift(uint32_t m) {
     return m >= 0x7F80u ? 0 : min(max(14 - ((int)(m >> 7) - 127), -126), 126);
 }

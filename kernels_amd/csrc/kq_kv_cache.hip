@@ -241,8 +241,8 @@ __device__ __forceinline__ void put8(uint8_t* to, const float (&y)[8]) {
 }
 
 // One wave reads SPAN tokens (16 or 64, an aligned span of the sequence) of one head's K or V. What bounds it is
-// the writes: 131k tokens of 8 heads of 128, e4m3 to fp16, 160 us for 805 MB, where a copy of that
-// size reaches 4.9 TB/s.
+// the writes: 131k tokens of 8 heads of 128, e4m3 to fp16, 167 us for 805 MB, 4.8 TB/s, where a copy of that
+// size reaches 4.9.
 template <int D, int TYPE, int F, int SPAN>
 __global__ __launch_bounds__(256) void kv_read_k(Cache c, Batch b, Rows K, Rows V, uint32_t groups) {
     const int lane = threadIdx.x & 63;

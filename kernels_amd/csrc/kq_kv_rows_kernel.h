@@ -1,5 +1,5 @@
 // kq_kv_rows_kernel.h -- attention over the 8-bit cache, many rows: the kernel of
-// kq_kv_attn_<D>.hip for prompts and for more than 16 rows a sequence and head.
+// kq_kv_attn_<D>.hip for prompts and chunks: calls of more than 64 rows a sequence and head.
 //
 // A workgroup of NW waves takes 32 NW rows (query tokens x the heads of a group) of a sequence
 // and head, 64 tokens at a time. The tokens' codes become fp16 once for all its waves, in
