@@ -111,7 +111,7 @@ def test_arrays_that_lie_beside_others(gpu, kind, max_q, heads, group):
 
 
 def mixed(gpu, rng, decode, chunk, heads, group, dim, window=0):
-    """A step of single tokens beside one chunk: in one call, and as INTEGRATION's two calls."""
+    """A step of single tokens beside one chunk: in one call, and in two: the tokens', the chunk's."""
     seqs = [(n, 1) for n in decode] + [chunk]
     b = kv.Batch(gpu, seqs, 16, rng, pad=1)
     oracle = _kv.Cache(b.n_pages, heads, dim)
