@@ -172,3 +172,51 @@ def test_two_streams_at_once(gpu):
         got.append(outs)
     assert all(torch.equal(a, c) for a, c in zip(*got))
     assert all(torch.equal(a, c) for a, c in zip(got[0], got[0][2:]))
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.3, 1.0])
+@pytest.mark.parametrize("dim,kind,dtype", [(64, "i8", "f16"), (128, "e4m3", "bf16"), (192, "i8", "bf16")])
+def test_scales_of_many_rows(gpu, dim, kind, dtype, scale):
+    kv.attn_case(gpu, [(100, 70), (65, 3), (0, 5), (300, 90)], 2, 2, dim, kind, dtype, scale=scale, sinks=scale < 0)
+
+
+def test_query_range_of_many_rows(gpu):
+    """Queries from the smallest to the largest of bf16, and rows of zeros, in the kernel for many rows."""
+    def tiny(b, q_heads):
+        return np.random.default_rng(1).normal(0, 1, (b.rows, q_heads, 64)) * 1e-36
+
+    def huge(b, q_heads):
+        x = np.random.default_rng(1).normal(0, 1, (b.rows, q_heads, 64)) * 1e36
+        x[::5] = 0.0
+        return x
+    kv.attn_case(gpu, [(100, 40), (65, 33)], 2, 2, 64, dtype="bf16", scale=1e35, q=tiny)
+    kv.attn_case(gpu, [(100, 40), (65, 33)], 2, 2, 64, "e4m3", dtype="bf16", scale=1e-37, q=huge)
+
+
+@pytest.mark.parametrize("seqs,heads,group,dim", [([(70, 1), (0, 1), (33, 3)], 2, 4, 64), ([(1500, 1), (100, 1)], 1, 2, 96), ([(2600, 1)] + [(30, 1)] * 200, 1, 2, 64),
+                                                  ([(64, 64), (90, 40)], 1, 3, 128), ([(2000, 70), (5, 5)], 1, 2, 256)])
+def test_layouts_of_queries_and_outputs(gpu, seqs, heads, group, dim):
+    """Heads of rows, rows with others' values between them, one row of queries for all: the same bits as rows of heads, and
+    nothing beside them written."""
+    rng = np.random.default_rng(dim)
+    b = kv.Batch(gpu, seqs, 16, rng, pad=2)
+    oracle = _kv.Cache(b.n_pages, heads, dim)
+    oracle.fill(rng)
+    cache = kv.upload(oracle, gpu)
+    n, q_heads = b.rows, heads * group
+    size = kq.kv_attn_workspace_size(cache, b.c, q_heads)
+    ws = torch.empty(size, dtype=torch.uint8, device=gpu)
+
+    def attend(q, out):
+        kq.kv_attn(cache, b.c, q, out, ws, size)
+        torch.cuda.synchronize()
+        return out
+    q = torch.randn((n, q_heads, dim), device=gpu).half()
+    want = attend(q, torch.full_like(q, 7.0))
+    by_head = torch.full((q_heads, n, dim), 7.0, dtype=torch.float16, device=gpu)
+    assert torch.equal(attend(q.transpose(0, 1).contiguous().transpose(0, 1), by_head.transpose(0, 1)), want)
+    wide = torch.full((n, 2 * q_heads + 1, dim + 8), 7.0, dtype=torch.float16, device=gpu)
+    assert torch.equal(attend(q, wide[:, 1:2 * q_heads:2, :dim]), want)
+    assert (wide[:, ::2] == 7.0).all() and (wide[:, :, dim:] == 7.0).all()
+    one = q[:1].expand(n, q_heads, dim)
+    assert torch.equal(attend(one, torch.full_like(q, 7.0)), attend(one.contiguous(), torch.full_like(q, 7.0)))
