@@ -2,8 +2,9 @@
  * kq.h -- C ABI of libkq, the MI355X (gfx950) decode hot path:
  *   int4 group-affine GEMV / batched skinny GEMM, codebook (VQ) dequant-GEMV,
  *   the three-kernel MoE block (router top-k, gathered gate/up + SwiGLU,
- *   gathered down + weighted combine), and an 8-bit paged key/value cache with
- *   the attention that reads it.
+ *   gathered down + weighted combine), an 8-bit paged key/value cache with the
+ *   attention that reads it, and a step of speculative decoding over it (rotary
+ *   positions, trees of drafted tokens, their verification).
  *
  * Every entry point is stream-ordered and asynchronous: it validates its
  * arguments on the host, enqueues kernels on `stream` and returns. Nothing
@@ -523,6 +524,86 @@ size_t kq_kv_attn_workspace_size(const kq_kv_cache* cache, const kq_kv_batch* ba
 kq_status kq_kv_attn(const kq_kv_cache* cache, const kq_kv_batch* batch, const kq_kv_attn_desc* d,
                      const kq_kv_rows* Q, const kq_kv_rows* O, kq_dtype dtype, float* lse,
                      void* ws, size_t ws_bytes, kq_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * Rotary positions
+ *
+ * Pairs (a, b) of a head's first `rot` columns are turned by the angle t = pos *
+ * inv_freq[i], i the pair:
+ *   y_a = A (x_a cos t - x_b sin t),  y_b = A (x_b cos t + x_a sin t)
+ * with (a, b) = (i, i + rot / 2) (KQ_ROPE_HALVES) or (2i, 2i + 1) (KQ_ROPE_PAIRS), A
+ * the amplitude. Columns from rot on stay as they are. `inverse` turns the other
+ * way, times A again: the gradient of x, given that of y.
+ * Angles, their cosines and sines and the products are 64-bit, so that far
+ * positions keep their angle (|t| < 2^32); y is rounded to 32 bits, then to its type.
+ *
+ * inv_freq  : float [rot / 2], device memory, finite (kq_rope_freqs makes them)
+ * rot       : even, 2 <= rot <= head_dim
+ * amplitude : finite
+ * No counterpart in the reference, which has no attention.
+ * ------------------------------------------------------------------------ */
+typedef enum kq_rope_layout { KQ_ROPE_HALVES = 0, KQ_ROPE_PAIRS = 1 } kq_rope_layout;
+typedef struct kq_rope_desc {
+    const float* inv_freq;
+    uint32_t rot;
+    uint32_t layout; /* kq_rope_layout */
+    float amplitude;
+    uint32_t inverse;
+} kq_rope_desc;
+
+/* Frequencies f_i = base^(-2i / rot) and their forms for contexts longer than a
+ * model was trained on (`original` tokens, stretched by `factor`), and the
+ * amplitude that goes with them (1 but for KQ_ROPE_YARN):
+ *   KQ_ROPE_PLAIN   f_i
+ *   KQ_ROPE_LINEAR  f_i / factor
+ *   KQ_ROPE_NTK     base * factor^(rot / (rot - 2)) for base
+ *   KQ_ROPE_BANDS   turns n_i = original f_i / 2 pi in the original context: f_i where n_i >
+ *                   high, f_i / factor where n_i < low, in between the mean of the two,
+ *                   (n_i - low) / (high - low) of the former
+ *   KQ_ROPE_YARN    f_i (1 - r) + f_i / factor r, r_i = (i - from) / (to - from) within [0, 1], from =
+ *                   floor(c(high)), to = ceil(c(low)), both within [0, rot - 1] (to + 0.001
+ *                   where they are the same), c(n) = rot ln(original / (2 pi n)) / (2 ln base);
+ *                   amplitude 0.1 ln(factor) + 1
+ * Host memory, computed in 64 bits; no GPU call. base > 1 (NTK: rot > 2), factor >= 1, 0 < low <
+ * high, original > 0 where they are used, all finite. */
+typedef enum kq_rope_kind {
+    KQ_ROPE_PLAIN = 0,
+    KQ_ROPE_LINEAR = 1,
+    KQ_ROPE_NTK = 2,
+    KQ_ROPE_BANDS = 3,
+    KQ_ROPE_YARN = 4
+} kq_rope_kind;
+typedef struct kq_rope_scaling {
+    uint32_t kind; /* kq_rope_kind */
+    uint32_t rot;
+    double base, factor, low, high, original;
+} kq_rope_scaling;
+kq_status kq_rope_freqs(const kq_rope_scaling* s, float* inv_freq, float* amplitude);
+
+/* Y = X turned, rows x heads x head_dim of dtype KQ_F16, KQ_BF16 or KQ_F32, row i at
+ * position pos[i] (int32 [n_rows], device memory; any values). Y may be X (the same
+ * address and strides), and overlaps it in no other way. A slice of a fused projection that holds the
+ * queries' and then the keys' heads is turned in one call. head_dim a multiple of 8,
+ * at most 512, heads <= 65535; the strides as kq_kv_rows has them. n_rows 0: the call does nothing.
+ * One launch. rot a multiple of 16 takes whole vectors; others go value by value. */
+kq_status kq_rope(const kq_rope_desc* d, const int32_t* pos, const kq_kv_rows* X, const kq_kv_rows* Y,
+                  uint32_t n_rows, uint32_t heads, uint32_t head_dim, kq_dtype dtype,
+                  kq_stream_t stream);
+
+/* kq_kv_write with the rotation on the way: the cache's keys are those that kq_rope
+ * leaves, rounded to their type as it rounds them (bit for bit what kq_rope and
+ * kq_kv_write leave one after the other), the values as in kq_kv_write. K itself is not
+ * changed. With Q (q_heads heads) its rows of the batch are turned into Qo too (which
+ * may be Q); Q NULL: none, Qo and q_heads are not looked at.
+ * pos: int32 [n_rows], device memory, the position of each row (of a tree: kq_kv_tree's);
+ * NULL: a row's place in its sequence, kv_len - n + j.
+ * rot a multiple of 16 (else KQ_EUNSUPPORTED: kq_rope first); q_heads <= 65535. One launch;
+ * KQ_EUNSUPPORTED too where kq_kv_write's workgroups and max_q * ceil(q_heads / 4) / 4 + 1
+ * more for the queries are over its bound. */
+kq_status kq_kv_write_rope(const kq_kv_cache* cache, const kq_kv_batch* batch,
+                           const kq_rope_desc* d, const int32_t* pos, const kq_kv_rows* Q,
+                           const kq_kv_rows* Qo, uint32_t q_heads, const kq_kv_rows* K,
+                           const kq_kv_rows* V, kq_dtype dtype, kq_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -9,6 +9,7 @@
 #include <hip/hip_runtime.h>
 
 #include <atomic>
+#include <cmath>
 #include <cstdint>
 #include <cstring>
 #include <utility>
@@ -206,16 +207,19 @@ bool rows_meet(uint64_t n, uint64_t m, uint64_t row, uint64_t head, uint32_t D) 
     return false;
 }
 
-kq_status check_kv_rows(const kq_kv_rows* r, const kq_kv_batch* b, uint32_t heads, uint32_t D, bool written) {
+kq_status check_rows(const kq_kv_rows* r, uint32_t n_rows, uint32_t heads, uint32_t D, bool written) {
     if (!r) return KQ_ENULL;
-    if (b->n_rows == 0) return KQ_OK;  // an empty tensor has no address
+    if (n_rows == 0) return KQ_OK;  // an empty tensor has no address
     if (!r->p) return KQ_ENULL;
     // the stride of a single row or head is never used
-    if ((b->n_rows > 1 && (r->row < 0 || r->row % 8)) || (heads > 1 && (r->head < 0 || r->head % 8))) return KQ_EINVAL;
+    if ((n_rows > 1 && (r->row < 0 || r->row % 8)) || (heads > 1 && (r->head < 0 || r->head % 8))) return KQ_EINVAL;
     // rows and heads that overlap cannot be written
-    if (written && ((b->n_rows > 1 && r->row < (int64_t)D) || (heads > 1 && r->head < (int64_t)D))) return KQ_EINVAL;
-    if (written && b->n_rows > 1 && heads > 1 && rows_meet(b->n_rows, heads, (uint64_t)r->row, (uint64_t)r->head, D)) return KQ_EINVAL;
+    if (written && ((n_rows > 1 && r->row < (int64_t)D) || (heads > 1 && r->head < (int64_t)D))) return KQ_EINVAL;
+    if (written && n_rows > 1 && heads > 1 && rows_meet(n_rows, heads, (uint64_t)r->row, (uint64_t)r->head, D)) return KQ_EINVAL;
     return aligned(r->p, 16) ? KQ_OK : KQ_EALIGN;
+}
+kq_status check_kv_rows(const kq_kv_rows* r, const kq_kv_batch* b, uint32_t heads, uint32_t D, bool written) {
+    return check_rows(r, b->n_rows, heads, D, written);
 }
 
 kq::kv::Cache kv_cache(const kq_kv_cache& c) {
@@ -227,13 +231,27 @@ kq::kv::Batch kv_batch(const kq_kv_batch& b) {
 }
 kq::kv::Rows kv_rows(const kq_kv_rows& r) { return {r.p, r.row, r.head}; }
 
-// Workgroups of a launch over the `unit`-token blocks of max_q tokens (grid.x).
+// Workgroups of a launch over the `unit`-token blocks of max_q tokens (grid.x), at most.
+uint64_t kv_block_groups(const kq_kv_cache* c, const kq_kv_batch* b, uint32_t unit) {
+    return ((uint64_t)(b->max_q / unit) + 2) * ((2 * c->heads + 3) / 4);
+}
 bool kv_blocks_fit(const kq_kv_cache* c, const kq_kv_batch* b, uint32_t unit) {
-    return ((uint64_t)(b->max_q / unit) + 2) * ((2 * c->heads + 3) / 4) <= kq::kv::kMostGroups;
+    return kv_block_groups(c, b, unit) <= kq::kv::kMostGroups;
 }
 
 kq_status check_kv_heads(const kq_kv_cache* c, uint32_t q_heads) {
     return q_heads == 0 || q_heads % c->heads || q_heads / c->heads > 64 ? KQ_EINVAL : KQ_OK;
+}
+
+// ---- rotary positions
+kq_status check_rope(const kq_rope_desc* d, uint32_t head_dim) {
+    if (!d || !d->inv_freq) return KQ_ENULL;
+    if (d->rot < 2 || d->rot % 2 || d->rot > head_dim) return KQ_EINVAL;
+    if (d->layout > KQ_ROPE_PAIRS || !std::isfinite(d->amplitude)) return KQ_EINVAL;
+    return aligned(d->inv_freq, 4) ? KQ_OK : KQ_EALIGN;
+}
+kq::rope::Rope rope_of(const kq_rope_desc& d) {
+    return {d.inv_freq, d.rot, d.layout == KQ_ROPE_PAIRS, d.amplitude, d.inverse ? -(double)d.amplitude : d.amplitude};
 }
 
 }  // namespace
@@ -671,6 +689,87 @@ kq_status kq_kv_attn(const kq_kv_cache* cache, const kq_kv_batch* batch, const k
                              (65536 + group - 1) / group, d->sinks, lse};
     return hip_status(kq::launch_kv_attn(c, b, cache->head_dim, (int)cache->type, a, kv_rows(*Q), kv_rows(*O),
                                          dtype == KQ_BF16, ws, reinterpret_cast<hipStream_t>(stream)));
+}
+
+// ------------------------------------------------------------ rotary positions
+kq_status kq_rope_freqs(const kq_rope_scaling* s, float* inv_freq, float* amplitude) {
+    if (!s || !inv_freq || !amplitude) return KQ_ENULL;
+    if (s->kind > KQ_ROPE_YARN || s->rot < 2 || s->rot % 2 || s->rot > kq::rope::kMostHead) return KQ_EINVAL;
+    if (!std::isfinite(s->base) || !(s->base > 1.0)) return KQ_EINVAL;
+    const bool bands = s->kind == KQ_ROPE_BANDS || s->kind == KQ_ROPE_YARN;
+    if (s->kind != KQ_ROPE_PLAIN && (!std::isfinite(s->factor) || !(s->factor >= 1.0))) return KQ_EINVAL;
+    if (bands && !(std::isfinite(s->high) && std::isfinite(s->original) && s->low > 0.0 && s->low < s->high && s->original > 0.0))
+        return KQ_EINVAL;
+    if (s->kind == KQ_ROPE_NTK && s->rot == 2) return KQ_EINVAL;
+    const double rot = s->rot, turn = 6.283185307179586;
+    const double base = s->kind == KQ_ROPE_NTK ? s->base * std::pow(s->factor, rot / (rot - 2.0)) : s->base;
+    double from = 0.0, to = 0.0;
+    if (s->kind == KQ_ROPE_YARN) {
+        auto place = [&](double turns) { return rot * std::log(s->original / (turns * turn)) / (2.0 * std::log(base)); };
+        auto within = [&](double x) { return x < 0.0 ? 0.0 : x > rot - 1.0 ? rot - 1.0 : x; };
+        from = within(std::floor(place(s->high)));
+        to = within(std::ceil(place(s->low)));
+        if (from == to) to += 0.001;
+    }
+    for (uint32_t i = 0; i < s->rot / 2; ++i) {
+        const double f = std::pow(base, -2.0 * i / rot);
+        double share = 1.0;  // of the frequency as it is
+        if (s->kind == KQ_ROPE_LINEAR) share = 0.0;
+        if (s->kind == KQ_ROPE_BANDS) share = (s->original * f / turn - s->low) / (s->high - s->low);
+        if (s->kind == KQ_ROPE_YARN) share = 1.0 - (i - from) / (to - from);
+        share = share < 0.0 ? 0.0 : share > 1.0 ? 1.0 : share;
+        inv_freq[i] = (float)(share == 1.0 ? f : f * share + f / s->factor * (1.0 - share));
+    }
+    *amplitude = s->kind == KQ_ROPE_YARN ? (float)(0.1 * std::log(s->factor) + 1.0) : 1.0f;
+    return KQ_OK;
+}
+
+kq_status kq_rope(const kq_rope_desc* d, const int32_t* pos, const kq_kv_rows* X, const kq_kv_rows* Y, uint32_t n_rows,
+                  uint32_t heads, uint32_t head_dim, kq_dtype dtype, kq_stream_t stream) {
+    if (head_dim == 0 || head_dim % 8 || heads == 0 || heads > 65535 || n_rows >= 0x7FFF0000u) return KQ_EINVAL;
+    if (head_dim > kq::rope::kMostHead) return KQ_EUNSUPPORTED;
+    kq_status st = check_rope(d, head_dim);
+    if (st != KQ_OK) return st;
+    if (!(dtype == KQ_F16 || dtype == KQ_BF16 || dtype == KQ_F32)) return KQ_EUNSUPPORTED;
+    st = check_rows(X, n_rows, heads, head_dim, false);
+    if (st == KQ_OK) st = check_rows(Y, n_rows, heads, head_dim, true);
+    if (st != KQ_OK || n_rows == 0) return st;
+    // in place: the same elements
+    if (X->p == Y->p && ((n_rows > 1 && X->row != Y->row) || (heads > 1 && X->head != Y->head))) return KQ_EINVAL;
+    if (!pos) return KQ_ENULL;
+    if (!aligned(pos, 4)) return KQ_EALIGN;
+    if (!kq::rope_fits(n_rows, heads, d->rot)) return KQ_EUNSUPPORTED;
+    return hip_status(kq::launch_rope(rope_of(*d), pos, kv_rows(*X), kv_rows(*Y), n_rows, heads, head_dim, dtype,
+                                      reinterpret_cast<hipStream_t>(stream)));
+}
+
+kq_status kq_kv_write_rope(const kq_kv_cache* cache, const kq_kv_batch* batch, const kq_rope_desc* d, const int32_t* pos,
+                           const kq_kv_rows* Q, const kq_kv_rows* Qo, uint32_t q_heads, const kq_kv_rows* K,
+                           const kq_kv_rows* V, kq_dtype dtype, kq_stream_t stream) {
+    kq_status st = check_kv(cache, batch);
+    if (st == KQ_OK) st = check_kv_pointers(cache, batch);
+    if (st == KQ_OK) st = check_rope(d, cache->head_dim);
+    if (st != KQ_OK) return st;
+    if (d->rot % 16 || !(dtype == KQ_F16 || dtype == KQ_BF16)) return KQ_EUNSUPPORTED;
+    if (!aligned(pos, 4)) return KQ_EALIGN;
+    st = check_kv_rows(K, batch, cache->heads, cache->head_dim, false);
+    if (st == KQ_OK) st = check_kv_rows(V, batch, cache->heads, cache->head_dim, false);
+    if (st != KQ_OK) return st;
+    uint64_t groups = kv_block_groups(cache, batch, cache->block);
+    if (Q) {
+        if (q_heads == 0 || q_heads > 65535) return KQ_EINVAL;
+        st = check_kv_rows(Q, batch, q_heads, cache->head_dim, false);
+        if (st == KQ_OK) st = check_kv_rows(Qo, batch, q_heads, cache->head_dim, true);
+        if (st != KQ_OK) return st;
+        if (Q->p && Q->p == Qo->p && ((batch->n_rows > 1 && Q->row != Qo->row) || (q_heads > 1 && Q->head != Qo->head))) return KQ_EINVAL;
+        groups += (uint64_t)batch->max_q * ((q_heads + 3) / 4) / 4 + 1;
+    }
+    if (groups > kq::kv::kMostGroups) return KQ_EUNSUPPORTED;
+    if (batch->n_rows == 0) return KQ_OK;
+    const kq::kv::Rows q = Q ? kv_rows(*Q) : kq::kv::Rows{}, qo = Q ? kv_rows(*Qo) : kq::kv::Rows{};
+    return hip_status(kq::launch_kv_write_rope(kv_cache(*cache), kv_batch(*batch), cache->head_dim, (int)cache->type,
+                                               kq::kv::Turn{rope_of(*d), pos}, Q ? &q : nullptr, &qo, q_heads, kv_rows(*K),
+                                               kv_rows(*V), dtype == KQ_BF16, reinterpret_cast<hipStream_t>(stream)));
 }
 
 }  // extern "C"

@@ -159,6 +159,17 @@ bool moe_one_supported(const kq_moe_desc& d, uint32_t batch);
 bool moe_atomic_supported(const kq_moe_desc& d, uint32_t batch);
 
 
+// Rotary positions (kq_rope.hip).
+namespace rope {
+// kq_rope_desc as the kernels take it: amplitude_sin carries the direction.
+struct Rope {
+    const float* freq;
+    uint32_t rot, pairs;
+    double amplitude, amplitude_sin;
+};
+constexpr uint32_t kMostHead = 512;  // columns of a head in kq_rope
+}  // namespace rope
+
 // 8-bit key/value cache (kq_kv_cache.hip, kq_kv_attn.hip).
 namespace kv {
 // The cache, with shifts for its powers of two.
@@ -174,6 +185,13 @@ struct Batch {
 struct Rows {
     void* p;
     int64_t row, head;
+};
+// Spans of `tokens` that max_q consecutive ones can touch.
+inline uint32_t spans(uint32_t max_q, uint32_t tokens) { return (max_q - 1) / tokens + 1 + (max_q > 1); }
+// How keys are turned on their way into the cache; pos NULL: by their places in the sequences.
+struct Turn {
+    rope::Rope rope;
+    const int32_t* pos;
 };
 // Workgroups of 256 threads that a launch can have: HIP counts its threads in 32 bits.
 constexpr uint64_t kMostGroups = (1ull << 24) - 1;
@@ -236,6 +254,13 @@ hipError_t by_dim(uint32_t D, int type, Fn f) {
 }  // namespace kv
 hipError_t launch_kv_write(const kv::Cache& c, const kv::Batch& b, uint32_t D, int type, const kv::Rows& K,
                            const kv::Rows& V, bool bf, hipStream_t s);
+// Q null: no queries.
+hipError_t launch_kv_write_rope(const kv::Cache& c, const kv::Batch& b, uint32_t D, int type, const kv::Turn& turn,
+                                const kv::Rows* Q, const kv::Rows* Qo, uint32_t q_heads, const kv::Rows& K, const kv::Rows& V,
+                                bool bf, hipStream_t s);
+hipError_t launch_rope(const rope::Rope& r, const int32_t* pos, const kv::Rows& X, const kv::Rows& Y, uint32_t n_rows,
+                       uint32_t heads, uint32_t D, kq_dtype f, hipStream_t s);
+bool rope_fits(uint32_t n_rows, uint32_t heads, uint32_t rot);
 hipError_t launch_kv_read(const kv::Cache& c, const kv::Batch& b, uint32_t D, int type, const kv::Rows& K,
                           const kv::Rows& V, kq_dtype f, hipStream_t s);
 namespace kv {

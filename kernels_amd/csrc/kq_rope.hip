@@ -1,0 +1,55 @@
+// kq_rope.hip -- rotary positions (kq_rope): rows of heads turned by their position's angles.
+#include "kq_rope_device.h"
+
+namespace kq {
+namespace rope {
+namespace {
+
+// A wave for a row and up to `each` of its heads; blockIdx.x = the waves, four of them.
+template <int F, int PAIRS>
+__global__ __launch_bounds__(256) void rope_k(Rope r, const int32_t* pos, kv::Rows X, kv::Rows Y, uint32_t n_rows,
+                                              uint32_t heads, uint32_t D, uint32_t parts, uint32_t each) {
+    __shared__ Factor tables[4][kMostHead / 2];
+    const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const uint64_t id = (uint64_t)blockIdx.x * 4 + wave;
+    const uint32_t row = (uint32_t)(id / parts), part = (uint32_t)(id % parts);
+    if (row >= n_rows) return;
+    constexpr int kSize = F == KQ_F32 ? 4 : 2;
+    turn_heads<F, PAIRS>(r, pos[row], static_cast<const uint8_t*>(X.p) + (int64_t)row * X.row * kSize,
+                         static_cast<uint8_t*>(Y.p) + (int64_t)row * Y.row * kSize, X.head, Y.head, part * each,
+                         min(heads, (part + 1) * each), D, tables[wave]);
+}
+
+template <int F>
+hipError_t rope_f(const Rope& r, const int32_t* pos, const kv::Rows& X, const kv::Rows& Y, uint32_t n_rows, uint32_t heads,
+                  uint32_t D, uint32_t parts, uint32_t each, uint32_t wgs, hipStream_t s) {
+    if (r.pairs) rope_k<F, 1><<<wgs, 256, 0, s>>>(r, pos, X, Y, n_rows, heads, D, parts, each);
+    else rope_k<F, 0><<<wgs, 256, 0, s>>>(r, pos, X, Y, n_rows, heads, D, parts, each);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+// Heads of a wave: as many as its lanes take at once, or all of them where there are rows enough.
+uint32_t heads_each(uint32_t n_rows, uint32_t heads, uint32_t rot) {
+    const uint32_t at_once = rot % 16 ? 1 : 64 / (rot / 16);
+    const uint64_t parts = (heads + at_once - 1) / at_once;
+    return (uint64_t)n_rows * parts > 16384 ? heads : at_once;
+}
+}  // namespace rope
+
+bool rope_fits(uint32_t n_rows, uint32_t heads, uint32_t rot) {
+    const uint32_t each = rope::heads_each(n_rows, heads, rot);
+    return ((uint64_t)n_rows * ((heads + each - 1) / each) + 3) / 4 <= kv::kMostGroups;
+}
+
+hipError_t launch_rope(const rope::Rope& r, const int32_t* pos, const kv::Rows& X, const kv::Rows& Y, uint32_t n_rows,
+                       uint32_t heads, uint32_t D, kq_dtype f, hipStream_t s) {
+    const uint32_t each = rope::heads_each(n_rows, heads, r.rot), parts = (heads + each - 1) / each;
+    const uint32_t wgs = (uint32_t)(((uint64_t)n_rows * parts + 3) / 4);
+    return f == KQ_F16    ? rope::rope_f<KQ_F16>(r, pos, X, Y, n_rows, heads, D, parts, each, wgs, s)
+           : f == KQ_BF16 ? rope::rope_f<KQ_BF16>(r, pos, X, Y, n_rows, heads, D, parts, each, wgs, s)
+                          : rope::rope_f<KQ_F32>(r, pos, X, Y, n_rows, heads, D, parts, each, wgs, s);
+}
+
+}  // namespace kq

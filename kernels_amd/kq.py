@@ -31,7 +31,8 @@ EXPORTS = ("kq_status_str", "kq_last_hip_error", "kq_version", "kq_int4_gemv",
            "kq_moe_down_combine", "kq_moe_block", "kq_moe_block_path", "kq_moe_block_noalloc",
            "kq_moe_unfused_workspace_size",
            "kq_moe_block_unfused", "kq_vq_quantize_workspace_size", "kq_vq_quantize",
-           "kq_kv_write", "kq_kv_read", "kq_kv_attn_workspace_size", "kq_kv_attn")
+           "kq_kv_write", "kq_kv_read", "kq_kv_attn_workspace_size", "kq_kv_attn",
+           "kq_rope_freqs", "kq_rope", "kq_kv_write_rope")
 
 
 class KQError(RuntimeError):
@@ -77,6 +78,18 @@ class _KVAttnC(C.Structure):
     """kq_kv_attn_desc."""
     _fields_ = [("q_heads", C.c_uint32), ("scale", C.c_float), ("causal", C.c_uint32),
                 ("window", C.c_uint32), ("sinks", C.c_void_p)]
+
+
+class _RopeC(C.Structure):
+    """kq_rope_desc."""
+    _fields_ = [("inv_freq", C.c_void_p), ("rot", C.c_uint32), ("layout", C.c_uint32),
+                ("amplitude", C.c_float), ("inverse", C.c_uint32)]
+
+
+class _RopeScalingC(C.Structure):
+    """kq_rope_scaling."""
+    _fields_ = [("kind", C.c_uint32), ("rot", C.c_uint32), ("base", C.c_double), ("factor", C.c_double),
+                ("low", C.c_double), ("high", C.c_double), ("original", C.c_double)]
 
 
 _lib = None
@@ -135,6 +148,9 @@ def lib():
         L.kq_kv_attn_workspace_size.argtypes = [vp, vp, u32]
         L.kq_kv_attn_workspace_size.restype = sz
         L.kq_kv_attn.argtypes = [vp, vp, vp, vp, vp, i32, vp, vp, sz, vp]
+        L.kq_rope_freqs.argtypes = [C.POINTER(_RopeScalingC), vp, C.POINTER(C.c_float)]
+        L.kq_rope.argtypes = [vp, vp, vp, vp, u32, u32, u32, i32, vp]
+        L.kq_kv_write_rope.argtypes = [vp, vp, vp, vp, vp, vp, u32, vp, vp, i32, vp]
         for name in EXPORTS:
             if name not in ("kq_status_str", "kq_last_hip_error", "kq_version",
                             "kq_moe_default_desc", "kq_moe_workspace_size",
@@ -556,3 +572,87 @@ def kv_attn(cache, batch, q, out, ws, ws_bytes, scale=None, causal=True, window=
     d = _pack_attn(q_heads, cache.scale if scale is None else scale, bool(causal), window, _ptr(sinks) or 0)
     _check(lib().kq_kv_attn(cache._ref, batch._packed(rows), d, a, b, _dt(q),
                             _ptr(lse), _ptr(ws), ws_bytes, s), "kq_kv_attn")
+
+
+# ---------------------------------------------------------------------------
+# Rotary positions
+# ---------------------------------------------------------------------------
+ROPE_KINDS = ("plain", "linear", "ntk", "bands", "yarn")  # kq_rope_kind
+
+
+def rope_freqs(rot, base=10000.0, kind="plain", factor=1.0, low=1.0, high=None, original=0.0, device=None):
+    """(inv_freq float32 [rot/2] on the device, amplitude): the frequencies of rotary positions, as they are
+    or for contexts `factor` times as long as the `original` tokens (kq_rope_freqs; high: 4 in bands, 32 in yarn)."""
+    import torch
+    _need(kind in ROPE_KINDS, f"kind: one of {', '.join(ROPE_KINDS)}")
+    _need(0 <= rot < 2**32, "rot: 32-bit")
+    got, amplitude = (C.c_float * max(rot // 2, 1))(), C.c_float(0.0)
+    d = _RopeScalingC(ROPE_KINDS.index(kind), rot, base, factor, low, (32.0 if kind == "yarn" else 4.0) if high is None else high,
+                      original)
+    _check(lib().kq_rope_freqs(C.byref(d), got, C.byref(amplitude)), "kq_rope_freqs")
+    return torch.tensor(list(got), dtype=torch.float32, device=device or "cuda"), amplitude.value
+
+
+class Rope:
+    """kq_rope_desc over a contiguous float32 tensor [rot/2] of frequencies, kept alive with it.
+
+    pairs: columns (2i, 2i + 1) are turned together, else (i, i + rot/2). inverse:
+    the other way, which is the gradient."""
+
+    def __init__(self, inv_freq, pairs=False, amplitude=1.0, inverse=False):
+        import torch
+        _need(inv_freq.dim() == 1, "inv_freq: [rot/2]")
+        _here(inv_freq, torch.float32, inv_freq.shape, "inv_freq")
+        self.inv_freq, self.device, self.rot = inv_freq, inv_freq.get_device(), 2 * inv_freq.shape[0]
+        self._c = _RopeC(inv_freq.data_ptr(), self.rot, bool(pairs), amplitude, bool(inverse))
+        self._ref = C.byref(self._c)
+
+
+def _on_current(stream, *tensors):
+    """The call's stream; refuses tensors of another device than the current one, whose stream it is."""
+    s = _stream(stream)
+    if _current is None:
+        _stream(None)
+    d = _current[1]()
+    for t in tensors:
+        if t is not None and t.get_device() != d:
+            raise ValueError(f"every tensor of the call is on the current device ({d})")
+    return s
+
+
+def _positions(pos, rows):
+    if pos is not None:
+        import torch
+        _here(pos, torch.int32, (rows,), "pos")
+    return _ptr(pos)
+
+
+def rope(x, out, pos, rope, stream=None):
+    """x [n_rows][heads][head_dim] (float16, bfloat16 or float32, any row and head strides) turned into out, which
+    may be x; pos: int32 [n_rows], each row's position."""
+    s = _on_current(stream, x, out, pos, rope.inv_freq)
+    shape, dtype = x.shape, x.dtype
+    if len(shape) != 3:
+        raise ValueError(f"x: [n_rows][heads][head_dim], not {tuple(shape)}")
+    a, b = _kv_rows(x, shape, dtype, "x"), _kv_rows(out, shape, dtype, "out")
+    _check(lib().kq_rope(rope._ref, _positions(pos, shape[0]), a, b, *shape, _dt(x), s), "kq_rope")
+
+
+def kv_write_rope(cache, batch, rope, k, v, q=None, q_out=None, pos=None, stream=None):
+    """kv_write with the keys turned on their way into the cache, and q [n_rows][q_heads][head_dim] into q_out
+    (which may be q). pos: int32 [n_rows], or None: the rows' places in their sequences."""
+    s = _kv_call(cache, batch, stream, k, v, q, q_out, pos, rope.inv_freq)
+    shape, dtype = k.shape, k.dtype
+    if len(shape) != 3 or shape[1] != cache.heads or shape[2] != cache.head_dim:
+        raise ValueError(f"k: [n_rows][{cache.heads}][{cache.head_dim}], not {tuple(shape)}")
+    _need((q is None) == (q_out is None), "q and q_out: both or none")
+    a, b = _kv_rows(k, shape, dtype, "k"), _kv_rows(v, shape, dtype, "v")
+    x = y = None
+    heads = 0
+    if q is not None:
+        if q.dim() != 3 or q.shape[0] != shape[0] or q.shape[2] != shape[2]:
+            raise ValueError(f"q: [{shape[0]}][q_heads][{shape[2]}], not {tuple(q.shape)}")
+        heads = q.shape[1]
+        x, y = _kv_rows(q, q.shape, dtype, "q"), _kv_rows(q_out, q.shape, dtype, "q_out")
+    _check(lib().kq_kv_write_rope(cache._ref, batch._packed(shape[0]), rope._ref, _positions(pos, shape[0]), x, y, heads, a, b,
+                                  _dt(k), s), "kq_kv_write_rope")

@@ -1,0 +1,149 @@
+"""The calls of a speculative step on the CPU: what the host refuses before any launch, and
+what it computes itself."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+from kernels_amd import kq
+from tests.test_kv_abi import BAD_BATCH, BAD_BATCH_P, BAD_CACHE, BAD_CACHE_P, FAKE, batch_c, cache_c, rows_c
+
+
+def rope_c(**kw):
+    a = dict(inv_freq=FAKE, rot=128, layout=0, amplitude=1.0, inverse=0)
+    a.update(kw)
+    return kq._RopeC(**a)
+
+
+def rope(d=None, pos=FAKE, X=None, Y=None, n=6, heads=8, dim=128, dt=kq.F16):
+    return kq.lib().kq_rope(C.byref(d or rope_c()), pos, C.byref(X or rows_c()), C.byref(Y or rows_c(p=FAKE * 2)), n, heads, dim, dt, None)
+
+
+def write(c=None, b=None, d=None, pos=None, Q=None, Qo=None, q_heads=32, K=None, V=None, dt=kq.F16, q=True):
+    Q, Qo = Q or rows_c(row=4096), Qo or rows_c(p=FAKE * 2, row=4096)
+    return kq.lib().kq_kv_write_rope(C.byref(c or cache_c()), C.byref(b or batch_c()), C.byref(d or rope_c()), pos,
+                                     C.byref(Q) if q else None, C.byref(Qo) if q else None, q_heads, C.byref(K or rows_c()),
+                                     C.byref(V or rows_c()), dt, None)
+
+
+@pytest.mark.parametrize("kw,status", [
+    (dict(inv_freq=None), kq.KQ_ENULL), (dict(inv_freq=FAKE + 2), kq.KQ_EALIGN), (dict(rot=0), kq.KQ_EINVAL), (dict(rot=63), kq.KQ_EINVAL),
+    (dict(rot=130), kq.KQ_EINVAL), (dict(layout=2), kq.KQ_EINVAL), (dict(amplitude=float("nan")), kq.KQ_EINVAL),
+    (dict(amplitude=float("inf")), kq.KQ_EINVAL)])
+def test_bad_rope(kw, status):
+    assert rope(rope_c(**kw)) == write(d=rope_c(**kw)) == status
+
+
+@pytest.mark.parametrize("kw,status", [
+    (dict(dim=0), kq.KQ_EINVAL), (dict(dim=132), kq.KQ_EINVAL), (dict(dim=520), kq.KQ_EUNSUPPORTED), (dict(heads=0), kq.KQ_EINVAL),
+    (dict(heads=65536), kq.KQ_EINVAL), (dict(n=0x7FFF0000), kq.KQ_EINVAL), (dict(dt=3), kq.KQ_EUNSUPPORTED), (dict(pos=None), kq.KQ_ENULL),
+    (dict(pos=FAKE + 2), kq.KQ_EALIGN), (dict(X=rows_c(p=None)), kq.KQ_ENULL), (dict(Y=rows_c(p=FAKE + 8)), kq.KQ_EALIGN),
+    (dict(X=rows_c(row=1028)), kq.KQ_EINVAL), (dict(Y=rows_c(row=0)), kq.KQ_EINVAL), (dict(Y=rows_c(head=64)), kq.KQ_EINVAL),
+    (dict(X=rows_c(row=2048), Y=rows_c(row=1024)), kq.KQ_EINVAL), (dict(X=rows_c(head=256, row=2048), Y=rows_c(row=2048)), kq.KQ_EINVAL)])
+def test_bad_rows(kw, status):
+    assert rope(**kw) == status
+
+
+def test_rope_of_no_rows_and_launch_limits():
+    none = rows_c(p=None)
+    assert rope(n=0, X=none, Y=none, pos=None) == kq.KQ_OK
+    assert rope(n=0, X=none, Y=none, dt=7) == kq.KQ_EUNSUPPORTED
+    assert rope(n=2**27, X=rows_c(row=1 << 17), Y=rows_c(p=FAKE * 2, row=1 << 17)) == kq.KQ_EUNSUPPORTED
+
+
+def test_null_structs():
+    L = kq.lib()
+    r, d = rows_c(), rope_c()
+    assert L.kq_rope(None, FAKE, C.byref(r), C.byref(r), 6, 8, 128, 0, None) == kq.KQ_ENULL
+    assert L.kq_rope(C.byref(d), FAKE, None, C.byref(r), 6, 8, 128, 0, None) == kq.KQ_ENULL
+    assert L.kq_kv_write_rope(C.byref(cache_c()), C.byref(batch_c()), None, None, None, None, 0, C.byref(r), C.byref(r), 0, None) == kq.KQ_ENULL
+    assert L.kq_kv_write_rope(C.byref(cache_c()), C.byref(batch_c()), C.byref(d), None, C.byref(rows_c(row=4096)), None, 32, C.byref(r), C.byref(r), 0, None) == kq.KQ_ENULL
+
+
+@pytest.mark.parametrize("kw,status", BAD_CACHE + BAD_CACHE_P)
+def test_bad_cache(kw, status):
+    assert write(cache_c(**kw)) == status
+
+
+@pytest.mark.parametrize("kw,status", BAD_BATCH + BAD_BATCH_P)
+def test_bad_batch(kw, status):
+    assert write(b=batch_c(**kw)) == status
+
+
+@pytest.mark.parametrize("kw,status", [
+    (dict(d=rope_c(rot=24)), kq.KQ_EUNSUPPORTED), (dict(dt=kq.F32), kq.KQ_EUNSUPPORTED), (dict(pos=FAKE + 2), kq.KQ_EALIGN),
+    (dict(q_heads=0), kq.KQ_EINVAL), (dict(q_heads=65536), kq.KQ_EINVAL), (dict(Q=rows_c(p=None)), kq.KQ_ENULL),
+    (dict(Qo=rows_c(row=120)), kq.KQ_EINVAL), (dict(Qo=rows_c(p=FAKE + 8, row=4096)), kq.KQ_EALIGN), (dict(Q=rows_c(row=8192), Qo=rows_c(row=4096)), kq.KQ_EINVAL),
+    (dict(K=rows_c(p=None)), kq.KQ_ENULL), (dict(V=rows_c(row=1028)), kq.KQ_EINVAL)])
+def test_bad_write(kw, status):
+    assert write(**kw) == status
+
+
+def test_write_of_no_rows_and_launch_limits():
+    none = rows_c(p=None)
+    assert write(b=batch_c(n_rows=0), K=none, V=none, Q=none, Qo=none) == kq.KQ_OK
+    assert write(b=batch_c(n_rows=0), K=none, V=none, q=False) == kq.KQ_OK
+    # without queries the blocks fit; the queries' rows are too many
+    b = batch_c(n_rows=0, max_q=2**24, max_len=2**24, max_pages=2**20)
+    assert write(b=b, K=none, V=none, q=False) == kq.KQ_OK
+    assert write(b=b, K=none, V=none, Q=none, Qo=none) == kq.KQ_EUNSUPPORTED
+
+
+# ---- frequencies, which the host computes
+
+def freqs(rot=64, **kw):
+    f, a = kq.rope_freqs(rot, device="cpu", **kw)
+    return f.double().numpy(), a
+
+
+def test_freqs_plain_linear_ntk():
+    i = np.arange(32)
+    want = 10000.0 ** (-2 * i / 64)
+    assert np.allclose(freqs()[0], want, rtol=2**-24, atol=0) and freqs()[1] == 1.0
+    assert np.allclose(freqs(kind="linear", factor=4.0)[0], want / 4, rtol=2**-24, atol=0)
+    got = freqs(kind="ntk", factor=8.0)[0]
+    # the fastest pair as it is, the slowest slower by the factor
+    assert got[0] == 1.0 and abs(got[-1] * 8.0 / want[-1] - 1) < 2**-22
+
+
+def test_freqs_bands():
+    want, got = freqs(base=500000.0)[0], freqs(base=500000.0, kind="bands", factor=8.0, low=1.0, high=4.0, original=8192.0)[0]
+    turns = 8192.0 * want / (2 * np.pi)
+    assert np.array_equal(got[turns > 4], want[turns > 4]) and (turns > 4).any()
+    assert np.allclose(got[turns < 1], want[turns < 1] / 8, rtol=2**-22, atol=0) and (turns < 1).any()
+    mid = (turns >= 1) & (turns <= 4)
+    share = (turns[mid] - 1) / 3
+    assert np.allclose(got[mid], want[mid] * share + want[mid] / 8 * (1 - share), rtol=2**-21, atol=0) and mid.any()
+
+
+def test_freqs_yarn():
+    want, (got, a) = freqs()[0], freqs(kind="yarn", factor=16.0, original=4096.0)
+    assert abs(a - (0.1 * np.log(16.0) + 1)) < 2**-22
+    c = [64 * np.log(4096 / (n * 2 * np.pi)) / (2 * np.log(10000.0)) for n in (32.0, 1.0)]
+    lo, hi = np.floor(c[0]), np.ceil(c[1])
+    r = np.clip((np.arange(32) - lo) / (hi - lo), 0, 1)
+    assert np.allclose(got, want * (1 - r) + want / 16 * r, rtol=2**-22, atol=0)
+    assert got[0] == 1.0 and got[-1] < want[-1] / 15
+    # a context so short that both ends meet
+    f, _ = freqs(kind="yarn", factor=2.0, original=1.0)
+    assert np.isfinite(f).all()
+
+
+@pytest.mark.parametrize("kw", [dict(rot=0), dict(rot=3), dict(rot=514), dict(base=1.0), dict(base=float("nan")), dict(base=float("inf")),
+                                dict(kind="linear", factor=0.5), dict(kind="linear", factor=float("nan")), dict(kind="ntk", rot=2, factor=2.0),
+                                dict(kind="bands", factor=2.0), dict(kind="bands", factor=2.0, original=100.0, low=4.0, high=4.0),
+                                dict(kind="yarn", factor=2.0, original=float("inf")), dict(kind="yarn", factor=2.0, original=-1.0)])
+def test_freqs_refused(kw):
+    with pytest.raises(kq.KQError) as e:
+        freqs(**kw)
+    assert e.value.status == kq.KQ_EINVAL
+
+
+def test_freqs_nulls_and_kinds():
+    L, d, a = kq.lib(), kq._RopeScalingC(0, 64, 1e4, 1, 1, 4, 0), C.c_float()
+    out = (C.c_float * 32)()
+    assert L.kq_rope_freqs(None, out, C.byref(a)) == L.kq_rope_freqs(C.byref(d), None, C.byref(a)) == L.kq_rope_freqs(C.byref(d), out, None) == kq.KQ_ENULL
+    d.kind = 5
+    assert L.kq_rope_freqs(C.byref(d), out, C.byref(a)) == kq.KQ_EINVAL
+    with pytest.raises(ValueError):
+        kq.rope_freqs(64, kind="other", device="cpu")
