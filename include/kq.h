@@ -605,6 +605,47 @@ kq_status kq_kv_write_rope(const kq_kv_cache* cache, const kq_kv_batch* batch,
                            const kq_kv_rows* Qo, uint32_t q_heads, const kq_kv_rows* K,
                            const kq_kv_rows* V, kq_dtype dtype, kq_stream_t stream);
 
+/* ------------------------------------------------------------------------
+ * Trees of drafted tokens
+ *
+ * A sequence's rows of a step as a tree: row 0 is the last token that is certain,
+ * rows 1 .. n - 1 are drafted, and row j continues row parent[j] < j. Their keys
+ * and values stand in the cache one after the other, as kq_kv_write puts them.
+ * No counterpart in the reference.
+ *
+ * kq_kv_tree: what the step's calls take of a tree, once for all layers.
+ * parent : int32 [n_rows], of each row the number of its parent among its
+ *          sequence's rows; one that is not in 0 .. j - 1 makes row j a root
+ * mask   : uint32 [n_rows][words], written: bit t of row j says that the row sees
+ *          its sequence's row t: itself and the rows it continues; with
+ *          window > 0 the nearest `window` of them alone. words >= max_q / 32, rounded up
+ * pos    : int32 [n_rows] or NULL, written: kv_len - n + the row's depth
+ * Rows of no sequence are left as they were. max_q <= 1024 (else KQ_EUNSUPPORTED). The
+ * batch's pages are not read. One launch. */
+kq_status kq_kv_tree(const kq_kv_batch* batch, const int32_t* parent, uint32_t* mask,
+                     uint32_t words, int32_t* pos, uint32_t window, kq_stream_t stream);
+
+/* kq_kv_attn of a tree's rows: a row sees the tokens of its sequence before the
+ * batch's rows -- with window > 0 those behind position pos - window -- and of the batch's
+ * rows of its sequence those whose bit is set in its mask, whatever they are (a mask of
+ * nothing is one, too). Everything else is kq_kv_attn's: sums, sinks, lse, rows that
+ * see nothing, limits of a launch. d->causal is not looked at.
+ * pos: int32 [n_rows], the rows' positions, below 2^31 - 2^16 and at least that of their
+ * sequence's first row (else they count as that); read with window > 0 alone, else NULL will do.
+ * words * 32 >= max_q, max_q <= 1024 (else KQ_EUNSUPPORTED).
+ * ws: kq_kv_attn_tree_workspace_size bytes, otherwise as kq_kv_attn's. */
+typedef struct kq_kv_nodes {
+    const uint32_t* mask;
+    const int32_t* pos;
+    uint32_t words;
+} kq_kv_nodes;
+size_t kq_kv_attn_tree_workspace_size(const kq_kv_cache* cache, const kq_kv_batch* batch,
+                                      uint32_t q_heads);
+kq_status kq_kv_attn_tree(const kq_kv_cache* cache, const kq_kv_batch* batch,
+                          const kq_kv_attn_desc* d, const kq_kv_nodes* nodes, const kq_kv_rows* Q,
+                          const kq_kv_rows* O, kq_dtype dtype, float* lse, void* ws,
+                          size_t ws_bytes, kq_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

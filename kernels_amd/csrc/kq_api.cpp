@@ -171,6 +171,7 @@ kq_status check_ws(const kq_moe_desc* d, uint32_t batch, const void* ws, size_t 
 // ---- 8-bit key/value cache
 uint32_t log2_of(uint32_t v) { return 31u - (uint32_t)__builtin_clz(v); }
 
+kq_status check_kv_batch(const kq_kv_batch* b);
 kq_status check_kv(const kq_kv_cache* c, const kq_kv_batch* b) {
     if (!c || !b) return KQ_ENULL;
     if (!(c->type == KQ_KV_I8 || c->type == KQ_KV_E4M3)) return KQ_EUNSUPPORTED;
@@ -179,6 +180,9 @@ kq_status check_kv(const kq_kv_cache* c, const kq_kv_batch* b) {
     if (!pow2(c->block) || c->block < 16 || c->block > 256) return KQ_EINVAL;
     if (!pow2(c->page) || c->page < c->block || c->page > 4096) return KQ_EINVAL;
     if (c->heads == 0 || c->heads > 1024 || c->n_pages == 0 || c->n_pages > 0x7FFFFFFFu) return KQ_EINVAL;
+    return check_kv_batch(b);
+}
+kq_status check_kv_batch(const kq_kv_batch* b) {
     constexpr uint32_t kMost = 0x7FFF0000u;  // tokens and rows are ints in the kernels, with room for a tile
     if (b->n_seq == 0 || b->n_seq > 65535 || b->max_pages == 0 || b->max_q == 0 || b->max_len == 0) return KQ_EINVAL;
     if (b->max_len >= kMost || b->max_q >= kMost || b->n_rows >= kMost) return KQ_EINVAL;
@@ -659,9 +663,11 @@ size_t kq_kv_attn_workspace_size(const kq_kv_cache* cache, const kq_kv_batch* ba
     return kq::kv_attn_ws_bytes(kv_cache(*cache), b, cache->head_dim, group);
 }
 
-kq_status kq_kv_attn(const kq_kv_cache* cache, const kq_kv_batch* batch, const kq_kv_attn_desc* d,
-                     const kq_kv_rows* Q, const kq_kv_rows* O, kq_dtype dtype, float* lse,
-                     void* ws, size_t ws_bytes, kq_stream_t stream) {
+namespace {
+// kq_kv_attn, or of a tree's nodes.
+kq_status kv_attn(const kq_kv_cache* cache, const kq_kv_batch* batch, const kq_kv_attn_desc* d, const kq_kv_nodes* nodes,
+                  const kq_kv_rows* Q, const kq_kv_rows* O, kq_dtype dtype, float* lse, void* ws, size_t ws_bytes,
+                  kq_stream_t stream) {
     kq_status st = check_kv(cache, batch);
     if (st == KQ_OK) st = check_kv_pointers(cache, batch);
     if (st != KQ_OK) return st;
@@ -670,7 +676,7 @@ kq_status kq_kv_attn(const kq_kv_cache* cache, const kq_kv_batch* batch, const k
     st = check_kv_heads(cache, d->q_heads);
     if (st != KQ_OK) return st;
     const float scale_log2 = d->scale * 1.4426950408889634f;
-    if (!(scale_log2 - scale_log2 == 0.0f) || (d->window && !d->causal)) return KQ_EINVAL;
+    if (!(scale_log2 - scale_log2 == 0.0f) || (d->window && !d->causal && !nodes)) return KQ_EINVAL;
     st = check_kv_rows(Q, batch, d->q_heads, cache->head_dim, false);
     if (st == KQ_OK) st = check_kv_rows(O, batch, d->q_heads, cache->head_dim, true);
     if (st != KQ_OK) return st;
@@ -678,17 +684,63 @@ kq_status kq_kv_attn(const kq_kv_cache* cache, const kq_kv_batch* batch, const k
     const kq::kv::Cache c = kv_cache(*cache);
     const kq::kv::Batch b = kv_batch(*batch);
     const uint32_t group = d->q_heads / cache->heads;
-    const uint32_t window = d->window < batch->max_len ? d->window : 0;  // as wide as all there is: none
-    if (!kq::kv_attn_fits(c, b, cache->head_dim, group)) return KQ_EUNSUPPORTED;
-    if (!ws || ws_bytes < kq::kv_attn_ws_bytes(c, b, cache->head_dim, group) ||
-        ws_bytes < kq::kv_attn_ws_need(c, b, cache->head_dim, group, window))  // never more than the former
+    uint32_t window = d->window < batch->max_len ? d->window : 0;  // as wide as all there is: none
+    if (nodes) {
+        window = d->window < 0x7FFF0000u ? d->window : 0x7FFF0000u;  // positions may pass max_len
+        if (batch->n_rows && (!nodes->mask || (window && !nodes->pos))) return KQ_ENULL;
+        if (!aligned(nodes->mask, 4) || !aligned(nodes->pos, 4)) return KQ_EALIGN;
+        if (batch->max_q > kq::kMostNodes) return KQ_EUNSUPPORTED;
+        if (nodes->words > 0x7FFFFFFFu || nodes->words < (batch->max_q + 31) / 32) return KQ_EINVAL;
+    }
+    if (!(nodes ? kq::kv_tree_fits : kq::kv_attn_fits)(c, b, cache->head_dim, group)) return KQ_EUNSUPPORTED;
+    if (!ws || ws_bytes < (nodes ? kq::kv_tree_ws_bytes : kq::kv_attn_ws_bytes)(c, b, cache->head_dim, group) ||
+        ws_bytes < (nodes ? kq::kv_tree_ws_need : kq::kv_attn_ws_need)(c, b, cache->head_dim, group, window))  // never more than the former
         return KQ_EWORKSPACE;
     if (!aligned(ws, 256)) return KQ_EALIGN;
     if (batch->n_rows == 0) return KQ_OK;
-    const kq::kv::Attn a = {scale_log2, group, d->causal != 0, window,
-                             (65536 + group - 1) / group, d->sinks, lse};
+    kq::kv::Attn a = {scale_log2, group, d->causal != 0, window, (65536 + group - 1) / group, d->sinks, lse, nullptr, nullptr, 0};
+    if (nodes) a.mask = nodes->mask, a.pos = nodes->pos, a.words = nodes->words;
     return hip_status(kq::launch_kv_attn(c, b, cache->head_dim, (int)cache->type, a, kv_rows(*Q), kv_rows(*O),
                                          dtype == KQ_BF16, ws, reinterpret_cast<hipStream_t>(stream)));
+}
+}  // namespace
+
+kq_status kq_kv_attn(const kq_kv_cache* cache, const kq_kv_batch* batch, const kq_kv_attn_desc* d,
+                     const kq_kv_rows* Q, const kq_kv_rows* O, kq_dtype dtype, float* lse,
+                     void* ws, size_t ws_bytes, kq_stream_t stream) {
+    return kv_attn(cache, batch, d, nullptr, Q, O, dtype, lse, ws, ws_bytes, stream);
+}
+
+// ------------------------------------------------------------ trees of drafted tokens
+kq_status kq_kv_tree(const kq_kv_batch* batch, const int32_t* parent, uint32_t* mask, uint32_t words, int32_t* pos,
+                     uint32_t window, kq_stream_t stream) {
+    if (!batch) return KQ_ENULL;
+    kq_status st = check_kv_batch(batch);
+    if (st != KQ_OK) return st;
+    if (!batch->kv_len || (batch->n_rows && (!parent || !mask))) return KQ_ENULL;
+    if (!aligned(batch->kv_len, 4) || !aligned(batch->q_start, 4) || !aligned(parent, 4) || !aligned(mask, 4) || !aligned(pos, 4))
+        return KQ_EALIGN;
+    if (batch->max_q > kq::kMostNodes) return KQ_EUNSUPPORTED;
+    if (words > 0x7FFFFFFFu || words < (batch->max_q + 31) / 32) return KQ_EINVAL;
+    if (batch->n_rows == 0) return KQ_OK;
+    kq::kv::Batch b = kv_batch(*batch);
+    b.max_pages = 0x7FFFFFFFu;  // lengths are cut to max_len alone: no pages are read
+    return hip_status(kq::launch_kv_tree(b, parent, mask, words, pos, window, reinterpret_cast<hipStream_t>(stream)));
+}
+
+size_t kq_kv_attn_tree_workspace_size(const kq_kv_cache* cache, const kq_kv_batch* batch, uint32_t q_heads) {
+    if (check_kv(cache, batch) != KQ_OK || check_kv_heads(cache, q_heads) != KQ_OK || batch->max_q > kq::kMostNodes) return 0;
+    const kq::kv::Batch b = kv_batch(*batch);
+    const uint32_t group = q_heads / cache->heads;
+    if (!kq::kv_tree_fits(kv_cache(*cache), b, cache->head_dim, group)) return 0;
+    return kq::kv_tree_ws_bytes(kv_cache(*cache), b, cache->head_dim, group);
+}
+
+kq_status kq_kv_attn_tree(const kq_kv_cache* cache, const kq_kv_batch* batch, const kq_kv_attn_desc* d,
+                          const kq_kv_nodes* nodes, const kq_kv_rows* Q, const kq_kv_rows* O, kq_dtype dtype,
+                          float* lse, void* ws, size_t ws_bytes, kq_stream_t stream) {
+    if (!nodes) return KQ_ENULL;
+    return kv_attn(cache, batch, d, nodes, Q, O, dtype, lse, ws, ws_bytes, stream);
 }
 
 // ------------------------------------------------------------ rotary positions

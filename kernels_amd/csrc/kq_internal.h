@@ -202,6 +202,10 @@ struct Attn {
     uint32_t group_inv;  // 2^16 / group, rounded up
     const float* sinks;
     float* lse;
+    // of trees: a row's bits, `words` of them, and its position (read with a window)
+    const uint32_t* mask;
+    const int32_t* pos;
+    uint32_t words;
 };
 // Launch of the kernel for few rows. A row of work is a sequence and head.
 struct FewPlan {
@@ -264,8 +268,8 @@ bool rope_fits(uint32_t n_rows, uint32_t heads, uint32_t rot);
 hipError_t launch_kv_read(const kv::Cache& c, const kv::Batch& b, uint32_t D, int type, const kv::Rows& K,
                           const kv::Rows& V, kq_dtype f, hipStream_t s);
 namespace kv {
-// The kernels, heads D wide (kq_kv_attn_<D>.hip).
-template <int D>
+// The kernels, heads D wide (kq_kv_attn_<D>.hip; of trees: kq_kv_tree_<D>.hip).
+template <int D, bool TREE>
 struct AttnKernels {
     static hipError_t few(int type, const Cache& c, const Batch& b, const Attn& a, const FewPlan& p, const Rows& Q,
                           const Rows& O, bool bf, float* ws, hipStream_t s);
@@ -278,7 +282,16 @@ struct AttnKernels {
 size_t kv_attn_ws_need(const kv::Cache& c, const kv::Batch& b, uint32_t D, uint32_t group, uint32_t window);
 size_t kv_attn_ws_bytes(const kv::Cache& c, const kv::Batch& b, uint32_t D, uint32_t group);
 bool kv_attn_fits(const kv::Cache& c, const kv::Batch& b, uint32_t D, uint32_t group);
+// The same of trees, whose rows see by masks.
+size_t kv_tree_ws_need(const kv::Cache& c, const kv::Batch& b, uint32_t D, uint32_t group, uint32_t window);
+size_t kv_tree_ws_bytes(const kv::Cache& c, const kv::Batch& b, uint32_t D, uint32_t group);
+bool kv_tree_fits(const kv::Cache& c, const kv::Batch& b, uint32_t D, uint32_t group);
 hipError_t launch_kv_attn(const kv::Cache& c, const kv::Batch& b, uint32_t D, int type, const kv::Attn& a,
                           const kv::Rows& Q, const kv::Rows& O, bool bf, void* ws, hipStream_t s);
+
+// Trees of drafted tokens (kq_spec.hip).
+constexpr uint32_t kMostNodes = 1024;  // rows of a sequence's tree
+hipError_t launch_kv_tree(const kv::Batch& b, const int32_t* parent, uint32_t* mask, uint32_t words, int32_t* pos,
+                          uint32_t window, hipStream_t s);
 
 }  // namespace kq

@@ -57,14 +57,32 @@ constexpr int kRowSum = sizeof(RowSum) / sizeof(float);
 struct Span {
     int lo, hi;
 };
+template <bool TREE>
 __device__ __forceinline__ Span span_of(const Seq& s, const Attn& a, int row, int rows) {
     Span v = {0, s.len};
-    if (a.causal) {
+    if constexpr (TREE) {
+        // any of the sequence's rows, and a window behind its first one's position
+        if (a.window) v.lo = max(s.len - s.n - (int)a.window + 1, 0) & ~(kTile - 1);
+    } else if (a.causal) {
         const int pos = s.len - s.n, last = min(row + rows, (int)(s.n * a.group)) - 1;
         v.hi = max(pos + last / (int)a.group + 1, 0);
         if (a.window) v.lo = max(pos + row / (int)a.group - (int)a.window + 1, 0) & ~(kTile - 1);
     }
     return v;
+}
+
+// Of a tree: what a row sees of the 16 tokens from t0 on, a bit for each. The sequence's rows are the tokens from
+// `first` on; before them the row sees from `lo` on, and nothing counts that is not below hi.
+__device__ __forceinline__ uint32_t low_bits(int n) { return n >= 16 ? 0xFFFFu : (1u << max(n, 0)) - 1; }
+__device__ __forceinline__ uint32_t tree_bits(const uint32_t* mask, int words, int t0, int first, int lo, int hi) {
+    uint32_t sees = low_bits(first - t0) & ~low_bits(lo - t0);
+    const int off = t0 - first;  // of the tokens' bits
+    if (off > -16) {
+        const int w = off >> 5;
+        const uint32_t a = w >= 0 && w < words ? mask[w] : 0u, b = w + 1 < words ? mask[w + 1] : 0u;
+        sees |= (uint32_t)(((uint64_t)b << 32 | a) >> (off & 31)) & 0xFFFFu & ~low_bits(-off);
+    }
+    return sees & low_bits(hi - t0);
 }
 
 __device__ __forceinline__ int row_splits(const Span& v, int chunk) {
@@ -212,8 +230,9 @@ __device__ __forceinline__ T load_codes(const T* p) {
 // A row of work that a cut goes through leaves partial sums: a group's first piece, if it continues a
 // row, in slot 2k, a last piece that begins a row and does not end it in slot 2k + 1 (k the group);
 // kv_join_k adds the row's parts up.
+template <bool TREE>
 __device__ __forceinline__ int units_of(const Seq& s, const Attn& a, int rows, int start) {
-    const Span v = span_of(s, a, 0, rows);
+    const Span v = span_of<TREE>(s, a, 0, rows);
     return s.n == 0 ? 0 : max((v.hi - v.lo + kTile - 1) / kTile, 1) + start;
 }
 
@@ -245,6 +264,7 @@ __device__ __forceinline__ int prefix64(int v) {
 
 // What group k does; each wave works it out for itself from the units of all sequences.
 // lds: kScan ints.
+template <bool TREE>
 __device__ inline Share share_of(const Cache& c, const Batch& b, const Attn& a, const FewPlan& p, uint32_t k, int rows,
                                  int* lds) {
     const int lane = threadIdx.x & 63, n = (int)b.n_seq;
@@ -253,14 +273,14 @@ __device__ inline Share share_of(const Cache& c, const Batch& b, const Attn& a, 
     if (p.mode == FewPlan::kRows) {
         w.seq = (int)(k / c.heads);
         w.head = k % c.heads;
-        w.units = units_of(sequence(b, c.page_log2, w.seq), a, rows, (int)p.start);
+        w.units = units_of<TREE>(sequence(b, c.page_log2, w.seq), a, rows, (int)p.start);
         return w;
     }
     int u0;  // of sequence `lane`
     if (n <= 64) {
-        u0 = lane < n ? units_of(sequence(b, c.page_log2, lane), a, rows, (int)p.start) : 0;
+        u0 = lane < n ? units_of<TREE>(sequence(b, c.page_log2, lane), a, rows, (int)p.start) : 0;
     } else {
-        for (int i = threadIdx.x; i < n; i += 256) lds[i] = units_of(sequence(b, c.page_log2, i), a, rows, (int)p.start);
+        for (int i = threadIdx.x; i < n; i += 256) lds[i] = units_of<TREE>(sequence(b, c.page_log2, i), a, rows, (int)p.start);
         __syncthreads();
         u0 = lds[lane];
     }
@@ -352,7 +372,7 @@ __device__ __forceinline__ float* slot_of(float* ws, const FewPlan& p, uint32_t 
 // (128 wide) is always on its way. ONCE: no other workgroup reads the codes, and they are loaded past the
 // caches' other lines (64 sequences of 2486 tokens 69 us without, 64 with); with two row tiles to
 // share them that costs more than it saves (28 us without, 31 with).
-template <int D, int TYPE, int R, bool ONCE>
+template <int D, int TYPE, int R, bool ONCE, bool TREE>
 __global__ __launch_bounds__(256, few_waves(D)) void kv_few_k(Cache c, Batch b, Attn a, FewPlan p, Rows Q, Rows O, int bf,
                                                               float* ws) {
     constexpr int C64 = D / 64, kHalf = D % 64 ? 1 : 0;  // 64-column pieces of a key, and a 32-column one
@@ -368,7 +388,7 @@ __global__ __launch_bounds__(256, few_waves(D)) void kv_few_k(Cache c, Batch b, 
     // the workgroups of a group side by side in one of eight XCDs: 8 groups' first tiles, their second, ...
     const uint32_t group = blockIdx.x / (8 * p.tiles) * 8 + blockIdx.x % 8, tile = blockIdx.x / 8 % p.tiles;
     const int all_rows = (int)(b.max_q * a.group), row0 = (int)tile * 16 * R;
-    const Share share = share_of(c, b, a, p, group, all_rows, ids);
+    const Share share = share_of<TREE>(c, b, a, p, group, all_rows, ids);
     Cut* const cuts = reinterpret_cast<Cut*>(ws);
     if (p.mode == FewPlan::kShares && !p.by_row && group < p.groups && tile == 0 && tid == 0) cuts[group].parts = 0;
     int left = share.units, unit = share.unit;
@@ -379,8 +399,8 @@ __global__ __launch_bounds__(256, few_waves(D)) void kv_few_k(Cache c, Batch b, 
         seq = __builtin_amdgcn_readfirstlane(seq);
         h = (uint32_t)__builtin_amdgcn_readfirstlane((int)h);
         const Seq s = sequence(b, c.page_log2, (uint32_t)seq);
-        const Span sp = span_of(s, a, 0, all_rows);  // the same for all row tiles
-        const int units = units_of(s, a, all_rows, (int)p.start), mine = min(left, units - unit);
+        const Span sp = span_of<TREE>(s, a, 0, all_rows);  // the same for all row tiles
+        const int units = units_of<TREE>(s, a, all_rows, (int)p.start), mine = min(left, units - unit);
         if (mine <= 0) {  // a sequence without rows
             ++seq;
             continue;
@@ -395,6 +415,8 @@ __global__ __launch_bounds__(256, few_waves(D)) void kv_few_k(Cache c, Batch b, 
             f16x8 q[R][D / 32];
             float m[R], l[R];  // of the row; l: this lane's tokens alone
             int q_exp[R], sees_lo[R], sees_hi[R], base = kBase;
+            const int first_row = max(s.len - s.n, 0);          // TREE: the token of the first row
+            const uint32_t* masks[R];                           // TREE: the row's bits, from that of token s.len - s.n on
             f32x4 o[R][D / 16];
 #pragma unroll
             for (int k = 0; k < R; ++k) {
@@ -402,8 +424,14 @@ __global__ __launch_bounds__(256, few_waves(D)) void kv_few_k(Cache c, Batch b, 
                 const bool there = 16 * k + r < rows;
                 const int row = there ? row0 + 16 * k + r : row0 + rows - 1, tok = token_of(a, row);
                 const int pos = s.len - s.n + tok;
-                sees_hi[k] = min(a.causal ? pos + 1 : s.len, hi);
-                sees_lo[k] = a.window ? pos + 1 - (int)a.window : 0;
+                if constexpr (TREE) {
+                    sees_hi[k] = min(first_row, hi);
+                    sees_lo[k] = a.window ? max(a.pos[s.row0 + tok], s.len - s.n) + 1 - (int)a.window : 0;
+                    masks[k] = a.mask + (uint64_t)(uint32_t)(s.row0 + tok) * a.words;
+                } else {
+                    sees_hi[k] = min(a.causal ? pos + 1 : s.len, hi);
+                    sees_lo[k] = a.window ? pos + 1 - (int)a.window : 0;
+                }
                 q_exp[k] = load_q<D>(Q, there, s.row0 + tok, h * a.group + (uint32_t)(row - tok * (int)a.group),
                                                              g, bf, a.scale_log2, q[k]);
                 m[k] = kLowest;
@@ -483,9 +511,16 @@ __global__ __launch_bounds__(256, few_waves(D)) void kv_few_k(Cache c, Batch b, 
                         // only the few tiles that need it: nothing of this is computed ahead of the branch
                         int first = from;
                         asm volatile("" : "+v"(first));
+                        if constexpr (TREE) {
+                            const uint32_t sees = pv < 0 ? 0u : tree_bits(masks[k], (int)a.words, tv, s.len - s.n, first + tv, hi);
 #pragma unroll
-                        for (int i = 0; i < 16; ++i)
-                            st[k][i / 4][i % 4] = i < first || i >= to ? -__builtin_inff() : __builtin_fmaf(st[k][i / 4][i % 4], f, e);
+                            for (int i = 0; i < 16; ++i)
+                                st[k][i / 4][i % 4] = sees >> i & 1 ? __builtin_fmaf(st[k][i / 4][i % 4], f, e) : -__builtin_inff();
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 16; ++i)
+                                st[k][i / 4][i % 4] = i < first || i >= to ? -__builtin_inff() : __builtin_fmaf(st[k][i / 4][i % 4], f, e);
+                        }
                         f = 1.0f;
                         e = 0.0f;
                     }
@@ -719,12 +754,12 @@ __global__ __launch_bounds__(256) void kv_join_k(Cache c, Batch b, Attn a, FewPl
                    (uint32_t)cut.head * a.group + (uint32_t)(row % (int)a.group), c.heads * a.group);
 }
 
-template <int D, int TYPE, int R>
+template <int D, int TYPE, int R, bool TREE>
 hipError_t few_r(const Cache& c, const Batch& b, const Attn& a, const FewPlan& p, const Rows& Q, const Rows& O, bool bf,
                  float* ws, hipStream_t s) {
     const uint32_t wgs = (p.groups + 7) / 8 * 8 * p.tiles;
-    if (p.tiles == 1) kv_few_k<D, TYPE, R, true><<<wgs, 256, 0, s>>>(c, b, a, p, Q, O, bf, ws);
-    else if constexpr (R == few_sixteens(D)) kv_few_k<D, TYPE, R, false><<<wgs, 256, 0, s>>>(c, b, a, p, Q, O, bf, ws);
+    if (p.tiles == 1) kv_few_k<D, TYPE, R, true, TREE><<<wgs, 256, 0, s>>>(c, b, a, p, Q, O, bf, ws);
+    else if constexpr (R == few_sixteens(D)) kv_few_k<D, TYPE, R, false, TREE><<<wgs, 256, 0, s>>>(c, b, a, p, Q, O, bf, ws);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.mode == FewPlan::kRows) return e;
     const uint32_t rows = b.max_q * a.group;
@@ -734,12 +769,12 @@ hipError_t few_r(const Cache& c, const Batch& b, const Attn& a, const FewPlan& p
     return hipGetLastError();
 }
 
-template <int D, int TYPE>
+template <int D, int TYPE, bool TREE>
 hipError_t few_d(const Cache& c, const Batch& b, const Attn& a, const FewPlan& p, const Rows& Q, const Rows& O, bool bf,
                  float* ws, hipStream_t s) {
     if constexpr (few_sixteens(D) > 1)
-        if (p.sixteens == 2) return few_r<D, TYPE, 2>(c, b, a, p, Q, O, bf, ws, s);
-    return few_r<D, TYPE, 1>(c, b, a, p, Q, O, bf, ws, s);
+        if (p.sixteens == 2) return few_r<D, TYPE, 2, TREE>(c, b, a, p, Q, O, bf, ws, s);
+    return few_r<D, TYPE, 1, TREE>(c, b, a, p, Q, O, bf, ws, s);
 }
 
 }  // namespace kv

@@ -32,7 +32,8 @@ EXPORTS = ("kq_status_str", "kq_last_hip_error", "kq_version", "kq_int4_gemv",
            "kq_moe_unfused_workspace_size",
            "kq_moe_block_unfused", "kq_vq_quantize_workspace_size", "kq_vq_quantize",
            "kq_kv_write", "kq_kv_read", "kq_kv_attn_workspace_size", "kq_kv_attn",
-           "kq_rope_freqs", "kq_rope", "kq_kv_write_rope")
+           "kq_rope_freqs", "kq_rope", "kq_kv_write_rope",
+           "kq_kv_tree", "kq_kv_attn_tree_workspace_size", "kq_kv_attn_tree")
 
 
 class KQError(RuntimeError):
@@ -78,6 +79,11 @@ class _KVAttnC(C.Structure):
     """kq_kv_attn_desc."""
     _fields_ = [("q_heads", C.c_uint32), ("scale", C.c_float), ("causal", C.c_uint32),
                 ("window", C.c_uint32), ("sinks", C.c_void_p)]
+
+
+class _KVNodesC(C.Structure):
+    """kq_kv_nodes."""
+    _fields_ = [("mask", C.c_void_p), ("pos", C.c_void_p), ("words", C.c_uint32)]
 
 
 class _RopeC(C.Structure):
@@ -151,11 +157,15 @@ def lib():
         L.kq_rope_freqs.argtypes = [C.POINTER(_RopeScalingC), vp, C.POINTER(C.c_float)]
         L.kq_rope.argtypes = [vp, vp, vp, vp, u32, u32, u32, i32, vp]
         L.kq_kv_write_rope.argtypes = [vp, vp, vp, vp, vp, vp, u32, vp, vp, i32, vp]
+        L.kq_kv_tree.argtypes = [vp, vp, vp, u32, vp, u32, vp]
+        L.kq_kv_attn_tree_workspace_size.argtypes = [vp, vp, u32]
+        L.kq_kv_attn_tree_workspace_size.restype = sz
+        L.kq_kv_attn_tree.argtypes = [vp, vp, vp, vp, vp, vp, i32, vp, vp, sz, vp]
         for name in EXPORTS:
             if name not in ("kq_status_str", "kq_last_hip_error", "kq_version",
                             "kq_moe_default_desc", "kq_moe_workspace_size",
                             "kq_moe_unfused_workspace_size", "kq_vq_quantize_workspace_size",
-                            "kq_kv_attn_workspace_size"):
+                            "kq_kv_attn_workspace_size", "kq_kv_attn_tree_workspace_size"):
                 getattr(L, name).restype = i32
         _lib = L
     return _lib
@@ -543,20 +553,19 @@ def kv_read(cache, batch, k, v, stream=None):
     _kv_move(lib().kq_kv_read, "kq_kv_read", cache, batch, k, v, stream)
 
 
-def kv_attn_workspace_size(cache, batch, q_heads):
+def _kv_attn_size(f, where, cache, batch, q_heads):
     rows = 0 if batch.q_start is not None else min(batch.n_seq * batch.max_q, 2**32 - 1)  # with q_start any number
-    n = lib().kq_kv_attn_workspace_size(cache._ref, batch._packed(rows), q_heads)
+    n = f(cache._ref, batch._packed(rows), q_heads)
     if n == 0:
-        raise KQError(KQ_EINVAL, "kq_kv_attn_workspace_size")
+        raise KQError(KQ_EINVAL, where)
     return n
 
 
-def kv_attn(cache, batch, q, out, ws, ws_bytes, scale=None, causal=True, window=0, sinks=None, lse=None,
-            stream=None):
-    """Attention of the rows q [n_rows][q_heads][head_dim] over their sequences in
-    the cache, into out (float16 or bfloat16 both). scale: None is
-    1 / sqrt(head_dim). window > 0: a row sees its own and the window - 1 tokens
-    before. sinks: float32 [q_heads]. lse: float32 [n_rows][q_heads], written."""
+def kv_attn_workspace_size(cache, batch, q_heads):
+    return _kv_attn_size(lib().kq_kv_attn_workspace_size, "kq_kv_attn_workspace_size", cache, batch, q_heads)
+
+
+def _kv_attn(f, where, cache, batch, nodes, q, out, ws, ws_bytes, scale, causal, window, sinks, lse, stream):
     s = _kv_call(cache, batch, stream, q, out, sinks, lse, None if isinstance(ws, int) else ws)
     shape, dtype = q.shape, q.dtype
     if len(shape) != 3 or shape[2] != cache.head_dim:
@@ -570,8 +579,62 @@ def kv_attn(cache, batch, q, out, ws, ws_bytes, scale=None, causal=True, window=
     if not 0 <= window < 2**32:
         raise ValueError("window: 32-bit")
     d = _pack_attn(q_heads, cache.scale if scale is None else scale, bool(causal), window, _ptr(sinks) or 0)
-    _check(lib().kq_kv_attn(cache._ref, batch._packed(rows), d, a, b, _dt(q),
-                            _ptr(lse), _ptr(ws), ws_bytes, s), "kq_kv_attn")
+    _check(f(cache._ref, batch._packed(rows), d, *nodes, a, b, _dt(q), _ptr(lse), _ptr(ws), ws_bytes, s), where)
+
+
+def kv_attn(cache, batch, q, out, ws, ws_bytes, scale=None, causal=True, window=0, sinks=None, lse=None,
+            stream=None):
+    """Attention of the rows q [n_rows][q_heads][head_dim] over their sequences in
+    the cache, into out (float16 or bfloat16 both). scale: None is
+    1 / sqrt(head_dim). window > 0: a row sees its own and the window - 1 tokens
+    before. sinks: float32 [q_heads]. lse: float32 [n_rows][q_heads], written."""
+    _kv_attn(lib().kq_kv_attn, "kq_kv_attn", cache, batch, (), q, out, ws, ws_bytes, scale, causal, window, sinks, lse, stream)
+
+
+# ---------------------------------------------------------------------------
+# Trees of drafted tokens
+# ---------------------------------------------------------------------------
+class KVTree:
+    """kq_kv_nodes over contiguous tensors, kept alive with it: mask int32 [n_rows][words], bit t of a row: it sees
+    its sequence's row t; pos int32 [n_rows], which attention with a window reads, or None."""
+
+    def __init__(self, mask, pos=None):
+        import torch
+        _need(mask.dim() == 2, "mask: [n_rows][words]")
+        _here(mask, torch.int32, mask.shape, "mask")
+        if pos is not None:
+            _here(pos, torch.int32, (mask.shape[0],), "pos")
+            _need(pos.device == mask.device, "mask and pos are on one device")
+        self.mask, self.pos, self.device = mask, pos, mask.get_device()
+        self._c = _KVNodesC(mask.data_ptr(), _ptr(pos) or 0, mask.shape[1])
+        self._ref = C.byref(self._c)
+
+
+def kv_tree(batch, parent, mask, pos=None, window=0, stream=None):
+    """Masks int32 [n_rows][words], words * 32 >= max_q, and positions int32 [n_rows] of the trees that parent int32
+    [n_rows] describes (a row's parent among its sequence's rows), for all the layers' calls of a step. Returns their
+    KVTree. window > 0: a row sees the nearest `window` of the rows it continues, itself among them."""
+    import torch
+    s = _on_current(stream, batch.kv_len, parent, mask, pos)
+    tree = KVTree(mask, pos)
+    rows = mask.shape[0]
+    _here(parent, torch.int32, (rows,), "parent")
+    _need(0 <= window < 2**32, "window: 32-bit")
+    _check(lib().kq_kv_tree(batch._packed(rows), _ptr(parent), _ptr(mask), mask.shape[1], _ptr(pos), window, s), "kq_kv_tree")
+    return tree
+
+
+def kv_attn_tree_workspace_size(cache, batch, q_heads):
+    return _kv_attn_size(lib().kq_kv_attn_tree_workspace_size, "kq_kv_attn_tree_workspace_size", cache, batch, q_heads)
+
+
+def kv_attn_tree(cache, batch, tree, q, out, ws, ws_bytes, scale=None, window=0, sinks=None, lse=None, stream=None):
+    """kv_attn of a tree's rows: each over the tokens before the batch's rows of its sequence (window > 0: behind its
+    position less the window) and the rows that its mask names."""
+    if tree.device != cache.device or tree.mask.shape[0] != q.shape[0]:
+        raise ValueError(f"tree: of {q.shape[0]} rows, on the cache's device")
+    _kv_attn(lib().kq_kv_attn_tree, "kq_kv_attn_tree", cache, batch, (tree._ref,), q, out, ws, ws_bytes, scale, True, window, sinks,
+             lse, stream)
 
 
 # ---------------------------------------------------------------------------

@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 
 from kernels_amd import kq
-from tests.test_kv_abi import BAD_BATCH, BAD_BATCH_P, BAD_CACHE, BAD_CACHE_P, FAKE, batch_c, cache_c, rows_c
+from tests.test_kv_abi import _Cache, BAD_BATCH, BAD_BATCH_P, BAD_CACHE, BAD_CACHE_P, FAKE, attn_c, batch_c, cache_c, rows_c
 
 
 def rope_c(**kw):
@@ -147,3 +147,103 @@ def test_freqs_nulls_and_kinds():
     assert L.kq_rope_freqs(C.byref(d), out, C.byref(a)) == kq.KQ_EINVAL
     with pytest.raises(ValueError):
         kq.rope_freqs(64, kind="other", device="cpu")
+
+
+# ---- trees
+
+def nodes_c(**kw):
+    a = dict(mask=FAKE, pos=FAKE, words=1)
+    a.update(kw)
+    return kq._KVNodesC(**a)
+
+
+def tree(b=None, parent=FAKE, mask=FAKE, words=1, pos=None, window=0):
+    return kq.lib().kq_kv_tree(C.byref(b or batch_c()), parent, mask, words, pos, window, None)
+
+
+def attn(c=None, b=None, d=None, t=None, Q=None, O=None, dt=kq.F16, lse=None, ws=FAKE, n=1 << 30):
+    return kq.lib().kq_kv_attn_tree(C.byref(c or cache_c()), C.byref(b or batch_c()), C.byref(d or attn_c()), C.byref(t or nodes_c()),
+                                    C.byref(Q or rows_c(row=4096)), C.byref(O or rows_c(row=4096)), dt, lse, ws, n, None)
+
+
+@pytest.mark.parametrize("kw,status", BAD_BATCH + [(dict(kv_len=None), kq.KQ_ENULL), (dict(kv_len=FAKE + 1), kq.KQ_EALIGN), (dict(q_start=FAKE + 2), kq.KQ_EALIGN),
+                                                   (dict(max_q=1025), kq.KQ_EUNSUPPORTED)])
+def test_tree_bad_batch(kw, status):
+    assert tree(batch_c(**kw), words=64) == status
+
+
+@pytest.mark.parametrize("kw,status", [
+    (dict(parent=None), kq.KQ_ENULL), (dict(mask=None), kq.KQ_ENULL), (dict(parent=FAKE + 2), kq.KQ_EALIGN), (dict(mask=FAKE + 1), kq.KQ_EALIGN),
+    (dict(pos=FAKE + 2), kq.KQ_EALIGN), (dict(words=0), kq.KQ_EINVAL), (dict(words=2**31), kq.KQ_EINVAL), (dict(b=batch_c(max_q=33)), kq.KQ_EINVAL)])
+def test_bad_tree(kw, status):
+    assert tree(**kw) == status
+
+
+@pytest.mark.parametrize("kw,status", BAD_CACHE + BAD_CACHE_P)
+def test_attention_bad_cache(kw, status):
+    assert attn(cache_c(**kw)) == status
+
+
+@pytest.mark.parametrize("kw,status", BAD_BATCH + BAD_BATCH_P)
+def test_attention_bad_batch(kw, status):
+    assert attn(b=batch_c(**kw), t=nodes_c(words=1 << 20)) in (status, kq.KQ_EUNSUPPORTED if kw.get("max_q", 0) > 1024 else status)
+
+
+@pytest.mark.parametrize("kw,status", [
+    (dict(t=nodes_c(mask=None)), kq.KQ_ENULL), (dict(t=nodes_c(pos=None), d=attn_c(window=5)), kq.KQ_ENULL), (dict(t=nodes_c(mask=FAKE + 2)), kq.KQ_EALIGN),
+    (dict(t=nodes_c(pos=FAKE + 2)), kq.KQ_EALIGN), (dict(t=nodes_c(words=0)), kq.KQ_EINVAL), (dict(b=batch_c(max_q=1025), t=nodes_c(words=64)), kq.KQ_EUNSUPPORTED),
+    (dict(dt=kq.F32), kq.KQ_EUNSUPPORTED), (dict(d=attn_c(q_heads=12)), kq.KQ_EINVAL), (dict(d=attn_c(scale=float("nan"))), kq.KQ_EINVAL),
+    (dict(ws=None), kq.KQ_EWORKSPACE), (dict(n=0), kq.KQ_EWORKSPACE), (dict(ws=FAKE + 16), kq.KQ_EALIGN), (dict(lse=FAKE + 2), kq.KQ_EALIGN),
+    (dict(O=rows_c(row=0)), kq.KQ_EINVAL)])
+def test_bad_attention(kw, status):
+    assert attn(**kw) == status
+
+
+def test_tree_of_no_rows():
+    none = rows_c(p=None)
+    assert tree(batch_c(n_rows=0), parent=None, mask=None) == kq.KQ_OK
+    assert attn(b=batch_c(n_rows=0), t=nodes_c(mask=None, pos=None), Q=none, O=none, d=attn_c(causal=0, window=3)) == kq.KQ_OK
+    L = kq.lib()
+    assert L.kq_kv_tree(None, FAKE, FAKE, 1, None, 0, None) == kq.KQ_ENULL
+    r = rows_c(row=4096)
+    assert L.kq_kv_attn_tree(C.byref(cache_c()), C.byref(batch_c()), C.byref(attn_c()), None, C.byref(r), C.byref(r), 0, None, FAKE, 1 << 30, None) == kq.KQ_ENULL
+
+
+def size(c=None, b=None, q_heads=32):
+    return kq.lib().kq_kv_attn_tree_workspace_size(C.byref(c or cache_c()), C.byref(b or batch_c()), q_heads)
+
+
+def test_tree_workspace():
+    for kw, _ in BAD_CACHE:
+        assert size(cache_c(**kw)) == 0
+    for kw, _ in BAD_BATCH + [(dict(max_q=1025), 0)]:
+        assert size(b=batch_c(**kw)) == 0
+    assert size(q_heads=0) == size(q_heads=12) == size(q_heads=8 * 65) == 0
+    b = batch_c(n_seq=1, max_q=64, max_len=9000, n_rows=64)
+    n = size(b=b)
+    assert n > 256 and n % 256 == 0
+    assert attn(b=b, t=nodes_c(words=2), n=n - 1) == kq.KQ_EWORKSPACE
+
+
+def test_tree_workspace_covers_every_window():
+    """What a call writes is within what kq_kv_attn_tree_workspace_size said, over the launch's forms."""
+    need = kq.lib()["_ZN2kq15kv_tree_ws_needERKNS_2kv5CacheERKNS0_5BatchEjjj"]
+    need.restype = C.c_size_t
+    rng = np.random.default_rng(0)
+    some = 0
+    for _ in range(3000):
+        heads, group = int(rng.choice([1, 2, 3, 8, 16, 64])), int(rng.choice([1, 2, 5, 8, 16, 64]))
+        dim, page = int(rng.choice([64, 96, 128, 192, 256])), int(rng.choice([16, 64, 1024]))
+        max_len, n_seq = int(2 ** rng.uniform(0, 31) * 0.99), int(2 ** rng.uniform(0, 14))
+        max_q = int(2 ** rng.uniform(0, rng.choice([3, 10])))
+        if n_seq * max_q * heads * group >= 2**31 - 2**16:
+            continue
+        b = batch_c(n_seq=n_seq, max_q=max_q, n_rows=n_seq * max_q, max_len=max(max_len, 1), max_pages=1 << 20)
+        said = size(cache_c(heads=heads, head_dim=dim, page=page), b, heads * group)
+        assert said > 0
+        c = _Cache(FAKE, FAKE, FAKE, FAKE, 64, heads, page.bit_length() - 1, 4)
+        for window in [0] + [int(2 ** rng.uniform(0, 31)) for _ in range(6)]:
+            n = need(C.byref(c), C.byref(b), C.c_uint32(dim), C.c_uint32(group), C.c_uint32(window))
+            assert n <= said, (heads, group, dim, max_len, n_seq, max_q, window)
+            some += window > 0 and n > 0
+    assert some > 1000
