@@ -547,7 +547,7 @@ typedef struct kq_rope_desc {
     const float* inv_freq;
     uint32_t rot;
     uint32_t layout; /* kq_rope_layout */
-    float amplitude;
+    double amplitude;
     uint32_t inverse;
 } kq_rope_desc;
 
@@ -578,7 +578,7 @@ typedef struct kq_rope_scaling {
     uint32_t rot;
     double base, factor, low, high, original;
 } kq_rope_scaling;
-kq_status kq_rope_freqs(const kq_rope_scaling* s, float* inv_freq, float* amplitude);
+kq_status kq_rope_freqs(const kq_rope_scaling* s, float* inv_freq, double* amplitude);
 
 /* Y = X turned, rows x heads x head_dim of dtype KQ_F16, KQ_BF16 or KQ_F32, row i at
  * position pos[i] (int32 [n_rows], device memory; any values). Y may be X (the same
@@ -645,6 +645,61 @@ kq_status kq_kv_attn_tree(const kq_kv_cache* cache, const kq_kv_batch* batch,
                           const kq_kv_attn_desc* d, const kq_kv_nodes* nodes, const kq_kv_rows* Q,
                           const kq_kv_rows* O, kq_dtype dtype, float* lse, void* ws,
                           size_t ws_bytes, kq_stream_t stream);
+
+/* Which drafted tokens are kept, and the token behind them, so that what comes out
+ * is distributed as the target's own draws are. From row 0 on: with P the target's
+ * probabilities after the row, S = 1, the rows that continue it are tried in order,
+ *   row c of token x, drawn from Q: kept if u[c] S Q(x) < P(x); if not,
+ *   P becomes max(P - S Q, 0) and S its sum
+ *   (a token picked outright: Q(x) = 1, and P(x) becomes 0, S less by what it was)
+ * and the way goes on from the one that is kept. Where none is, the last token is
+ * the first whose sum of P up to it is over u[row 0] times P's whole sum (if that is
+ * 0: the first of the largest probability of the row). All of it is 64-bit.
+ *
+ * p      : float [n_rows][vocab], row stride p_row: after each row, adding up to 1
+ * q      : float [n_q][vocab], row stride q_row, or NULL: every token is picked outright
+ * q_index: int32 [n_rows] or NULL: the row of q that a row's token was drawn from; outside
+ *          [0, n_q): picked outright. NULL: the row's own (n_q >= n_rows)
+ * token  : int32 [n_rows] (a row 0's is not looked at); outside [0, vocab): never kept
+ * parent : int32 [n_rows] or NULL: each row continues the one before. Rows whose
+ *          parent is not in 0 .. j - 1 are never reached
+ * u      : float [n_rows], in [0, 1)
+ * start  : int32 [n_seq + 1], ascending, or NULL: max_q rows each
+ * Probabilities that are negative or not finite count as 0. 64-bit sums of many are taken
+ * in one order, whatever the run.
+ * Written: keep int32 [n_seq][max_q], the kept rows' numbers (row 0 first), n_keep int32
+ * [n_seq], how many (0: the sequence has no rows), out int32 [n_seq][max_q], n_keep
+ * tokens: those of the kept rows but row 0, then the last one. Behind them keep
+ * and out are -1. No two written arrays, and none that is read, overlap.
+ * max_q <= 1024, vocab < 2^31 - 2^16 (else KQ_EUNSUPPORTED); 1 <= n_seq <= 65535.
+ * ws: kq_draft_verify_workspace_size bytes, 256-byte aligned, no initialisation and nothing
+ * kept in it; calls that share one must be stream-ordered. */
+typedef struct kq_draft {
+    const float* p;
+    const float* q;
+    int64_t p_row, q_row;
+    const int32_t *q_index, *token, *parent, *start;
+    const float* u;
+    uint32_t n_seq, max_q, n_rows, n_q, vocab;
+} kq_draft;
+size_t kq_draft_verify_workspace_size(uint32_t n_seq, uint32_t max_q, uint32_t vocab);
+kq_status kq_draft_verify(const kq_draft* d, int32_t* keep, int32_t* n_keep, int32_t* out, void* ws,
+                          size_t ws_bytes, kq_stream_t stream);
+
+/* Moves the kept rows of each sequence together: row keep[i][j] of sequence i's newest
+ * tokens goes to the place of its row j, j < n_keep[i]. keep: int32 [n_seq][max_q],
+ * ascending (so that keep[i][j] >= j); n_keep: int32 [n_seq], cut to max_q and the
+ * sequence's rows. An entry that is less than its j or that of the row before, or no row, ends
+ * the list there. The sequence then holds kv_len - n + n_keep tokens, which
+ * is the caller's to set; what is behind them may be overwritten by the next step.
+ * Codes are moved as they are where the two blocks' exponents are the same. A
+ * block that rows are moved into takes the largest exponent of its own and of those
+ * they come from; all its tokens below kv_len go by it, rounded to nearest even
+ * where it grows. Tokens of a page id outside [0, n_pages) are read as zeros, of the
+ * smallest exponent, and not written. A page that the call writes must belong to one sequence of it.
+ * max_q <= 1024 (else KQ_EUNSUPPORTED). One launch. */
+kq_status kq_kv_keep(const kq_kv_cache* cache, const kq_kv_batch* batch, const int32_t* keep,
+                     const int32_t* n_keep, kq_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -255,7 +255,7 @@ kq_status check_rope(const kq_rope_desc* d, uint32_t head_dim) {
     return aligned(d->inv_freq, 4) ? KQ_OK : KQ_EALIGN;
 }
 kq::rope::Rope rope_of(const kq_rope_desc& d) {
-    return {d.inv_freq, d.rot, d.layout == KQ_ROPE_PAIRS, d.amplitude, d.inverse ? -(double)d.amplitude : d.amplitude};
+    return {d.inv_freq, d.rot, d.layout == KQ_ROPE_PAIRS, d.amplitude, d.inverse ? -d.amplitude : d.amplitude};
 }
 
 }  // namespace
@@ -743,8 +743,44 @@ kq_status kq_kv_attn_tree(const kq_kv_cache* cache, const kq_kv_batch* batch, co
     return kv_attn(cache, batch, d, nodes, Q, O, dtype, lse, ws, ws_bytes, stream);
 }
 
+size_t kq_draft_verify_workspace_size(uint32_t n_seq, uint32_t max_q, uint32_t vocab) {
+    if (n_seq == 0 || n_seq > 65535 || max_q == 0 || max_q > kq::kMostNodes || vocab == 0 || vocab >= 0x7FFF0000u) return 0;
+    return kq::draft_verify_ws_bytes(n_seq, max_q, vocab);
+}
+
+kq_status kq_draft_verify(const kq_draft* d, int32_t* keep, int32_t* n_keep, int32_t* out, void* ws, size_t ws_bytes,
+                          kq_stream_t stream) {
+    if (!d) return KQ_ENULL;
+    if (d->n_seq == 0 || d->n_seq > 65535 || d->max_q == 0 || d->vocab == 0 || d->n_rows >= 0x7FFF0000u) return KQ_EINVAL;
+    if (d->max_q > kq::kMostNodes || d->vocab >= 0x7FFF0000u) return KQ_EUNSUPPORTED;
+    if (!d->start && (uint64_t)d->n_seq * d->max_q > d->n_rows) return KQ_EINVAL;
+    if (d->n_rows && (!d->p || !d->token || !d->u)) return KQ_ENULL;
+    if (!keep || !n_keep || !out) return KQ_ENULL;
+    if ((d->n_rows > 1 && d->p_row < 0) || (d->q && d->n_q > 1 && d->q_row < 0)) return KQ_EINVAL;
+    if (d->q && (d->n_q >= 0x7FFF0000u || (!d->q_index && d->n_q < d->n_rows))) return KQ_EINVAL;
+    for (const void* p : {(const void*)d->p, (const void*)d->q, (const void*)d->q_index, (const void*)d->token, (const void*)d->parent,
+                          (const void*)d->start, (const void*)d->u, (const void*)keep, (const void*)n_keep, (const void*)out})
+        if (!aligned(p, 4)) return KQ_EALIGN;
+    if (!ws || ws_bytes < kq::draft_verify_ws_bytes(d->n_seq, d->max_q, d->vocab)) return KQ_EWORKSPACE;
+    if (!aligned(ws, 256)) return KQ_EALIGN;
+    return hip_status(kq::launch_draft_verify(*d, keep, n_keep, out, ws, reinterpret_cast<hipStream_t>(stream)));
+}
+
+kq_status kq_kv_keep(const kq_kv_cache* cache, const kq_kv_batch* batch, const int32_t* keep, const int32_t* n_keep,
+                     kq_stream_t stream) {
+    kq_status st = check_kv(cache, batch);
+    if (st == KQ_OK) st = check_kv_pointers(cache, batch);
+    if (st != KQ_OK) return st;
+    if (!keep || !n_keep) return KQ_ENULL;
+    if (!aligned(keep, 4) || !aligned(n_keep, 4)) return KQ_EALIGN;
+    if (batch->max_q > kq::kMostNodes) return KQ_EUNSUPPORTED;
+    if (batch->n_rows == 0) return KQ_OK;
+    return hip_status(kq::launch_kv_keep(kv_cache(*cache), kv_batch(*batch), cache->head_dim, (int)cache->type, keep, n_keep,
+                                         reinterpret_cast<hipStream_t>(stream)));
+}
+
 // ------------------------------------------------------------ rotary positions
-kq_status kq_rope_freqs(const kq_rope_scaling* s, float* inv_freq, float* amplitude) {
+kq_status kq_rope_freqs(const kq_rope_scaling* s, float* inv_freq, double* amplitude) {
     if (!s || !inv_freq || !amplitude) return KQ_ENULL;
     if (s->kind > KQ_ROPE_YARN || s->rot < 2 || s->rot % 2 || s->rot > kq::rope::kMostHead) return KQ_EINVAL;
     if (!std::isfinite(s->base) || !(s->base > 1.0)) return KQ_EINVAL;
@@ -772,7 +808,7 @@ kq_status kq_rope_freqs(const kq_rope_scaling* s, float* inv_freq, float* amplit
         share = share < 0.0 ? 0.0 : share > 1.0 ? 1.0 : share;
         inv_freq[i] = (float)(share == 1.0 ? f : f * share + f / s->factor * (1.0 - share));
     }
-    *amplitude = s->kind == KQ_ROPE_YARN ? (float)(0.1 * std::log(s->factor) + 1.0) : 1.0f;
+    *amplitude = s->kind == KQ_ROPE_YARN ? 0.1 * std::log(s->factor) + 1.0 : 1.0;
     return KQ_OK;
 }
 

@@ -293,5 +293,9 @@ hipError_t launch_kv_attn(const kv::Cache& c, const kv::Batch& b, uint32_t D, in
 constexpr uint32_t kMostNodes = 1024;  // rows of a sequence's tree
 hipError_t launch_kv_tree(const kv::Batch& b, const int32_t* parent, uint32_t* mask, uint32_t words, int32_t* pos,
                           uint32_t window, hipStream_t s);
+size_t draft_verify_ws_bytes(uint32_t n_seq, uint32_t max_q, uint32_t vocab);
+hipError_t launch_draft_verify(const kq_draft& d, int32_t* keep, int32_t* n_keep, int32_t* out, void* ws, hipStream_t s);
+hipError_t launch_kv_keep(const kv::Cache& c, const kv::Batch& b, uint32_t D, int type, const int32_t* keep, const int32_t* n_keep,
+                          hipStream_t s);
 
 }  // namespace kq

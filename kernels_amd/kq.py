@@ -33,7 +33,8 @@ EXPORTS = ("kq_status_str", "kq_last_hip_error", "kq_version", "kq_int4_gemv",
            "kq_moe_block_unfused", "kq_vq_quantize_workspace_size", "kq_vq_quantize",
            "kq_kv_write", "kq_kv_read", "kq_kv_attn_workspace_size", "kq_kv_attn",
            "kq_rope_freqs", "kq_rope", "kq_kv_write_rope",
-           "kq_kv_tree", "kq_kv_attn_tree_workspace_size", "kq_kv_attn_tree")
+           "kq_kv_tree", "kq_kv_attn_tree_workspace_size", "kq_kv_attn_tree",
+           "kq_draft_verify_workspace_size", "kq_draft_verify", "kq_kv_keep")
 
 
 class KQError(RuntimeError):
@@ -89,7 +90,7 @@ class _KVNodesC(C.Structure):
 class _RopeC(C.Structure):
     """kq_rope_desc."""
     _fields_ = [("inv_freq", C.c_void_p), ("rot", C.c_uint32), ("layout", C.c_uint32),
-                ("amplitude", C.c_float), ("inverse", C.c_uint32)]
+                ("amplitude", C.c_double), ("inverse", C.c_uint32)]
 
 
 class _RopeScalingC(C.Structure):
@@ -154,18 +155,23 @@ def lib():
         L.kq_kv_attn_workspace_size.argtypes = [vp, vp, u32]
         L.kq_kv_attn_workspace_size.restype = sz
         L.kq_kv_attn.argtypes = [vp, vp, vp, vp, vp, i32, vp, vp, sz, vp]
-        L.kq_rope_freqs.argtypes = [C.POINTER(_RopeScalingC), vp, C.POINTER(C.c_float)]
+        L.kq_rope_freqs.argtypes = [C.POINTER(_RopeScalingC), vp, C.POINTER(C.c_double)]
         L.kq_rope.argtypes = [vp, vp, vp, vp, u32, u32, u32, i32, vp]
         L.kq_kv_write_rope.argtypes = [vp, vp, vp, vp, vp, vp, u32, vp, vp, i32, vp]
         L.kq_kv_tree.argtypes = [vp, vp, vp, u32, vp, u32, vp]
         L.kq_kv_attn_tree_workspace_size.argtypes = [vp, vp, u32]
         L.kq_kv_attn_tree_workspace_size.restype = sz
         L.kq_kv_attn_tree.argtypes = [vp, vp, vp, vp, vp, vp, i32, vp, vp, sz, vp]
+        L.kq_draft_verify_workspace_size.argtypes = [u32, u32, u32]
+        L.kq_draft_verify_workspace_size.restype = sz
+        L.kq_draft_verify.argtypes = [vp, vp, vp, vp, vp, sz, vp]
+        L.kq_kv_keep.argtypes = [vp, vp, vp, vp, vp]
         for name in EXPORTS:
             if name not in ("kq_status_str", "kq_last_hip_error", "kq_version",
                             "kq_moe_default_desc", "kq_moe_workspace_size",
                             "kq_moe_unfused_workspace_size", "kq_vq_quantize_workspace_size",
-                            "kq_kv_attn_workspace_size", "kq_kv_attn_tree_workspace_size"):
+                            "kq_kv_attn_workspace_size", "kq_kv_attn_tree_workspace_size",
+                            "kq_draft_verify_workspace_size"):
                 getattr(L, name).restype = i32
         _lib = L
     return _lib
@@ -424,9 +430,9 @@ def moe_block_unfused(pool, desc, R, x, idx, wgt, H, y, ws, ws_bytes, batch=1, x
 # ---------------------------------------------------------------------------
 KV_I8, KV_E4M3 = 0, 1  # kq_kv_type
 
-# kq_kv_batch, kq_kv_rows and kq_kv_attn_desc as bytes: a call makes up to four of them, and a
+# kq_kv_batch, kq_kv_rows, kq_kv_attn_desc and kq_draft as bytes: a call makes up to four of them, and a
 # ctypes.Structure costs several times as much
-_pack_batch, _pack_rows, _pack_attn = (struct.Struct("@" + f).pack for f in ("3P5I4x", "Pqq", "If2IP"))
+_pack_batch, _pack_rows, _pack_attn, _pack_draft = (struct.Struct("@" + f).pack for f in ("3P5I4x", "Pqq", "If2IP", "2P2q5P5I4x"))
 
 
 def _need(ok, what):
@@ -637,6 +643,59 @@ def kv_attn_tree(cache, batch, tree, q, out, ws, ws_bytes, scale=None, window=0,
              lse, stream)
 
 
+def draft_verify_workspace_size(n_seq, max_q, vocab):
+    n = lib().kq_draft_verify_workspace_size(n_seq, max_q, vocab)
+    if n == 0:
+        raise KQError(KQ_EINVAL, "kq_draft_verify_workspace_size")
+    return n
+
+
+def _probabilities(t, dtype, rows, vocab, what):
+    if t.dtype != dtype or t.dim() != 2 or t.shape[1] != vocab or (rows is not None and t.shape[0] < rows):
+        raise ValueError(f"{what}: a {dtype} tensor [{'any' if rows is None else rows}][{vocab}], not {t.dtype} {tuple(t.shape)}")
+    if t.stride(1) != 1 and vocab > 1 and t.shape[0]:
+        raise ValueError(f"{what}: contiguous in its last dimension, not strides {t.stride()}")
+
+
+def draft_verify(p, token, u, keep, n_keep, out, ws, ws_bytes, q=None, q_index=None, parent=None, start=None, stream=None):
+    """Drafted tokens against the target's probabilities p float32 [n_rows][vocab] (any row stride), with given
+    random numbers u float32 [n_rows]: kept rows into keep int32 [n_seq][max_q], how many into n_keep int32 [n_seq], their
+    tokens and the one behind them into out int32 [n_seq][max_q].
+
+    token: int32 [n_rows]. parent: int32 [n_rows] (None: a chain). start: int32 [n_seq + 1] (None: max_q rows
+    each). q: float32 [n_q][vocab], the probabilities that the tokens were drawn from, row q_index[i] (int32 [n_rows],
+    -1: picked outright) or i for row i; None: all were picked outright."""
+    import torch
+    f32, i32 = torch.float32, torch.int32
+    s = _on_current(stream, p, token, u, keep, n_keep, out, q, q_index, parent, start, None if isinstance(ws, int) else ws)
+    _need(keep.dim() == 2 and p.dim() == 2, "keep: [n_seq][max_q], p: [n_rows][vocab]")
+    (n_seq, max_q), (rows, vocab) = keep.shape, p.shape
+    _probabilities(p, f32, rows, vocab, "p")
+    for t, dtype, shape, what in ((token, i32, (rows,), "token"), (u, f32, (rows,), "u"), (keep, i32, (n_seq, max_q), "keep"),
+                                  (n_keep, i32, (n_seq,), "n_keep"), (out, i32, (n_seq, max_q), "out"), (parent, i32, (rows,), "parent"),
+                                  (start, i32, (n_seq + 1,), "start"), (q_index, i32, (rows,), "q_index")):
+        if t is not None:
+            _here(t, dtype, shape, what)
+    n_q = q_row = 0
+    if q is not None:
+        _probabilities(q, f32, rows if q_index is None else None, vocab, "q")
+        n_q, q_row = q.shape[0], q.stride(0)
+    d = _pack_draft(p.data_ptr(), _ptr(q) or 0, p.stride(0), q_row, _ptr(q_index) or 0, token.data_ptr(), _ptr(parent) or 0,
+                    _ptr(start) or 0, u.data_ptr(), n_seq, max_q, rows, n_q, vocab)
+    _check(lib().kq_draft_verify(d, keep.data_ptr(), n_keep.data_ptr(), out.data_ptr(), _ptr(ws), ws_bytes, s), "kq_draft_verify")
+
+
+def kv_keep(cache, batch, keep, n_keep, stream=None):
+    """The rows keep[i][:n_keep[i]] (int32 [n_seq][max_q] and [n_seq], as draft_verify leaves them) of each sequence's
+    newest tokens moved together in the cache; the sequence then ends behind them, which is for kv_len to say."""
+    import torch
+    s = _kv_call(cache, batch, stream, keep, n_keep)
+    _here(keep, torch.int32, (batch.n_seq, batch.max_q), "keep")
+    _here(n_keep, torch.int32, (batch.n_seq,), "n_keep")
+    rows = batch.n_seq * batch.max_q if batch.q_start is None else 0x7FFF0000 - 1  # with q_start: no tensor has them
+    _check(lib().kq_kv_keep(cache._ref, batch._packed(rows), keep.data_ptr(), n_keep.data_ptr(), s), "kq_kv_keep")
+
+
 # ---------------------------------------------------------------------------
 # Rotary positions
 # ---------------------------------------------------------------------------
@@ -649,7 +708,7 @@ def rope_freqs(rot, base=10000.0, kind="plain", factor=1.0, low=1.0, high=None, 
     import torch
     _need(kind in ROPE_KINDS, f"kind: one of {', '.join(ROPE_KINDS)}")
     _need(0 <= rot < 2**32, "rot: 32-bit")
-    got, amplitude = (C.c_float * max(rot // 2, 1))(), C.c_float(0.0)
+    got, amplitude = (C.c_float * max(rot // 2, 1))(), C.c_double(0.0)
     d = _RopeScalingC(ROPE_KINDS.index(kind), rot, base, factor, low, (32.0 if kind == "yarn" else 4.0) if high is None else high,
                       original)
     _check(lib().kq_rope_freqs(C.byref(d), got, C.byref(amplitude)), "kq_rope_freqs")

@@ -7,7 +7,7 @@ def turned(x, pos, freqs, pairs=False, amplitude=1.0, inverse=False):
     """x float64 [rows][heads][dim] turned by pos [rows] times freqs float32 [rot / 2], by complex numbers."""
     rot = 2 * len(freqs)
     angle = np.asarray(pos, np.float64)[:, None, None] * np.asarray(freqs, np.float64)
-    by = float(np.float32(amplitude)) * np.exp((-1j if inverse else 1j) * angle)
+    by = amplitude * np.exp((-1j if inverse else 1j) * angle)
     y = np.array(x, np.float64)
     a, b = (slice(0, rot, 2), slice(1, rot, 2)) if pairs else (slice(0, rot // 2), slice(rot // 2, rot))
     z = (y[..., a] + 1j * y[..., b]) * by

@@ -83,3 +83,94 @@ def attend(cache, table, length, q, scale, sees, pos=None, window=0, sinks=None)
 def attend_tolerance(want, dim, eps, tiny):
     """The arithmetic is kq_kv_attn's, and so is the bound."""
     return _kv.attend_tolerance(*want, dim, eps, tiny)
+
+
+# ---- verification, and the kept rows
+
+def verify(p, tokens, u, parents, q=None, q_rows=None):
+    """A sequence: p [n][vocab], tokens, u and parents [n], q [n_q][vocab], q_rows [n] (below 0: picked outright), in
+    64 bits -> (kept rows, tokens, margin): margin is how far, relative to what is compared, the nearest decision
+    was from going the other way."""
+    clean = lambda a: np.where(np.isfinite(a) & (a > 0), a, 0.0).astype(np.float64)  # noqa: E731
+    n, vocab = p.shape
+    at, kept, out, margin = 0, [0], [], np.inf
+
+    def differs(a, b):
+        nonlocal margin
+        margin = min(margin, abs(a - b) / max(abs(a), abs(b), 1e-300))
+
+    while True:
+        left, mass, went = clean(p[at]), 1.0, None
+        for c in [c for c in range(1, n) if 0 <= parents[c] < c and parents[c] == at]:
+            x, outright = int(tokens[c]), q is None or q_rows[c] < 0
+            real = 0 <= x < vocab
+            prob = 1.0 if outright else float(clean(q[q_rows[c], x])) if real else 0.0
+            there = float(left[x]) if real else 0.0
+            if there or u[c] * mass * prob:
+                differs(u[c] * mass * prob, there)
+            if u[c] * mass * prob < there:
+                went = c
+                break
+            if outright:
+                mass -= there
+                if real:
+                    left[x] = 0.0
+            else:
+                left = np.maximum(left - mass * clean(q[q_rows[c]]), 0.0)
+                mass = float(left.sum())
+        if went is None:
+            break
+        at = went
+        kept.append(went)
+        out.append(int(tokens[went]))
+    up = np.cumsum(left)
+    if up[-1] > 0:
+        aim = u[0] * up[-1]
+        x = int(np.argmax(up > aim))
+        differs(aim, up[x])
+        if x and up[x - 1]:
+            differs(aim, up[x - 1])
+        out.append(x)
+    else:
+        out.append(int(np.argmax(clean(p[at]))))
+    return kept, out, margin
+
+
+def keep_rows(cache, which, table, length, n, kept):
+    """kq_kv_keep of one sequence: the rows `kept` of its last n tokens, into a _kv.Cache."""
+    first = length - n
+    rows = []
+    for j, k in enumerate(kept):
+        if not (j <= k < n and (not rows or k > rows[-1])):
+            break
+        rows.append(k)
+    block, page = cache.block, cache.page
+    src = {first + j: first + k for j, k in enumerate(rows) if k != j and first + j >= 0}
+    before = {w: x[which].copy() for w, x in (("codes", cache.codes), ("exps", cache.exps))}
+
+    def of(t):
+        """(codes [heads][dim], exponent bytes [heads]) of a token as it was, or None."""
+        p = table[t // page]
+        return (before["codes"][p, :, t % page], before["exps"][p, :, t % page // block].astype(int)) if 0 <= p < cache.n_pages else None
+
+    for b in sorted({t // block for t in src}):
+        t0 = b * block
+        p, s = table[t0 // page], t0 % page
+        if not 0 <= p < cache.n_pages:
+            continue
+        own = before["exps"][p, :, s // block].astype(int)
+        e = own.copy()
+        for t, a in src.items():
+            if t // block == b and of(a) is not None:
+                e = np.maximum(e, of(a)[1])
+        for t in range(t0, min(t0 + block, length)):
+            got = of(src.get(t, t))
+            for h in range(cache.heads):
+                if got is None:
+                    codes = np.zeros(cache.dim, np.uint8)
+                elif got[1][h] == e[h]:
+                    codes = got[0][h]
+                else:
+                    codes = _kv.encode(_kv.decode(got[0][h], cache.kind) * 2.0 ** float(got[1][h] - e[h]), cache.kind)
+                cache.codes[which][p, h, t % page] = codes
+        cache.exps[which][p, :, s // block] = e

@@ -118,7 +118,7 @@ def test_freqs_bands():
 
 def test_freqs_yarn():
     want, (got, a) = freqs()[0], freqs(kind="yarn", factor=16.0, original=4096.0)
-    assert abs(a - (0.1 * np.log(16.0) + 1)) < 2**-22
+    assert abs(a - (0.1 * np.log(16.0) + 1)) < 2**-50
     c = [64 * np.log(4096 / (n * 2 * np.pi)) / (2 * np.log(10000.0)) for n in (32.0, 1.0)]
     lo, hi = np.floor(c[0]), np.ceil(c[1])
     r = np.clip((np.arange(32) - lo) / (hi - lo), 0, 1)
@@ -140,7 +140,7 @@ def test_freqs_refused(kw):
 
 
 def test_freqs_nulls_and_kinds():
-    L, d, a = kq.lib(), kq._RopeScalingC(0, 64, 1e4, 1, 1, 4, 0), C.c_float()
+    L, d, a = kq.lib(), kq._RopeScalingC(0, 64, 1e4, 1, 1, 4, 0), C.c_double()
     out = (C.c_float * 32)()
     assert L.kq_rope_freqs(None, out, C.byref(a)) == L.kq_rope_freqs(C.byref(d), None, C.byref(a)) == L.kq_rope_freqs(C.byref(d), out, None) == kq.KQ_ENULL
     d.kind = 5
@@ -247,3 +247,66 @@ def test_tree_workspace_covers_every_window():
             assert n <= said, (heads, group, dim, max_len, n_seq, max_q, window)
             some += window > 0 and n > 0
     assert some > 1000
+
+
+# ---- verification, and the kept rows
+
+def draft(**kw):
+    a = dict(p=FAKE, q=FAKE, p_row=100, q_row=100, q_index=FAKE, token=FAKE, parent=FAKE, start=FAKE, u=FAKE, n_seq=2, max_q=3, n_rows=6,
+             n_q=6, vocab=100)
+    a.update(kw)
+    return kq._pack_draft(*((v or 0) for v in a.values()))
+
+
+def verify(d=None, keep=FAKE, n_keep=FAKE, out=FAKE, ws=FAKE, n=1 << 40):
+    return kq.lib().kq_draft_verify(d or draft(), keep, n_keep, out, ws, n, None)
+
+
+@pytest.mark.parametrize("kw,status", [
+    (dict(n_seq=0), kq.KQ_EINVAL), (dict(n_seq=65536), kq.KQ_EINVAL), (dict(max_q=0), kq.KQ_EINVAL), (dict(max_q=1025), kq.KQ_EUNSUPPORTED),
+    (dict(vocab=0), kq.KQ_EINVAL), (dict(vocab=0x7FFF0000), kq.KQ_EUNSUPPORTED), (dict(n_rows=0x7FFF0000), kq.KQ_EINVAL),
+    (dict(start=None, n_rows=5), kq.KQ_EINVAL), (dict(p=None), kq.KQ_ENULL), (dict(token=None), kq.KQ_ENULL), (dict(u=None), kq.KQ_ENULL),
+    (dict(p_row=-1), kq.KQ_EINVAL), (dict(q_row=-100), kq.KQ_EINVAL), (dict(q_index=None, n_q=5), kq.KQ_EINVAL), (dict(n_q=0x7FFF0000), kq.KQ_EINVAL),
+    (dict(p=FAKE + 2), kq.KQ_EALIGN), (dict(q=FAKE + 1), kq.KQ_EALIGN), (dict(q_index=FAKE + 2), kq.KQ_EALIGN), (dict(token=FAKE + 2), kq.KQ_EALIGN),
+    (dict(parent=FAKE + 2), kq.KQ_EALIGN), (dict(start=FAKE + 2), kq.KQ_EALIGN), (dict(u=FAKE + 2), kq.KQ_EALIGN)])
+def test_bad_draft(kw, status):
+    assert verify(draft(**kw)) == status
+
+
+@pytest.mark.parametrize("kw,status", [
+    (dict(keep=None), kq.KQ_ENULL), (dict(n_keep=None), kq.KQ_ENULL), (dict(out=None), kq.KQ_ENULL), (dict(keep=FAKE + 2), kq.KQ_EALIGN),
+    (dict(n_keep=FAKE + 2), kq.KQ_EALIGN), (dict(out=FAKE + 1), kq.KQ_EALIGN), (dict(ws=None), kq.KQ_EWORKSPACE), (dict(n=255), kq.KQ_EWORKSPACE),
+    (dict(ws=FAKE + 16), kq.KQ_EALIGN)])
+def test_bad_verify(kw, status):
+    assert verify(**kw) == status
+
+
+def test_verify_workspace():
+    size = kq.lib().kq_draft_verify_workspace_size
+    assert size(0, 3, 100) == size(65536, 3, 100) == size(2, 0, 100) == size(2, 1025, 100) == size(2, 3, 0) == size(2, 3, 0x7FFF0000) == 0
+    assert kq.lib().kq_draft_verify(None, FAKE, FAKE, FAKE, FAKE, 1 << 40, None) == kq.KQ_ENULL
+    for n_seq, max_q, vocab in ((1, 1, 1), (2, 3, 100), (65535, 1024, 300000), (1, 1024, 0x7FFEFFFF)):
+        n = size(n_seq, max_q, vocab)
+        assert n % 256 == 0 and n >= n_seq * (16 * max_q + 8 * -(-vocab // 4096) + 16)
+    d = draft(n_seq=64, max_q=5, n_rows=320, vocab=128256, n_q=320)
+    assert verify(d, n=size(64, 5, 128256) - 1) == kq.KQ_EWORKSPACE
+
+
+def keep(c=None, b=None, rows=FAKE, n=FAKE):
+    return kq.lib().kq_kv_keep(C.byref(c or cache_c()), C.byref(b or batch_c()), rows, n, None)
+
+
+@pytest.mark.parametrize("kw,status", BAD_CACHE + BAD_CACHE_P)
+def test_keep_bad_cache(kw, status):
+    assert keep(cache_c(**kw)) == status
+
+
+@pytest.mark.parametrize("kw,status", BAD_BATCH + BAD_BATCH_P + [(dict(max_q=1025), kq.KQ_EUNSUPPORTED)])
+def test_keep_bad_batch(kw, status):
+    assert keep(b=batch_c(**kw)) == status
+
+
+@pytest.mark.parametrize("kw,status", [(dict(rows=None), kq.KQ_ENULL), (dict(n=None), kq.KQ_ENULL), (dict(rows=FAKE + 2), kq.KQ_EALIGN),
+                                       (dict(n=FAKE + 2), kq.KQ_EALIGN), (dict(b=batch_c(n_rows=0)), kq.KQ_OK)])
+def test_bad_keep(kw, status):
+    assert keep(**kw) == status
