@@ -214,7 +214,7 @@ struct FewPlan {
         kParts,   // rows of work in equal parts, a group each
         kShares,  // all of it in equal shares, whatever rows they begin and end in
     };
-    uint32_t sixteens;  // rows of a workgroup, in sixteens: 1 or 2
+    uint32_t sixteens;  // rows of a workgroup, in sixteens: 1 or 2 (many rows of trees: 8 or 16)
     uint32_t tiles;     // workgroups that take the same tokens for other rows
     uint32_t groups;    // of such workgroups
     uint32_t mode;
@@ -268,12 +268,20 @@ bool rope_fits(uint32_t n_rows, uint32_t heads, uint32_t rot);
 hipError_t launch_kv_read(const kv::Cache& c, const kv::Batch& b, uint32_t D, int type, const kv::Rows& K,
                           const kv::Rows& V, kq_dtype f, hipStream_t s);
 namespace kv {
-// The kernels, heads D wide (kq_kv_attn_<D>.hip; of trees: kq_kv_tree_<D>.hip).
-template <int D, bool TREE>
+// The kernels, heads D wide (kq_kv_attn_<D>.hip).
+template <int D>
 struct AttnKernels {
     static hipError_t few(int type, const Cache& c, const Batch& b, const Attn& a, const FewPlan& p, const Rows& Q,
                           const Rows& O, bool bf, float* ws, hipStream_t s);
     static hipError_t rows(int type, const Cache& c, const Batch& b, const Attn& a, const RowPlan& p, const Rows& Q,
+                           const Rows& O, bool bf, float* ws, hipStream_t s);
+};
+// Those of trees (kq_kv_tree_<D>.hip); rows: FewPlan's sixteens are 8 or 16.
+template <int D>
+struct TreeKernels {
+    static hipError_t few(int type, const Cache& c, const Batch& b, const Attn& a, const FewPlan& p, const Rows& Q,
+                          const Rows& O, bool bf, float* ws, hipStream_t s);
+    static hipError_t rows(int type, const Cache& c, const Batch& b, const Attn& a, const FewPlan& p, const Rows& Q,
                            const Rows& O, bool bf, float* ws, hipStream_t s);
 };
 }  // namespace kv

@@ -57,12 +57,12 @@ size_t few_ws_bytes(const FewPlan& p, uint32_t D) {
 uint64_t row_splits_wanted(const Cache& c, const Batch& b, const RowPlan& p) {
     return ceil_div((uint64_t)cu_count() * (p.rows == 256 ? 1 : 2), (uint64_t)b.n_seq * p.tiles * c.heads);
 }
-RowPlan row_plan(const Cache& c, const Batch& b, uint32_t D, uint32_t group, uint32_t window, bool tree) {
+RowPlan row_plan(const Cache& c, const Batch& b, uint32_t D, uint32_t group, uint32_t window) {
     RowPlan p;
     const uint64_t rows = (uint64_t)b.max_q * group;
     p.rows = rows <= 128 ? 128 : row_most(D);
     p.tiles = (uint32_t)ceil_div(rows, p.rows);
-    const uint64_t longest = longest_span(b, p.rows, window, tree);
+    const uint64_t longest = longest_span(b, p.rows, window, false);
     p.chunk = (uint32_t)std::max<uint64_t>(ceil_div(ceil_div(longest, row_splits_wanted(c, b, p)), kTile) * kTile, kRound);
     p.splits = (uint32_t)ceil_div(longest, p.chunk);
     return p;
@@ -71,9 +71,35 @@ size_t row_ws_bytes(const Cache& c, const Batch& b, const RowPlan& p, uint64_t s
     return splits > 1 ? (size_t)b.n_seq * splits * p.tiles * c.heads * p.rows * (D + kRowSum) * 4 : 0;
 }
 
+// Many rows of trees: shares and parts as for few rows, of whole units of 64 tokens, among the workgroups that the
+// device holds at once.
+FewPlan tree_plan(const Cache& c, const Batch& b, uint32_t D, uint32_t group, uint32_t window) {
+    FewPlan p = {};
+    const uint64_t q_rows = (uint64_t)b.max_q * group;
+    const uint32_t tile = q_rows <= 128 ? 128 : row_most(D);
+    p.sixteens = tile / 16;
+    p.tiles = (uint32_t)ceil_div(q_rows, tile);
+    const uint64_t rounds = ceil_div(longest_span(b, q_rows, window, true), kTile);
+    const uint64_t rows = (uint64_t)b.n_seq * c.heads, at_once = (uint64_t)cu_count() * (tile == 256 || D >= 192 ? 1 : 2);
+    const uint64_t fit = std::max<uint64_t>(at_once / p.tiles, 1);
+    p.groups = (uint32_t)std::min<uint64_t>(fit, rows * rounds);
+    p.mode = 2 * rows <= p.groups ? FewPlan::kParts : FewPlan::kShares;
+    constexpr uint32_t start = 5;
+    if (rounds <= (p.mode == FewPlan::kShares ? 4 : 1) || b.n_seq > kScan || b.n_seq * (ceil_div(b.max_len, kTile) + start) >= 0x7FFFFFFF) {
+        p.mode = FewPlan::kRows;
+        p.groups = (uint32_t)rows;
+        return p;
+    }
+    p.start = p.mode == FewPlan::kShares && rows * rounds >= 4 * fit ? start : 0;
+    p.by_row = rows <= p.groups;
+    p.cuts = p.by_row ? (uint32_t)rows : p.groups;
+    return p;
+}
+
 size_t ws_need(const Cache& c, const Batch& b, uint32_t D, uint32_t group, uint32_t window, bool tree) {
     if (few(b, group)) return few_ws_bytes(few_plan(c, b, D, group, window, tree), D);
-    const RowPlan p = row_plan(c, b, D, group, window, tree);
+    if (tree) return few_ws_bytes(tree_plan(c, b, D, group, window), D);
+    const RowPlan p = row_plan(c, b, D, group, window);
     return row_ws_bytes(c, b, p, p.splits, D);
 }
 
@@ -81,8 +107,8 @@ size_t ws_need(const Cache& c, const Batch& b, uint32_t D, uint32_t group, uint3
 // are not as orderly: no window makes more than are wanted, nor of less than a round.
 size_t ws_bytes(const Cache& c, const Batch& b, uint32_t D, uint32_t group, bool tree) {
     size_t n = ws_need(c, b, D, group, 0, tree);
-    if (!few(b, group)) {
-        const RowPlan p = row_plan(c, b, D, group, 0, tree);
+    if (!few(b, group) && !tree) {
+        const RowPlan p = row_plan(c, b, D, group, 0);
         n = row_ws_bytes(c, b, p, std::min(row_splits_wanted(c, b, p), ceil_div(b.max_len, kRound)), D);
     }
     return n > 256 ? (n + 255) / 256 * 256 : 256;
@@ -93,7 +119,12 @@ bool fits(const Cache& c, const Batch& b, uint32_t D, uint32_t group, bool tree)
     // Shares, parts and splits are made of few rows of work, and are few.
     const uint64_t rows = (uint64_t)b.n_seq * c.heads;
     if (few(b, group)) return (rows + 7) / 8 * 8 * few_plan(c, b, D, group, 0, tree).tiles <= kMostGroups;
-    const RowPlan p = row_plan(c, b, D, group, 0, tree);
+    // of 512 threads count as two
+    if (tree) {
+        const FewPlan p = tree_plan(c, b, D, group, 0);
+        return (rows + 7) / 8 * 8 * p.tiles * (p.sixteens / 8) <= kMostGroups;
+    }
+    const RowPlan p = row_plan(c, b, D, group, 0);
     return rows * p.tiles * (p.rows / 128) <= kMostGroups;
 }
 
@@ -114,17 +145,15 @@ bool kv_tree_fits(const kv::Cache& c, const kv::Batch& b, uint32_t D, uint32_t g
 hipError_t launch_kv_attn(const kv::Cache& c, const kv::Batch& b, uint32_t D, int type, const kv::Attn& a,
                           const kv::Rows& Q, const kv::Rows& O, bool bf, void* ws, hipStream_t s) {
     float* const w = static_cast<float*>(ws);
-    const bool tree = a.mask != nullptr;
     return kv::by_dim(D, type, [&](auto d, auto) {
         constexpr int N = decltype(d)::value;
-        if (kv::few(b, a.group)) {
-            const kv::FewPlan p = kv::few_plan(c, b, D, a.group, a.window, tree);
-            return tree ? kv::AttnKernels<N, true>::few(type, c, b, a, p, Q, O, bf, w, s)
-                        : kv::AttnKernels<N, false>::few(type, c, b, a, p, Q, O, bf, w, s);
-        }
-        const kv::RowPlan p = kv::row_plan(c, b, D, a.group, a.window, tree);
-        return tree ? kv::AttnKernels<N, true>::rows(type, c, b, a, p, Q, O, bf, w, s)
-                    : kv::AttnKernels<N, false>::rows(type, c, b, a, p, Q, O, bf, w, s);
+        if (a.mask)
+            return kv::few(b, a.group)
+                       ? kv::TreeKernels<N>::few(type, c, b, a, kv::few_plan(c, b, D, a.group, a.window, true), Q, O, bf, w, s)
+                       : kv::TreeKernels<N>::rows(type, c, b, a, kv::tree_plan(c, b, D, a.group, a.window), Q, O, bf, w, s);
+        return kv::few(b, a.group)
+                   ? kv::AttnKernels<N>::few(type, c, b, a, kv::few_plan(c, b, D, a.group, a.window, false), Q, O, bf, w, s)
+                   : kv::AttnKernels<N>::rows(type, c, b, a, kv::row_plan(c, b, D, a.group, a.window), Q, O, bf, w, s);
     });
 }
 

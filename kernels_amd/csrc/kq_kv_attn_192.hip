@@ -5,17 +5,17 @@ namespace kq {
 namespace kv {
 
 template <>
-hipError_t AttnKernels<192, false>::few(int type, const Cache& c, const Batch& b, const Attn& a, const FewPlan& p, const Rows& Q,
+hipError_t AttnKernels<192>::few(int type, const Cache& c, const Batch& b, const Attn& a, const FewPlan& p, const Rows& Q,
                               const Rows& O, bool bf, float* ws, hipStream_t s) {
     return type == KQ_KV_I8 ? few_d<192, KQ_KV_I8, false>(c, b, a, p, Q, O, bf, ws, s)
                             : few_d<192, KQ_KV_E4M3, false>(c, b, a, p, Q, O, bf, ws, s);
 }
 
 template <>
-hipError_t AttnKernels<192, false>::rows(int type, const Cache& c, const Batch& b, const Attn& a, const RowPlan& p, const Rows& Q,
+hipError_t AttnKernels<192>::rows(int type, const Cache& c, const Batch& b, const Attn& a, const RowPlan& p, const Rows& Q,
                                const Rows& O, bool bf, float* ws, hipStream_t s) {
-    return type == KQ_KV_I8 ? rows_d<192, KQ_KV_I8, false>(c, b, a, p, Q, O, bf, ws, s)
-                            : rows_d<192, KQ_KV_E4M3, false>(c, b, a, p, Q, O, bf, ws, s);
+    return type == KQ_KV_I8 ? rows_d<192, KQ_KV_I8>(c, b, a, p, Q, O, bf, ws, s)
+                            : rows_d<192, KQ_KV_E4M3>(c, b, a, p, Q, O, bf, ws, s);
 }
 
 }  // namespace kv

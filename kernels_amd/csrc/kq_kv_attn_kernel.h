@@ -75,14 +75,12 @@ __device__ __forceinline__ Span span_of(const Seq& s, const Attn& a, int row, in
 // `first` on; before them the row sees from `lo` on, and nothing counts that is not below hi.
 __device__ __forceinline__ uint32_t low_bits(int n) { return n >= 16 ? 0xFFFFu : (1u << max(n, 0)) - 1; }
 __device__ __forceinline__ uint32_t tree_bits(const uint32_t* mask, int words, int t0, int first, int lo, int hi) {
-    uint32_t sees = low_bits(first - t0) & ~low_bits(lo - t0);
-    const int off = t0 - first;  // of the tokens' bits
-    if (off > -16) {
-        const int w = off >> 5;
-        const uint32_t a = w >= 0 && w < words ? mask[w] : 0u, b = w + 1 < words ? mask[w + 1] : 0u;
-        sees |= (uint32_t)(((uint64_t)b << 32 | a) >> (off & 31)) & 0xFFFFu & ~low_bits(-off);
-    }
-    return sees & low_bits(hi - t0);
+    // of the tokens' bits; words that there are not are read as others, and their bits not taken
+    const int off = t0 - first, w = off >> 5;
+    const uint32_t a = mask[min(max(w, 0), words - 1)], b = mask[min(max(w + 1, 0), words - 1)];
+    const uint32_t lower = w >= 0 && w < words ? a : 0u, upper = w >= -1 && w + 1 < words ? b : 0u;
+    const uint32_t of_rows = (uint32_t)(((uint64_t)upper << 32 | lower) >> (off & 31)) & 0xFFFFu & ~low_bits(-off);
+    return ((low_bits(first - t0) & ~low_bits(lo - t0)) | of_rows) & low_bits(hi - t0);
 }
 
 __device__ __forceinline__ int row_splits(const Span& v, int chunk) {
@@ -263,8 +261,8 @@ __device__ __forceinline__ int prefix64(int v) {
 }
 
 // What group k does; each wave works it out for itself from the units of all sequences.
-// lds: kScan ints.
-template <bool TREE>
+// lds: kScan ints. LEAST: units of a part, at least.
+template <bool TREE, int LEAST = kRound / kTile>
 __device__ inline Share share_of(const Cache& c, const Batch& b, const Attn& a, const FewPlan& p, uint32_t k, int rows,
                                  int* lds) {
     const int lane = threadIdx.x & 63, n = (int)b.n_seq;
@@ -313,7 +311,7 @@ __device__ inline Share share_of(const Cache& c, const Batch& b, const Attn& a, 
     if (p.mode == FewPlan::kParts) {
         // c from the mean on; the last is enough for any lengths: sum ceil(u / c) <= sum u / c + rows of work
         const uint32_t most = p.groups / c.heads;
-        uint32_t size = max((uint32_t)((all + most - 1) / most), (uint32_t)(kRound / kTile)), count = 0;
+        uint32_t size = max((uint32_t)((all + most - 1) / most), (uint32_t)LEAST), count = 0;
         for (int tries = 0; tries < 4; ++tries, ++size) {
             count = (uint32_t)sum([&](int v) { return (int)(((uint32_t)v + size - 1) / size); });
             if (count <= most) break;

@@ -26,7 +26,7 @@ struct RowTile {
     int exps[8];  // exponent bytes of the four 16-token blocks: K's (-1: no page), V's (kBase: no page or token)
 };
 
-template <int D, int TYPE, int NW, bool TREE>
+template <int D, int TYPE, int NW>
 __global__ __launch_bounds__(64 * NW, D >= 192 ? 1 : 2) void kv_rows_k(Cache c, Batch b, Attn a, RowPlan p, Rows Q, Rows O,
                                                                        int bf, float* ws) {
     constexpr int T = 64 * NW, RT = 32 * NW;
@@ -45,7 +45,7 @@ __global__ __launch_bounds__(64 * NW, D >= 192 ? 1 : 2) void kv_rows_k(Cache c, 
     const Seq s = sequence(b, c.page_log2, seq);
     const int row0 = (int)tile * RT, rows = s.n * (int)a.group;
     if (row0 >= rows) return;
-    const Span sp = span_of<TREE>(s, a, row0, RT);
+    const Span sp = span_of<false>(s, a, row0, RT);
     const int n_splits = row_splits(sp, (int)p.chunk);
     if ((int)split >= max(n_splits, 1)) return;
     const int lo = sp.lo + (int)(split * p.chunk), hi = (int)min((int64_t)sp.hi, (int64_t)lo + p.chunk);
@@ -56,12 +56,7 @@ __global__ __launch_bounds__(64 * NW, D >= 192 ? 1 : 2) void kv_rows_k(Cache c, 
     const uint32_t q_heads = c.heads * a.group, head = h * a.group + (uint32_t)(row % (int)a.group);
     const bool there = row0 + wave * 32 + n < rows;
     const int pos = s.len - s.n + tok;
-    // TREE: the tokens before the first row, from a window on; of those from it on the row's bits
-    const bool busy = row0 + wave * 32 < rows;
-    const int first_row = s.len - s.n;
-    const int sees_hi = !busy ? 0 : TREE ? min(max(first_row, 0), hi) : min(a.causal ? pos + 1 : s.len, hi);
-    const int sees_lo = a.window ? (TREE ? max(a.pos[s.row0 + tok], first_row) : pos) + 1 - (int)a.window : 0;
-    const uint32_t* const mask = TREE ? a.mask + (uint64_t)(uint32_t)(s.row0 + tok) * a.words : nullptr;
+    const int sees_hi = row0 + wave * 32 < rows ? min(a.causal ? pos + 1 : s.len, hi) : 0, sees_lo = a.window ? pos + 1 - (int)a.window : 0;
 
     // Q as the second operand: 8 of each 16 columns
     f16x8 q[D / 16];
@@ -161,11 +156,7 @@ __global__ __launch_bounds__(64 * NW, D >= 192 ? 1 : 2) void kv_rows_k(Cache c, 
     int base = kBase;  // of l
     f32x16v o[D / 32] = {};
     auto compute = [&](int t0, const RowTile<D>& in) {
-        if constexpr (TREE) {
-            if (!__any(busy && t0 + 64 > min(sees_lo, first_row))) return;
-        } else {
-            if (!__any(t0 < sees_hi && t0 + 64 > sees_lo)) return;  // no token of it in sight of the wave
-        }
+        if (!__any(t0 < sees_hi && t0 + 64 > sees_lo)) return;  // no token of it in sight of the wave
         f32x16v st[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
@@ -186,19 +177,11 @@ __global__ __launch_bounds__(64 * NW, D >= 192 ? 1 : 2) void kv_rows_k(Cache c, 
             const int end = first + sees_hi - sees_lo;
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                if constexpr (TREE) {
-                    const uint32_t sees = !busy || (u ? k1 : k0) < 0 ? 0u
-                                              : tree_bits(mask, (int)a.words, t0 + 32 * u + 16 * g, first_row, first + t0 + 16 * g, hi);
 #pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        st[u][i] = sees >> i & 1 ? __builtin_fmaf(st[u][i], f[u], e[u]) : -__builtin_inff();
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const int t = 32 * u + i;
-                        st[u][i] = t < first || t >= end || (u ? k1 : k0) < 0 ? -__builtin_inff()
-                                                                             : __builtin_fmaf(st[u][i], f[u], e[u]);
-                    }
+                for (int i = 0; i < 16; ++i) {
+                    const int t = 32 * u + i;
+                    st[u][i] = t < first || t >= end || (u ? k1 : k0) < 0 ? -__builtin_inff()
+                                                                         : __builtin_fmaf(st[u][i], f[u], e[u]);
                 }
                 f[u] = 1.0f;
                 e[u] = 0.0f;
@@ -295,7 +278,7 @@ __global__ __launch_bounds__(64 * NW, D >= 192 ? 1 : 2) void kv_rows_k(Cache c, 
 }
 
 // Adds up the splits of kv_rows_k: a wave takes one (token, query head).
-template <int D, bool TREE>
+template <int D>
 __global__ __launch_bounds__(256) void kv_rows_join_k(Cache c, Batch b, Attn a, RowPlan p, Rows O, int bf, const float* ws) {
     const uint32_t q_heads = c.heads * a.group, id = blockIdx.x * 4 + (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const uint32_t head = id % q_heads, h = head / a.group, j = id / q_heads % b.max_q, seq = id / q_heads / b.max_q;
@@ -303,7 +286,7 @@ __global__ __launch_bounds__(256) void kv_rows_join_k(Cache c, Batch b, Attn a, 
     const Seq s = sequence(b, c.page_log2, seq);
     if ((int)j >= s.n) return;
     const int RT = (int)p.rows, row = (int)(j * a.group + head % a.group), tile = row / RT, in = row % RT;
-    const int n = row_splits(span_of<TREE>(s, a, tile * RT, RT), (int)p.chunk);
+    const int n = row_splits(span_of<false>(s, a, tile * RT, RT), (int)p.chunk);
     if (n <= 1) return;
     const uint64_t size = (uint64_t)RT * (D + kRowSum);
     const float* const first = ws + (((uint64_t)seq * p.splits * p.tiles + tile) * c.heads + h) * size;
@@ -312,19 +295,19 @@ __global__ __launch_bounds__(256) void kv_rows_join_k(Cache c, Batch b, Attn a, 
                    [&](int i) { return first + i * step + RT * D + in * kRowSum; }, nullptr, O, bf, s.row0 + (int)j, head, q_heads);
 }
 
-template <int D, int TYPE, bool TREE>
+template <int D, int TYPE>
 hipError_t rows_d(const Cache& c, const Batch& b, const Attn& a, const RowPlan& p, const Rows& Q, const Rows& O, bool bf,
                   float* ws, hipStream_t s) {
     const uint32_t wgs = b.n_seq * p.splits * p.tiles * c.heads;
     if constexpr (row_most(D) > 128) {
-        if (p.rows > 128) kv_rows_k<D, TYPE, 8, TREE><<<wgs, 512, 0, s>>>(c, b, a, p, Q, O, bf, ws);
-        else kv_rows_k<D, TYPE, 4, TREE><<<wgs, 256, 0, s>>>(c, b, a, p, Q, O, bf, ws);
+        if (p.rows > 128) kv_rows_k<D, TYPE, 8><<<wgs, 512, 0, s>>>(c, b, a, p, Q, O, bf, ws);
+        else kv_rows_k<D, TYPE, 4><<<wgs, 256, 0, s>>>(c, b, a, p, Q, O, bf, ws);
     } else {
-        kv_rows_k<D, TYPE, 4, TREE><<<wgs, 256, 0, s>>>(c, b, a, p, Q, O, bf, ws);
+        kv_rows_k<D, TYPE, 4><<<wgs, 256, 0, s>>>(c, b, a, p, Q, O, bf, ws);
     }
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.splits == 1) return e;
-    kv_rows_join_k<D, TREE><<<(b.n_seq * b.max_q * c.heads * a.group + 3) / 4, 256, 0, s>>>(c, b, a, p, O, bf, ws);
+    kv_rows_join_k<D><<<(b.n_seq * b.max_q * c.heads * a.group + 3) / 4, 256, 0, s>>>(c, b, a, p, O, bf, ws);
     return hipGetLastError();
 }
 

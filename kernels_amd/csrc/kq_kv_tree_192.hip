@@ -1,21 +1,21 @@
 // kq_kv_tree_192.hip -- attention of trees over the 8-bit cache, heads 192 wide.
-#include "kq_kv_rows_kernel.h"
+#include "kq_kv_tree_kernel.h"
 
 namespace kq {
 namespace kv {
 
 template <>
-hipError_t AttnKernels<192, true>::few(int type, const Cache& c, const Batch& b, const Attn& a, const FewPlan& p, const Rows& Q,
+hipError_t TreeKernels<192>::few(int type, const Cache& c, const Batch& b, const Attn& a, const FewPlan& p, const Rows& Q,
                               const Rows& O, bool bf, float* ws, hipStream_t s) {
     return type == KQ_KV_I8 ? few_d<192, KQ_KV_I8, true>(c, b, a, p, Q, O, bf, ws, s)
                             : few_d<192, KQ_KV_E4M3, true>(c, b, a, p, Q, O, bf, ws, s);
 }
 
 template <>
-hipError_t AttnKernels<192, true>::rows(int type, const Cache& c, const Batch& b, const Attn& a, const RowPlan& p, const Rows& Q,
+hipError_t TreeKernels<192>::rows(int type, const Cache& c, const Batch& b, const Attn& a, const FewPlan& p, const Rows& Q,
                                const Rows& O, bool bf, float* ws, hipStream_t s) {
-    return type == KQ_KV_I8 ? rows_d<192, KQ_KV_I8, true>(c, b, a, p, Q, O, bf, ws, s)
-                            : rows_d<192, KQ_KV_E4M3, true>(c, b, a, p, Q, O, bf, ws, s);
+    return type == KQ_KV_I8 ? tree_rows_d<192, KQ_KV_I8>(c, b, a, p, Q, O, bf, ws, s)
+                            : tree_rows_d<192, KQ_KV_E4M3>(c, b, a, p, Q, O, bf, ws, s);
 }
 
 }  // namespace kv
