@@ -22,6 +22,7 @@ constexpr uint32_t kChunk = 4096;
 // picked outright and turned down there, the rows of q that others were drawn from, and how many are kept.
 struct End {
     int row, n_out, n_q, count;
+    double u;  // the sequence's number for it
 };
 // A sequence's part of the workspace: End, then the three lists, then the chunks' sums.
 struct Places {
@@ -113,7 +114,7 @@ __device__ __forceinline__ End walk(const kq_draft& d, uint32_t i, const Rows& r
         r.q[j] = from < 0 ? 1.0 : real ? prob(d.q[(int64_t)from * d.q_row + x]) : 0.0;
     }
     __syncthreads();
-    End e = {s.n ? s.row0 : -1, 0, 0, s.n ? 1 : 0};
+    End e = {s.n ? s.row0 : -1, 0, 0, s.n ? 1 : 0, s.n ? (double)r.u[0] : 0.0};
     if (writer && tid == 0 && s.n) keep[0] = 0;
     int at = 0, last = 0;  // the present row, and the latest one tried there
     double mass = 1.0;
@@ -156,7 +157,7 @@ __device__ __forceinline__ End walk(const kq_draft& d, uint32_t i, const Rows& r
                 keep[e.count] = j;
                 out[e.count - 1] = x;
             }
-            e = {s.row0 + j, 0, 0, e.count + 1};
+            e = {s.row0 + j, 0, 0, e.count + 1, e.u};
             mass = 1.0;
             stale = false;
             continue;
@@ -329,13 +330,14 @@ __global__ __launch_bounds__(256) void verify_draw_k(kq_draft d, int32_t* out, c
     const Rows r = rows_in(row_lds, d.max_q);
     const int tid = threadIdx.x;
     ws += at.size * blockIdx.x;
-    const End e = get_end<256>(ws, at, r);
-    if (e.row < 0) return;
-    const double u = d.u[sequence(d, blockIdx.x).row0];
     const double* const sums = reinterpret_cast<const double*>(ws + at.sums);
     const uint32_t each = (chunks + 255) / 256, mine = min(tid * each, chunks), end = min(mine + each, chunks);
+    // on their way together with the rest (of a sequence without rows: whatever stands there)
     double part = 0.0;
     for (uint32_t c = mine; c < end; ++c) part += sums[c];
+    const End e = get_end<256>(ws, at, r);
+    if (e.row < 0) return;
+    const double u = e.u;
     ends[tid] = block_prefix(part, scratch);
     if (tid == 0) found = -1;
     __syncthreads();

@@ -9,7 +9,7 @@ namespace {
 
 template <int D, int TYPE, int BF>
 __global__ __launch_bounds__(256) void kv_write_k(Cache c, Batch b, Rows K, Rows V, uint32_t groups) {
-    write_block<D, TYPE, BF, -1>(c, b, K, V, groups, blockIdx.x, Turn{});
+    write_block<D, TYPE, BF, -1>(c, b, K, V, groups, blockIdx.x, Turn{}, nullptr);
 }
 
 // F: the type of the rows.

@@ -11,12 +11,15 @@ namespace {
 template <int D, int TYPE, int BF, int TURN>
 __global__ __launch_bounds__(256) void kv_write_rope_k(Cache c, Batch b, Rows K, Rows V, uint32_t groups, uint32_t blocks, Turn turn,
                                                        Rows Q, Rows Qo, uint32_t q_heads, uint32_t q_parts, uint32_t q_each) {
-    __shared__ rope::Factor tables[4][D / 2];
+    // a wave's turned keys, or the factors of a row
+    constexpr int kKept = (D + 63) / 64 * 2 * 64 * kept_subs(D);
+    static_assert(kKept * sizeof(u32x4) >= D / 2 * sizeof(rope::Factor));
+    __shared__ u32x4 kept[4][kKept];
+    const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     if (blockIdx.x < blocks) {
-        write_block<D, TYPE, BF, TURN>(c, b, K, V, groups, blockIdx.x, turn);
+        write_block<D, TYPE, BF, TURN>(c, b, K, V, groups, blockIdx.x, turn, kept[wave]);
         return;
     }
-    const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const uint32_t id = (blockIdx.x - blocks) * 4 + wave;
     const Seq s = sequence(b, c.page_log2, blockIdx.y);
     const int j = (int)(id / q_parts);
@@ -25,14 +28,15 @@ __global__ __launch_bounds__(256) void kv_write_rope_k(Cache c, Batch b, Rows K,
     const int row = s.row0 + j, pos = turn.pos ? turn.pos[row] : s.len - s.n + j;
     rope::turn_heads<BF, TURN>(turn.rope, pos, static_cast<const uint8_t*>(Q.p) + (int64_t)row * Q.row * 2,
                                static_cast<uint8_t*>(Qo.p) + (int64_t)row * Qo.row * 2, Q.head, Qo.head, h0,
-                               min(q_heads, h0 + q_each), D, tables[wave]);
+                               min(q_heads, h0 + q_each), D, reinterpret_cast<rope::Factor*>(kept[wave]));
 }
 
 template <int D, int TYPE, int BF>
 hipError_t write_rope_d(const Cache& c, const Batch& b, const Turn& turn, const Rows* Q, const Rows* Qo, uint32_t q_heads,
                         const Rows& K, const Rows& V, hipStream_t s) {
     const uint32_t groups = (2 * c.heads + 3) / 4, blocks = spans(b.max_q, 1u << c.block_log2) * groups;
-    const uint32_t each = 64 / (turn.rope.rot / 16), parts = Q ? (q_heads + each - 1) / each : 0;
+    const uint32_t each = Q ? rope_heads_each((uint64_t)b.max_q * b.n_seq, q_heads, turn.rope.rot) : 1;
+    const uint32_t parts = Q ? (q_heads + each - 1) / each : 0;
     const dim3 grid(blocks + (uint32_t)(((uint64_t)b.max_q * parts + 3) / 4), b.n_seq);
     const Rows q = Q ? *Q : Rows{}, qo = Q ? *Qo : Rows{};
     if (turn.rope.pairs) kv_write_rope_k<D, TYPE, BF, 1><<<grid, 256, 0, s>>>(c, b, K, V, groups, blocks, turn, q, qo, q_heads, parts, each);

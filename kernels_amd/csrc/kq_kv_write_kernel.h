@@ -57,10 +57,12 @@ __device__ __forceinline__ uint32_t four_codes(float a, float b, float c, float 
 // TURN: the layout of the pairs that keys are turned by (0: HALVES, 1: PAIRS), or none
 // (-1). A lane then holds units of 16 columns that are turned together, in place of
 // chunks of 8 in order; everything behind is the same. Angles are computed anew by each head's
-// wave.
+// wave, and once: blocks of up to kept_subs(D) x 16 tokens wait in LDS, turned, for their scale (48 trees of 9-26 rows into
+// blocks of 32, 64 and 8 heads of 128: turned twice 22.0 us, so 16.6).
+constexpr int kept_subs(int D) { return D <= 128 ? 256 / D : 1; }
 template <int D, int TYPE, int BF, int TURN>
 __device__ __forceinline__ void write_block(const Cache& c, const Batch& b, const Rows& K, const Rows& V, uint32_t groups, uint32_t block_x,
-                                            const Turn& turn) {
+                                            const Turn& turn, u32x4* kept) {
     const int lane = threadIdx.x & 63;
     const uint32_t job = (block_x % groups) * 4 + (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     if (job >= 2 * c.heads) return;
@@ -143,12 +145,29 @@ __device__ __forceinline__ void write_block(const Cache& c, const Batch& b, cons
     load(lo & ~15);  // on its way while the page id is
     if (page < 0) return;
     rotate(lo & ~15);
+    // The tokens of `sub` once more, for the passes behind the first; put by: into LDS.
+    const bool wait = TURN >= 0 && !is_v && B > 16 && B <= 16 * kept_subs(D);
+    auto put_by = [&](int sub) __attribute__((always_inline)) {
+        if constexpr (TURN >= 0)
+            if (wait)
+#pragma unroll
+                for (int j = 0; j < NK; ++j) kept[(sub / 16 * NK + j) * 64 + lane] = xk[j];
+    };
+    auto again = [&](int sub) __attribute__((always_inline)) {
+        if (wait && sub >= (lo & ~15)) {
+#pragma unroll
+            for (int j = 0; j < NK; ++j) xk[j] = kept[(sub / 16 * NK + j) * 64 + lane];
+        } else {
+            load(sub), rotate(sub);
+        }
+    };
     uint8_t* const codes = (is_v ? c.v : c.k) + code_offset(c, D, page, h, t0);
     uint8_t* const ep = (is_v ? c.v_exp : c.k_exp) + exp_offset(c, page, h, t0);
     const int was = lo > 0 ? (int)*ep - 127 : -127;
     uint32_t m = 0;
     for (int sub = lo & ~15; sub < hi; sub += 16) {
         if (sub > lo) load(sub), rotate(sub);
+        put_by(sub);
         if (!is_v) {
 #pragma unroll
             for (int j = 0; j < NK; ++j)
@@ -166,7 +185,7 @@ __device__ __forceinline__ void write_block(const Cache& c, const Batch& b, cons
     if (!finite) {  // once more, without infinities and NaN
         m = 0;
         for (int sub = lo & ~15; sub < hi; sub += 16) {
-            if (B > 16) load(sub), rotate(sub);
+            if (B > 16) again(sub);
             if (!is_v) {
 #pragma unroll
                 for (int j = 0; j < NK; ++j)
@@ -191,7 +210,7 @@ __device__ __forceinline__ void write_block(const Cache& c, const Batch& b, cons
     auto write = [&](auto plain) __attribute__((always_inline)) {
         constexpr bool P = decltype(plain)::value;
         for (int sub = grew ? 0 : lo & ~15; sub < hi; sub += 16) {
-            if (B > 16) load(sub), rotate(sub);
+            if (B > 16) again(sub);
             if (!is_v) {
 #pragma unroll
                 for (int j = 0; j < NK; ++j) {

@@ -29,23 +29,23 @@ hipError_t rope_f(const Rope& r, const int32_t* pos, const kv::Rows& X, const kv
 }
 
 }  // namespace
-
-// Heads of a wave: as many as its lanes take at once, or all of them where there are rows enough.
-uint32_t heads_each(uint32_t n_rows, uint32_t heads, uint32_t rot) {
-    const uint32_t at_once = rot % 16 ? 1 : 64 / (rot / 16);
-    const uint64_t parts = (heads + at_once - 1) / at_once;
-    return (uint64_t)n_rows * parts > 16384 ? heads : at_once;
-}
 }  // namespace rope
 
+// As many as its lanes take at once, or all of them where there are rows enough.
+uint32_t rope_heads_each(uint64_t n_rows, uint32_t heads, uint32_t rot) {
+    const uint32_t at_once = rot % 16 ? 1 : 64 / (rot / 16);
+    const uint64_t parts = (heads + at_once - 1) / at_once;
+    return n_rows * parts > 16384 ? heads : at_once;
+}
+
 bool rope_fits(uint32_t n_rows, uint32_t heads, uint32_t rot) {
-    const uint32_t each = rope::heads_each(n_rows, heads, rot);
+    const uint32_t each = rope_heads_each(n_rows, heads, rot);
     return ((uint64_t)n_rows * ((heads + each - 1) / each) + 3) / 4 <= kv::kMostGroups;
 }
 
 hipError_t launch_rope(const rope::Rope& r, const int32_t* pos, const kv::Rows& X, const kv::Rows& Y, uint32_t n_rows,
                        uint32_t heads, uint32_t D, kq_dtype f, hipStream_t s) {
-    const uint32_t each = rope::heads_each(n_rows, heads, r.rot), parts = (heads + each - 1) / each;
+    const uint32_t each = rope_heads_each(n_rows, heads, r.rot), parts = (heads + each - 1) / each;
     const uint32_t wgs = (uint32_t)(((uint64_t)n_rows * parts + 3) / 4);
     return f == KQ_F16    ? rope::rope_f<KQ_F16>(r, pos, X, Y, n_rows, heads, D, parts, each, wgs, s)
            : f == KQ_BF16 ? rope::rope_f<KQ_BF16>(r, pos, X, Y, n_rows, heads, D, parts, each, wgs, s)

@@ -620,11 +620,10 @@ def kv_tree(batch, parent, mask, pos=None, window=0, stream=None):
     """Masks int32 [n_rows][words], words * 32 >= max_q, and positions int32 [n_rows] of the trees that parent int32
     [n_rows] describes (a row's parent among its sequence's rows), for all the layers' calls of a step. Returns their
     KVTree. window > 0: a row sees the nearest `window` of the rows it continues, itself among them."""
-    import torch
     s = _on_current(stream, batch.kv_len, parent, mask, pos)
     tree = KVTree(mask, pos)
     rows = mask.shape[0]
-    _here(parent, torch.int32, (rows,), "parent")
+    _ints(parent, rows, "parent")
     _need(0 <= window < 2**32, "window: 32-bit")
     _check(lib().kq_kv_tree(batch._packed(rows), _ptr(parent), _ptr(mask), mask.shape[1], _ptr(pos), window, s), "kq_kv_tree")
     return tree
@@ -643,6 +642,19 @@ def kv_attn_tree(cache, batch, tree, q, out, ws, ws_bytes, scale=None, window=0,
              lse, stream)
 
 
+_int32 = _float32 = None  # torch's, from the first call on
+
+
+def _ints(t, n, what):
+    """t: a contiguous int32 tensor [n]."""
+    global _int32, _float32
+    if _int32 is None:
+        import torch
+        _int32, _float32 = torch.int32, torch.float32
+    if t.dtype is not _int32 or t.dim() != 1 or t.numel() != n or not t.is_contiguous():
+        _here(t, _int32, (n,), what)
+
+
 def draft_verify_workspace_size(n_seq, max_q, vocab):
     n = lib().kq_draft_verify_workspace_size(n_seq, max_q, vocab)
     if n == 0:
@@ -650,11 +662,11 @@ def draft_verify_workspace_size(n_seq, max_q, vocab):
     return n
 
 
-def _probabilities(t, dtype, rows, vocab, what):
-    if t.dtype != dtype or t.dim() != 2 or t.shape[1] != vocab or (rows is not None and t.shape[0] < rows):
-        raise ValueError(f"{what}: a {dtype} tensor [{'any' if rows is None else rows}][{vocab}], not {t.dtype} {tuple(t.shape)}")
-    if t.stride(1) != 1 and vocab > 1 and t.shape[0]:
-        raise ValueError(f"{what}: contiguous in its last dimension, not strides {t.stride()}")
+def _probabilities(t, what):
+    """The shape of a float32 tensor of rows, contiguous and at any stride."""
+    if t.dim() != 2 or t.dtype is not _float32 or (t.stride(1) != 1 and t.shape[1] > 1 and t.shape[0]):
+        raise ValueError(f"{what}: a float32 tensor of rows, contiguous in its last dimension, not {t.dtype} {tuple(t.shape)} of strides {t.stride()}")
+    return t.shape
 
 
 def draft_verify(p, token, u, keep, n_keep, out, ws, ws_bytes, q=None, q_index=None, parent=None, start=None, stream=None):
@@ -665,33 +677,37 @@ def draft_verify(p, token, u, keep, n_keep, out, ws, ws_bytes, q=None, q_index=N
     token: int32 [n_rows]. parent: int32 [n_rows] (None: a chain). start: int32 [n_seq + 1] (None: max_q rows
     each). q: float32 [n_q][vocab], the probabilities that the tokens were drawn from, row q_index[i] (int32 [n_rows],
     -1: picked outright) or i for row i; None: all were picked outright."""
-    import torch
-    f32, i32 = torch.float32, torch.int32
     s = _on_current(stream, p, token, u, keep, n_keep, out, q, q_index, parent, start, None if isinstance(ws, int) else ws)
     _need(keep.dim() == 2 and p.dim() == 2, "keep: [n_seq][max_q], p: [n_rows][vocab]")
-    (n_seq, max_q), (rows, vocab) = keep.shape, p.shape
-    _probabilities(p, f32, rows, vocab, "p")
-    for t, dtype, shape, what in ((token, i32, (rows,), "token"), (u, f32, (rows,), "u"), (keep, i32, (n_seq, max_q), "keep"),
-                                  (n_keep, i32, (n_seq,), "n_keep"), (out, i32, (n_seq, max_q), "out"), (parent, i32, (rows,), "parent"),
-                                  (start, i32, (n_seq + 1,), "start"), (q_index, i32, (rows,), "q_index")):
+    n_seq, max_q = keep.shape
+    _ints(n_keep, n_seq, "n_keep")
+    rows, vocab = _probabilities(p, "p")
+    _ints(token, rows, "token")
+    if out.shape != keep.shape or out.dtype is not _int32 or not out.is_contiguous() or keep.dtype is not _int32 or not keep.is_contiguous():
+        raise ValueError(f"keep, out: contiguous int32 tensors [{n_seq}][{max_q}]")
+    if u.dtype is not _float32 or u.dim() != 1 or u.numel() != rows or not u.is_contiguous():
+        raise ValueError(f"u: a contiguous float32 tensor [{rows}]")
+    for t, n, what in ((parent, rows, "parent"), (start, n_seq + 1, "start"), (q_index, rows, "q_index")):
         if t is not None:
-            _here(t, dtype, shape, what)
-    n_q = q_row = 0
+            _ints(t, n, what)
+    at_q = n_q = q_row = 0
     if q is not None:
-        _probabilities(q, f32, rows if q_index is None else None, vocab, "q")
-        n_q, q_row = q.shape[0], q.stride(0)
-    d = _pack_draft(p.data_ptr(), _ptr(q) or 0, p.stride(0), q_row, _ptr(q_index) or 0, token.data_ptr(), _ptr(parent) or 0,
-                    _ptr(start) or 0, u.data_ptr(), n_seq, max_q, rows, n_q, vocab)
+        n_q, wide = _probabilities(q, "q")
+        if wide != vocab or (q_index is None and n_q < rows):
+            raise ValueError(f"q: {'a row for each of p' if q_index is None else 'rows'}, {vocab} wide, not {tuple(q.shape)}")
+        at_q, q_row = q.data_ptr(), q.stride(0)
+    d = _pack_draft(p.data_ptr(), at_q, p.stride(0), q_row, _ptr(q_index) or 0, token.data_ptr(), _ptr(parent) or 0, _ptr(start) or 0,
+                    u.data_ptr(), n_seq, max_q, rows, n_q, vocab)
     _check(lib().kq_draft_verify(d, keep.data_ptr(), n_keep.data_ptr(), out.data_ptr(), _ptr(ws), ws_bytes, s), "kq_draft_verify")
 
 
 def kv_keep(cache, batch, keep, n_keep, stream=None):
     """The rows keep[i][:n_keep[i]] (int32 [n_seq][max_q] and [n_seq], as draft_verify leaves them) of each sequence's
     newest tokens moved together in the cache; the sequence then ends behind them, which is for kv_len to say."""
-    import torch
     s = _kv_call(cache, batch, stream, keep, n_keep)
-    _here(keep, torch.int32, (batch.n_seq, batch.max_q), "keep")
-    _here(n_keep, torch.int32, (batch.n_seq,), "n_keep")
+    _ints(n_keep, batch.n_seq, "n_keep")
+    if keep.dtype is not _int32 or keep.shape != (batch.n_seq, batch.max_q) or not keep.is_contiguous():
+        raise ValueError(f"keep: a contiguous int32 tensor [{batch.n_seq}][{batch.max_q}]")
     rows = batch.n_seq * batch.max_q if batch.q_start is None else 0x7FFF0000 - 1  # with q_start: no tensor has them
     _check(lib().kq_kv_keep(cache._ref, batch._packed(rows), keep.data_ptr(), n_keep.data_ptr(), s), "kq_kv_keep")
 
@@ -743,21 +759,23 @@ def _on_current(stream, *tensors):
 
 
 def _positions(pos, rows):
-    if pos is not None:
-        import torch
-        _here(pos, torch.int32, (rows,), "pos")
-    return _ptr(pos)
+    if pos is None:
+        return None
+    _ints(pos, rows, "pos")
+    return pos.data_ptr()
 
 
 def rope(x, out, pos, rope, stream=None):
     """x [n_rows][heads][head_dim] (float16, bfloat16 or float32, any row and head strides) turned into out, which
     may be x; pos: int32 [n_rows], each row's position."""
-    s = _on_current(stream, x, out, pos, rope.inv_freq)
+    s = _on_current(stream, x, out, pos)
+    _need(rope.device == _current[1](), "the rotation's frequencies are on the current device")
     shape, dtype = x.shape, x.dtype
     if len(shape) != 3:
         raise ValueError(f"x: [n_rows][heads][head_dim], not {tuple(shape)}")
     a, b = _kv_rows(x, shape, dtype, "x"), _kv_rows(out, shape, dtype, "out")
-    _check(lib().kq_rope(rope._ref, _positions(pos, shape[0]), a, b, *shape, _dt(x), s), "kq_rope")
+    at = _positions(pos, shape[0])
+    _check(lib().kq_rope(rope._ref, at, a, b, *shape, _dt(x), s), "kq_rope")
 
 
 def kv_write_rope(cache, batch, rope, k, v, q=None, q_out=None, pos=None, stream=None):
@@ -769,6 +787,7 @@ def kv_write_rope(cache, batch, rope, k, v, q=None, q_out=None, pos=None, stream
         raise ValueError(f"k: [n_rows][{cache.heads}][{cache.head_dim}], not {tuple(shape)}")
     _need((q is None) == (q_out is None), "q and q_out: both or none")
     a, b = _kv_rows(k, shape, dtype, "k"), _kv_rows(v, shape, dtype, "v")
+    at = _positions(pos, shape[0])
     x = y = None
     heads = 0
     if q is not None:
@@ -776,5 +795,5 @@ def kv_write_rope(cache, batch, rope, k, v, q=None, q_out=None, pos=None, stream
             raise ValueError(f"q: [{shape[0]}][q_heads][{shape[2]}], not {tuple(q.shape)}")
         heads = q.shape[1]
         x, y = _kv_rows(q, q.shape, dtype, "q"), _kv_rows(q_out, q.shape, dtype, "q_out")
-    _check(lib().kq_kv_write_rope(cache._ref, batch._packed(shape[0]), rope._ref, _positions(pos, shape[0]), x, y, heads, a, b,
-                                  _dt(k), s), "kq_kv_write_rope")
+    _check(lib().kq_kv_write_rope(cache._ref, batch._packed(shape[0]), rope._ref, at, x, y, heads, a, b, _dt(k), s),
+           "kq_kv_write_rope")

@@ -310,3 +310,75 @@ def test_keep_bad_batch(kw, status):
                                        (dict(n=FAKE + 2), kq.KQ_EALIGN), (dict(b=batch_c(n_rows=0)), kq.KQ_OK)])
 def test_bad_keep(kw, status):
     assert keep(**kw) == status
+
+
+# ---- the Python layer's own refusals (on the CPU: every tensor is on device -1)
+
+@pytest.fixture
+def no_gpu(monkeypatch):
+    """The wrappers' checks without a device: calls that pass them raise KeyError in place of a launch."""
+    import torch
+
+    class Lib:
+        def __getattr__(self, name):
+            raise KeyError(name)
+
+    monkeypatch.setattr(kq, "_stream", lambda s: 0)
+    monkeypatch.setattr(kq, "_current", (lambda d: 0, lambda: -1))
+    monkeypatch.setattr(kq, "_lib", Lib())
+    return torch
+
+
+def test_python_refusals(no_gpu):
+    t = no_gpu
+    i32, f32, f16 = t.int32, t.float32, t.float16
+    z = lambda *s, dtype=i32: t.zeros(s, dtype=dtype)  # noqa: E731
+    good = dict(p=z(6, 50, dtype=f32), token=z(6), u=z(6, dtype=f32), keep=z(2, 3), n_keep=z(2), out=z(2, 3), ws=0, ws_bytes=0)
+    with pytest.raises(KeyError):
+        kq.draft_verify(**good)
+    with pytest.raises(KeyError):
+        kq.draft_verify(**good, q=z(9, 50, dtype=f32), q_index=z(6), parent=z(6), start=z(3))
+    for kw in (dict(p=z(6, 50)), dict(p=z(6, dtype=f32)), dict(p=z(50, 6, dtype=f32).t()), dict(token=z(5)), dict(token=z(6, dtype=t.int64)),
+               dict(u=z(6)), dict(u=z(7, dtype=f32)), dict(keep=z(2, 4)), dict(keep=z(3, 2).t()), dict(n_keep=z(3)), dict(out=z(2, 3, dtype=t.int64)),
+               dict(parent=z(5)), dict(start=z(2)), dict(q=z(5, 50, dtype=f32)), dict(q=z(6, 49, dtype=f32)), dict(q_index=z(7)),
+               dict(q=z(6, 50, dtype=f16))):
+        with pytest.raises(ValueError):
+            kq.draft_verify(**{**good, **kw})
+    x, pos, f = z(4, 2, 64, dtype=f16), z(4), kq.Rope(z(32, dtype=f32))
+    with pytest.raises(KeyError):
+        kq.rope(x, x, pos, f)
+    for a in ((z(4, 64, dtype=f16), x, pos), (x, z(4, 2, 32, dtype=f16), pos), (x, z(4, 2, 64, dtype=f32), pos), (x, x, z(3)), (x, x, z(4, dtype=t.int64)),
+              (x, x, z(8)[::2]), (x.transpose(1, 2), x.transpose(1, 2), pos)):
+        with pytest.raises(ValueError):
+            kq.rope(*a, f)
+    for a in (z(32), z(2, 32, dtype=f32)):
+        with pytest.raises(ValueError):
+            kq.Rope(a)
+    cache = kq.KVCache(z(4, 2, 16, 64, dtype=t.int8), z(4, 2, 1, 64, 16, dtype=t.int8), *(z(4, 2, 1, dtype=t.uint8) for _ in "kv"))
+    b = kq.KVBatch(z(2, 2), z(2), 32, max_q=2)
+    k, q = x, z(4, 6, 64, dtype=f16)
+    with pytest.raises(KeyError):
+        kq.kv_write_rope(cache, b, f, k, k, q=q, q_out=q, pos=pos)
+    for kw in (dict(q=q), dict(q_out=q), dict(q=z(3, 6, 64, dtype=f16), q_out=q), dict(q=q, q_out=z(4, 5, 64, dtype=f16)),
+               dict(q=q.bfloat16(), q_out=q.bfloat16()), dict(pos=z(3))):
+        with pytest.raises(ValueError):
+            kq.kv_write_rope(cache, b, f, k, k, **kw)
+    with pytest.raises(ValueError):
+        kq.kv_write_rope(cache, b, f, z(4, 3, 64, dtype=f16), k)
+    with pytest.raises(KeyError):
+        kq.kv_keep(cache, b, z(2, 2), z(2))
+    for a in ((z(2, 3), z(2)), (z(2, 2), z(3)), (z(2, 2, dtype=t.int64), z(2))):
+        with pytest.raises(ValueError):
+            kq.kv_keep(cache, b, *a)
+    tree = kq.KVTree(z(4, 1), z(4))
+    with pytest.raises(KeyError):
+        kq.kv_attn_tree(cache, b, tree, q, q.clone(), 0, 0)
+    for bad in (kq.KVTree(z(3, 1)),):
+        with pytest.raises(ValueError):
+            kq.kv_attn_tree(cache, b, bad, q, q.clone(), 0, 0)
+    for a in ((z(4), None), (z(4, 1, dtype=t.int64), None), (z(4, 1), z(3))):
+        with pytest.raises(ValueError):
+            kq.KVTree(*a)
+    for kw in (dict(parent=z(3)), dict(window=-1), dict(pos=z(3)), dict(mask=z(4))):
+        with pytest.raises(ValueError):
+            kq.kv_tree(b, **{**dict(parent=z(4), mask=z(4, 1)), **kw})
