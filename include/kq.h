@@ -585,7 +585,8 @@ kq_status kq_rope_freqs(const kq_rope_scaling* s, float* inv_freq, double* ampli
  * address and strides), and overlaps it in no other way. A slice of a fused projection that holds the
  * queries' and then the keys' heads is turned in one call. head_dim a multiple of 8,
  * at most 512, heads <= 65535; the strides as kq_kv_rows has them. n_rows 0: the call does nothing.
- * One launch. rot a multiple of 16 takes whole vectors; others go value by value. */
+ * One launch. rot a multiple of 16 takes whole vectors, 64 / (rot / 16) heads of a row a wave; others go value
+ * by value, one head a wave up to 1024 rows, then a row. KQ_EUNSUPPORTED where these are more than 4 * (2^24 - 1) waves. */
 kq_status kq_rope(const kq_rope_desc* d, const int32_t* pos, const kq_kv_rows* X, const kq_kv_rows* Y,
                   uint32_t n_rows, uint32_t heads, uint32_t head_dim, kq_dtype dtype,
                   kq_stream_t stream);
@@ -629,11 +630,13 @@ kq_status kq_kv_tree(const kq_kv_batch* batch, const int32_t* parent, uint32_t* 
  * batch's rows -- with window > 0 those behind position pos - window -- and of the batch's
  * rows of its sequence those whose bit is set in its mask, whatever they are (a mask of
  * nothing is one, too). Everything else is kq_kv_attn's: sums, sinks, lse, rows that
- * see nothing, limits of a launch. d->causal is not looked at.
+ * see nothing. d->causal is not looked at. Limits of a launch: kq_kv_attn's, n_seq * heads rounded up
+ * to a multiple of 8; where max_q * (q_heads / heads) > 64, for each 128 of those rows (of 96 or 128 columns, where they are more
+ * than 128: two for each 256).
  * pos: int32 [n_rows], the rows' positions, below 2^31 - 2^16 and at least that of their
  * sequence's first row (else they count as that); read with window > 0 alone, else NULL will do.
  * words * 32 >= max_q, max_q <= 1024 (else KQ_EUNSUPPORTED).
- * ws: kq_kv_attn_tree_workspace_size bytes, otherwise as kq_kv_attn's. */
+ * ws: kq_kv_attn_tree_workspace_size bytes (up to some 70 MB), otherwise as kq_kv_attn's. */
 typedef struct kq_kv_nodes {
     const uint32_t* mask;
     const int32_t* pos;

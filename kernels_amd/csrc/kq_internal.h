@@ -265,8 +265,6 @@ hipError_t launch_kv_write_rope(const kv::Cache& c, const kv::Batch& b, uint32_t
 hipError_t launch_rope(const rope::Rope& r, const int32_t* pos, const kv::Rows& X, const kv::Rows& Y, uint32_t n_rows,
                        uint32_t heads, uint32_t D, kq_dtype f, hipStream_t s);
 bool rope_fits(uint32_t n_rows, uint32_t heads, uint32_t rot);
-// Heads of a row that a wave turns, of n_rows rows.
-uint32_t rope_heads_each(uint64_t n_rows, uint32_t heads, uint32_t rot);
 hipError_t launch_kv_read(const kv::Cache& c, const kv::Batch& b, uint32_t D, int type, const kv::Rows& K,
                           const kv::Rows& V, kq_dtype f, hipStream_t s);
 namespace kv {

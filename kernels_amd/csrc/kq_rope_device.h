@@ -3,7 +3,9 @@
 // An angle pos * inv_freq of a far position needs 64 bits: at position 131072 a float holds the
 // angle of the fastest pair to 0.008. MI355X runs float64 sums and products at the float32 rate, so cosines, sines
 // and the rotation itself are 64-bit too, and what comes out (keys rounded once, blocks' exponents) does not
-// depend on how it is computed. Two lanes never compute the same pair's angle for one row.
+// depend on how it is computed.
+// Rows of queries share their pairs' angles among up to 64 / (rot / 16) heads, through LDS; keys on their way into a cache
+// compute them anew for each head, as one wave is at one head's block.
 #pragma once
 #include "kq_device.h"
 #include "kq_internal.h"

@@ -197,6 +197,14 @@ def test_shares(gpu, n, heads, group, longest, new, kw):
     tree_case(gpu, ragged(n, longest, n, new), heads, group, **{"dim": 64, "nan": True, "pad": 1, **kw})
 
 
+# shares of many rows: a cut for each row of work, and for each workgroup; tiles of 128 and 256 rows, one and two
+@pytest.mark.parametrize("n,heads,group,longest,kw", [
+    (300, 1, 16, 2300, {}), (150, 4, 16, 2300, dict(kind="e4m3")), (150, 1, 32, 2200, dict(dim=128)), (100, 3, 32, 2200, dict(dim=128, kind="e4m3")),
+    (150, 2, 32, 2300, dict(window=2100, sinks=True)), (140, 2, 16, 2200, dict(dim=192)), (90, 2, 24, 2400, dict(dim=96, page=64, block=32))])
+def test_shares_of_many_rows(gpu, n, heads, group, longest, kw):
+    tree_case(gpu, ragged(n, longest, n + group, 8), heads, group, **{"dim": 64, "nan": True, "pad": 1, **kw})
+
+
 def test_long_and_bounds_above(gpu):
     tree_case(gpu, [(9001, 9), (30, 4)], 1, 4, 64, max_len=20000)
     tree_case(gpu, [(4000, 70), (71, 70)], 1, 2, 64, max_len=50000, page=64, block=32)
