@@ -9,7 +9,7 @@
 // down and another continues the same row (trees with Q alone): a workgroup per sequence walks those first. Elsewhere
 // every chunk's workgroup finds the way for itself, which takes less than a launch between.
 //
-// One tree of 26 rows, without Q, over 128256 tokens: 5.8 + 7.1 us, latencies one behind the other (lengths and parents,
+// One tree of 60 rows, without Q, over 128256 tokens: 5.8 + 7.1 us, latencies one behind the other (lengths and parents,
 // probabilities, the way, the row; then sums, their prefix, the chunk, its prefix). 64 chains of 5 rows with Q: 16.5 +
 // 8.8 us for 66 MB, 4 TB/s in the first: each workgroup finds the way before it asks for its 16 KB of P and of Q.
 #include <algorithm>

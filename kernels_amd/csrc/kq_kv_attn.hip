@@ -77,7 +77,7 @@ size_t row_ws_bytes(const Cache& c, const Batch& b, const RowPlan& p, uint64_t s
 // 20-30 rows a sequence; 64 sequences of 1024: 106 us, in shares 134; 32 of 2048: 96, 126; 40 of 256 to 2048: 106, 98;
 // 24 of 512 to 4096: 144, 97; 48 of 4096: 287, 272), up to 192 instead of parts (one sequence of 128: 14.0, in parts 15.9;
 // 192: 16.2, 16.0; 256: 18.4, 16.2; 1024: 43.9, 22.0). A row's beginning is priced as 5 units of 64 tokens (16 sequences of
-// up to 9000 tokens and 26 rows: 203 us, priced as 2: 213, as 8: 209, as 14: 220).
+// 300 to 12000 tokens and 33 to 64 rows: 203 us, priced as 2: 213, as 8: 209, as 14: 220).
 FewPlan tree_plan(const Cache& c, const Batch& b, uint32_t D, uint32_t group, uint32_t window) {
     FewPlan p = {};
     const uint64_t q_rows = (uint64_t)b.max_q * group;

@@ -15,8 +15,8 @@ struct Sources {
 // One wave moves the rows of one head's K or V. A row moves down, or stays: blocks of 16 places are taken in
 // order, and everything that comes into one is in registers before any of it is written, so that no source
 // is overwritten before it is read. Exponent bytes are written after their block. What bounds it is
-// one way to memory after the other: lengths, rows, page ids, exponents, codes. (64 sequences, 8 heads of 128, about 4 of 5-9 rows
-// kept: 7.1 us; the 4.5 MB that it moves would take 0.9. One sequence whose kept rows come first: 1.8 us.)
+// one way to memory after the other: lengths, rows, page ids, exponents, codes. (64 sequences' trees of 26 to 64 rows, 8
+// heads of 64: 7.2 us; what it moves would take 0.9. One sequence of 60 rows, 8 heads of 128: 1.8 us.)
 template <int D, int TYPE>
 __global__ __launch_bounds__(256) void kv_keep_k(Cache c, Batch b, const int32_t* keep, const int32_t* n_keep) {
     __shared__ int rows[kMostNodes];

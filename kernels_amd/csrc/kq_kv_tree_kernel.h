@@ -10,10 +10,10 @@
 // one does, loads beyond an end are of the last element again. (Copies that the compiler makes of registers where
 // lanes meet again behind a branch have been of the masked lanes alone, in kernels that need more than 256 registers.)
 //
-// Two waves a SIMD (some 220 registers) and the instructions that they issue bound it: 16 trees of 26 rows over up to 9000 tokens, 64
+// Two waves a SIMD (some 220 registers) and the instructions that they issue bound it: 16 trees of 33 to 64 rows over 300 to 12000 tokens, 64
 // heads over 8 of 128, take 177 us, 27 of them the join (96 GFLOP; a large matrix product's rate would take 77); 60 rows over
 // 131072 tokens, 32 heads over 8 of 128: 176, 8 of them the join (129 GFLOP, 103). A 32x32x16 product keeps its unit for 33 cycles and the issue for 11, a
-// vector instruction the issue for 4, an exponential 8; of 64 tokens the issue is 1.1 times as long as the products.
+// vector instruction the issue for 4, an exponential 8.
 // Left out one at a time, products, loads from LDS and loads from memory are worth about a tenth each, exponentials
 // nothing. No faster: the next keys' product beside the exponentials (180 us against 182), three tiles in LDS, half of
 // the waves half a tile ahead, 64 rows a wave with one wave a SIMD (250).
