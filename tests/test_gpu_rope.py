@@ -215,6 +215,21 @@ def test_write_rope_positions_and_in_place(gpu):
         write_both(gpu, b, oracle, kq.Rope(fd, pairs=True), "bf16", 5, pos, x, in_place=True)
 
 
+# more heads of queries than a wave takes of a row; blocks whose keys wait in LDS, and one that is too large for it
+@pytest.mark.parametrize("dim,rot,q_heads,page,block", [(256, 256, 37, 16, 16), (128, 128, 70, 32, 32), (64, 64, 129, 64, 64), (64, 64, 3, 128, 128),
+                                                        (96, 96, 43, 32, 16), (64, 48, 1, 32, 32)])
+def test_write_rope_query_heads(gpu, dim, rot, q_heads, page, block):
+    rng = np.random.default_rng(dim + rot + q_heads)
+    b = Batch(gpu, [(150, 40), (9, 9), (33, 1), (7, 0), (70, 70)], page, rng, pad=2)
+    oracle = _kv.Cache(b.n_pages, 1, dim, page, block)
+    oracle.fill(rng)
+    _, fd = freqs_of(rot, gpu)
+    pos = rng.integers(-5, 200000, b.rows).astype(np.int32)
+    x, _ = to(rng.normal(0, 1, (b.rows, q_heads + 2, dim)), "bf16", gpu)
+    write_both(gpu, b, oracle, kq.Rope(fd), "bf16", q_heads, pos, x.clone())
+    write_both(gpu, b, oracle, kq.Rope(fd, pairs=True), "bf16", q_heads, pos, x, in_place=True)
+
+
 def test_write_rope_without_queries(gpu):
     rng = np.random.default_rng(10)
     b = Batch(gpu, [(50, 20), (9, 9)], 16, rng)
