@@ -585,8 +585,9 @@ kq_status kq_rope_freqs(const kq_rope_scaling* s, float* inv_freq, double* ampli
  * address and strides), and overlaps it in no other way. A slice of a fused projection that holds the
  * queries' and then the keys' heads is turned in one call. head_dim a multiple of 8,
  * at most 512, heads <= 65535; the strides as kq_kv_rows has them. n_rows 0: the call does nothing.
- * One launch. rot a multiple of 16 takes whole vectors, 64 / (rot / 16) heads of a row a wave; others go value
- * by value, one head a wave up to 1024 rows, then a row. KQ_EUNSUPPORTED where these are more than 4 * (2^24 - 1) waves. */
+ * One launch. rot a multiple of 16 takes whole vectors, 64 / (rot / 16) heads of a row a wave, and twice that
+ * beyond 1024 rows; others go value by value, one head a wave, and beyond 1024 rows all of a row.
+ * KQ_EUNSUPPORTED where these are more than 4 * (2^24 - 1) waves. */
 kq_status kq_rope(const kq_rope_desc* d, const int32_t* pos, const kq_kv_rows* X, const kq_kv_rows* Y,
                   uint32_t n_rows, uint32_t heads, uint32_t head_dim, kq_dtype dtype,
                   kq_stream_t stream);

@@ -2,8 +2,8 @@
 // (kq_kv_write_rope): keys turned before their block's scale is taken, queries turned beside them.
 //
 // Long prompts are bound by the writes and by 64-bit sums for the angles of keys, which each head's wave computes for itself
-// (five prompts of 1201 to 5003 new tokens, 8 heads of 128 and 32 of queries: 83 us); single tokens by a chain of
-// accesses (5.2 us), as kv_write_k's are.
+// (five prompts of 1201 to 5003 new tokens, 8 heads of 128 and 32 of queries: 80 us); single tokens by a chain of
+// accesses (5.3 us), as kv_write_k's are.
 #include "kq_kv_write_kernel.h"
 
 namespace kq {
@@ -40,8 +40,8 @@ hipError_t write_rope_d(const Cache& c, const Batch& b, const Turn& turn, const 
                         const Rows& K, const Rows& V, hipStream_t s) {
     const uint32_t groups = (2 * c.heads + 3) / 4, blocks = spans(b.max_q, 1u << c.block_log2) * groups;
     // heads of a row of queries a wave: four times as many as its lanes take at once. Waves are few beside the keys' (whose
-    // registers and LDS they share), so that angles saved count for more than in kq_rope (32 heads of 128, bf16: 16384
-    // rows 87.4 us, one time as many 91.3; 48 sequences of 20 rows 11.8, 15.4; one row 4.9 both)
+    // registers and LDS they share), so that angles saved count for more than in kq_rope (32 heads of 128, bf16: 4
+    // sequences of 2048 rows 42.8 us, one time as many 48.6; 48 of 20 rows 12.0, 15.7; one row 5.1 both)
     const uint32_t each = 4 * (64 / (turn.rope.rot / 16));
     const uint32_t parts = Q ? (q_heads + each - 1) / each : 0;
     const dim3 grid(blocks + (uint32_t)(((uint64_t)b.max_q * parts + 3) / 4), b.n_seq);

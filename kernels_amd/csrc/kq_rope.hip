@@ -34,14 +34,15 @@ hipError_t rope_f(const Rope& r, const int32_t* pos, const kv::Rows& X, const kv
 }  // namespace
 }  // namespace rope
 
-// Heads of a row that a wave turns. As many as its lanes take at once: all heads in one wave save most of the angles and cost more than that by their
-// loads one after the other (16384 rows of 40 x 128 bf16: 60.9 us, all heads a wave 65.8; 64 rows: 2.8, 4.3; of 8
-// heads the two are the same). Value by value a wave is at one head for long, and the angles count: one head a wave
-// while the rows are too few for the device's SIMDs (rot 40 of 128 columns, 40 heads, 512 rows: 8.8 us, all heads 12.6;
-// 2048 rows: 32.1, all heads 23.7).
+// Heads of a row that a wave turns, in registers as many as its lanes take at once, and twice that where there are rows
+// enough for the device's SIMDs: the angles count for more then (8192 rows of 40 x 128 bf16: 32.8 us, one time as many 34.1, all
+// heads 34.5; 2048 rows: 9.0, 10.1, 8.5; 64 rows: 2.8 one time, 3.1 twice, 3.8 all). Value by value a wave is
+// at one head for long: one head a wave, or all of them (rot 40 of 128 columns, 40 heads, 512 rows: 8.8 us, all heads
+// 12.6; 2048 rows: 32.1, all heads 23.7).
 static uint32_t rope_heads_each(uint64_t n_rows, uint32_t heads, uint32_t rot) {
-    if (rot % 16 == 0) return 64 / (rot / 16);
-    return n_rows > 1024 ? heads : 1;
+    const bool many = n_rows > 1024;
+    if (rot % 16 == 0) return 64 / (rot / 16) << many;
+    return many ? heads : 1;
 }
 
 bool rope_fits(uint32_t n_rows, uint32_t heads, uint32_t rot) {

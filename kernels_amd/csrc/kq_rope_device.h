@@ -145,27 +145,35 @@ __device__ __forceinline__ void turn_heads(const Rope& r, int pos, const uint8_t
                                            int64_t y_head, uint32_t h0, uint32_t h1, uint32_t D, Factor* table) {
     constexpr int kSize = F == KQ_F32 ? 4 : 2;
     const uint32_t lane = threadIdx.x & 63, pairs = r.rot / 2;
+    // whole vectors: asked for before the angles, and the next heads' before these are turned
+    const bool vectors = r.rot % 16 == 0;
+    const uint32_t units = vectors ? r.rot / 16 : 1, at_once = 64 / units, u = lane % units;
+    const uint32_t ca = first_eight<PAIRS>(u) * kSize, cb = second_eight<PAIRS>(u, r.rot) * kSize;
+    uint32_t h = vectors && lane < at_once * units ? h0 + lane / units : h1;
+    Eight<F> a, b;
+    auto load = [&](uint32_t head) {
+        if (head >= h1) return;
+        const uint8_t* const from = x + (int64_t)head * x_head * kSize;
+        a.load(from + ca);
+        b.load(from + cb);
+    };
+    load(h);
     for (uint32_t i = lane; i < pairs; i += 64) factors(r, pos, i, table[i].c, table[i].s);
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-    if (r.rot % 16 == 0) {
-        const uint32_t units = r.rot / 16, at_once = 64 / units;
-        if (lane < at_once * units) {
-            const uint32_t u = lane % units;
-            const uint32_t ca = first_eight<PAIRS>(u) * kSize, cb = second_eight<PAIRS>(u, r.rot) * kSize;
+    if (vectors) {
+        if (h < h1) {
             Factor f[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) f[e] = table[8 * u + e];
-            for (uint32_t h = h0 + lane / units; h < h1; h += at_once) {
-                const uint8_t* const from = x + (int64_t)h * x_head * kSize;
+            for (; h < h1; h += at_once) {
                 uint8_t* const to = y + (int64_t)h * y_head * kSize;
-                Eight<F> a, b;
-                a.load(from + ca);
-                b.load(from + cb);
-                turn_eight<F, PAIRS>(a, b, [&](int e, double& c, double& s) { c = f[e].c, s = f[e].s; });
-                a.store(to + ca);
-                b.store(to + cb);
+                Eight<F> ya = a, yb = b;
+                load(h + at_once);
+                turn_eight<F, PAIRS>(ya, yb, [&](int e, double& c, double& s) { c = f[e].c, s = f[e].s; });
+                ya.store(to + ca);
+                yb.store(to + cb);
             }
         }
     } else {
@@ -177,15 +185,15 @@ __device__ __forceinline__ void turn_heads(const Rope& r, int pos, const uint8_t
             if constexpr (F == KQ_F32) *reinterpret_cast<float*>(p) = v;
             else *reinterpret_cast<uint16_t*>(p) = (uint16_t)kv::pair16<F == KQ_BF16>(v, 0.0f);
         };
-        for (uint32_t h = h0; h < h1; ++h) {
+        for (h = h0; h < h1; ++h) {
             const uint8_t* const from = x + (int64_t)h * x_head * kSize;
             uint8_t* const to = y + (int64_t)h * y_head * kSize;
             for (uint32_t i = lane; i < pairs; i += 64) {
-                const uint32_t a = (PAIRS ? 2 * i : i) * kSize, b = (PAIRS ? 2 * i + 1 : pairs + i) * kSize;
+                const uint32_t one = (PAIRS ? 2 * i : i) * kSize, two = (PAIRS ? 2 * i + 1 : pairs + i) * kSize;
                 float ya, yb;
-                turn(get(from + a), get(from + b), table[i].c, table[i].s, ya, yb);
-                put(to + a, ya);
-                put(to + b, yb);
+                turn(get(from + one), get(from + two), table[i].c, table[i].s, ya, yb);
+                put(to + one, ya);
+                put(to + two, yb);
             }
         }
     }
@@ -194,16 +202,16 @@ __device__ __forceinline__ void turn_heads(const Rope& r, int pos, const uint8_t
     const uint32_t rest = D - r.rot;
     if (r.rot % 8 == 0) {
         for (uint32_t i = lane; i < (h1 - h0) * (rest / 8); i += 64) {
-            const uint32_t h = h0 + i / (rest / 8), d = (r.rot + i % (rest / 8) * 8) * kSize;
+            const uint32_t head = h0 + i / (rest / 8), d = (r.rot + i % (rest / 8) * 8) * kSize;
             Eight<F> v;
-            v.load(x + (int64_t)h * x_head * kSize + d);
-            v.store(y + (int64_t)h * y_head * kSize + d);
+            v.load(x + (int64_t)head * x_head * kSize + d);
+            v.store(y + (int64_t)head * y_head * kSize + d);
         }
     } else {
         for (uint32_t i = lane; i < (h1 - h0) * rest; i += 64) {
-            const uint32_t h = h0 + i / rest, d = (r.rot + i % rest) * kSize;
-            const uint8_t* const from = x + (int64_t)h * x_head * kSize + d;
-            uint8_t* const to = y + (int64_t)h * y_head * kSize + d;
+            const uint32_t head = h0 + i / rest, d = (r.rot + i % rest) * kSize;
+            const uint8_t* const from = x + (int64_t)head * x_head * kSize + d;
+            uint8_t* const to = y + (int64_t)head * y_head * kSize + d;
             if constexpr (F == KQ_F32) *reinterpret_cast<uint32_t*>(to) = *reinterpret_cast<const uint32_t*>(from);
             else *reinterpret_cast<uint16_t*>(to) = *reinterpret_cast<const uint16_t*>(from);
         }
