@@ -256,3 +256,43 @@ def test_graph(gpu):
         step()
         torch.cuda.synchronize()
         assert torch.equal(got, out)
+
+
+@pytest.mark.parametrize("seqs", [[(3000, 40), (500, 33)], [(3000, 5), (500, 3)]])
+def test_two_streams_and_two_graphs(gpu, seqs):
+    """Two calls at once, each with a workspace of its own; then two graphs that share one, replayed in turn."""
+    b, cache, q, out, lse = tree_case(gpu, seqs, 2, 4, 64, trees=[list(range(-1, m - 1)) for _, m in seqs])
+    parent = dev(np.concatenate([np.arange(-1, m - 1) for _, m in seqs]).astype(np.int32), gpu)
+    tree = kq.kv_tree(b.c, parent, torch.zeros((b.rows, 2), dtype=torch.int32, device=gpu))
+    n = kq.kv_attn_tree_workspace_size(cache, b.c, 8)
+    ws = [torch.full((n,), 0xA5, dtype=torch.uint8, device=gpu) for _ in range(2)]
+    qs = [q, -q]
+    outs = [torch.full_like(out, 7.0) for _ in range(2)]
+
+    def call(i, w):
+        kq.kv_attn_tree(cache, b.c, tree, qs[i], outs[i], ws[w], n)
+
+    call(1, 1)
+    torch.cuda.synchronize()
+    want = [out, outs[1].clone()]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(3):
+        for o in outs:
+            o.fill_(7.0)
+        torch.cuda.synchronize()
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                call(i, i)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, c) for a, c in zip(outs, want)), "two streams"
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    for i, g in enumerate(graphs):
+        with torch.cuda.graph(g):
+            call(i, 0)
+    for _ in range(3):
+        for o in outs:
+            o.fill_(7.0)
+        for g in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, c) for a, c in zip(outs, want)), "two graphs"
