@@ -76,7 +76,10 @@ __device__ __forceinline__ void write_block(const Cache& c, const Batch& b, cons
     const int t0 = (int)t0u;
     const int page = page_of(c, b.pages + (uint64_t)blockIdx.y * b.max_pages, t0);
     const int lo = max(first0 - t0, 0), hi = min(s.len - t0, B);  // the block's new tokens
-    const Rows& R = is_v ? V : K;
+    // field by field: from a reference to one of the two the compiler makes more offsets of rows ahead, and takes 268
+    // registers at 192 columns and one wave a SIMD in place of 179 and two (five prompts of 331 to 5001 tokens, 8 heads,
+    // bf16: 59 us in place of 38), 104 at 96 in place of 92 (17.1 and 15.7)
+    const Rows R = {is_v ? V.p : K.p, is_v ? V.row : K.row, is_v ? V.head : K.head};
     const uint16_t* const x = static_cast<const uint16_t*>(R.p) + (int64_t)(s.row0 + t0 - first) * R.row +
                               (int64_t)h * R.head;  // token t0's values
 
