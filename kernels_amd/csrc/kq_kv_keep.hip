@@ -71,8 +71,9 @@ __global__ __launch_bounds__(256) void kv_keep_k(Cache c, Batch b, const int32_t
             __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
             __builtin_amdgcn_wave_barrier();
             __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-            // 2^(its exponent - e) of a token (below 2^-126 every code rounds to zero all the same); no page: zero
-            auto keeps = [&](int exp) { return exp < 0 ? 0.0f : pow2f(max(exp - e, -126)); };
+            // 2^(its exponent - e) of a token (below 2^-126 every code rounds to zero all the same). Of no page: codes of
+            // zero, whatever was read in their place (times zero a negative e4m3 value would leave its sign)
+            auto keeps = [&](int exp) { return pow2f(max(exp - e, -126)); };
             uint8_t* const to = codes + code_offset(c, D, page, h, sub);
             if (!is_v) {
                 constexpr int N = D / 32;
@@ -88,7 +89,8 @@ __global__ __launch_bounds__(256) void kv_keep_k(Cache c, Batch b, const int32_t
                     const int i = lane + 64 * j, t = i / (D / 8), exp = src.exp[t];
                     if (sub + t >= hi || (src.in[t] < 0 && !grew)) continue;
                     const float f = keeps(exp);
-                    const u32x2 y = exp == e ? w[j] : u32x2{rounded_anew<TYPE>(w[j].x, f), rounded_anew<TYPE>(w[j].y, f)};
+                    u32x2 y = exp == e ? w[j] : u32x2{rounded_anew<TYPE>(w[j].x, f), rounded_anew<TYPE>(w[j].y, f)};
+                    if (exp < 0) y = u32x2{0, 0};
                     *reinterpret_cast<u32x2*>(to + i * 8) = y;
                 }
                 continue;
@@ -106,7 +108,7 @@ __global__ __launch_bounds__(256) void kv_keep_k(Cache c, Batch b, const int32_t
                     const int exp = src.exp[t];
                     uint32_t byte = in < 0 ? w[j][t / 4] >> 8 * (t % 4) & 0xFF : codes[src.code[t] + (uint32_t)(col * 16 + in)];
                     if (sub + t >= hi) continue;
-                    if (exp != e) byte = rounded_anew<TYPE>(byte, keeps(exp)) & 0xFF;
+                    if (exp != e) byte = exp < 0 ? 0 : rounded_anew<TYPE>(byte, keeps(exp)) & 0xFF;
                     w[j][t / 4] = (w[j][t / 4] & ~(0xFFu << 8 * (t % 4))) | byte << 8 * (t % 4);
                 }
             }

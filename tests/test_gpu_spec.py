@@ -12,7 +12,7 @@ from kernels_amd import kq
 from tests import _kv, _rope, _spec
 from tests._util import dev
 from tests.test_gpu_graphs import replay_check
-from tests.test_gpu_kv import Batch, same_cache, to, upload
+from tests.test_gpu_kv import Batch, codes_of, same_cache, to, upload
 
 pytestmark = pytest.mark.gpu
 NEAR = 2.0**-30
@@ -361,3 +361,36 @@ def test_step(gpu, kind, dtype, page, block):
         tol, _ = _kv.attend_tolerance(*want, dim, eps, tiny)
         assert (np.abs(out1[i:i + 1].double().cpu().numpy() - want[0]) <= tol).all(), i
     same_cache(cache, oracle, "step")
+
+
+@pytest.mark.parametrize("kind", ["i8", "e4m3"])
+@pytest.mark.parametrize("dim,page,block", [(64, 16, 16), (96, 32, 16), (256, 64, 32)])
+def test_keep_of_no_page(gpu, dim, page, block, kind):
+    """Rows whose page is none come as codes of zero, whatever the cache's other pages hold (negative values here, and
+    codes that are no values)."""
+    rng = np.random.default_rng(dim)
+    n, m = 6 * page, 3 * page
+    b = Batch(gpu, [(n, m), (n, m)], page, rng)
+    b.table[0, 4], b.table[1, 5] = -1, b.n_pages
+    b.c.pages.copy_(torch.from_numpy(b.table))
+    oracle = _kv.Cache(b.n_pages, 2, dim, page, block, kind)
+    oracle.fill(rng)
+    for w in "kv":
+        oracle.codes[w] |= 0x80
+        oracle.codes[w][(oracle.codes[w] & 0x7F) == (0x7F if kind == "e4m3" else 0)] ^= 1
+    rows = list(range(1, m, 2))
+    none = [int(p) for p in b.table[:, 3:].ravel() if 0 <= p < b.n_pages]
+    oracle.codes["k"][[p for p in range(b.n_pages) if p not in b.table]] = 0xFF  # pages of no sequence
+    assert none and len(rows) < b.max_q
+    cache = upload(oracle, gpu)
+    keep = np.full((2, b.max_q), -1, np.int32)
+    keep[:, :len(rows)] = rows
+    kq.kv_keep(cache, b.c, dev(keep, gpu), dev(np.full(2, len(rows), np.int32), gpu))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for w in "kv":
+            _spec.keep_rows(oracle, w, b.table[i], n, m, rows)
+    same_cache(cache, oracle, "keep")
+    codes, _ = codes_of(cache)
+    for w in "kv":
+        assert np.array_equal(codes[w], oracle.codes[w]), f"{w}: the bytes"
