@@ -637,7 +637,8 @@ kq_status kq_kv_tree(const kq_kv_batch* batch, const int32_t* parent, uint32_t* 
  * pos: int32 [n_rows], the rows' positions, below 2^31 - 2^16 and at least that of their
  * sequence's first row (else they count as that); read with window > 0 alone, else NULL will do.
  * words * 32 >= max_q, max_q <= 1024 (else KQ_EUNSUPPORTED).
- * ws: kq_kv_attn_tree_workspace_size bytes (up to some 70 MB), otherwise as kq_kv_attn's. */
+ * ws: kq_kv_attn_tree_workspace_size bytes (up to some 70 MB while max_q * (q_heads / heads) is 32768 at most,
+ * and some 140 beyond, of heads of 256), otherwise as kq_kv_attn's. */
 typedef struct kq_kv_nodes {
     const uint32_t* mask;
     const int32_t* pos;

@@ -382,3 +382,19 @@ def test_python_refusals(no_gpu):
     for kw in (dict(parent=z(3)), dict(window=-1), dict(pos=z(3)), dict(mask=z(4))):
         with pytest.raises(ValueError):
             kq.kv_tree(b, **{**dict(parent=z(4), mask=z(4, 1)), **kw})
+
+
+@pytest.mark.parametrize("dim", [64, 96, 128, 192, 256])
+def test_tree_workspace_at_most(dim):
+    """The sizes that kq.h names: some 70 MB while a sequence and head has up to 32768 rows, and some 140 beyond."""
+    most = {False: 0, True: 0}
+    for heads in (1, 2, 8, 64):
+        for group in (1, 3, 8, 33, 64):
+            for max_q in (1, 2, 9, 33, 128, 257, 512, 513, 516, 1000, 1024):
+                for n_seq in (1, 7, 200):
+                    for max_len in (100, 3000, 2**20):
+                        b = batch_c(n_seq=n_seq, max_q=max_q, n_rows=n_seq * max_q, max_len=max_len, max_pages=2**17)
+                        many = max_q * group > 32768
+                        most[many] = max(most[many], size(cache_c(head_dim=dim, heads=heads), b, heads * group))
+    assert 0 < most[False] <= 70e6 and most[True] <= 140e6
+    assert dim < 192 or most[True] > 100e6
