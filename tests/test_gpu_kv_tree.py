@@ -296,3 +296,41 @@ def test_two_streams_and_two_graphs(gpu, seqs):
             g.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, c) for a, c in zip(outs, want)), "two graphs"
+
+
+@pytest.mark.parametrize("dim,kind", [(192, "i8"), (256, "e4m3"), (128, "i8"), (64, "e4m3")])
+@pytest.mark.parametrize("max_q", [520, 1024])
+def test_bounds_of_many_tiles(gpu, dim, kind, max_q):
+    """A bound of rows far above what the sequences have: more tiles than workgroups that the device holds at once (of 128
+    rows, at 64 heads a key), one group, the largest workspaces."""
+    def bound(b, gpu):
+        b.max_q = max_q
+        b.c = kq.KVBatch(b.c.pages, b.c.kv_len, b.max_len, q_start=b.c.q_start, max_q=max_q)
+
+    tree_case(gpu, [(700, 5), (0, 0), (80, 1), (9, 3)], 2, 64, dim, kind, nan=True, pad=1, max_len=5000, spoil=bound)
+    tree_case(gpu, [(300, 3), (90, 2)], 1, 64, dim, kind, "bf16", window=70, sinks=True, spoil=bound)
+
+
+def test_most_sequences(gpu):
+    """65535 sequences: masks, positions, and a tree's attention of equal values, which is that value."""
+    n = 65535
+    cache = kq.kv_cache(n, 1, 64, device=gpu)
+    cache.v.fill_(3)
+    cache.v_exp.fill_(127)
+    pages = torch.arange(n, dtype=torch.int32, device=gpu).flip(0)[:, None].contiguous()
+    kv_len = torch.arange(n, dtype=torch.int32, device=gpu) % 14 + 3
+    b = kq.KVBatch(pages, kv_len, 16, max_q=3)
+    mask, pos = torch.full((3 * n, 1), 77, dtype=torch.int32, device=gpu), torch.full((3 * n,), 77, dtype=torch.int32, device=gpu)
+    tree = kq.kv_tree(b, torch.tensor([-1, 0, 0], dtype=torch.int32, device=gpu).repeat(n), mask, pos)
+    torch.cuda.synchronize()
+    assert torch.equal(mask.view(n, 3).cpu(), torch.tensor([[1, 3, 5]], dtype=torch.int32).repeat(n, 1))
+    assert torch.equal(pos.view(n, 3), kv_len[:, None] - 3 + torch.tensor([0, 1, 1], dtype=torch.int32, device=gpu))
+    q = torch.randn((3 * n, 2, 64), device=gpu).half()
+    out, lse = torch.zeros_like(q), torch.zeros((3 * n, 2), device=gpu)
+    size = kq.kv_attn_tree_workspace_size(cache, b, 2)
+    kq.kv_attn_tree(cache, b, tree, q, out, torch.empty(size, dtype=torch.uint8, device=gpu), size, lse=lse)
+    torch.cuda.synchronize()
+    assert (out == 3).all()
+    seen = (kv_len[:, None] - 3 + torch.tensor([1, 2, 2], device=gpu)).view(-1, 1).float()
+    # keys of zero: lse is the logarithm of the tokens' number, below 4: four roundings of 2^-22 (sum, logarithm, factor, torch's)
+    assert ((lse - seen.log()).abs() <= 2.0**-20).all()

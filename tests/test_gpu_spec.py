@@ -394,3 +394,51 @@ def test_keep_of_no_page(gpu, dim, page, block, kind):
     codes, _ = codes_of(cache)
     for w in "kv":
         assert np.array_equal(codes[w], oracle.codes[w]), f"{w}: the bytes"
+
+
+def test_verify_most_sequences(gpu):
+    """65535 chains of one token picked outright, in a vocabulary of 7."""
+    n, vocab, rng = 65535, 7, np.random.default_rng(0)
+    p = softmax(rng.normal(0, 1.5, (2 * n, vocab)))
+    token = rng.integers(0, vocab, 2 * n).astype(np.int32)
+    u = rng.random(2 * n).astype(np.float32)
+    keep, out = (torch.full((n, 2), 77, dtype=torch.int32, device=gpu) for _ in "ko")
+    n_keep = torch.full((n,), 77, dtype=torch.int32, device=gpu)
+    size = kq.draft_verify_workspace_size(n, 2, vocab)
+    kq.draft_verify(dev(p, gpu), dev(token, gpu), dev(u, gpu), keep, n_keep, out, torch.empty(size, dtype=torch.uint8, device=gpu), size)
+    torch.cuda.synchronize()
+    i, x, u0, u1 = np.arange(n), token[1::2], u[0::2].astype(np.float64), u[1::2].astype(np.float64)
+    there = p[0::2][i, x].astype(np.float64)
+    kept = u1 < there
+    left = p[0::2].astype(np.float64)
+    left[i, x] = 0.0
+    left[kept] = p[1::2][kept]
+    up = left.cumsum(1)
+    aim = u0 * up[:, -1]
+    last = (up <= aim[:, None]).sum(1)
+    sure = np.abs(up - aim[:, None]).min(1) > NEAR  # nearer to a border either place is right
+    assert sure.mean() > 0.999
+    got = out.cpu().numpy()
+    assert np.array_equal(n_keep.cpu().numpy(), 1 + kept)
+    assert np.array_equal(keep.cpu().numpy(), np.stack([np.zeros(n), np.where(kept, 1, -1)], 1))
+    assert np.array_equal(got[kept, 0], x[kept]) and (got[~kept, 1] == -1).all()
+    assert np.array_equal(got[i, kept.astype(int)][sure], last[sure])
+
+
+def test_keep_most_sequences(gpu):
+    """65535 sequences of a page each, two rows of four moved, exponents all the same: codes as they were."""
+    n = 65535
+    cache = kq.kv_cache(n, 1, 64, device=gpu)
+    g = torch.Generator(device=gpu)
+    g.manual_seed(0)
+    for t in (cache.k, cache.v):
+        t.copy_(torch.randint(-127, 128, t.shape, generator=g, device=gpu, dtype=torch.int8))
+    pages = torch.arange(n, dtype=torch.int32, device=gpu).flip(0)[:, None].contiguous()
+    kv_len = torch.full((n,), 16, dtype=torch.int32, device=gpu)
+    k, v = cache.k.clone(), cache.v.clone()
+    k[:, :, 12:14], v[..., 12:14] = k[:, :, 13::2].clone(), v[..., 13::2].clone()
+    kq.kv_keep(cache, kq.KVBatch(pages, kv_len, 16, max_q=4), torch.tensor([1, 3, -1, -1], dtype=torch.int32, device=gpu).repeat(n, 1),
+               torch.full((n,), 2, dtype=torch.int32, device=gpu))
+    torch.cuda.synchronize()
+    assert torch.equal(cache.k, k) and torch.equal(cache.v, v)
+    assert (cache.k_exp == 63).all() and (cache.v_exp == 63).all()
