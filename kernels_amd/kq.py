@@ -724,7 +724,7 @@ def rope_freqs(rot, base=10000.0, kind="plain", factor=1.0, low=1.0, high=None, 
     import torch
     _need(kind in ROPE_KINDS, f"kind: one of {', '.join(ROPE_KINDS)}")
     _need(0 <= rot < 2**32, "rot: 32-bit")
-    got, amplitude = (C.c_float * max(rot // 2, 1))(), C.c_double(0.0)
+    got, amplitude = (C.c_float * max(min(rot, 512) // 2, 1))(), C.c_double(0.0)  # beyond 512 the call refuses
     d = _RopeScalingC(ROPE_KINDS.index(kind), rot, base, factor, low, (32.0 if kind == "yarn" else 4.0) if high is None else high,
                       original)
     _check(lib().kq_rope_freqs(C.byref(d), got, C.byref(amplitude)), "kq_rope_freqs")

@@ -398,3 +398,18 @@ def test_tree_workspace_at_most(dim):
                         most[many] = max(most[many], size(cache_c(head_dim=dim, heads=heads), b, heads * group))
     assert 0 < most[False] <= 70e6 and most[True] <= 140e6
     assert dim < 192 or most[True] > 100e6
+
+
+def test_freqs_refused_without_memory():
+    """A rot that is refused takes no memory for its frequencies first."""
+    import tracemalloc
+    tracemalloc.start()
+    try:
+        for rot in (514, 2**20, 2**26):
+            with pytest.raises(kq.KQError):
+                kq.rope_freqs(rot, device="cpu")
+        assert tracemalloc.get_traced_memory()[1] < 2**20
+    finally:
+        tracemalloc.stop()
+    got, _ = kq.rope_freqs(512, device="cpu")
+    assert got.shape == (256,)
