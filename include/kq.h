@@ -623,15 +623,15 @@ kq_status kq_kv_write_rope(const kq_kv_cache* cache, const kq_kv_batch* batch,
  *          window > 0 the nearest `window` of them alone. words >= max_q / 32, rounded up
  * pos    : int32 [n_rows] or NULL, written: kv_len - n + the row's depth
  * Rows of no sequence are left as they were. max_q <= 1024 (else KQ_EUNSUPPORTED). The
- * batch's pages are not read. One launch. */
+ * batch's pages are not read (lengths are cut to max_len alone). One launch. */
 kq_status kq_kv_tree(const kq_kv_batch* batch, const int32_t* parent, uint32_t* mask,
                      uint32_t words, int32_t* pos, uint32_t window, kq_stream_t stream);
 
 /* kq_kv_attn of a tree's rows: a row sees the tokens of its sequence before the
  * batch's rows -- with window > 0 those behind position pos - window -- and of the batch's
  * rows of its sequence those whose bit is set in its mask, whatever they are (a mask of
- * nothing is one, too). Everything else is kq_kv_attn's: sums, sinks, lse, rows that
- * see nothing. d->causal is not looked at. Limits of a launch: kq_kv_attn's, n_seq * heads rounded up
+ * nothing is one, too). Everything else is kq_kv_attn's: sums and roundings (probabilities and
+ * queries as fp16 in the products), sinks, lse, rows that see nothing. d->causal is not looked at. Limits of a launch: kq_kv_attn's, n_seq * heads rounded up
  * to a multiple of 8; where max_q * (q_heads / heads) > 64, for each 128 of those rows (of 96 or 128 columns, where they are more
  * than 128: two for each 256).
  * pos: int32 [n_rows], the rows' positions, below 2^31 - 2^16 and at least that of their
@@ -694,7 +694,7 @@ kq_status kq_draft_verify(const kq_draft* d, int32_t* keep, int32_t* n_keep, int
 /* Moves the kept rows of each sequence together: row keep[i][j] of sequence i's newest
  * tokens goes to the place of its row j, j < n_keep[i]. keep: int32 [n_seq][max_q],
  * ascending (so that keep[i][j] >= j); n_keep: int32 [n_seq], cut to max_q and the
- * sequence's rows. An entry that is less than its j or that of the row before, or no row, ends
+ * sequence's rows. An entry that is less than its j, not more than the one before it, or no row, ends
  * the list there. The sequence then holds kv_len - n + n_keep tokens, which
  * is the caller's to set; what is behind them may be overwritten by the next step.
  * Codes are moved as they are where the two blocks' exponents are the same. A

@@ -11,7 +11,10 @@
 //
 // One tree of 60 rows, without Q, over 128256 tokens: 5.8 + 7.1 us, latencies one behind the other (lengths and parents,
 // probabilities, the way, the row; then sums, their prefix, the chunk, its prefix). 64 chains of 5 rows with Q: 16.5 +
-// 8.8 us for 66 MB, 4 TB/s in the first: each workgroup finds the way before it asks for its 16 KB of P and of Q.
+// 8.8 us for 66 MB, 4 TB/s in the first: each workgroup finds the way before it asks for its 16 KB of P and of Q. Trees with Q are
+// far from what their bytes take: of 16 rows that share their parents' Q, 46 us in the walk for one sequence, 197 for 16 and 423 for 64, then
+// 13 to 23. A workgroup sums a row up alone for each sibling behind one that was turned down, from P and all the Q so far, a value at a time for
+// each thread.
 #include <algorithm>
 
 #include "kq_device.h"

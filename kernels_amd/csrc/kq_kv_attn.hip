@@ -76,8 +76,10 @@ size_t row_ws_bytes(const Cache& c, const Batch& b, const RowPlan& p, uint64_t s
 // of 128 columns: 135 KB): one workgroup for each row of work up to 2048 tokens instead of shares (64 heads over 8 of 128,
 // 20-30 rows a sequence; 64 sequences of 1024: 106 us, in shares 134; 32 of 2048: 96, 126; 40 of 256 to 2048: 106, 98;
 // 24 of 512 to 4096: 144, 97; 48 of 4096: 287, 272), up to 192 instead of parts (one sequence of 128: 14.0, in parts 15.9;
-// 192: 16.2, 16.0; 256: 18.4, 16.2; 1024: 43.9, 22.0). A row's beginning is priced as 5 units of 64 tokens (16 sequences of
-// 300 to 12000 tokens and 33 to 64 rows: 203 us, priced as 2: 213, as 8: 209, as 14: 220).
+// 192: 16.2, 16.0; 256: 18.4, 16.2; 1024: 43.9, 22.0). A row's beginning is priced as 5 units of 64 tokens (measured on one batch
+// alone, 16 sequences of 300 to 12000 tokens and 33 to 64 rows: 203 us, priced as 2: 213, as 8: 209, as 14: 220). One
+// long sequence was faster in splits by the host's bounds, which kq_kv_attn's rows have (60 rows over 131071 tokens: 166 us, in
+// shares 176, for a cause not known); that batch took 359 in them.
 FewPlan tree_plan(const Cache& c, const Batch& b, uint32_t D, uint32_t group, uint32_t window) {
     FewPlan p = {};
     const uint64_t q_rows = (uint64_t)b.max_q * group;

@@ -539,7 +539,7 @@ __global__ __launch_bounds__(256, few_waves(D)) void kv_few_k(Cache c, Batch b, 
                     for (int i = 0; i < 16; ++i) {
                         const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(st[k][i / 4][i % 4], f, down));
                         sum += y;
-                        w[k][i / 8][i % 8] = (_Float16)y;
+                        w[k][i / 8][i % 8] = (_Float16)y;  // for the product: codes are exact in fp16, probabilities 2^-11 of each
                     }
                     l[k] += sum * un_v;
                 }

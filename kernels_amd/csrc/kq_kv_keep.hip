@@ -15,8 +15,10 @@ struct Sources {
 // One wave moves the rows of one head's K or V. A row moves down, or stays: blocks of 16 places are taken in
 // order, and everything that comes into one is in registers before any of it is written, so that no source
 // is overwritten before it is read. Exponent bytes are written after their block. What bounds it is
-// one way to memory after the other: lengths, rows, page ids, exponents, codes. (64 sequences' trees of 26 to 64 rows, 8
-// heads of 64: 7.2 us; what it moves would take 0.9. One sequence of 60 rows, 8 heads of 128: 1.8 us.)
+// one way to memory after the other: lengths, rows, page ids, exponents, codes; of V, whose columns hold 16 tokens each, then a moved token's
+// byte in each column, waited for before the next token's is asked for. (One sequence of 60 rows, 8 heads of 128, every eighth of
+// the rows kept: 6.6 us; 64 trees of 26 to 64 rows, 8 heads of 64: 7.4, where what it moves would take 0.9. Rows that
+// all stay, and the wave has nothing to do: 1.6.)
 template <int D, int TYPE>
 __global__ __launch_bounds__(256) void kv_keep_k(Cache c, Batch b, const int32_t* keep, const int32_t* n_keep) {
     __shared__ int rows[kMostNodes];

@@ -2,8 +2,12 @@
 // (kq_kv_write_rope): keys turned before their block's scale is taken, queries turned beside them.
 //
 // Long prompts are bound by the writes and by 64-bit sums for the angles of keys, which each head's wave computes for itself
-// (five prompts of 1201 to 5003 new tokens, 8 heads of 128 and 32 of queries: 80 us); single tokens by a chain of
-// accesses (5.3 us), as kv_write_k's are.
+// (five prompts of 1201 to 5003 new tokens, 8 heads of 128 and 32 of queries: 78 us, as long as kq_rope and then kq_kv_write take, 75).
+// At 192 and 256 columns the two calls are faster (blocks of 16: 120 and 154 us, in one call 153 and 177; blocks of 64, whose keys
+// are turned twice, 122 and 182 at 192): the queries' waves hold the keys' registers and LDS, two waves a SIMD.
+// Single tokens are bound by a chain of accesses (5.3 us), as kv_write_k's are; batches of trees by that chain with the angles in it and by the
+// queries' rows, a wave each: 48 trees of 9 to 26 rows, 64 heads of queries over 8 of 128, 64 columns turned, 15.3 us, without
+// queries 11.3 (kq_kv_write 9.3), with all columns turned 13.0: those that are not turned come last, a load, a wait and a store at a time.
 #include "kq_kv_write_kernel.h"
 
 namespace kq {

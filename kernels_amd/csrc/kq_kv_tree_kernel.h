@@ -10,10 +10,18 @@
 // one does, loads beyond an end are of the last element again. (Copies that the compiler makes of registers where
 // lanes meet again behind a branch have been of the masked lanes alone, in kernels that need more than 256 registers.)
 //
-// Two waves a SIMD (some 220 registers) and the instructions that they issue bound it: 16 trees of 33 to 64 rows over 300 to 12000 tokens, 64
-// heads over 8 of 128, take 177 us, 27 of them the join (96 GFLOP; a large matrix product's rate would take 77); 60 rows over
-// 131072 tokens, 32 heads over 8 of 128: 176, 8 of them the join (129 GFLOP, 103). A 32x32x16 product keeps its unit for 33 cycles and the issue for 11, a
-// vector instruction the issue for 4, an exponential 8.
+// What bounds it is time that two waves a SIMD (some 220 registers) leave open. By counters, of a wave's time a half is waits for loads,
+// for LDS and for the others at each tile's barrier (60 rows over 131072 tokens: 50%, 16 trees of 33 to 64 rows: 56), a seventh
+// waits for the issue, a third issues (35, 29). No unit is full: matrix products 39% of a SIMD's time (30), vector instructions 50 (40), LDS
+// 28 (24, a tenth of it bank conflicts). Those 16 trees, over 300 to 12000 tokens, 64 heads over 8 of 128, take 177 us, 27 of
+// them the join (96 GFLOP; a large matrix product's rate would take 77; of their waves 22%, weighted by tokens, have no rows); 60 rows over
+// 131072 tokens, 32 heads over 8 of 128: 176, 8 of them the join (129 GFLOP, 103). A 32x32x16 product keeps its unit for 32 cycles and
+// the issue for 11, a vector instruction the issue for 4, an exponential 8.
+//
+// Probabilities are rounded to fp16 for their product with V (2^-11 of each at most), as in kv_rows_k: codes are exact in fp16, whose products run
+// at sixteen times the rate of 32-bit ones. Sums, statistics and the denominator, which adds up what was not rounded, are 32 bits. Against 64 bits outputs
+// are off by 0.16390% of their size over those 16 trees, bf16, of which the output's own rounding is 0.1636; 0.16074 over the long sequence, of 0.1607;
+// in fp16 (26 rows over 701 tokens) 0.0207, of 0.0205.
 // Left out one at a time, products, loads from LDS and loads from memory are worth about a tenth each, exponentials
 // nothing. No faster: the next keys' product beside the exponentials (180 us against 182), three tiles in LDS, half of
 // the waves half a tile ahead, 64 rows a wave with one wave a SIMD (250).
@@ -200,7 +208,7 @@ __device__ __forceinline__ void tree_piece(const Cache& c, const Batch& b, const
             for (int i = 0; i < 16; ++i) {
                 const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(st[u][i], f[u], down));
                 sum += y;
-                w[i / 8][i % 8] = (_Float16)y;
+                w[i / 8][i % 8] = (_Float16)y;  // what the product takes (above)
             }
             l += sum * pow2f(base - (u ? v1 : v0));
 #pragma unroll

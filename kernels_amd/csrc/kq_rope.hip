@@ -38,7 +38,7 @@ hipError_t rope_f(const Rope& r, const int32_t* pos, const kv::Rows& X, const kv
 // enough for the device's SIMDs: the angles count for more then (8192 rows of 40 x 128 bf16: 32.8 us, one time as many 34.1, all
 // heads 34.5; 2048 rows: 9.0, 10.1, 8.5; 64 rows: 2.8 one time, 3.1 twice, 3.8 all). Value by value a wave is
 // at one head for long: one head a wave, or all of them (rot 40 of 128 columns, 40 heads, 512 rows: 8.8 us, all heads
-// 12.6; 2048 rows: 32.1, all heads 23.7).
+// 12.6; 2048 rows: 32.1, all heads 23.7). Its accesses of two bytes bound it: 2.8 times what a copy of those rows takes (rot 64: 8.5).
 static uint32_t rope_heads_each(uint64_t n_rows, uint32_t heads, uint32_t rot) {
     const bool many = n_rows > 1024;
     if (rot % 16 == 0) return 64 / (rot / 16) << many;

@@ -18,7 +18,7 @@ __device__ __forceinline__ void each_ancestor(const int* parent, int j, Fn f) {
 
 // A workgroup a sequence, a thread a row: it walks up its own ancestors. They come in falling order, so
 // that each word of the mask is whole before the next begins. Latency bounds it: a step of
-// the way is one read of LDS.
+// the way is one read of LDS (one tree of 60 rows 2.7 us, 64 of 64 rows 3.8, 16 of 1024 rows, up to 130 deep, 44).
 __global__ __launch_bounds__(256) void kv_tree_k(Batch b, const int32_t* parents, uint32_t* mask, uint32_t words, int32_t* pos,
                                                  uint32_t window) {
     __shared__ int parent[kMostNodes];
