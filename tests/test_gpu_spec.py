@@ -442,3 +442,84 @@ def test_keep_most_sequences(gpu):
     torch.cuda.synchronize()
     assert torch.equal(cache.k, k) and torch.equal(cache.v, v)
     assert (cache.k_exp == 63).all() and (cache.v_exp == 63).all()
+
+
+@pytest.mark.parametrize("draft", ["none", "shared"])
+def test_verify_two_streams_and_two_graphs(gpu, draft):
+    """Two calls at once, each with a workspace of its own; then two graphs that share one, replayed in turn, with
+    other numbers between the replays."""
+    rng = np.random.default_rng(11)
+    trees = [_spec.random_tree(rng, n) for n in (20, 33, 5)]
+    starts = np.concatenate([[0], np.cumsum([len(t) for t in trees])]).astype(np.int32)
+    vocab, rows, max_q = 9000, int(starts[-1]), 33
+    size = kq.draft_verify_workspace_size(3, max_q, vocab)
+    ws = [torch.full((size,), 0xA5, dtype=torch.uint8, device=gpu) for _ in range(2)]
+    parent, start = dev(np.concatenate(trees).astype(np.int32), gpu), dev(starts, gpu)
+    calls, outs, us, ins = [], [], [], []
+    for i in range(2):
+        parts = [draft_of(rng, t, vocab, 3.0, 0.5, draft) for t in trees]
+        p, tok, u = (np.concatenate([d[k] for d in parts]) for k in range(3))
+        rows_of = np.concatenate([np.where(d[4] < 0, -1, d[4] + s) for d, s in zip(parts, starts)]).astype(np.int32)
+        q = None if draft == "none" else dev(np.concatenate([d[3] for d in parts]), gpu)
+        out = [torch.full((3, max_q), 77, dtype=torch.int32, device=gpu) for _ in "ko"] + [torch.full((3,), 77, dtype=torch.int32, device=gpu)]
+        args = dict(q=q, q_index=None if q is None else dev(rows_of, gpu), parent=parent, start=start)
+        pd, td, ud = dev(p, gpu), dev(tok, gpu), dev(u, gpu)
+        calls.append(lambda w, pd=pd, td=td, ud=ud, out=out, args=args: kq.draft_verify(pd, td, ud, out[0], out[2], out[1], ws[w], size, **args))
+        outs.append(out), us.append(ud), ins.append(parts)
+
+    def check(i):
+        u = us[i].cpu().numpy()
+        for s, (t, d) in enumerate(zip(trees, ins[i])):
+            kept, toks, margin = _spec.verify(d[0], d[1], u[starts[s]:starts[s + 1]], t, d[3], d[4])
+            assert margin > NEAR
+            n = int(outs[i][2][s])
+            assert n == len(kept) and outs[i][0][s].tolist() == kept + [-1] * (max_q - n) and outs[i][1][s].tolist() == toks + [-1] * (max_q - n)
+
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                calls[i](i)
+        torch.cuda.synchronize()
+        check(0), check(1)
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    for i, g in enumerate(graphs):
+        with torch.cuda.graph(g):
+            calls[i](0)
+    for _ in range(3):
+        for u in us:
+            u.copy_(torch.from_numpy(rng.random(rows).astype(np.float32)))
+        for g in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        check(0), check(1)
+
+
+def test_keep_graph(gpu):
+    """kq_kv_keep captured, replayed on lengths, rows and codes that change between replays."""
+    rng = np.random.default_rng(4)
+    seqs = [(150, 20), (90, 20), (33, 20)]
+    b = Batch(gpu, seqs, 32, rng, q_start=False)
+    first = _kv.Cache(b.n_pages, 2, 128, 32, 32, "e4m3")
+    first.fill(rng)
+    cache = upload(first, gpu)
+    keep, n_keep = torch.zeros((3, 20), dtype=torch.int32, device=gpu), torch.zeros(3, dtype=torch.int32, device=gpu)
+    kq.kv_keep(cache, b.c, keep, n_keep)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        kq.kv_keep(cache, b.c, keep, n_keep)
+    torch.cuda.synchronize()
+    oracle = first.copy()
+    for r in range(4):
+        rows = [sorted(rng.permutation(20)[:rng.integers(1, 20)].tolist()) for _ in seqs]
+        lens = [n - 3 * r for n, _ in seqs]
+        b.c.kv_len.copy_(torch.tensor(lens, dtype=torch.int32))
+        keep.copy_(torch.tensor([x + [-1] * (20 - len(x)) for x in rows], dtype=torch.int32))
+        n_keep.copy_(torch.tensor([len(x) for x in rows], dtype=torch.int32))
+        g.replay()
+        torch.cuda.synchronize()
+        for i, n in enumerate(lens):
+            for w in "kv":
+                _spec.keep_rows(oracle, w, b.table[i], n, 20, rows[i])
+        same_cache(cache, oracle, f"replay {r}")
